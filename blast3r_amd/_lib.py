@@ -140,6 +140,35 @@ class BaTangentArgs(ctypes.Structure):
                 ('H_z', c_p), ('workspace', c_p), ('workspace_bytes', c_i64)]
 
 
+c_p2 = c_p * 2
+c_i64x2 = c_i64 * 2
+
+
+class BaRotaryArgs(ctypes.Structure):
+    _fields_ = [('x', c_p2), ('y', c_p2), ('x_sb', c_i64x2), ('x_st', c_i64x2), ('x_sh', c_i64x2),
+                ('y_sb', c_i64x2), ('y_st', c_i64x2), ('y_sh', c_i64x2), ('heads', c_int * 2), ('n_x', c_int),
+                ('dtype', c_int), ('B', c_i64), ('T', c_i64), ('dim', c_int), ('part', c_int), ('axes', c_int),
+                ('interleaved', c_int), ('inverse', c_int), ('pos_int64', c_int), ('positions', c_p),
+                ('pos_sb', c_i64), ('pos_st', c_i64), ('pos_sa', c_i64), ('turns', c_p), ('factor', c_f)]
+
+
+class BaKvArgs(ctypes.Structure):
+    _fields_ = [('k', c_p), ('v', c_p), ('scales', c_p), ('n_blocks', c_i64), ('heads', c_int), ('dim', c_int),
+                ('bits', c_int), ('n_seqs', c_int), ('pages', c_p), ('pages_stride', c_i64), ('n_pages', c_int),
+                ('dtype', c_int), ('starts', c_p), ('offsets', c_p), ('n_rows', c_i64), ('rows_per_seq', c_i64),
+                ('max_rows', c_i64), ('rk', c_p), ('rv', c_p), ('rk_st', c_i64), ('rk_sh', c_i64), ('rv_st', c_i64),
+                ('rv_sh', c_i64)]
+
+
+class BaKvAttendArgs(ctypes.Structure):
+    _fields_ = [('k', c_p), ('v', c_p), ('scales', c_p), ('n_blocks', c_i64), ('heads', c_int), ('dim', c_int),
+                ('bits', c_int), ('n_seqs', c_int), ('pages', c_p), ('pages_stride', c_i64), ('n_pages', c_int),
+                ('dtype', c_int), ('lengths', c_p), ('offsets', c_p), ('n_rows', c_i64), ('rows_per_seq', c_i64),
+                ('max_rows', c_i64), ('q', c_p), ('o', c_p), ('lse', c_p), ('q_st', c_i64), ('q_sh', c_i64),
+                ('o_st', c_i64), ('o_sh', c_i64), ('q_heads', c_int), ('causal', c_int), ('window', c_i64),
+                ('scale', c_f), ('n_splits', c_int), ('workspace', c_p), ('workspace_bytes', c_i64)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     'ba_last_error': (ctypes.c_char_p, []),
@@ -214,6 +243,12 @@ _SIGS = {
     'ba_tangent_workspace_bytes': (c_i64, [c_i64, c_int, c_int, c_int, c_int, c_int, c_int]),
     'ba_planar_confidence': (c_int, [c_p, c_int, c_int, c_f, c_p, c_p]),
     'ba_add_z_prior': (c_int, [c_p, c_p, c_p, c_p, c_p, c_p, c_i64, c_int, c_int, c_int, c_p]),
+    'ba_rotary': (c_int, [ctypes.POINTER(BaRotaryArgs), c_p]),
+    'ba_kv_write': (c_int, [ctypes.POINTER(BaKvArgs), c_p]),
+    'ba_kv_read': (c_int, [ctypes.POINTER(BaKvArgs), c_p]),
+    'ba_kv_attend': (c_int, [ctypes.POINTER(BaKvAttendArgs), c_p]),
+    'ba_kv_attend_splits': (c_int, [c_int, c_int, c_int, c_int, c_i64, c_int]),
+    'ba_kv_attend_workspace_bytes': (c_i64, [c_i64, c_int, c_int, c_int]),
 }
 
 EXPORTED = tuple(_SIGS)
@@ -222,7 +257,8 @@ EXPORTED = tuple(_SIGS)
 ABI_STRUCTS = {'ba_huber': BaHuber, 'ba_layout': BaLayout, 'ba_lin_args': BaLinArgs, 'ba_pm_args': BaPmArgs,
                'ba_pcg_args': BaPcgArgs, 'ba_pcg_pairs': BaPcgPairs, 'ba_pcg_resident': BaPcgResident, 'ba_chol_args': BaCholArgs, 'ba_sample_args': BaSampleArgs,
                'ba_obs_set': BaObsSet, 'ba_gather_args': BaGatherArgs, 'ba_remove_args': BaRemoveArgs,
-               'ba_tangent_args': BaTangentArgs}
+               'ba_tangent_args': BaTangentArgs, 'ba_rotary_args': BaRotaryArgs, 'ba_kv_args': BaKvArgs,
+               'ba_kv_attend_args': BaKvAttendArgs}
 
 
 def _check_abi(L):

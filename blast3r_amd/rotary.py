@@ -1,0 +1,182 @@
+"""Rotary positions of a transformer's queries and keys on the device (``ba_rotary``, libba_hip.so).
+
+The depth and matching networks in front of a bundle adjustment place the patches of an image by row and column
+(src/blast3r/extensions/curope: two or three axes, each with its part of the head, members of a pair half a section
+apart); sequence models place tokens by one position, with pairs half a head apart or side by side, and may scale
+their frequencies for long contexts.  ``Rotary`` holds one such choice::
+
+    rot = Rotary(64, axes=2)                    # a head of 64, rows in its first half, columns in the other
+    q, k = rot(positions, q, k)                 # one launch for both; differentiable
+
+Nothing here falls back to torch: the rotation runs in libba_hip.so on device tensors.
+"""
+import ctypes
+import math
+
+import torch
+
+from ._lib import BaRotaryArgs, check, lib, stream_ptr
+
+__all__ = ['Rotary', 'rotary_frequencies']
+
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def rotary_frequencies(n, base=10000.0, scaling=None):
+    """(angle per position of each of the n / 2 pairs of a section of n elements, factor of the result), 64 bits.
+
+    base^(-2p/n) for pair p, and with ``scaling``
+      dict(kind='linear', factor=s)   divided by s: positions are squeezed into the trained range;
+      dict(kind='base', factor=s)     with base * s^(n / (n - 2)): the slowest pair turns s times slower, the fastest as
+                                      before;
+      dict(kind='ramp', factor=s, length=L, fast=32, slow=1)
+                                      by the turns that a pair makes over the trained length L: as before from `fast`
+                                      turns on, divided by s up to `slow`, a mixture in between; the result is
+                                      multiplied by 0.1 ln s + 1.
+    """
+    if n < 2 or n % 2:
+        raise ValueError(f'rotary: a section must be whole pairs, got {n} elements')
+    if not base > 0:
+        raise ValueError(f'rotary: base must be positive, got {base}')
+    kind = scaling['kind'] if scaling else None
+    s = float(scaling['factor']) if scaling else 1.0
+    if kind not in (None, 'linear', 'base', 'ramp') or not s >= 1.0:
+        raise ValueError(f'rotary: unknown scaling {scaling!r} (linear, base or ramp, by a factor of at least 1)')
+    if kind == 'base':
+        base = base * s ** (n / max(n - 2, 1))
+    f = [base ** (-2.0 * p / n) for p in range(n // 2)]
+    if kind == 'linear':
+        f = [x / s for x in f]
+    if kind == 'ramp':
+        fast, slow = float(scaling.get('fast', 32.0)), float(scaling.get('slow', 1.0))
+        if not fast > slow:
+            raise ValueError(f'rotary: fast must exceed slow, got {fast} and {slow}')
+        keep = [min(1.0, max(0.0, (scaling['length'] * x / (2 * math.pi) - slow) / (fast - slow))) for x in f]
+        f = [g * x + (1.0 - g) * x / s for g, x in zip(keep, f)]
+        return f, 0.1 * math.log(s) + 1.0
+    return f, 1.0
+
+
+class _Turn(torch.autograd.Function):
+    """The rotation with its gradient, which is the opposite rotation."""
+
+    @staticmethod
+    def forward(ctx, rot, positions, inverse, *xs):
+        ctx.rot, ctx.inverse = rot, inverse
+        ctx.save_for_backward(positions)
+        return rot._run(positions, xs, None, inverse)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        positions, = ctx.saved_tensors
+        need = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[3 + i]]
+        out = [None] * len(grads)
+        if need:
+            gs = [g if g.stride(-1) == 1 else g.contiguous() for g in (grads[i] for i in need)]
+            for i, y in zip(need, ctx.rot._run(positions, gs, None, not ctx.inverse)):
+                out[i] = y
+        return (None, None, None, *out)
+
+
+class Rotary:
+    """Rotary positions of heads of ``head_dim`` elements.
+
+    rotary_dim  the first elements of a head that are rotated (default: all); the rest is copied
+    base        of the frequencies base^(-2p/n)
+    layout      'half': pair p of a section of n is (p, p + n/2); 'interleaved': (2p, 2p + 1)
+    axes        coordinates of a position; each rotates rotary_dim / axes elements
+    scaling     see ``rotary_frequencies``
+    """
+
+    def __init__(self, head_dim, rotary_dim=None, base=10000.0, layout='half', axes=1, scaling=None, device='cuda'):
+        part = head_dim if rotary_dim is None else rotary_dim
+        if layout not in ('half', 'interleaved'):
+            raise ValueError(f"rotary: layout must be 'half' or 'interleaved', got {layout!r}")
+        if axes < 1 or part < 2 or part > head_dim or part % (2 * axes):
+            raise ValueError(f'rotary: {part} of {head_dim} elements are not whole pairs for each of {axes} axes')
+        if layout == 'interleaved' and head_dim % 2:
+            raise ValueError('rotary: an interleaved head must be even')
+        self.head_dim, self.rotary_dim, self.layout, self.axes = head_dim, part, layout, axes
+        self.frequencies, self.factor = rotary_frequencies(part // axes, base, scaling)
+        # turns per position in units of 2^-64 (a frequency of 2 pi or more wraps, as its angle does)
+        turns = [round(x / (2 * math.pi) * 2.0 ** 64) % (1 << 64) for x in self.frequencies]
+        self.turns = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device)
+        if not self.turns.is_cuda:
+            raise RuntimeError('rotary needs a GPU (it runs in libba_hip.so)')
+
+    def __call__(self, positions, *xs, out=None, inverse=False):
+        """The rotated tensors of ``xs``: one or two of shape (tokens, heads, head_dim) or (B, T, heads, head_dim), fp32,
+        fp16 or bf16, any strides with contiguous elements; a single tensor comes back as itself, two as a tuple.
+
+        positions   int32 or int64, the tokens' shape ((T,) serves every batch), with more than one axis a last
+                    dimension of ``axes``
+        out         tensors to write to, one for each x (x itself rotates in place); not differentiable
+        inverse     rotate by the opposite angles
+        """
+        if not 1 <= len(xs) <= 2:
+            raise ValueError(f'rotary: one or two tensors at a time, got {len(xs)}')
+        if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+            if out is not None:
+                raise ValueError('rotary: out cannot be given where gradients are recorded')
+            ys = _Turn.apply(self, positions, bool(inverse), *xs)
+        else:
+            ys = self._run(positions, xs, out, inverse)
+        return ys if len(xs) == 2 else ys[0]
+
+    def _run(self, positions, xs, out, inverse):
+        x = xs[0]
+        lead = x.shape[:-2]
+        dev = self.turns.device
+        if len(lead) not in (1, 2):
+            raise ValueError(f'rotary: tensors are (tokens, heads, dim) or (B, T, heads, dim), got {tuple(x.shape)}')
+        if x.dtype not in DTYPES:
+            raise ValueError(f'rotary: fp32, fp16 or bf16 tensors, got {x.dtype}')
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != dev:
+            raise ValueError(f'rotary: positions must be int32 or int64 on {dev}')
+        p = positions
+        if self.axes > 1:
+            if p.dim() < 2 or p.shape[-1] != self.axes:
+                raise ValueError(f'rotary: positions need a last dimension of {self.axes} axes, got {tuple(p.shape)}')
+            p_lead, sa = p.shape[:-1], p.stride(-1)
+        else:
+            p_lead, sa = p.shape, 0
+        if tuple(p_lead) != tuple(lead) and not (len(lead) == 2 and tuple(p_lead) == tuple(lead[1:])):
+            raise ValueError(f'rotary: positions of shape {tuple(p.shape)} for tokens {tuple(lead)}')
+        if out is None:
+            ys = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in xs]
+        else:
+            ys = list(out) if isinstance(out, (tuple, list)) else [out]
+            if len(ys) != len(xs):
+                raise ValueError(f'rotary: {len(ys)} outputs for {len(xs)} tensors')
+        a = BaRotaryArgs()
+        for i, (t, y) in enumerate(zip(xs, ys)):
+            shape = t.shape
+            if (len(shape) != len(lead) + 2 or shape[:-2] != lead or shape[-1] != self.head_dim or t.dtype != x.dtype or
+                    t.device != dev):
+                raise ValueError(f'rotary: tensors must share tokens, type and device, with heads of {self.head_dim}: got '
+                                 f'{tuple(shape)} {t.dtype} on {t.device}')
+            if y.shape != shape or y.dtype != t.dtype or y.device != dev:
+                raise ValueError('rotary: an output must be like its tensor')
+            xs_, ys_ = t.stride(), y.stride()
+            if xs_[-1] != 1 or ys_[-1] != 1:
+                raise ValueError('rotary: the elements of a head must be contiguous')
+            a.x[i], a.y[i] = t.data_ptr(), y.data_ptr()
+            a.heads[i] = shape[-2]
+            a.x_sh[i], a.y_sh[i] = xs_[-2], ys_[-2]
+            a.x_st[i], a.y_st[i] = xs_[-3], ys_[-3]
+            if len(lead) == 2:
+                a.x_sb[i], a.y_sb[i] = xs_[0], ys_[0]
+        a.n_x, a.dtype = len(xs), DTYPES[x.dtype]
+        a.T = lead[-1]
+        a.B = lead[0] if len(lead) == 2 else 1
+        a.dim, a.part, a.axes = self.head_dim, self.rotary_dim, self.axes
+        a.interleaved, a.inverse = self.layout == 'interleaved', bool(inverse)
+        a.pos_int64, a.positions = p.dtype == torch.int64, p.data_ptr()
+        st = p.stride()
+        a.pos_st, a.pos_sa = st[len(p_lead) - 1], sa
+        a.pos_sb = st[0] if len(p_lead) == 2 else 0
+        a.turns, a.factor = self.turns.data_ptr(), self.factor
+        if a.B * a.T > 0 and all(h > 0 for h in a.heads[:len(xs)]):
+            with torch.cuda.device(dev):
+                check(lib().ba_rotary(ctypes.byref(a), stream_ptr(dev)))
+        return tuple(ys)

@@ -624,6 +624,108 @@ int ba_planar_confidence(const float* D0, int32_t H, int32_t W, float alpha, flo
 int ba_add_z_prior(void* S_pairs, const int32_t* diag_pair, void* e_img, void* dg_img, const void* H_z,
                    const void* g_z, int64_t n_imgs, int32_t d, int32_t C, int32_t real32, void* stream);
 
+/* ------------------------------------------------------------------ token operators */
+/* What the networks whose depth maps and tracks the adjustment reads do with a frame's tokens (no counterpart in the
+ * reference's native module for the cache).  dtype of a tensor: 0 fp32, 1 fp16, 2 bf16; strides are in elements, the
+ * last dimension of every tensor has stride 1. */
+
+/* Rotary positions of one or two tensors (B, T, heads, dim) that share the tokens' positions: the first `part`
+ * elements of a head are `axes` sections, one per coordinate of the position; pair p of a section of n elements, (p,
+ * p + n/2) or, interleaved, (2p, 2p + 1), is turned by position * turns[p] / 2^64 of a circle and multiplied by
+ * factor; the rest of the head is copied.  inverse: by the opposite angle (the gradient).  y may be x. */
+typedef struct {
+    const void* x[2];
+    void* y[2];
+    int64_t x_sb[2], x_st[2], x_sh[2];
+    int64_t y_sb[2], y_st[2], y_sh[2];
+    int32_t heads[2];
+    int32_t n_x;
+    int32_t dtype;
+    int64_t B, T;
+    int32_t dim, part, axes;
+    int32_t interleaved, inverse;
+    int32_t pos_int64;         /* positions hold int64 (else int32) */
+    const void* positions;     /* at b * pos_sb + t * pos_st + axis * pos_sa; any value, negative ones too */
+    int64_t pos_sb, pos_st, pos_sa;
+    const uint64_t* turns;     /* (part / axes / 2,) turns per position in units of 2^-64 */
+    float factor;
+} ba_rotary_args;
+
+int ba_rotary(const ba_rotary_args* args, void* stream);
+
+/* A key/value cache in 8 bits.  Blocks of 64 tokens: k (n_blocks, heads, 64, dim), v (n_blocks, heads, dim, 64), one
+ * byte each (bits 0: e4m3, 1: two's complement in [-127, 127]), scales (n_blocks, heads, 2) fp32: the factors of a
+ * block's keys and values.  pages (n_seqs, pages_stride): the blocks of each sequence, in order.  dim is 32, 64, 96,
+ * 128 or 256.  Sequence s of a call has the rows offsets[s] .. offsets[s + 1] of the row tensors (n_rows rows in
+ * all), or rows_per_seq rows each where offsets is NULL; max_rows bounds the rows of a sequence: what is over it is
+ * left out.  Entries of pages outside [0, n_blocks), tokens past the width of pages and rows past n_rows are left
+ * out too: not written, read as zeros, hidden from queries. */
+typedef struct {
+    void* k;
+    void* v;
+    float* scales;
+    int64_t n_blocks;
+    int32_t heads, dim, bits;
+    int32_t n_seqs;
+    const int32_t* pages;
+    int64_t pages_stride;
+    int32_t n_pages;           /* width of pages */
+    int32_t dtype;             /* of the row tensors */
+    const int32_t* starts;     /* (n_seqs,) tokens of a sequence before the first row */
+    const int32_t* offsets;    /* (n_seqs + 1,) or NULL */
+    int64_t n_rows, rows_per_seq, max_rows;
+    void* rk;                  /* (n_rows, heads, dim) keys and values: read by ba_kv_write, written by ba_kv_read */
+    void* rv;
+    int64_t rk_st, rk_sh, rv_st, rv_sh;
+} ba_kv_args;
+
+/* Rows appended to the cache at starts[s] ...  The factor of a block and head is fit(largest magnitude of its new
+ * values), and not less than its present factor where the block held tokens before starts[s]; those are then recoded
+ * with the new factor if it grew.  fit: e4m3: the least power of two, from 2^-60 on, with largest <= 448 * factor;
+ * int8: max(largest / 127, 2^-60).  Codes: nearest to x * (1 / factor), ties to even.  A block with a NaN or an
+ * infinity among its values (or with a factor over 2^60) gets a NaN factor and zero codes: it reads as NaN until a
+ * token is written to its first place again. */
+int ba_kv_write(const ba_kv_args* args, void* stream);
+/* The values of tokens starts[s] .. of each sequence, code * factor, as rows. */
+int ba_kv_read(const ba_kv_args* args, void* stream);
+
+/* Attention of query rows (n_rows, q_heads, dim) over the cached tokens of their sequences:
+ * o = softmax(scale * q k^T) v over the keys j that row i of its sequence's n rows sees, at position p = lengths[s] - n
+ * + i: j < lengths[s], with causal also j <= p, with window > 0 also j > p - window.  A row that sees no key gives
+ * zeros (lse -inf); one that sees a block with a NaN factor gives NaN (lse too).  Query head h reads cache head h / (q_heads / heads).  lse (n_rows, q_heads) fp32 or NULL: the
+ * natural logarithm of the sum of exp(scale * q k^T).  n_splits: parts that a sequence's keys are cut into
+ * (ba_kv_attend_splits gives the number that fills the GPU); above 1, workspace holds their partial sums
+ * (ba_kv_attend_workspace_bytes), which are added in order. */
+typedef struct {
+    const void* k;
+    const void* v;
+    const float* scales;
+    int64_t n_blocks;
+    int32_t heads, dim, bits;
+    int32_t n_seqs;
+    const int32_t* pages;
+    int64_t pages_stride;
+    int32_t n_pages;
+    int32_t dtype;             /* of q and o: 1 fp16 or 2 bf16 */
+    const int32_t* lengths;    /* (n_seqs,) tokens of a sequence that the cache holds, the queries' own among them */
+    const int32_t* offsets;    /* (n_seqs + 1,) or NULL */
+    int64_t n_rows, rows_per_seq, max_rows;
+    const void* q;
+    void* o;
+    float* lse;
+    int64_t q_st, q_sh, o_st, o_sh;
+    int32_t q_heads, causal;
+    int64_t window;
+    float scale;
+    int32_t n_splits;
+    void* workspace;
+    int64_t workspace_bytes;
+} ba_kv_attend_args;
+
+int ba_kv_attend(const ba_kv_attend_args* args, void* stream);
+int32_t ba_kv_attend_splits(int32_t n_seqs, int32_t heads, int32_t q_heads, int32_t dim, int64_t max_rows, int32_t n_pages);
+int64_t ba_kv_attend_workspace_bytes(int64_t n_rows, int32_t q_heads, int32_t dim, int32_t n_splits);
+
 #ifdef __cplusplus
 }
 #endif
