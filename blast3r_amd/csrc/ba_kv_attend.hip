@@ -30,6 +30,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "ba_common.h"
 #include "ba_error.h"
 #include "ba_hip.h"
@@ -44,7 +46,7 @@ typedef float f16 __attribute__((ext_vector_type(16)));
 
 #define AT_T 256
 #define AT_WAVES 4
-#define AT_MIN_BLOCKS 4      // a split part has at least so many blocks: one for each wave
+#define AT_MIN_BLOCKS 16     // a part has at least so many blocks: below that a second launch costs more than it saves
 
 template <int COLS> struct Mma;
 template <> struct Mma<16> {
@@ -105,25 +107,29 @@ __device__ __forceinline__ AtSeq at_seq(const ba_kv_attend_args& a, int s) {
     return {row0, (int)n, (int)len, (int)(n < a.max_rows ? n : a.max_rows)};
 }
 
-// Blocks [lo, hi) that rows [row, row + rows) (of n * group rows) see, and of these the ones of part sp.
-__device__ __forceinline__ void at_blocks(const ba_kv_attend_args& a, const AtSeq& q, int group, int64_t row, int rows, int sp,
-                                          int& lo, int& hi) {
+// Blocks [lo, hi) that rows [row, row + rows) (of n * group rows) see, cut into parts of `per` blocks.
+struct AtBlocks {
+    int lo, hi, per;
+};
+
+__device__ __forceinline__ AtBlocks at_blocks(const ba_kv_attend_args& a, const AtSeq& q, int group, int64_t row, int rows) {
     const int64_t all = (int64_t)q.rows * group, last = row + rows < all ? row + rows : all;
-    if (row >= last) { lo = hi = 0; return; }
+    if (row >= last) return {0, 0, 1};
     const int64_t p0 = (int64_t)q.len - q.n + row / group, p1 = (int64_t)q.len - q.n + (last - 1) / group;
     const int64_t keys = a.causal ? p1 + 1 : (int64_t)q.len;
     int64_t first = a.window > 0 ? p0 - a.window + 1 : 0;
     if (first < 0) first = 0;
-    if (keys <= first) { lo = hi = 0; return; }
-    const int b0 = (int)(first / 64), b1 = (int)((keys + 63) / 64);
-    int per = (b1 - b0 + a.n_splits - 1) / a.n_splits;
-    per = per < AT_MIN_BLOCKS ? AT_MIN_BLOCKS : per;
-    lo = b0 + sp * per < b1 ? b0 + sp * per : b1;
-    hi = lo + per < b1 ? lo + per : b1;
+    if (keys <= first) return {0, 0, 1};
+    const int b0 = (int)(first / 64), b1 = (int)((keys + 63) / 64), per = (b1 - b0 + a.n_splits - 1) / a.n_splits;
+    return {b0, b1, per < AT_MIN_BLOCKS ? AT_MIN_BLOCKS : per};
 }
 
-// rows of a workgroup's tile
-template <int COLS, int NCB, int WR> constexpr int tile_rows() { return COLS * NCB * WR; }
+// Part sp of them.
+__device__ __forceinline__ void at_part(const AtBlocks& b, int sp, int& lo, int& hi) {
+    const int64_t x = b.lo + (int64_t)sp * b.per;
+    lo = x < b.hi ? (int)x : b.hi;
+    hi = lo + b.per < b.hi ? lo + b.per : b.hi;
+}
 
 // partial sums of a row and part: dim floats, and the reference and the denominator
 __device__ __forceinline__ float* part_sum(const ba_kv_attend_args& a, int64_t row, int head, int sp) {
@@ -150,47 +156,21 @@ __device__ __forceinline__ void store_out4(const ba_kv_attend_args& a, int64_t r
 #define AT_NONE -1.0e30f      // reference of a row that has seen no key
 #define AT_MOVE 8.0f          // m is moved when a score passes it by so much (log2)
 #define AT_LIFT 6.0f          // weights at m are 2^6: with AT_MOVE at most 2^14, and fp16 is normal down to 2^-20 of m
+#define AT_MOST 32768.0f      // a lane's sum of 16 weights above it moves m too: each of them fits fp16
 
-// WR waves split the rows of the workgroup's tile, 4 / WR the blocks.
-template <int D, int KT, int COLS, int NCB, int WR>
-__global__ void __launch_bounds__(AT_T, COLS == 16 && D <= 128 ? 3 : 1) k_kv_attend(ba_kv_attend_args a, int n_tiles, int wide) {
-    typedef Mma<COLS> M;
-    typedef typename M::acc acc;
-    constexpr int NG = 64 / COLS, NB = NG, CREG = COLS * COLS / 64, TPL = 64 / NG;
-    constexpr int KS = D / (8 * NG), DB = D / COLS, PS = TPL / 8, WK = AT_WAVES / WR, ROWS = tile_rows<COLS, NCB, WR>();
-    __shared__ float2 ref_sh[WK > 1 ? AT_WAVES * COLS * NCB : 1];
-    __shared__ f4 sum_sh[WK > 1 ? 2 * COLS * NCB * D / 4 : 1];
-
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wr = wave % WR, wk = wave / WR;
-    const int n = lane % COLS, g = lane / COLS;
-    unsigned id = xcd_block(blockIdx.x, gridDim.x);
-    const int tile = (int)(id % (unsigned)n_tiles);
-    id /= (unsigned)n_tiles;
-    const int sp = (int)(id % (unsigned)a.n_splits);
-    id /= (unsigned)a.n_splits;
-    const int kh = (int)(id % (unsigned)a.heads), s = (int)(id / (unsigned)a.heads);
-    const int group = a.q_heads / a.heads;
-    const AtSeq q = at_seq(a, s);
-    const int64_t all = (int64_t)q.rows * group, tile0 = (int64_t)tile * ROWS;
-    if (tile0 >= all) return;
-    int lo, hi;
-    at_blocks(a, q, group, tile0, ROWS, sp, lo, hi);
-    if (lo >= hi && a.n_splits > 1) return;                  // k_kv_join knows which parts there are
-
-    // queries: row, its position, its elements as fp16 and the power of two that they were divided by
-    const int64_t row0 = tile0 + wr * COLS * NCB;
-    if constexpr (WK == 1)
-        if (row0 >= all) return;
-    h8 qf[NCB][KS];
-    float qc[NCB];
-    int64_t pos[NCB];
+// Query rows row0 .. of a wave (NCB tiles of COLS): their positions, their elements as fp16 (lane (n, g) holds those of
+// row n that pair with its pieces of a key) divided by a power of two of the row, and the constant that a score is
+// multiplied by before the key factor: softmax scale, log2(e) and that power.
+template <int D, int COLS, int NCB>
+__device__ __forceinline__ void load_queries(const ba_kv_attend_args& a, const AtSeq& q, int kh, int group, int64_t row0, int64_t all,
+                                             int n, int g, bool wide, h8 (&qf)[NCB][D * COLS / 512], float (&qc)[NCB], int (&pos)[NCB]) {
+    constexpr int NG = 64 / COLS, KS = D / (8 * NG);
 #pragma unroll
     for (int c = 0; c < NCB; ++c) {
         const int64_t r = row0 + c * COLS + n, rc = r < all ? r : all - 1;
         const int64_t i = rc / group;
         const int head = kh * group + (int)(rc - i * group);
-        pos[c] = (int64_t)q.len - q.n + i;
+        pos[c] = q.len - q.n + (int)i;
         float x[KS][8];
         uint32_t top = 0;
         const int64_t at = (q.row0 + i) * a.q_st + head * a.q_sh + g * (D / NG);
@@ -219,24 +199,91 @@ __global__ void __launch_bounds__(AT_T, COLS == 16 && D <= 128 ? 3 : 1) k_kv_att
 #pragma unroll
             for (int j = 0; j < 8; ++j) qf[c][t][j] = (_Float16)(x[t][j] * up);
     }
-    // positions of the wave's rows, for the choice between blocks that all rows see whole and others
-    const int64_t last = row0 + COLS * NCB < all ? row0 + COLS * NCB : all;
-    const int64_t pmin = (int64_t)q.len - q.n + row0 / group, pmax = (int64_t)q.len - q.n + (last - 1) / group;
-    const int64_t whole_hi = a.causal ? pmin + 1 : (int64_t)q.len;                 // tokens below it are seen by all rows
-    const int64_t whole_lo = a.window > 0 ? pmax - a.window + 1 : 0;               // from it on too
+}
 
-    if constexpr (WR > 1) {                                  // the blocks that this wave's rows see
-        if (a.causal && (int64_t)hi * 64 > pmax + 64) hi = pmax < 0 ? lo : (int)(pmax / 64) + 1;
-        const int64_t first = a.window > 0 ? pmin - a.window + 1 : 0;
-        if (first / 64 > lo) lo = (int)(first / 64 < hi ? first / 64 : hi);
-    }
-
-    acc o[NCB][DB];
-    float m[NCB], l[NCB];
+// The result of a wave's rows, or their partial sums.
+template <int D, int COLS, int NCB, typename A>
+__device__ __forceinline__ void store_rows(const ba_kv_attend_args& a, const AtSeq& q, int kh, int group, int64_t row0, int64_t all, int sp,
+                                           int n, int g, bool wide, const A (&o)[NCB][D / COLS], const float (&m)[NCB], const float (&l)[NCB]) {
+    constexpr int CREG = COLS * COLS / 64, DB = D / COLS;
+    typedef Mma<COLS> M;
 #pragma unroll
     for (int c = 0; c < NCB; ++c) {
-        m[c] = AT_NONE;
+        const int64_t r = row0 + c * COLS + n;
+        if (r >= all) continue;
+        const int64_t i = r / group, row = q.row0 + i;
+        const int head = kh * group + (int)(r - i * group);
+        if (a.n_splits > 1) {
+            float* w = part_sum(a, row, head, sp);
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int k = 0; k < CREG; k += 4)
+                    *(f4*)(w + d * COLS + M::row(g, k)) = (f4){o[c][d][k], o[c][d][k + 1], o[c][d][k + 2], o[c][d][k + 3]};
+            if (g == 0) *part_ref(a, row, head, sp) = make_float2(m[c], l[c]);
+            continue;
+        }
+        const float inv = l[c] == 0.0f ? 0.0f : 1.0f / l[c];         // l is 0 in a row that saw no key
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int k = 0; k < CREG; k += 4)
+                store_out4(a, row, head, d * COLS + M::row(g, k),
+                           (f4){o[c][d][k] * inv, o[c][d][k + 1] * inv, o[c][d][k + 2] * inv, o[c][d][k + 3] * inv}, wide);
+        if (a.lse && g == 0)
+            a.lse[row * a.q_heads + head] = l[c] == 0.0f ? -__builtin_inff() : 0.693147180559945309f * (m[c] - AT_LIFT + __builtin_amdgcn_logf(l[c]));
+    }
+}
+
+// waves of a SIMD that the registers are to leave room for
+constexpr int at_waves(int d, int cols) { return cols == 16 ? (d <= 64 ? 4 : d <= 128 ? 2 : 1) : d <= 128 ? 2 : 1; }
+
+// Few rows: the four waves have the same COLS rows and split the blocks; every wave reads and converts its own.
+template <int D, int KT, int COLS>
+__global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_attend_args a, int n_tiles, int wide) {
+    typedef Mma<COLS> M;
+    typedef typename M::acc acc;
+    constexpr int NG = 64 / COLS, NB = NG, CREG = COLS * COLS / 64, TPL = 64 / NG;
+    constexpr int KS = D / (8 * NG), DB = D / COLS, PS = TPL / 8, WK = AT_WAVES, NCB = 1, ROWS = COLS;
+    __shared__ float2 ref_sh[AT_WAVES * COLS * NCB];
+    __shared__ f4 sum_sh[2 * COLS * NCB * D / 4];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = wave;
+    const int n = lane % COLS, g = lane / COLS;
+    unsigned id = xcd_block(blockIdx.x, gridDim.x);
+    const int tile = (int)(id % (unsigned)n_tiles);
+    id /= (unsigned)n_tiles;
+    const int sp = (int)(id % (unsigned)a.n_splits);
+    id /= (unsigned)a.n_splits;
+    const int kh = (int)(id % (unsigned)a.heads), s = (int)(id / (unsigned)a.heads);
+    const int group = a.q_heads / a.heads;
+    const AtSeq q = at_seq(a, s);
+    const int64_t all = (int64_t)q.rows * group, tile0 = (int64_t)tile * ROWS;
+    if (tile0 >= all) return;
+    int lo, hi;
+    at_part(at_blocks(a, q, group, tile0, ROWS), sp, lo, hi);
+    if (lo >= hi && a.n_splits > 1) return;                  // k_kv_join knows which parts there are
+
+    h8 qf[NCB][KS];
+    float qc[NCB];
+    int pos[NCB];
+    load_queries<D, COLS, NCB>(a, q, kh, group, tile0, all, n, g, wide != 0, qf, qc, pos);
+    // tokens [whole_lo, whole_hi) are seen by all rows of the wave: their blocks need no comparisons
+    const int64_t last = tile0 + ROWS < all ? tile0 + ROWS : all;
+    const int pmin = q.len - q.n + (int)(tile0 / group), pmax = q.len - q.n + (int)((last - 1) / group);
+    const int64_t window = a.window > 0 ? a.window : (int64_t)1 << 40;
+    const int whole_hi = a.causal ? pmin + 1 : q.len;
+    const int whole_lo = pmax - window + 1 > 0 ? (int)(pmax - window + 1) : 0;
+    if (a.n_blocks == 0) hi = lo;
+
+    acc o[NCB][DB];
+    // weights are exp2(z + lv - m + AT_LIFT); `move`: an exponent above it moves m (any does in a row that has no m yet)
+    float m[NCB], l[NCB], move[NCB];
+#pragma unroll
+    for (int c = 0; c < NCB; ++c) {
+        m[c] = 0.0f;
         l[c] = 0.0f;
+        move[c] = -3.0e38f;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -248,10 +295,18 @@ __global__ void __launch_bounds__(AT_T, COLS == 16 && D <= 128 ? 3 : 1) k_kv_att
     const uint8_t* vb = (const uint8_t*)a.v + (int64_t)kh * 64 * D;
     const int64_t step = (int64_t)a.heads * 64 * D;
     uint2 kr[NB][KS], vr[DB][PS];
-    auto load_keys = [&](int64_t page) {
+    // a block that is not there is read as block 0 and hidden
+    auto page_of = [&](int b) { return b < hi ? pages[b] : 0; };
+    auto there = [&](int p) { return p >= 0 && p < a.n_blocks; };
+    auto factors = [&](int p) {
+        const float2 f = *(const float2*)(a.scales + ((int64_t)(there(p) ? p : 0) * a.heads + kh) * 2);
+        return there(p) ? f : make_float2(1.0f, 1.0f);
+    };
+    auto load_keys = [&](int page) {
+        const uint8_t* base = kb + (there(page) ? page : 0) * step;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const uint8_t* p = kb + page * step + M::token(b, n) * D + g * (D / NG);
+            const uint8_t* p = base + M::token(b, n) * D + g * (D / NG);
             if constexpr (KS % 2 == 0) {
 #pragma unroll
                 for (int t = 0; t < KS; t += 2) {
@@ -265,10 +320,11 @@ __global__ void __launch_bounds__(AT_T, COLS == 16 && D <= 128 ? 3 : 1) k_kv_att
             }
         }
     };
-    auto load_values = [&](int64_t page) {
+    auto load_values = [&](int page) {
+        const uint8_t* base = vb + (there(page) ? page : 0) * step;
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-            const uint8_t* p = vb + page * step + (d * COLS + n) * 64 + g * TPL;
+            const uint8_t* p = base + (d * COLS + n) * 64 + g * TPL;
 #pragma unroll
             for (int t = 0; t < PS; t += 2) {
                 const uint4 w = *(const uint4*)(p + 8 * t);
@@ -277,126 +333,144 @@ __global__ void __launch_bounds__(AT_T, COLS == 16 && D <= 128 ? 3 : 1) k_kv_att
             }
         }
     };
-    auto page_of = [&](int b) -> int64_t {
-        const int64_t p = b < hi ? pages[b] : -1;
-        return p < a.n_blocks ? p : -1;
-    };
 
     int blk = lo + wk;
-    int64_t page = page_of(blk);
-    if (page >= 0) { load_keys(page); load_values(page); }
-    while (blk < hi) {
-        const int64_t next = page_of(blk + WK);
-        if (page >= 0) {
-            const float2 f = *(const float2*)(a.scales + (page * a.heads + kh) * 2);
-            acc sc[NCB][NB];
+    int page = page_of(blk), next = page_of(blk + WK);
+    float2 f = make_float2(1.0f, 1.0f);
+    if (blk < hi) {
+        f = factors(page);
+        load_keys(page);
+        load_values(page);
+    }
+    for (; blk < hi; blk += WK) {
+        const int after = page_of(blk + 2 * WK);
+        const float2 fn = factors(next);
+        acc sc[NCB][NB];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
+        for (int b = 0; b < NB; ++b) {
 #pragma unroll
-                for (int c = 0; c < NCB; ++c)
+            for (int c = 0; c < NCB; ++c)
 #pragma unroll
-                    for (int r = 0; r < CREG; ++r) sc[c][b][r] = 0.0f;
+                for (int r = 0; r < CREG; ++r) sc[c][b][r] = 0.0f;
 #pragma unroll
-                for (int t = 0; t < KS; ++t) {
-                    const h8 kf = codes8<KT>(kr[b][t]);
+            for (int t = 0; t < KS; ++t) {
+                const h8 kf = codes8<KT>(kr[b][t]);
 #pragma unroll
-                    for (int c = 0; c < NCB; ++c) sc[c][b] = M::run(kf, qf[c][t], sc[c][b]);
-                }
+                for (int c = 0; c < NCB; ++c) sc[c][b] = M::run(kf, qf[c][t], sc[c][b]);
             }
-            if (next >= 0) load_keys(next);
-            const float lv = __builtin_amdgcn_logf(f.y), iv = 1.0f / f.y;
-            const int64_t t0 = (int64_t)blk * 64;
-            const bool masked = t0 + 64 > whole_hi || t0 < whole_lo;
-            if (t0 + 64 > q.len) {                           // tokens that were never written: their codes may be anything
-                const int over = q.len - (int)t0 - g * TPL;  // the lane's tokens from here on
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int t = 0; t < PS; ++t) {
-                        const int x = over - 8 * t, y = x - 4;
-                        vr[d][t].x &= x >= 4 ? ~0u : x <= 0 ? 0u : (1u << (8 * x)) - 1u;
-                        vr[d][t].y &= y >= 4 ? ~0u : y <= 0 ? 0u : (1u << (8 * y)) - 1u;
-                    }
-            }
-            h8 pf[NCB][PS];
-#pragma unroll
-            for (int c = 0; c < NCB; ++c) {
-                const float cz = f.x * qc[c];
-                int seen_lo = 0, seen_hi = TPL - 1;          // the lane's tokens that the row sees
-                if (masked) {
-                    const int64_t base = t0 + g * TPL;
-                    const int64_t e = (a.causal && pos[c] < q.len ? pos[c] : (int64_t)q.len - 1) - base;
-                    const int64_t b = a.window > 0 ? pos[c] - a.window + 1 - base : -1;
-                    seen_hi = (int)(e < -1 ? -1 : e > TPL - 1 ? TPL - 1 : e);
-                    seen_lo = (int)(b < 0 ? 0 : b > TPL ? TPL : b);
-#pragma unroll
-                    for (int b2 = 0; b2 < NB; ++b2)
-#pragma unroll
-                        for (int r = 0; r < CREG; ++r) {
-                            const int t = b2 * CREG + r;
-                            sc[c][b2][r] = t >= seen_lo && t <= seen_hi ? sc[c][b2][r] : -3.0e38f;
-                        }
-                }
-                float top = sc[c][0][0];
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int r = 0; r < CREG; ++r) top = fmaxf(top, sc[c][b][r]);
-                top = seen_lo <= seen_hi ? fmaf(top, cz, lv) : AT_NONE;         // a block without a seen token moves nothing
-                if (__any(top > m[c] + AT_MOVE)) {
-                    float now = fmaxf(top, m[c]);
-#pragma unroll
-                    for (int k = COLS; k < 64; k <<= 1) now = fmaxf(now, __shfl_xor(now, k));
-                    const float by = __builtin_amdgcn_exp2f(m[c] - now);
-                    m[c] = now;
-                    l[c] *= by;
-#pragma unroll
-                    for (int d = 0; d < DB; ++d)
-#pragma unroll
-                        for (int r = 0; r < CREG; ++r) o[c][d][r] *= by;
-                }
-                const float off = lv - m[c] + AT_LIFT;
-                float sum = 0.0f;
-#pragma unroll
-                for (int t = 0; t < PS; ++t)
-#pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
-                        const int k = 8 * t + j;
-                        float x = __builtin_amdgcn_exp2f(fmaf(sc[c][k / CREG][k % CREG], cz, off));
-                        float y = __builtin_amdgcn_exp2f(fmaf(sc[c][(k + 1) / CREG][(k + 1) % CREG], cz, off));
-                        if (masked) {
-                            x = k >= seen_lo && k <= seen_hi ? x : 0.0f;
-                            y = k + 1 >= seen_lo && k + 1 <= seen_hi ? y : 0.0f;
-                        }
-                        const h2 p = {(_Float16)x, (_Float16)y};
-                        sum += x + y;                        // before rounding: see the factors above
-                        pf[c][t][j] = p[0];
-                        pf[c][t][j + 1] = p[1];
-                    }
-                l[c] = fmaf(sum, iv, l[c]);
-            }
+        }
+        if (blk + WK < hi) load_keys(next);
+
+        const float lv = __builtin_amdgcn_logf(f.y), iv = __builtin_amdgcn_rcpf(f.y);
+        const int t0 = blk * 64, len = there(page) ? q.len : t0;
+        const bool masked = t0 + 64 > whole_hi || t0 < whole_lo || t0 + 64 > len;
+        if (t0 + 64 > len) {                                 // places without a token: their codes may be anything
+            const int over = len - t0 - g * TPL;             // the lane's tokens from here on
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
                 for (int t = 0; t < PS; ++t) {
-                    const h8 vf = codes8<KT>(vr[d][t]);
-#pragma unroll
-                    for (int c = 0; c < NCB; ++c) o[c][d] = M::run(vf, pf[c][t], o[c][d]);
+                    const int x = over - 8 * t, y = x - 4;
+                    const uint32_t mx = x >= 4 ? ~0u : x <= 0 ? 0u : (1u << (8 * x & 31)) - 1u;
+                    const uint32_t my = y >= 4 ? ~0u : y <= 0 ? 0u : (1u << (8 * y & 31)) - 1u;
+                    vr[d][t].x &= mx;
+                    vr[d][t].y &= my;
                 }
-            if (next >= 0) load_values(next);
-        } else if (next >= 0) {
-            load_keys(next);
-            load_values(next);
         }
+        // exponents of the weights, in place of the scores
+        float top[NCB];
+#pragma unroll
+        for (int c = 0; c < NCB; ++c) {
+            const float cz = f.x * qc[c], off = lv - m[c] + AT_LIFT;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int r = 0; r < CREG; ++r) sc[c][b][r] = fmaf(sc[c][b][r], cz, off);
+        }
+        if (masked) {
+#pragma unroll
+            for (int c = 0; c < NCB; ++c) {
+                // the lane's tokens that the row sees
+                const int base = t0 + g * TPL;
+                const int e = (a.causal && pos[c] < len ? pos[c] : len - 1) - base;
+                const int64_t w = pos[c] - window + 1 - base;
+                const int seen_lo = w < 0 ? 0 : w > 64 ? 64 : (int)w;
+#pragma unroll
+                for (int t = 0; t < TPL; ++t)
+                    if (t < seen_lo || t > e) sc[c][t / CREG][t % CREG] = -__builtin_inff();
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < NCB; ++c) {
+            top[c] = sc[c][0][0];
+#pragma unroll
+            for (int t = 1; t < TPL; ++t) top[c] = fmaxf(top[c], sc[c][t / CREG][t % CREG]);
+        }
+        bool up = false;
+#pragma unroll
+        for (int c = 0; c < NCB; ++c) up = up || top[c] > move[c];
+        if (__any(up)) {
+#pragma unroll
+            for (int c = 0; c < NCB; ++c) {
+                float x = top[c];
+#pragma unroll
+                for (int k = COLS; k < 64; k <<= 1) x = fmaxf(x, __shfl_xor(x, k));
+                const bool none = move[c] < 0.0f;            // no m yet
+                const float by = none ? (x > -1.0e38f ? x - AT_LIFT : 0.0f) : fmaxf(x - AT_LIFT, 0.0f);
+                const float shrink = none ? 1.0f : __builtin_amdgcn_exp2f(-by);
+                if (x > -1.0e38f) move[c] = AT_LIFT + AT_MOVE;
+                m[c] += by;
+                l[c] *= shrink;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int r = 0; r < CREG; ++r) o[c][d][r] *= shrink;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int r = 0; r < CREG; ++r) sc[c][b][r] -= by;
+            }
+        }
+        h8 pf[NCB][PS];
+#pragma unroll
+        for (int c = 0; c < NCB; ++c) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int t = 0; t < PS; ++t)
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const int k = 8 * t + j;
+                    const float x = __builtin_amdgcn_exp2f(sc[c][k / CREG][k % CREG]);
+                    const float y = __builtin_amdgcn_exp2f(sc[c][(k + 1) / CREG][(k + 1) % CREG]);
+                    sum += x + y;                            // before rounding: see the factors above
+                    pf[c][t][j] = (_Float16)x;
+                    pf[c][t][j + 1] = (_Float16)y;
+                }
+            // a row that sees nothing of a block takes nothing from a factor that is NaN
+            l[c] = masked && sum == 0.0f ? l[c] : fmaf(sum, iv, l[c]);
+        }
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int t = 0; t < PS; ++t) {
+                const h8 vf = codes8<KT>(vr[d][t]);
+#pragma unroll
+                for (int c = 0; c < NCB; ++c) o[c][d] = M::run(vf, pf[c][t], o[c][d]);
+            }
+        if (blk + WK < hi) load_values(next);
         page = next;
-        blk += WK;
+        next = after;
+        f = fn;
     }
+#pragma unroll
+    for (int c = 0; c < NCB; ++c)
+        if (move[c] < 0.0f) m[c] = AT_NONE;
 #pragma unroll
     for (int c = 0; c < NCB; ++c)
 #pragma unroll
         for (int k = COLS; k < 64; k <<= 1) l[c] += __shfl_xor(l[c], k);
 
-    if constexpr (WK > 1) {                                  // one reference for the waves, then their sums in order
+    {                                                        // one reference for the waves, then their sums in order
         if (g == 0)
 #pragma unroll
             for (int c = 0; c < NCB; ++c) ref_sh[wave * COLS * NCB + c * COLS + n] = make_float2(m[c], l[c]);
@@ -452,33 +526,317 @@ __global__ void __launch_bounds__(AT_T, COLS == 16 && D <= 128 ? 3 : 1) k_kv_att
         add(0);
     }
 
+    store_rows<D, COLS, NCB>(a, q, kh, group, tile0, all, sp, n, g, wide != 0, o, m, l);
+}
+
+// Many rows: the four waves have 32 * NCB rows each and share the blocks.  A block's codes are fetched once for the
+// workgroup, a block ahead, and converted into LDS in the order in which lanes read operands (16 bytes a lane, one lane
+// after the other).  Half a block (32 tokens) at a time, the scores of the next half are made while the weights of the
+// present one are: the matrix unit and the vector unit have independent work throughout.  Keys have two buffers and values
+// three, as the products with a block's second half run when others convert the next block: one barrier a block.
+template <int D, int KT, int NCB, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_attend_tile(ba_kv_attend_args a, int n_tiles, int wide) {
+    typedef Mma<32> M;
+    typedef M::acc acc;
+    constexpr int KS = D / 16, DB = D / 32, T = 64 * WAVES, ROWS = WAVES * 32 * NCB, PC = (4 * D + T - 1) / T;
+    __shared__ h8 k_sh[2][8 * D];
+    __shared__ h8 v_sh[3][8 * D];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane % 32, g = lane / 32;
+    unsigned id = xcd_block(blockIdx.x, gridDim.x);
+    const int tile = (int)(id % (unsigned)n_tiles);
+    id /= (unsigned)n_tiles;
+    const int sp = (int)(id % (unsigned)a.n_splits);
+    id /= (unsigned)a.n_splits;
+    const int kh = (int)(id % (unsigned)a.heads), s = (int)(id / (unsigned)a.heads);
+    const int group = a.q_heads / a.heads;
+    const AtSeq q = at_seq(a, s);
+    const int64_t all = (int64_t)q.rows * group, tile0 = (int64_t)tile * ROWS;
+    if (tile0 >= all) return;
+    int lo, hi;
+    at_part(at_blocks(a, q, group, tile0, ROWS), sp, lo, hi);
+    if (lo >= hi && a.n_splits > 1) return;                  // k_kv_join knows which parts there are
+    if (a.n_blocks == 0) hi = lo;
+
+    const int64_t row0 = tile0 + wave * 32 * NCB;
+    h8 qf[NCB][KS];
+    float qc[NCB];
+    int pos[NCB];
+    load_queries<D, 32, NCB>(a, q, kh, group, row0, all, n, g, wide != 0, qf, qc, pos);
+    // tokens [whole_lo, whole_hi) are seen by all rows of the wave: their blocks need no comparisons
+    const int64_t first = row0 < all ? row0 : all - 1, last = row0 + 32 * NCB < all ? row0 + 32 * NCB : all;
+    const int pmin = q.len - q.n + (int)(first / group), pmax = q.len - q.n + (int)((last - 1) / group);
+    const int64_t window = a.window > 0 ? a.window : (int64_t)1 << 40;
+    const int whole_hi = a.causal ? pmin + 1 : q.len;
+    const int whole_lo = pmax - window + 1 > 0 ? (int)(pmax - window + 1) : 0;
+
+    acc o[NCB][DB];
+    float m[NCB], l[NCB];                                    // weights are exp2(z + lv - m + AT_LIFT)
+    bool seen[NCB];                                          // the row has an m
 #pragma unroll
     for (int c = 0; c < NCB; ++c) {
-        const int64_t r = row0 + c * COLS + n;
-        if (r >= all) continue;
-        const int64_t i = r / group, row = q.row0 + i;
-        const int head = kh * group + (int)(r - i * group);
-        if (a.n_splits > 1) {
-            float* w = part_sum(a, row, head, sp);
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int k = 0; k < CREG; k += 4)
-                    *(f4*)(w + d * COLS + M::row(g, k)) = (f4){o[c][d][k], o[c][d][k + 1], o[c][d][k + 2], o[c][d][k + 3]};
-            if (g == 0) *part_ref(a, row, head, sp) = make_float2(m[c], l[c]);
-            continue;
-        }
-        // !(l == 0): a row without keys has l = 0, a NaN among its keys or queries has to come through
-        const float inv = l[c] == 0.0f ? 0.0f : 1.0f / l[c];
+        m[c] = 0.0f;
+        l[c] = 0.0f;
+        seen[c] = false;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int k = 0; k < CREG; k += 4)
-                store_out4(a, row, head, d * COLS + M::row(g, k),
-                           (f4){o[c][d][k] * inv, o[c][d][k + 1] * inv, o[c][d][k + 2] * inv, o[c][d][k + 3] * inv}, wide != 0);
-        if (a.lse && g == 0)
-            a.lse[row * a.q_heads + head] = l[c] == 0.0f ? -__builtin_inff() : 0.693147180559945309f * (m[c] - AT_LIFT + __builtin_amdgcn_logf(l[c]));
+            for (int r = 0; r < 16; ++r) o[c][d][r] = 0.0f;
     }
+
+    const int32_t* pages = a.pages + (int64_t)s * a.pages_stride;
+    const uint8_t* kb = (const uint8_t*)a.k + (int64_t)kh * 64 * D;
+    const uint8_t* vb = (const uint8_t*)a.v + (int64_t)kh * 64 * D;
+    const int64_t step = (int64_t)a.heads * 64 * D;
+    // a block that is not there is read as block 0 and hidden
+    auto page_of = [&](int b) { return b < hi ? pages[b] : 0; };
+    auto there = [&](int p) { return p >= 0 && p < a.n_blocks; };
+    auto factors = [&](int p) {
+        const float2 f = *(const float2*)(a.scales + ((int64_t)(there(p) ? p : 0) * a.heads + kh) * 2);
+        return there(p) ? f : make_float2(1.0f, 1.0f);
+    };
+    uint4 kr[PC], vr[PC];                                    // the thread's 16-byte pieces of a block
+    auto fetch = [&](int page) {
+        const int64_t base = (there(page) ? page : 0) * step;
+#pragma unroll
+        for (int i = 0; i < PC; ++i) {
+            const int u = tid + i * T;
+            if (4 * D % T == 0 || u < 4 * D) {
+                kr[i] = *(const uint4*)(kb + base + 16 * u);
+                vr[i] = *(const uint4*)(vb + base + 16 * u);
+            }
+        }
+    };
+    auto hide = [&](int blk, int page) {                     // places without a token: their codes may be anything
+        const int len = there(page) ? q.len : blk * 64;
+        if (blk * 64 + 64 <= len) return;
+#pragma unroll
+        for (int i = 0; i < PC; ++i) {
+            const int over = len - blk * 64 - 16 * ((tid + i * T) % 4);
+            auto keep = [&](uint32_t w, int x) { return w & (x >= 4 ? ~0u : x <= 0 ? 0u : (1u << (8 * x & 31)) - 1u); };
+            vr[i].x = keep(vr[i].x, over);
+            vr[i].y = keep(vr[i].y, over - 4);
+            vr[i].z = keep(vr[i].z, over - 8);
+            vr[i].w = keep(vr[i].w, over - 12);
+        }
+    };
+    // LDS places of the thread's pieces.  An operand is 64 slots of 16 bytes, one for each lane; slots are exchanged (by
+    // t / 2 and g) so that 8 threads in a row, whose pieces differ in t and g, write to different banks.
+    constexpr int SWZ_T = D >= 128 ? 0 : 1, SWZ_G = D == 96 ? 8 : 4;
+    int k_at[PC], v_at[PC];
+#pragma unroll
+    for (int i = 0; i < PC; ++i) {
+        const int u = tid + i * T, token = u / (D / 16), e = u % (D / 16) * 16, kg = e / (D / 2), x = (e - kg * (D / 2)) / 8;
+        const int b = token >> 4 & 1, kn = (token >> 2 & 3) * 8 + (token >> 5) * 4 + (token & 3);      // M::token turned round
+        k_at[i] = (b * KS + x) * 64 + ((kg * 32 + kn) ^ (x / 2 << SWZ_T) ^ (kg * SWZ_G));
+        const int d = u / 4, c = u % 4;
+        v_at[i] = (d / 32 * 4 + c % 2 * 2) * 64 + ((c / 2 * 32 + d % 32) ^ (c % 2 * 2) ^ (c / 2 * 4));
+    }
+    const int k_lane = lane ^ (g * SWZ_G), v_lane = lane ^ (g * 4);
+    auto convert = [&](int unit, h8* k, h8* v) {             // a quarter of a piece
+        const int i = unit / 4;
+        if (4 * D % T != 0 && tid + i * T >= 4 * D) return;
+        switch (unit % 4) {
+            case 0: k[k_at[i]] = codes8<KT>(make_uint2(kr[i].x, kr[i].y)); break;
+            case 1: k[k_at[i] + 64] = codes8<KT>(make_uint2(kr[i].z, kr[i].w)); break;
+            case 2: v[v_at[i]] = codes8<KT>(make_uint2(vr[i].x, vr[i].y)); break;
+            case 3: v[v_at[i] + 64] = codes8<KT>(make_uint2(vr[i].z, vr[i].w)); break;
+        }
+    };
+    // exponents e0 .. e1 of the 16 * NCB that a lane makes from its scores
+    auto exponents = [&](acc (&t)[NCB], const float (&cz)[NCB], const float (&off)[NCB], int e0, int e1) {
+#pragma unroll
+        for (int e = e0; e < e1; ++e) t[e / 16][e % 16] = fmaf(t[e / 16][e % 16], cz[e / 16], off[e / 16]);
+    };
+    // moves the reference of rows: m, l and the sums, and the exponents at hand
+    auto move_by = [&](acc (&t)[NCB], int c, float by) {
+        const float shrink = __builtin_amdgcn_exp2f(-by);
+        m[c] += by;
+        l[c] *= shrink;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[c][d][r] *= shrink;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t[c][r] -= by;
+    };
+    auto largest = [&](const acc (&t)[NCB], int c) {
+        float x = t[c][0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) x = fmaxf(x, t[c][r]);
+        return fmaxf(x, __shfl_xor(x, 32));
+    };
+    // what most blocks do not need: tokens hidden from rows, and the first reference of a row
+    bool unset = true;                                       // a row of the wave has none
+    auto settle = [&](acc (&t)[NCB], int blk, int page, int b) {
+        const int t0 = blk * 64, len = there(page) ? q.len : t0;
+        const bool masked = t0 + 64 > whole_hi || t0 < whole_lo || t0 + 64 > len;
+        if (!masked && !unset) return;
+        bool none = false;
+#pragma unroll
+        for (int c = 0; c < NCB; ++c) {
+            if (masked) {                                    // the lane's tokens that the row sees
+                const int base = t0 + 32 * g + 16 * b;
+                const int e = (a.causal && pos[c] < len ? pos[c] : len - 1) - base;
+                const int64_t w = pos[c] - window + 1 - base;
+                const int seen_lo = w < 0 ? 0 : w > 64 ? 64 : (int)w;
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (r < seen_lo || r > e) t[c][r] = -__builtin_inff();
+            }
+            if (unset) {
+                const float x = largest(t, c);
+                const bool sets = !seen[c] && x > -1.0e38f;
+                if (sets) {                                  // its sums are zeros
+                    m[c] = x - AT_LIFT;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) t[c][r] -= m[c];
+                    seen[c] = true;
+                }
+                none = none || !seen[c];
+            }
+        }
+        if (unset) unset = __any(none);
+    };
+    // One half block: the scores of another half (keys k, at half kb2 of their block; factors fn) into tn, the weights and
+    // products of the present one (exponents t, values v at half vb2, factors f).  The matrix unit takes a product every
+    // 32 clocks; vector instructions stand between them in the order that the fences keep.  Operands are read AHEAD
+    // products ahead, with `carry` through the end of the half into the second half of k, the next one's keys.
+    constexpr int AHEAD = D == 32 ? 2 : 4, READS = KS + 2 * DB, STEPS = 2 * DB;
+    h8 ring[AHEAD];
+    auto key = [&](const h8* k, int b, int x) { return k[(b * KS + x) * 64 + (k_lane ^ (x / 2 << SWZ_T))]; };
+    auto half = [&](acc (&t)[NCB], acc (&tn)[NCB], const h8* k, int kb2, const h8* v, int vb2, float2 f, float2 fn, auto carry, auto extra) {
+        constexpr int PAIRS = 8 * NCB, EL = 16 * NCB;
+        auto read = [&](int i) {
+            if (i < KS) ring[i % AHEAD] = key(k, kb2, i);
+            else if (i < READS) ring[i % AHEAD] = v[((i - KS) % DB * 4 + 2 * vb2 + (i - KS) / DB) * 64 + (v_lane ^ (2 * vb2))];
+            else if constexpr (decltype(carry)::value) ring[i % AHEAD] = key(k, 1, i - READS);
+        };
+        h8 pf[NCB][2];
+        float sum[NCB];
+        auto weigh = [&](int i0, int i1) {
+#pragma unroll
+            for (int i = i0; i < i1; ++i) {
+                const int c = i % NCB, j = i / NCB * 2;
+                const float y = __builtin_amdgcn_exp2f(t[c][j]), z = __builtin_amdgcn_exp2f(t[c][j + 1]);
+                sum[c] += y + z;                             // before rounding: see the factors above
+                pf[c][j / 8][j % 8] = (_Float16)y;
+                pf[c][j / 8][j % 8 + 1] = (_Float16)z;
+            }
+        };
+#pragma unroll
+        for (int c = 0; c < NCB; ++c) {
+            sum[c] = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) tn[c][r] = 0.0f;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int x = 0; x < KS; ++x) {
+#pragma unroll
+            for (int c = 0; c < NCB; ++c) tn[c] = M::run(ring[x % AHEAD], qf[c][x], tn[c]);
+            read(x + AHEAD);
+            weigh(x * PAIRS / KS, (x + 1) * PAIRS / KS);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // weights that fp16 could not hold show in their sum: no maximum is formed until then
+        bool big = false;
+#pragma unroll
+        for (int c = 0; c < NCB; ++c) big = big || sum[c] > AT_MOST;
+        if (__any(big)) {
+#pragma unroll
+            for (int c = 0; c < NCB; ++c) {
+                const float x = largest(t, c);
+                move_by(t, c, x > AT_LIFT ? x - AT_LIFT : 0.0f);
+                sum[c] = 0.0f;
+            }
+            weigh(0, PAIRS);
+        }
+        const float iv = __builtin_amdgcn_rcpf(f.y), lv = __builtin_amdgcn_logf(fn.y);
+        float cz[NCB], off[NCB];
+#pragma unroll
+        for (int c = 0; c < NCB; ++c) {
+            // a row that sees nothing of a block takes nothing from a factor that is NaN
+            l[c] = sum[c] == 0.0f ? l[c] : fmaf(sum[c], iv, l[c]);
+            cz[c] = fn.x * qc[c];
+            off[c] = lv - m[c] + AT_LIFT;
+        }
+#pragma unroll
+        for (int x = 0; x < STEPS; ++x) {
+#pragma unroll
+            for (int c = 0; c < NCB; ++c) o[c][x % DB] = M::run(ring[(KS + x) % AHEAD], pf[c][x / DB], o[c][x % DB]);
+            read(KS + x + AHEAD);
+            extra(x);
+            if (x > 0) exponents(tn, cz, off, (x - 1) * EL / (STEPS - 1), x * EL / (STEPS - 1));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto preload = [&](const h8* k, int b) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) ring[i] = key(k, b, i);
+    };
+    // LDS written before is visible after; global loads may be in flight across it
+    auto meet = [&] {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+
+    if (lo < hi) {
+        int page = page_of(lo), next = page_of(lo + 1);
+        float2 f = factors(page);
+        acc t0[NCB], t1[NCB];
+        fetch(page);
+        hide(lo, page);
+#pragma unroll
+        for (int i = 0; i < 4 * PC; ++i) convert(i, k_sh[0], v_sh[0]);
+        fetch(next);
+        meet();
+        {                                                    // scores of the first half
+            float cz[NCB], off[NCB];
+#pragma unroll
+            for (int c = 0; c < NCB; ++c) {
+                cz[c] = f.x * qc[c];
+                off[c] = __builtin_amdgcn_logf(f.y) + AT_LIFT;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) t0[c][r] = 0.0f;
+#pragma unroll
+                for (int x = 0; x < KS; ++x) t0[c] = M::run(key(k_sh[0], 0, x), qf[c][x], t0[c]);
+            }
+            exponents(t0, cz, off, 0, 16 * NCB);
+        }
+        settle(t0, lo, page, 0);
+        preload(k_sh[0], 1);
+        int kc = 0, vc = 0;                                  // buffers of the present block
+        for (int blk = lo; blk < hi; ++blk) {
+            // after the last block the next one is block 0, converted into free buffers and not used
+            const int after = page_of(blk + 2), vn = vc == 2 ? 0 : vc + 1;
+            const float2 fn = factors(next);
+            hide(blk + 1, next);
+            half(t0, t1, k_sh[kc], 1, v_sh[vc], 0, f, f, std::false_type(), [&](int x) {
+#pragma unroll
+                for (int i = x * 4 * PC / STEPS; i < (x + 1) * 4 * PC / STEPS; ++i) convert(i, k_sh[kc ^ 1], v_sh[vn]);
+                if (x == STEPS - 1) fetch(after);            // the registers that were converted are free
+            });
+            settle(t1, blk, page, 1);
+            meet();
+            preload(k_sh[kc ^ 1], 0);
+            half(t1, t0, k_sh[kc ^ 1], 0, v_sh[vc], 1, f, fn, std::true_type(), [](int) {});
+            if (blk + 1 < hi) settle(t0, blk + 1, next, 0);
+            kc ^= 1;
+            vc = vn;
+            page = next;
+            next = after;
+            f = fn;
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < NCB; ++c) {
+        if (!seen[c]) m[c] = AT_NONE;
+        l[c] += __shfl_xor(l[c], 32);
+    }
+    store_rows<D, 32, NCB>(a, q, kh, group, row0, all, sp, n, g, wide != 0, o, m, l);
 }
 
 // The parts of each row joined: a thread takes 4 elements, `lanes` groups of threads the parts in turn.
@@ -487,14 +845,15 @@ __global__ void __launch_bounds__(AT_T) k_kv_join(ba_kv_attend_args a, int tile_
     __shared__ float den_sh[AT_T];
     const int quads = a.dim / 4, unit = threadIdx.x / quads, d = threadIdx.x % quads * 4;
     const int per_wg = AT_T / quads / lanes;                 // rows of a workgroup
-    const int64_t rh = (int64_t)blockIdx.x * per_wg + unit / lanes;
+    const unsigned rh = blockIdx.x * (unsigned)per_wg + unit / lanes;
     const int lane = unit % lanes;
-    const int64_t row = rh / a.q_heads;
-    const int head = (int)(rh - row * a.q_heads);
+    const int64_t row = rh / (unsigned)a.q_heads;
+    const int head = (int)(rh - (unsigned)row * a.q_heads);
     const bool mine = unit / lanes < per_wg && row < a.n_rows;
     f4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     float den = 0.0f, top = AT_NONE;
     bool covered = false;
+    int n = 0;                                               // parts of the row
     if (mine) {
         int s = 0;                                           // the row's sequence
         if (a.offsets) {
@@ -512,22 +871,24 @@ __global__ void __launch_bounds__(AT_T) k_kv_join(ba_kv_attend_args a, int tile_
         const int group = a.q_heads / a.heads;
         covered = i >= 0 && i < q.rows;
         if (covered) {
-            const int64_t r = i * group + head % group, tile0 = r / tile_rows * tile_rows;
-            int n = 0, lo, hi;
-            for (; n < a.n_splits; ++n) {
-                at_blocks(a, q, group, tile0, tile_rows, n, lo, hi);
-                if (lo >= hi) break;
-            }
-            for (int p = 0; p < n; ++p) top = fmaxf(top, part_ref(a, row, head, p)->x);
-            for (int p = lane; p < n; p += lanes) {
-                const float2 f = *part_ref(a, row, head, p);
-                const float by = __builtin_amdgcn_exp2f(f.x - top);
-                const f4 x = *(const f4*)(part_sum(a, row, head, p) + d);
-                den = fmaf(f.y, by, den);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) sum[k] = fmaf(x[k], by, sum[k]);
-            }
+            const int64_t r = i * group + head % group;
+            const AtBlocks b = at_blocks(a, q, group, r / tile_rows * tile_rows, tile_rows);
+            n = (b.hi - b.lo + b.per - 1) / b.per;
+            for (int p = lane; p < n; p += lanes) top = fmaxf(top, part_ref(a, row, head, p)->x);
         }
+    }
+    // one reference for the row
+    den_sh[threadIdx.x] = top;
+    __syncthreads();
+    for (int k = 0; k < lanes; ++k) top = fmaxf(top, den_sh[threadIdx.x + (k - lane) * quads]);
+    __syncthreads();
+    for (int p = lane; p < n; p += lanes) {
+        const float2 f = *part_ref(a, row, head, p);
+        const float by = __builtin_amdgcn_exp2f(f.x - top);
+        const f4 x = *(const f4*)(part_sum(a, row, head, p) + d);
+        den = fmaf(f.y, by, den);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] = fmaf(x[k], by, sum[k]);
     }
     sum_sh[threadIdx.x] = sum;
     den_sh[threadIdx.x] = den;
@@ -543,22 +904,28 @@ __global__ void __launch_bounds__(AT_T) k_kv_join(ba_kv_attend_args a, int tile_
         a.lse[row * a.q_heads + head] = den == 0.0f ? -__builtin_inff() : 0.693147180559945309f * (top - AT_LIFT + __builtin_amdgcn_logf(den));
 }
 
-// The variant for a call: at most 16 rows of a cache head go through 16 columns, more through 32 (one or two
-// tiles of them to a wave), and from 65 rows on the waves split the rows.
-struct AtShape { int cols, ncb, wr; };
+// The kernel for a call by the rows that share a cache head: up to 16 in 16 columns and up to 32 in 32 with the waves
+// splitting the blocks; more in workgroups of 128 rows or, from 129 on, of 256 that share the converted blocks (128 where
+// heads of 256 leave a wave registers for 32 rows only).  256 rows are 4 waves of 64 rows up to 64 elements a head, and 8
+// waves of 32 above: then two waves fit a SIMD (2 x 2048 rows over 16384 tokens: 64 elements 615 us against 690 with 8
+// waves, 128 elements 1077 us against 1375 with 4).  `fit`: workgroups that a CU holds.
+struct AtShape { int cols, ncb, waves, rows, fit; };
 static AtShape at_shape(int64_t rows, int dim) {
-    if (rows <= 16) return {16, 1, 1};
-    if (rows <= 32) return {32, 1, 1};
-    if (rows <= 128 || dim > 128) return {32, 1, 4};
-    return {32, 2, 4};
+    if (rows <= 16) return {16, 0, 4, 16, dim <= 64 ? 4 : dim <= 128 ? 2 : 1};
+    if (rows <= 32) return {32, 0, 4, 32, dim <= 128 ? 2 : 1};
+    if (rows <= 128 || dim > 128) return {32, 1, 4, 128, dim <= 64 ? 3 : dim <= 128 ? 2 : 1};
+    if (dim <= 64) return {32, 2, 4, 256, 2};
+    return {32, 1, 8, 256, 1};
 }
 
 template <int D, int KT>
 static int launch_attend(const ba_kv_attend_args& a, AtShape v, unsigned nb, int tiles, int wide, hipStream_t st) {
-    if (v.cols == 16) hipLaunchKernelGGL((k_kv_attend<D, KT, 16, 1, 1>), dim3(nb), dim3(AT_T), 0, st, a, tiles, wide);
-    else if (v.wr == 1) hipLaunchKernelGGL((k_kv_attend<D, KT, 32, 1, 1>), dim3(nb), dim3(AT_T), 0, st, a, tiles, wide);
-    else if (v.ncb == 1) hipLaunchKernelGGL((k_kv_attend<D, KT, 32, 1, 4>), dim3(nb), dim3(AT_T), 0, st, a, tiles, wide);
-    else if constexpr (D <= 128) hipLaunchKernelGGL((k_kv_attend<D, KT, 32, 2, 4>), dim3(nb), dim3(AT_T), 0, st, a, tiles, wide);
+    const dim3 grid(nb), block(64 * v.waves);
+    if (v.cols == 16) hipLaunchKernelGGL((k_kv_attend<D, KT, 16>), grid, block, 0, st, a, tiles, wide);
+    else if (v.ncb == 0) hipLaunchKernelGGL((k_kv_attend<D, KT, 32>), grid, block, 0, st, a, tiles, wide);
+    else if (v.rows == 128) hipLaunchKernelGGL((k_kv_attend_tile<D, KT, 1, 4>), grid, block, 0, st, a, tiles, wide);
+    else if constexpr (D <= 64) hipLaunchKernelGGL((k_kv_attend_tile<D, KT, 2, 4>), grid, block, 0, st, a, tiles, wide);
+    else if constexpr (D <= 128) hipLaunchKernelGGL((k_kv_attend_tile<D, KT, 1, 8>), grid, block, 0, st, a, tiles, wide);
     BA_LAUNCHED();
     return BA_OK;
 }
@@ -572,9 +939,12 @@ extern "C" int32_t ba_kv_attend_splits(int32_t n_seqs, int32_t heads, int32_t q_
     if (n_seqs < 1 || heads < 1 || q_heads < heads || max_rows < 1 || n_pages < 1) return 1;
     const int64_t rows = max_rows * (q_heads / heads);
     const AtShape v = at_shape(rows, dim);
-    const int64_t tile = v.cols * v.ncb * v.wr, base = (int64_t)n_seqs * heads * ((rows + tile - 1) / tile);
+    const int64_t base = (int64_t)n_seqs * heads * ((rows + v.rows - 1) / v.rows);
     const int64_t most = (n_pages + AT_MIN_BLOCKS - 1) / AT_MIN_BLOCKS;
-    int64_t n = (1024 + base - 1) / base;                    // four workgroups for each of 256 CUs
+    // Many rows: as many workgroups as the CUs hold at a time.  Few rows read memory: one and a half per CU do, and
+    // at least two parts for sequences of different lengths.
+    int64_t n = v.ncb ? 256 * v.fit / base : (384 + base - 1) / base;
+    if (v.ncb == 0 && n < 2) n = 2;
     n = n < most ? n : most;
     return (int32_t)(n < 1 ? 1 : n);
 }
@@ -606,7 +976,7 @@ extern "C" int ba_kv_attend(const ba_kv_attend_args* args, void* stream) {
     const int group = a.q_heads / a.heads;
     const int64_t rows = a.max_rows * group;
     const AtShape v = at_shape(rows, a.dim);
-    const int tile = v.cols * v.ncb * v.wr;
+    const int tile = v.rows;
     const int64_t tiles = (rows + tile - 1) / tile;
     // a launch has less than 2^32 threads
     BA_REQUIRE(tiles <= ((int64_t)1 << 23) / a.n_seqs / a.heads / a.n_splits, "attention: too many tiles for a call (max_rows is the bound that counts)");
@@ -624,11 +994,12 @@ extern "C" int ba_kv_attend(const ba_kv_attend_args* args, void* stream) {
     switch (a.dim) { BA_AT_D(32) BA_AT_D(64) BA_AT_D(96) BA_AT_D(128) BA_AT_D(256) }
 #undef BA_AT_D
     if (rc != BA_OK || a.n_splits == 1) return rc;
-    int lanes = 1;
-    while (lanes < a.n_splits && 2 * lanes * (a.dim / 4) <= AT_T) lanes *= 2;
-    const int per_wg = AT_T / (a.dim / 4) / lanes;
     const int64_t jobs = a.n_rows * a.q_heads;
-    BA_REQUIRE((jobs + per_wg - 1) / per_wg < (int64_t)1 << 24, "attention: too many rows for a call");
+    // the parts of a row are shared among threads while the chip has room for more of them
+    int lanes = 1;
+    while (lanes < a.n_splits && 2 * lanes * (a.dim / 4) <= AT_T && jobs * (a.dim / 4) * lanes < 256 * 1024) lanes *= 2;
+    const int per_wg = AT_T / (a.dim / 4) / lanes;
+    BA_REQUIRE(jobs < (int64_t)1 << 31 && (jobs + per_wg - 1) / per_wg < (int64_t)1 << 24, "attention: too many rows for a call");
     hipLaunchKernelGGL(k_kv_join, dim3((unsigned)((jobs + per_wg - 1) / per_wg)), dim3(AT_T), 0, st, a, tile, lanes, wide);
     BA_LAUNCHED();
     return BA_OK;
