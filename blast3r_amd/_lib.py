@@ -140,13 +140,12 @@ class BaTangentArgs(ctypes.Structure):
                 ('H_z', c_p), ('workspace', c_p), ('workspace_bytes', c_i64)]
 
 
-c_p2 = c_p * 2
-c_i64x2 = c_i64 * 2
-
-
 class BaRotaryArgs(ctypes.Structure):
-    _fields_ = [('x', c_p2), ('y', c_p2), ('x_sb', c_i64x2), ('x_st', c_i64x2), ('x_sh', c_i64x2),
-                ('y_sb', c_i64x2), ('y_st', c_i64x2), ('y_sh', c_i64x2), ('heads', c_int * 2), ('n_x', c_int),
+    # the header's arrays of two, element by element
+    _fields_ = [('x0', c_p), ('x1', c_p), ('y0', c_p), ('y1', c_p),
+                ('x_sb0', c_i64), ('x_sb1', c_i64), ('x_st0', c_i64), ('x_st1', c_i64), ('x_sh0', c_i64), ('x_sh1', c_i64),
+                ('y_sb0', c_i64), ('y_sb1', c_i64), ('y_st0', c_i64), ('y_st1', c_i64), ('y_sh0', c_i64), ('y_sh1', c_i64),
+                ('heads0', c_int), ('heads1', c_int), ('n_x', c_int),
                 ('dtype', c_int), ('B', c_i64), ('T', c_i64), ('dim', c_int), ('part', c_int), ('axes', c_int),
                 ('interleaved', c_int), ('inverse', c_int), ('pos_int64', c_int), ('positions', c_p),
                 ('pos_sb', c_i64), ('pos_st', c_i64), ('pos_sa', c_i64), ('turns', c_p), ('factor', c_f)]
@@ -298,6 +297,22 @@ def check(status):
 
 def stream_ptr(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+
+
+def launch(call, args, device):
+    """One launch of ``call(args, stream)`` on the current stream of ``device``, as tensors on it expect (the short way
+    for calls whose host time counts: no stream object, no device guard where the device is the current one)."""
+    index = device.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return check(call(ctypes.byref(args), torch.cuda.current_stream(index).cuda_stream))
+    stream = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+    status = call(ctypes.byref(args), stream)
+    if status:
+        check(status)
 
 
 def ptr(t):

@@ -22,16 +22,20 @@
 #include "ba_hip.h"
 #include "ba_token.h"
 
+// every variant of the kernel rounds alike: fused steps are written as fmaf
+#pragma clang fp contract(off)
+
 namespace ba {
 
 #define ROT_T 256
+#define ROT_B 4
 
 struct RotGrid {
     unsigned n;              // threads that work
     unsigned units, groups;  // vectors (or vector pairs) of a head row; groups of heads
     unsigned rot_units;      // units that rotate; the others copy
     unsigned per;            // heads of a thread
-    int64_t first;           // token of thread 0
+    int64_t first, batch;    // token and batch of thread 0
 };
 
 __device__ __forceinline__ void turn_sincos(uint64_t frac, float& s, float& c) {
@@ -61,11 +65,10 @@ __global__ void __launch_bounds__(ROT_T) k_rotary(ba_rotary_args a, RotGrid g) {
     if (id >= g.n) return;
     const unsigned u = id % g.units, rest = id / g.units;
     const unsigned hg = rest % g.groups;
-    const int64_t token = g.first + rest / g.groups;
-    const int64_t b = token / a.T, t = token - b * a.T;
+    const int64_t t = g.first + rest / g.groups, b = g.batch + blockIdx.y;
     const bool copy = u >= g.rot_units;
     const int n = a.part / a.axes;                                      // elements of a section
-    int e0, e1 = 0, p0 = 0, ax = 0;
+    int e0, p0 = 0, ax = 0;
     if (copy) {
         e0 = a.part + (int)(u - g.rot_units) * V;
     } else if (INTER) {
@@ -77,7 +80,6 @@ __global__ void __launch_bounds__(ROT_T) k_rotary(ba_rotary_args a, RotGrid g) {
         ax = (int)u / per_sec;
         p0 = ((int)u - ax * per_sec) * V;
         e0 = ax * n + p0;
-        e1 = e0 + n / 2;
     }
     float sn[NP], cs[NP];
     if (!copy) {
@@ -90,39 +92,39 @@ __global__ void __launch_bounds__(ROT_T) k_rotary(ba_rotary_args a, RotGrid g) {
             cs[i] *= a.factor;
         }
     }
-    const int heads = a.heads[0] + a.heads[1];
-#pragma unroll 4
-    for (unsigned k = 0; k < g.per; ++k) {
-        const int h = (int)(hg + k * g.groups);
-        if (h >= heads) break;
-        const int w = h < a.heads[0] ? 0 : 1;
-        const int hh = w ? h - a.heads[0] : h;
-        const T* x = (const T*)a.x[w] + b * a.x_sb[w] + t * a.x_st[w] + hh * a.x_sh[w];
-        T* y = (T*)a.y[w] + b * a.y_sb[w] + t * a.y_st[w] + hh * a.y_sh[w];
-        float v0[V], v1[V];
-        load_vec<T, V>(x + e0, v0);
-        if (copy) {
-            store_vec<T, V>(y + e0, v0);
-            continue;
+    // ROT_B heads at a time: all their loads are under way before the first is used
+    const unsigned heads = (unsigned)(a.heads[0] + a.heads[1]);
+    const T* xt[2] = {(const T*)a.x[0] + b * a.x_sb[0] + t * a.x_st[0] + e0, (const T*)a.x[1] + b * a.x_sb[1] + t * a.x_st[1] + e0};
+    T* yt[2] = {(T*)a.y[0] + b * a.y_sb[0] + t * a.y_st[0] + e0, (T*)a.y[1] + b * a.y_sb[1] + t * a.y_st[1] + e0};
+    for (unsigned k = 0; k < g.per; k += ROT_B) {
+        float v0[ROT_B][V], v1[ROT_B][V];
+        T* y[ROT_B];
+#pragma unroll
+        for (unsigned j = 0; j < ROT_B; ++j) {
+            const unsigned h = hg + (k + j) * g.groups;
+            if (k + j >= g.per || h >= heads) break;
+            const bool first = h < (unsigned)a.heads[0];
+            const int hh = (int)(first ? h : h - a.heads[0]);        // strides of heads are below 2^31: one multiply-add each
+            const T* x = (first ? xt[0] : xt[1]) + (int64_t)hh * (first ? (int)a.x_sh[0] : (int)a.x_sh[1]);
+            y[j] = (first ? yt[0] : yt[1]) + (int64_t)hh * (first ? (int)a.y_sh[0] : (int)a.y_sh[1]);
+            load_vec<T, V>(x, v0[j]);
+            if (!INTER && !copy) load_vec<T, V>(x + n / 2, v1[j]);
         }
-        if (INTER) {
 #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const float p = v0[2 * i], q = v0[2 * i + 1];
-                v0[2 * i] = p * cs[i] - q * sn[i];
-                v0[2 * i + 1] = p * sn[i] + q * cs[i];
-            }
-            store_vec<T, V>(y + e0, v0);
-        } else {
-            load_vec<T, V>(x + e1, v1);
+        for (unsigned j = 0; j < ROT_B; ++j) {
+            if (k + j >= g.per || hg + (k + j) * g.groups >= heads) break;
+            if (!copy) {
 #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const float p = v0[i], q = v1[i];
-                v0[i] = p * cs[i] - q * sn[i];
-                v1[i] = p * sn[i] + q * cs[i];
+                for (int i = 0; i < NP; ++i) {
+                    float& p = INTER ? v0[j][2 * i] : v0[j][i];
+                    float& q = INTER ? v0[j][2 * i + 1] : v1[j][i];
+                    const float x = p, z = q;
+                    p = fmaf(x, cs[i], -(z * sn[i]));
+                    q = fmaf(x, sn[i], z * cs[i]);
+                }
+                if (!INTER) store_vec<T, V>(y[j] + n / 2, v1[j]);
             }
-            store_vec<T, V>(y + e0, v0);
-            store_vec<T, V>(y + e1, v1);
+            store_vec<T, V>(y[j], v0[j]);
         }
     }
 }
@@ -142,14 +144,15 @@ static int launch_rotary(const ba_rotary_args& a, hipStream_t st) {
     while (g.per < 8 && (int)g.per < heads && tokens * g.units * (heads / (2 * (int)g.per)) >= 256 * 2048) g.per *= 2;
     g.groups = (unsigned)((heads + (int)g.per - 1) / (int)g.per);
     const int64_t per_token = (int64_t)g.units * g.groups, most = ((int64_t)1 << 31) / per_token;
-    for (g.first = 0; g.first < tokens; g.first += most) {              // thread numbers stay in 32 bits
-        const int64_t now = tokens - g.first < most ? tokens - g.first : most;
-        g.n = (unsigned)(now * per_token);
-        const unsigned nb = (g.n + ROT_T - 1) / ROT_T;
-        if (a.interleaved) hipLaunchKernelGGL((k_rotary<T, V < 2 ? 2 : V, true>), dim3(nb), dim3(ROT_T), 0, st, a, g);
-        else hipLaunchKernelGGL((k_rotary<T, V, false>), dim3(nb), dim3(ROT_T), 0, st, a, g);
-        BA_LAUNCHED();
-    }
+    for (g.batch = 0; g.batch < a.B; g.batch += 65535)
+        for (g.first = 0; g.first < a.T; g.first += most) {             // thread numbers stay in 32 bits
+            const int64_t now = a.T - g.first < most ? a.T - g.first : most, nb = a.B - g.batch < 65535 ? a.B - g.batch : 65535;
+            g.n = (unsigned)(now * per_token);
+            const dim3 grid((g.n + ROT_T - 1) / ROT_T, (unsigned)nb);
+            if (a.interleaved) hipLaunchKernelGGL((k_rotary<T, V < 2 ? 2 : V, true>), grid, dim3(ROT_T), 0, st, a, g);
+            else hipLaunchKernelGGL((k_rotary<T, V, false>), grid, dim3(ROT_T), 0, st, a, g);
+            BA_LAUNCHED();
+        }
     return BA_OK;
 }
 
@@ -178,6 +181,15 @@ extern "C" int ba_rotary(const ba_rotary_args* args, void* stream) {
     BA_REQUIRE(a.B >= 0 && a.T >= 0 && a.heads[0] >= 1 && (a.n_x == 1 || a.heads[1] >= 1), "rotary: bad sizes");
     BA_REQUIRE(a.T == 0 || a.B <= ((int64_t)1 << 40) / a.T, "rotary: bad sizes");
     if (a.n_x == 1) a.heads[1] = 0;
+    for (int w = 0; w < a.n_x; ++w)
+        BA_REQUIRE(a.x_sh[w] > -((int64_t)1 << 31) && a.x_sh[w] < (int64_t)1 << 31 && a.y_sh[w] > -((int64_t)1 << 31) && a.y_sh[w] < (int64_t)1 << 31,
+                   "rotary: strides of heads must be below 2^31");
+    if (a.T == 1) {                                                     // single tokens: the batch takes their place
+        a.T = a.B;
+        a.B = 1;
+        a.pos_st = a.pos_sb;
+        for (int w = 0; w < 2; ++w) { a.x_st[w] = a.x_sb[w]; a.y_st[w] = a.y_sb[w]; }
+    }
     BA_REQUIRE(a.heads[0] <= 65536 && a.heads[1] <= 65536, "rotary: bad sizes");
     BA_REQUIRE(a.dim >= 2 && a.dim <= 65536, "rotary: head size must be in [2, 65536]");
     BA_REQUIRE(a.axes >= 1 && a.part >= 2 && a.part <= a.dim && a.part % (2 * a.axes) == 0,

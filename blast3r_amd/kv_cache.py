@@ -15,12 +15,11 @@ Sequences of a call have the same number of rows each, or ``offsets`` (n_seqs + 
 workgroups.  Lengths, offsets and pages are device tensors, never read by the host: nothing here synchronises, and a
 call can be captured in a graph.  What they say out of range is left out (include/ba_hip.h).
 """
-import ctypes
 import math
 
 import torch
 
-from ._lib import BaKvArgs, BaKvAttendArgs, check, lib, stream_ptr
+from ._lib import BaKvArgs, BaKvAttendArgs, launch, lib
 
 __all__ = ['KVCache', 'BLOCK']
 
@@ -74,25 +73,26 @@ class KVCache:
         self.k, self.v, self.scales = k, v, scales
         self.n_blocks, self.heads, self.head_dim = n, h, d
         self.device, self.dtype = k.device, k.dtype
-
-    def _index(self, t, name, shape):
-        if t.dtype != torch.int32 or t.device != self.device or tuple(t.shape) != shape or not t.is_contiguous():
-            raise ValueError(f'cache: {name} must be a contiguous int32 tensor of shape {shape} on {self.device}')
-        return t.data_ptr()
+        # the fields of every call
+        same = dict(k=k.data_ptr(), v=v.data_ptr(), scales=scales.data_ptr(), n_blocks=n, heads=h, dim=d, bits=BITS[k.dtype])
+        self._lib, self._args = lib(), BaKvArgs(**same)
+        self._attend_args = BaKvAttendArgs(n_splits=1, scale=1.0 / math.sqrt(d), **same)
 
     def _fill(self, a, pages, firsts, name, offsets, n_rows, max_rows):
-        """The fields that every call has; returns the largest number of rows of a sequence."""
-        if pages.dim() != 2 or pages.dtype != torch.int32 or pages.device != self.device or pages.stride(1) != 1:
-            raise ValueError(f'cache: pages must be (n_seqs, blocks) int32 on {self.device} with contiguous rows')
-        S = pages.shape[0]
-        a.k, a.v, a.scales = self.k.data_ptr(), self.v.data_ptr(), self.scales.data_ptr()
-        a.n_blocks, a.heads, a.dim, a.bits = self.n_blocks, self.heads, self.head_dim, BITS[self.dtype]
-        a.n_seqs, a.pages, a.pages_stride, a.n_pages = S, pages.data_ptr(), pages.stride(0), pages.shape[1]
-        firsts_at = self._index(firsts, name, (S,))
+        """The fields of a call that the arguments of every call give."""
+        dev = self.device
+        if pages.dim() != 2 or pages.dtype is not torch.int32 or pages.device != dev or pages.stride(1) != 1:
+            raise ValueError(f'cache: pages must be (n_seqs, blocks) int32 on {dev} with contiguous rows')
+        S, a.n_pages = pages.shape
+        a.n_seqs, a.pages, a.pages_stride = S, pages.data_ptr(), pages.stride(0)
+        if firsts.dtype is not torch.int32 or firsts.device != dev or firsts.shape != (S,) or not firsts.is_contiguous():
+            raise ValueError(f'cache: {name} must be a contiguous int32 tensor of shape {(S,)} on {dev}')
         a.n_rows = n_rows
         if offsets is not None:
-            a.offsets = self._index(offsets, 'offsets', (S + 1,))
-            most = n_rows if max_rows is None else min(int(max_rows), n_rows)
+            if offsets.dtype is not torch.int32 or offsets.device != dev or offsets.shape != (S + 1,) or not offsets.is_contiguous():
+                raise ValueError(f'cache: offsets must be a contiguous int32 tensor of shape {(S + 1,)} on {dev}')
+            a.offsets = offsets.data_ptr()
+            most = n_rows if max_rows is None or max_rows > n_rows else int(max_rows)
             if most < 0:
                 raise ValueError('cache: a negative bound on rows')
         else:
@@ -101,50 +101,51 @@ class KVCache:
             most = n_rows // S if S else 0
             a.rows_per_seq = most
         a.max_rows = most
-        return firsts_at, most
+        return most
 
     def _rows(self, t, name, heads):
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.head_dim or t.device != self.device:
+        shape = t.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or t.device != self.device:
             raise ValueError(f'cache: {name} must be (tokens, {heads}, {self.head_dim}) on {self.device}, got '
-                             f'{tuple(t.shape)} on {t.device}')
-        if t.stride(2) != 1:
+                             f'{tuple(shape)} on {t.device}')
+        st, sh, one = t.stride()
+        if one != 1:
             raise ValueError(f'cache: the elements of a head of {name} must be contiguous')
+        return st, sh
 
     def append(self, k, v, pages, lengths, offsets=None, max_new=None):
         """Write the rows of k and v (tokens, heads, head_dim; fp32, fp16 or bf16) after the first ``lengths`` (n_seqs,)
         int32 tokens of their sequences.  ``lengths`` stays as it is.  No two sequences of a call may append to the
         same block."""
-        self._rows(k, 'k', self.heads)
-        self._rows(v, 'v', self.heads)
-        if k.shape != v.shape or k.dtype != v.dtype or k.dtype not in DTYPES:
+        a = BaKvArgs.from_buffer_copy(self._args)
+        a.rk_st, a.rk_sh = self._rows(k, 'k', self.heads)
+        a.rv_st, a.rv_sh = self._rows(v, 'v', self.heads)
+        code = DTYPES.get(k.dtype)
+        if code is None or k.shape != v.shape or k.dtype is not v.dtype:
             raise ValueError(f'cache: k and v must be alike, in fp32, fp16 or bf16: got {tuple(k.shape)} {k.dtype} and '
                              f'{tuple(v.shape)} {v.dtype}')
-        a = BaKvArgs()
-        a.starts, most = self._fill(a, pages, lengths, 'lengths', offsets, k.shape[0], max_new)
-        self._move(a, k, v, most, lib().ba_kv_write)
+        a.starts, a.dtype, a.rk, a.rv = lengths.data_ptr(), code, k.data_ptr(), v.data_ptr()
+        if self._fill(a, pages, lengths, 'lengths', offsets, k.shape[0], max_new):
+            launch(self._lib.ba_kv_write, a, self.device)
 
     def read(self, pages, starts, offsets, n_rows, max_count=None, dtype=torch.bfloat16):
         """(k, v) of tokens ``starts[s]`` and on, ``offsets[s + 1] - offsets[s]`` of each sequence (n_rows / n_seqs where
         offsets is None), as (n_rows, heads, head_dim) tensors of ``dtype``: code * factor, rounded once."""
-        if dtype not in DTYPES:
+        code = DTYPES.get(dtype)
+        if code is None:
             raise ValueError(f'cache: fp32, fp16 or bf16 values, got {dtype}')
         if n_rows < 0:
             raise ValueError(f'cache: {n_rows} rows')
-        k = torch.empty((n_rows, self.heads, self.head_dim), dtype=dtype, device=self.device)
-        v = torch.empty_like(k)
-        a = BaKvArgs()
-        a.starts, most = self._fill(a, pages, starts, 'starts', offsets, n_rows, max_count)
-        self._move(a, k, v, most, lib().ba_kv_read)
-        return k, v
-
-    def _move(self, a, k, v, most, call):
-        a.dtype = DTYPES[k.dtype]
-        a.rk, a.rv = k.data_ptr(), v.data_ptr()
-        a.rk_st, a.rk_sh, _ = k.stride()
-        a.rv_st, a.rv_sh, _ = v.stride()
-        if a.n_rows > 0 and most > 0:
-            with torch.cuda.device(self.device):
-                check(call(ctypes.byref(a), stream_ptr(self.device)))
+        a = BaKvArgs.from_buffer_copy(self._args)
+        both = torch.empty((2, n_rows, self.heads, self.head_dim), dtype=dtype, device=self.device)
+        a.rk_st = a.rv_st = self.heads * self.head_dim
+        a.rk_sh = a.rv_sh = self.head_dim
+        at = both.data_ptr()
+        a.starts, a.dtype, a.rk = starts.data_ptr(), code, at
+        a.rv = at + n_rows * self.heads * self.head_dim * both.element_size()
+        if self._fill(a, pages, starts, 'starts', offsets, n_rows, max_count):
+            launch(self._lib.ba_kv_read, a, self.device)
+        return both[0], both[1]
 
     def attend(self, q, pages, lengths, offsets=None, max_new=None, causal=True, window=None, scale=None, out=None,
                return_lse=False):
@@ -160,41 +161,44 @@ class KVCache:
         A row that sees no token gives zeros.  q_heads is a multiple of the cache's heads; query head h reads cache
         head h // (q_heads // heads).  With ``return_lse`` also log(sum(exp(scale q k^T))) as (tokens, q_heads) fp32,
         -inf where no token is seen, with which results over different tokens can be joined."""
-        if q.dim() != 3 or q.shape[1] % self.heads or q.shape[1] == 0:
-            raise ValueError(f'cache: q must be (tokens, a multiple of {self.heads} heads, {self.head_dim}), got {tuple(q.shape)}')
-        n_rows, q_heads = q.shape[0], q.shape[1]
-        self._rows(q, 'q', q_heads)
-        if q.dtype not in (torch.float16, torch.bfloat16):
-            raise ValueError(f'cache: queries must be fp16 or bf16, got {q.dtype}')
-        if window is not None and window < 1:
-            raise ValueError(f'cache: window must be at least 1, got {window}')
-        scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
-        if not 0.0 < scale < 1e30:
-            raise ValueError(f'cache: scale must be positive, got {scale}')
+        shape = q.shape
+        if len(shape) != 3 or shape[1] % self.heads or shape[1] == 0:
+            raise ValueError(f'cache: q must be (tokens, a multiple of {self.heads} heads, {self.head_dim}), got {tuple(shape)}')
+        n_rows, q_heads, dim = shape
+        a = BaKvAttendArgs.from_buffer_copy(self._attend_args)
+        a.q_st, a.q_sh = self._rows(q, 'q', q_heads)
+        dtype, dev = q.dtype, self.device
+        if dtype is not torch.bfloat16 and dtype is not torch.float16:
+            raise ValueError(f'cache: queries must be fp16 or bf16, got {dtype}')
+        if window is not None:
+            if window < 1:
+                raise ValueError(f'cache: window must be at least 1, got {window}')
+            a.window = window
+        if scale is not None:
+            if not 0.0 < scale < 1e30:
+                raise ValueError(f'cache: scale must be positive, got {scale}')
+            a.scale = scale
         if out is None:
-            out = torch.empty((n_rows, q_heads, self.head_dim), dtype=q.dtype, device=self.device)
+            out = torch.empty(shape, dtype=dtype, device=dev)
+            a.o_st, a.o_sh = q_heads * dim, dim
         else:
-            if out.shape != q.shape or out.dtype != q.dtype:
+            if out.shape != shape or out.dtype is not dtype:
                 raise ValueError('cache: out must be like q')
-            self._rows(out, 'out', q_heads)
-        lse = torch.empty((n_rows, q_heads), dtype=torch.float32, device=self.device) if return_lse else None
-        a = BaKvAttendArgs()
-        a.lengths, most = self._fill(a, pages, lengths, 'lengths', offsets, n_rows, max_new)
-        if n_rows > 0 and most > 0:
-            L = lib()
-            a.dtype = DTYPES[q.dtype]
-            a.q, a.o = q.data_ptr(), out.data_ptr()
-            a.q_st, a.q_sh, _ = q.stride()
-            a.o_st, a.o_sh, _ = out.stride()
-            if lse is not None:
-                a.lse = lse.data_ptr()
-            a.q_heads, a.causal, a.window, a.scale = q_heads, bool(causal), window or 0, scale
-            with torch.cuda.device(self.device):
-                n = L.ba_kv_attend_splits(a.n_seqs, a.heads, q_heads, a.dim, most, a.n_pages)
+            a.o_st, a.o_sh = self._rows(out, 'out', q_heads)
+        lse = None
+        if return_lse:
+            lse = torch.empty((n_rows, q_heads), dtype=torch.float32, device=dev)
+            a.lse = lse.data_ptr()
+        a.lengths, a.dtype, a.q, a.o = lengths.data_ptr(), DTYPES[dtype], q.data_ptr(), out.data_ptr()
+        a.q_heads, a.causal = q_heads, 1 if causal else 0
+        most = self._fill(a, pages, lengths, 'lengths', offsets, n_rows, max_new)
+        if most:
+            L = self._lib
+            n = L.ba_kv_attend_splits(a.n_seqs, self.heads, q_heads, dim, most, a.n_pages)
+            if n > 1:                        # the partial sums live until the launches on this stream are done
                 a.n_splits = n
-                if n > 1:                    # the partial sums live until the launches on this stream are done
-                    size = L.ba_kv_attend_workspace_bytes(n_rows, q_heads, a.dim, n)
-                    work = torch.empty(size, dtype=torch.uint8, device=self.device)
-                    a.workspace, a.workspace_bytes = work.data_ptr(), size
-                check(L.ba_kv_attend(ctypes.byref(a), stream_ptr(self.device)))
+                size = L.ba_kv_attend_workspace_bytes(n_rows, q_heads, dim, n)
+                work = torch.empty(size, dtype=torch.uint8, device=dev)
+                a.workspace, a.workspace_bytes = work.data_ptr(), size
+            launch(L.ba_kv_attend, a, dev)
         return (out, lse) if return_lse else out

@@ -10,12 +10,11 @@ their frequencies for long contexts.  ``Rotary`` holds one such choice::
 
 Nothing here falls back to torch: the rotation runs in libba_hip.so on device tensors.
 """
-import ctypes
 import math
 
 import torch
 
-from ._lib import BaRotaryArgs, check, lib, stream_ptr
+from ._lib import BaRotaryArgs, launch, lib
 
 __all__ = ['Rotary', 'rotary_frequencies']
 
@@ -103,6 +102,11 @@ class Rotary:
         self.turns = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device)
         if not self.turns.is_cuda:
             raise RuntimeError('rotary needs a GPU (it runs in libba_hip.so)')
+        self.device = self.turns.device
+        # the fields of every call
+        self._args = BaRotaryArgs(n_x=1, B=1, dim=head_dim, part=part, axes=axes, interleaved=layout == 'interleaved',
+                                  turns=self.turns.data_ptr(), factor=self.factor)
+        self._call = lib().ba_rotary
 
     def __call__(self, positions, *xs, out=None, inverse=False):
         """The rotated tensors of ``xs``: one or two of shape (tokens, heads, head_dim) or (B, T, heads, head_dim), fp32,
@@ -115,7 +119,7 @@ class Rotary:
         """
         if not 1 <= len(xs) <= 2:
             raise ValueError(f'rotary: one or two tensors at a time, got {len(xs)}')
-        if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        if torch.is_grad_enabled() and (xs[0].requires_grad or xs[-1].requires_grad):
             if out is not None:
                 raise ValueError('rotary: out cannot be given where gradients are recorded')
             ys = _Turn.apply(self, positions, bool(inverse), *xs)
@@ -125,58 +129,71 @@ class Rotary:
 
     def _run(self, positions, xs, out, inverse):
         x = xs[0]
-        lead = x.shape[:-2]
-        dev = self.turns.device
-        if len(lead) not in (1, 2):
-            raise ValueError(f'rotary: tensors are (tokens, heads, dim) or (B, T, heads, dim), got {tuple(x.shape)}')
-        if x.dtype not in DTYPES:
-            raise ValueError(f'rotary: fp32, fp16 or bf16 tensors, got {x.dtype}')
-        if positions.dtype not in (torch.int32, torch.int64) or positions.device != dev:
+        dtype, shape, dev = x.dtype, x.shape, self.device
+        lead = shape[:-2]
+        n_lead = len(lead)
+        if n_lead != 1 and n_lead != 2:
+            raise ValueError(f'rotary: tensors are (tokens, heads, dim) or (B, T, heads, dim), got {tuple(shape)}')
+        code = DTYPES.get(dtype)
+        if code is None:
+            raise ValueError(f'rotary: fp32, fp16 or bf16 tensors, got {dtype}')
+        wide = positions.dtype is torch.int64
+        if not wide and positions.dtype is not torch.int32 or positions.device != dev:
             raise ValueError(f'rotary: positions must be int32 or int64 on {dev}')
-        p = positions
+        p_lead, p_stride = positions.shape, positions.stride()
         if self.axes > 1:
-            if p.dim() < 2 or p.shape[-1] != self.axes:
-                raise ValueError(f'rotary: positions need a last dimension of {self.axes} axes, got {tuple(p.shape)}')
-            p_lead, sa = p.shape[:-1], p.stride(-1)
-        else:
-            p_lead, sa = p.shape, 0
-        if tuple(p_lead) != tuple(lead) and not (len(lead) == 2 and tuple(p_lead) == tuple(lead[1:])):
-            raise ValueError(f'rotary: positions of shape {tuple(p.shape)} for tokens {tuple(lead)}')
+            if len(p_lead) < 2 or p_lead[-1] != self.axes:
+                raise ValueError(f'rotary: positions need a last dimension of {self.axes} axes, got {tuple(p_lead)}')
+            p_lead = p_lead[:-1]
+        if p_lead != lead and (n_lead == 1 or p_lead != lead[1:]):
+            raise ValueError(f'rotary: positions of shape {tuple(positions.shape)} for tokens {tuple(lead)}')
         if out is None:
-            ys = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in xs]
+            ys = [torch.empty_like(x) for x in xs]
+            for i, y in enumerate(ys):
+                if y.stride()[-1] != 1:                     # expanded tensors may come back in another order
+                    ys[i] = torch.empty(y.shape, dtype=dtype, device=dev)
         else:
             ys = list(out) if isinstance(out, (tuple, list)) else [out]
             if len(ys) != len(xs):
                 raise ValueError(f'rotary: {len(ys)} outputs for {len(xs)} tensors')
-        a = BaRotaryArgs()
-        for i, (t, y) in enumerate(zip(xs, ys)):
-            shape = t.shape
-            if (len(shape) != len(lead) + 2 or shape[:-2] != lead or shape[-1] != self.head_dim or t.dtype != x.dtype or
-                    t.device != dev):
-                raise ValueError(f'rotary: tensors must share tokens, type and device, with heads of {self.head_dim}: got '
-                                 f'{tuple(shape)} {t.dtype} on {t.device}')
-            if y.shape != shape or y.dtype != t.dtype or y.device != dev:
-                raise ValueError('rotary: an output must be like its tensor')
-            xs_, ys_ = t.stride(), y.stride()
-            if xs_[-1] != 1 or ys_[-1] != 1:
-                raise ValueError('rotary: the elements of a head must be contiguous')
-            a.x[i], a.y[i] = t.data_ptr(), y.data_ptr()
-            a.heads[i] = shape[-2]
-            a.x_sh[i], a.y_sh[i] = xs_[-2], ys_[-2]
-            a.x_st[i], a.y_st[i] = xs_[-3], ys_[-3]
-            if len(lead) == 2:
-                a.x_sb[i], a.y_sb[i] = xs_[0], ys_[0]
-        a.n_x, a.dtype = len(xs), DTYPES[x.dtype]
-        a.T = lead[-1]
-        a.B = lead[0] if len(lead) == 2 else 1
-        a.dim, a.part, a.axes = self.head_dim, self.rotary_dim, self.axes
-        a.interleaved, a.inverse = self.layout == 'interleaved', bool(inverse)
-        a.pos_int64, a.positions = p.dtype == torch.int64, p.data_ptr()
-        st = p.stride()
-        a.pos_st, a.pos_sa = st[len(p_lead) - 1], sa
-        a.pos_sb = st[0] if len(p_lead) == 2 else 0
-        a.turns, a.factor = self.turns.data_ptr(), self.factor
-        if a.B * a.T > 0 and all(h > 0 for h in a.heads[:len(xs)]):
-            with torch.cuda.device(dev):
-                check(lib().ba_rotary(ctypes.byref(a), stream_ptr(dev)))
+            for x, y in zip(xs, ys):
+                if y.shape != x.shape or y.dtype != x.dtype or y.device != x.device or y.stride(-1) != 1:
+                    raise ValueError('rotary: an output must be like its tensor, with contiguous elements of a head')
+        a = BaRotaryArgs.from_buffer_copy(self._args)
+        t, y = xs[0], ys[0]
+        xs_, ys_ = self._strides(t, lead, dtype), y.stride()
+        a.x0, a.y0, a.heads0 = t.data_ptr(), y.data_ptr(), t.shape[-2]
+        a.x_sh0, a.x_st0, a.y_sh0, a.y_st0 = xs_[-2], xs_[-3], ys_[-2], ys_[-3]
+        if n_lead == 2:
+            a.x_sb0, a.y_sb0, a.B = xs_[0], ys_[0], lead[0]
+        if len(xs) == 2:
+            t, y = xs[1], ys[1]
+            xs_, ys_ = self._strides(t, lead, dtype), y.stride()
+            a.x1, a.y1, a.heads1 = t.data_ptr(), y.data_ptr(), t.shape[-2]
+            a.x_sh1, a.x_st1, a.y_sh1, a.y_st1 = xs_[-2], xs_[-3], ys_[-2], ys_[-3]
+            a.n_x = 2
+            if n_lead == 2:
+                a.x_sb1, a.y_sb1 = xs_[0], ys_[0]
+        a.dtype, a.T = code, lead[-1]
+        if inverse:
+            a.inverse = 1
+        if wide:
+            a.pos_int64 = 1
+        a.positions, a.pos_st = positions.data_ptr(), p_stride[len(p_lead) - 1]
+        if self.axes > 1:
+            a.pos_sa = p_stride[-1]
+        if len(p_lead) == 2:
+            a.pos_sb = p_stride[0]
+        if a.T and a.B:
+            launch(self._call, a, dev)
         return tuple(ys)
+
+    def _strides(self, t, lead, dtype):
+        shape, stride = t.shape, t.stride()
+        if (len(shape) != len(lead) + 2 or shape[:-2] != lead or shape[-1] != self.head_dim or shape[-2] == 0 or
+                t.dtype is not dtype or t.device != self.device):
+            raise ValueError(f'rotary: tensors must share tokens, type and device, with heads of {self.head_dim}: got '
+                             f'{tuple(shape)} {t.dtype} on {t.device}')
+        if stride[-1] != 1:
+            raise ValueError('rotary: the elements of a head must be contiguous')
+        return stride

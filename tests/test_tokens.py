@@ -101,7 +101,7 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu():
             setattr(a, n, x)
 
     r = _lib.BaRotaryArgs(n_x=1, dtype=2, B=1, T=4, dim=64, part=64, axes=2)
-    r.heads[0] = 2
+    r.heads0 = 2
     assert L.ba_rotary(None, None) != 0
     refused(L.ba_rotary, r, 'null pointer')
     refused(L.ba_rotary, r, 'one or two', n_x=3)
@@ -112,7 +112,7 @@ def test_entry_points_refuse_bad_arguments_without_a_gpu():
     refused(L.ba_rotary, r, 'dtype', dtype=3)
     refused(L.ba_rotary, r, 'bad sizes', T=-1)
     refused(L.ba_rotary, r, 'bad sizes', T=1 << 41)
-    assert L.ba_rotary(ctypes.byref(_lib.BaRotaryArgs(n_x=1, B=1, T=0, dim=64, part=64, axes=2, heads=(1, 0))), None) == 0
+    assert L.ba_rotary(ctypes.byref(_lib.BaRotaryArgs(n_x=1, B=1, T=0, dim=64, part=64, axes=2, heads0=1)), None) == 0
 
     kv = dict(n_blocks=2, heads=2, dim=64, bits=0, n_seqs=1, n_pages=2, pages_stride=2, dtype=2, n_rows=3, rows_per_seq=3, max_rows=3)
     for call, a in ((L.ba_kv_write, _lib.BaKvArgs(**kv)), (L.ba_kv_read, _lib.BaKvArgs(**kv)),
