@@ -51,8 +51,10 @@ __device__ __forceinline__ bool kv_share(const ba_kv_args& a, int s, int slot_of
     r.row = row0 + lo - start;
     r.at = (int)(lo - slot * 64);
     r.n = (int)(hi - lo);
-    return r.page >= 0 && r.page < a.n_blocks;
+    return true;
 }
+
+__device__ __forceinline__ bool kv_there(const ba_kv_args& a, const KvShare& r) { return r.page >= 0 && r.page < a.n_blocks; }
 
 __device__ __forceinline__ uint32_t f32_bits(float x) { return __builtin_bit_cast(uint32_t, x); }
 
@@ -75,8 +77,11 @@ __device__ __forceinline__ uint32_t kv_code4(float a, float b, float c, float d)
         const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
         return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
     }
-    auto one = [](float x) { return (uint32_t)(int)fminf(fmaxf(rintf(x), -127.0f), 127.0f) & 255u; };
-    return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+    // 1.5 * 2^23 + x is x rounded to a whole number, ties to even, with its low byte last; |x| is at most 127 by the
+    // choice of the factor
+    auto one = [](float x) { return __builtin_bit_cast(uint32_t, x + 12582912.0f); };
+    const uint32_t lo = __builtin_amdgcn_perm(one(b), one(a), 0x0c0c0400u), hi = __builtin_amdgcn_perm(one(d), one(c), 0x0c0c0400u);
+    return hi << 16 | lo;
 }
 
 template <int KT>
@@ -118,12 +123,8 @@ __device__ void kv_write_block(const ba_kv_args& a, const KvShare& sh, int h, bo
     constexpr int N = PER_ROW * (64 / ROWS), UNITS = (N + KV_T - 1) / KV_T;
     const int tid = threadIdx.x;
     const T* x = (const T*)(KEYS ? a.rk : a.rv);
-    const int64_t st = KEYS ? a.rk_st : a.rv_st;
+    const int st = (int)(KEYS ? a.rk_st : a.rv_st);         // below 2^31: a row's address is one multiply-add
     x += sh.row * st + h * (KEYS ? a.rk_sh : a.rv_sh);
-    uint8_t* base = (uint8_t*)(KEYS ? a.k : a.v) + (sh.page * a.heads + h) * (int64_t)(64 * D);
-    float* factor = a.scales + (sh.page * a.heads + h) * 2 + (KEYS ? 0 : 1);
-    const float old = sh.at ? *factor : 0.0f;
-
     // tokens of a unit are block places sh.at + t; a values unit starts at a place that is a multiple of 4
     const int at4 = KEYS ? sh.at : sh.at & ~3;
     float v[UNITS][ROWS][W];
@@ -135,15 +136,24 @@ __device__ void kv_write_block(const ba_kv_args& a, const KvShare& sh, int h, bo
         for (int r = 0; r < ROWS; ++r) {
             const int t = place + r - sh.at;
             if (u < N && t >= 0 && t < sh.n) {
-                load_row<T, W>(x + t * st + e, wide, v[i][r]);
-#pragma unroll
-                for (int j = 0; j < W; ++j) top = max(top, f32_bits(v[i][r][j]) & 0x7fffffffu);
+                load_row<T, W>(x + (int64_t)t * st + e, wide, v[i][r]);
             } else {
 #pragma unroll
                 for (int j = 0; j < W; ++j) v[i][r][j] = 0.0f;
             }
         }
     }
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+            for (int j = 0; j < W; ++j) top = max(top, f32_bits(v[i][r][j]) & 0x7fffffffu);
+    // the rows were under way before the block's number was needed
+    if (!kv_there(a, sh)) return;
+    uint8_t* base = (uint8_t*)(KEYS ? a.k : a.v) + (sh.page * a.heads + h) * (int64_t)(64 * D);
+    float* factor = a.scales + (sh.page * a.heads + h) * 2 + (KEYS ? 0 : 1);
+    const float old = sh.at ? *factor : 0.0f;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m));
     if ((tid & 63) == 0) red[tid >> 6] = top;
@@ -253,9 +263,9 @@ __global__ void __launch_bounds__(KV_T) k_kv_read(ba_kv_args a, int slots, int w
     id /= (unsigned)a.heads;
     const int s = (int)(id / (unsigned)slots), slot = (int)(id % (unsigned)slots);
     KvShare sh;
-    const bool held = kv_share(a, s, slot, sh);
+    const bool held = kv_share(a, s, slot, sh) && kv_there(a, sh);
     T* y = (T*)(keys ? a.rk : a.rv);
-    const int64_t st = keys ? a.rk_st : a.rv_st;
+    const int st = (int)(keys ? a.rk_st : a.rv_st);         // below 2^31: a row's address is one multiply-add
     y += h * (keys ? a.rk_sh : a.rv_sh);
     if (!held) {                                             // rows of the call that no block holds are zeros
         int64_t row0 = (int64_t)s * a.rows_per_seq, count = a.rows_per_seq;
@@ -286,7 +296,7 @@ __global__ void __launch_bounds__(KV_T) k_kv_read(ba_kv_args a, int slots, int w
             kv_values4<KT>(((const uint32_t*)base)[sh.at * (D / 4) + q], v);
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] *= f;
-            store4(y + q / (D / 4) * st + q % (D / 4) * 4, v);
+            store4(y + (int64_t)(q / (D / 4)) * st + q % (D / 4) * 4, v);
         }
         return;
     }
@@ -303,7 +313,7 @@ __global__ void __launch_bounds__(KV_T) k_kv_read(ba_kv_args a, int slots, int w
             const int t = place + r - sh.at;
             if (t < 0 || t >= sh.n) continue;
             const float o[4] = {v[0][r] * f, v[1][r] * f, v[2][r] * f, v[3][r] * f};
-            store4(y + t * st + e, o);
+            store4(y + (int64_t)t * st + e, o);
         }
     }
 }
@@ -335,6 +345,9 @@ static int kv_call(const ba_kv_args* args, void* stream, bool write) {
     BA_REQUIRE(a.starts && a.rk && a.rv, "null pointer");
     BA_REQUIRE((a.n_pages == 0 || a.pages) && (a.n_blocks == 0 || (a.k && a.v && a.scales)), "null pointer");
     BA_REQUIRE((uintptr_t)a.k % 16 == 0 && (uintptr_t)a.v % 16 == 0, "cache: k and v must be aligned to 16 bytes");
+    const int64_t strides[4] = {a.rk_st, a.rk_sh, a.rv_st, a.rv_sh};
+    for (int i = 0; i < 4; ++i)
+        BA_REQUIRE(strides[i] > -((int64_t)1 << 31) && strides[i] < (int64_t)1 << 31, "cache: strides of rows and heads must be below 2^31");
     const int64_t slots = (a.max_rows + 62) / 64 + 1;
     // a launch has less than 2^32 threads
     BA_REQUIRE(slots <= ((int64_t)1 << 23) / a.n_seqs / a.heads - 1, "cache: too many blocks for a call (max_rows is the bound that counts)");
