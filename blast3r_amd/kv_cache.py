@@ -81,7 +81,8 @@ class KVCache:
     def _fill(self, a, pages, firsts, name, offsets, n_rows, max_rows):
         """The fields of a call that the arguments of every call give."""
         dev = self.device
-        if pages.dim() != 2 or pages.dtype is not torch.int32 or pages.device != dev or pages.stride(1) != 1:
+        if (pages.dim() != 2 or pages.dtype is not torch.int32 or pages.device != dev or
+                pages.stride(1) != 1 and pages.shape[0] > 0 and pages.shape[1] > 1):
             raise ValueError(f'cache: pages must be (n_seqs, blocks) int32 on {dev} with contiguous rows')
         S, a.n_pages = pages.shape
         a.n_seqs, a.pages, a.pages_stride = S, pages.data_ptr(), pages.stride(0)
@@ -117,6 +118,8 @@ class KVCache:
         """Write the rows of k and v (tokens, heads, head_dim; fp32, fp16 or bf16) after the first ``lengths`` (n_seqs,)
         int32 tokens of their sequences.  ``lengths`` stays as it is.  No two sequences of a call may append to the
         same block."""
+        if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+            raise RuntimeError('cache: codes carry no gradient: append under torch.no_grad()')
         a = BaKvArgs.from_buffer_copy(self._args)
         a.rk_st, a.rk_sh = self._rows(k, 'k', self.heads)
         a.rv_st, a.rv_sh = self._rows(v, 'v', self.heads)
@@ -161,6 +164,8 @@ class KVCache:
         A row that sees no token gives zeros.  q_heads is a multiple of the cache's heads; query head h reads cache
         head h // (q_heads // heads).  With ``return_lse`` also log(sum(exp(scale q k^T))) as (tokens, q_heads) fp32,
         -inf where no token is seen, with which results over different tokens can be joined."""
+        if q.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError('cache: attention over codes has no gradient: call it under torch.no_grad()')
         shape = q.shape
         if len(shape) != 3 or shape[1] % self.heads or shape[1] == 0:
             raise ValueError(f'cache: q must be (tokens, a multiple of {self.heads} heads, {self.head_dim}), got {tuple(shape)}')

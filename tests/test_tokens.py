@@ -450,6 +450,11 @@ ATTEND = [
     (256, 2, 1, [650], [1], True, None),
     (32, 1, 16, [4000], [1], True, None),
     (64, 1, 1, [3000], [1], True, 700),
+    (256, 1, 4, [300], [6], True, None),                           # 24 rows of the largest head
+    (32, 1, 5, [1500], [6], False, None),
+    (96, 2, 3, [190, 2500], [70, 1], True, None),                  # 210 rows, and one token that shares their call
+    (64, 2, 1, [70, 0, 1, 2100], [70, 0, 1, 300], True, 200),      # sequences without rows or tokens among others
+    (128, 1, 2, [1300], [200], True, 500),
 ]
 
 
@@ -500,10 +505,54 @@ def test_attend_ranges(bits, counts):
     o = _mirror(c, bits)
     _check(c, o, q, pages, [n], counts, window=64 * 10)
     _check(c, o, q, pages, [n], counts)
+    c.scales[int(pages[0, 19]), 0] = torch.tensor([1.0, math.nan], device=DEV)      # its values: rows that see it in part or not
+    o = _mirror(c, bits)
+    _check(c, o, q, pages, [n], counts, window=64 * 10)
     q = q.clone()
     q[0, 1, 5] = math.nan
     o2 = _mirror(c, bits)
     _check(c, o2, q, pages, [64 * 19], counts, window=64 * 12)
+
+
+@pytest.mark.gpu
+def test_attend_bounds():
+    """max_new below a sequence's rows leaves the others as they are; lengths past the block list and below zero, offsets
+    out of order and a cache without blocks stay inside the buffers."""
+    from blast3r_amd.kv_cache import KVCache
+    rng = np.random.default_rng(4)
+    c, o = _cache(8, 2, 64, 'fp8')
+    pages = _pages(rng, [4, 4], 8, 4)
+    x = torch.tensor(rng.normal(size=(300, 2, 64)), dtype=torch.float32, device=DEV).bfloat16()
+    print('attend bounds', flush=True)
+    for n, most in ((10, 7), (150, 40)):
+        off, lens = _i32([0, n, n + 3]), [200, 100]
+        y = torch.full_like(x[:n + 3], 7.0)
+        c.attend(x[:n + 3], _i32(pages), _i32(lens), offsets=off, max_new=most, out=y)
+        want, _, size = otok.attend(o, _np(x[:n + 3]), pages, lens, [n, 3], 0.125)
+        done = np.r_[0:most, n:n + 3]
+        assert np.all(np.abs(_np(y) - want)[done] <= 1.2e-3 * size[done] + 2.0 ** -8 * np.abs(want[done]))
+        rest = _np(y)[most:n]                               # up to a tile of them may be done all the same
+        assert np.all((rest == 7.0) | (np.abs(rest - want[most:n]) <= 1.2e-3 * size[most:n] + 2.0 ** -8 * np.abs(want[most:n])))
+    # 256 tokens is all that four blocks hold
+    got = c.attend(x[:2], _i32(pages), _i32([100000, -5]))
+    want, _, size = otok.attend(o, _np(x[:2]), pages, [256, 0], [1, 1], 0.125)
+    assert np.all(np.abs(_np(got) - want) <= 1.2e-3 * size + 2.0 ** -8 * np.abs(want)) and not got[1].any()
+    y = torch.full_like(x[:6], 7.0)
+    c.attend(x[:6], _i32(pages), _i32([50, 60]), offsets=_i32([9, -2, 4]), out=y)
+    assert bool((y == 7.0).all())
+    none = KVCache(0, 2, 64, device=DEV)
+    for n in (2, 40, 400):
+        q = x[:1].expand(n, 2, 64)
+        got, lse = none.attend(q, _i32(np.zeros((2, 3))), _i32([150, 20]), return_lse=True)
+        assert not got.any() and bool((lse == -math.inf).all())
+        assert not none.attend(q, _i32(np.zeros((2, 0))), _i32([150, 20])).any()
+    none.append(x[:2], x[:2], _i32(np.zeros((2, 3))), _i32([0, 64]))
+    assert not none.read(_i32(np.zeros((2, 3))), _i32([0, 64]), None, 4)[0].any()
+    assert c.attend(x[:0], _i32(np.zeros((0, 3))), _i32([])).shape == (0, 2, 64)
+    with pytest.raises(RuntimeError):
+        c.attend(x[:2].requires_grad_(), _i32(pages), _i32([5, 6]))
+    with pytest.raises(RuntimeError):
+        c.append(x[:2].clone().requires_grad_(), x[:2], _i32(pages), _i32([5, 6]))
 
 
 @pytest.mark.gpu
