@@ -649,3 +649,20 @@ def test_tokens_in_a_graph_and_on_a_side_stream():
         lens += 1
     for c in caches[1:]:
         assert torch.equal(c.k.view(torch.uint8), caches[0].k.view(torch.uint8)) and torch.equal(c.scales, caches[0].scales)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits,bar', [('fp8', 0.13), ('int8', 0.04)])
+def test_example_of_online_frames(bits, bar):
+    """examples/online_frames.py: rotary, append, attend over chosen frames and depth sampling together.  Attention over
+    codes against attention over the unrounded keys and values: e4m3 is off by at most 2^-4 of a value (twice: keys through
+    the weights, values), int8 by half of 1/127 of a block's largest value, about 2% of a value of ordinary size."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'examples', 'online_frames.py')
+    spec = importlib.util.spec_from_file_location('online_frames', path)
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    error, depths, net = ex.run(frames=4, layers=2, width=512, heads=8, like=2, bits=BITS[bits], device=DEV)
+    assert 0.0 < error < bar
+    assert depths.shape == (1000, 6) and bool(torch.isfinite(depths).all())
