@@ -45,7 +45,6 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16 __attribute__((ext_vector_type(16)));
 
 #define AT_T 256
-#define AT_WAVES 4
 #define AT_MIN_BLOCKS 16     // a part has at least so many blocks: below that a second launch costs more than it saves
 
 template <int COLS> struct Mma;
@@ -112,15 +111,15 @@ struct AtBlocks {
     int lo, hi, per;
 };
 
-__device__ __forceinline__ AtBlocks at_blocks(const ba_kv_attend_args& a, const AtSeq& q, int group, int64_t row, int rows) {
-    const int64_t all = (int64_t)q.rows * group, last = row + rows < all ? row + rows : all;
+__device__ __forceinline__ AtBlocks at_blocks(const ba_kv_attend_args& a, const AtSeq& q, int group, int row, int rows) {
+    const int all = q.rows * group, last = row + rows < all ? row + rows : all;
     if (row >= last) return {0, 0, 1};
-    const int64_t p0 = (int64_t)q.len - q.n + row / group, p1 = (int64_t)q.len - q.n + (last - 1) / group;
-    const int64_t keys = a.causal ? p1 + 1 : (int64_t)q.len;
-    int64_t first = a.window > 0 ? p0 - a.window + 1 : 0;
-    if (first < 0) first = 0;
+    const int p0 = q.len - q.n + (int)((unsigned)row / (unsigned)group), p1 = q.len - q.n + (int)((unsigned)(last - 1) / (unsigned)group);
+    const int keys = a.causal ? p1 + 1 : q.len;
+    const int64_t from = a.window > 0 ? p0 - a.window + 1 : 0;
+    const int first = from < 0 ? 0 : from < q.len ? (int)from : q.len;
     if (keys <= first) return {0, 0, 1};
-    const int b0 = (int)(first / 64), b1 = (int)((keys + 63) / 64), per = (b1 - b0 + a.n_splits - 1) / a.n_splits;
+    const int b0 = first / 64, b1 = (keys + 63) / 64, per = (b1 - b0 + a.n_splits - 1) / a.n_splits;
     return {b0, b1, per < AT_MIN_BLOCKS ? AT_MIN_BLOCKS : per};
 }
 
@@ -162,15 +161,15 @@ __device__ __forceinline__ void store_out4(const ba_kv_attend_args& a, int64_t r
 // row n that pair with its pieces of a key) divided by a power of two of the row, and the constant that a score is
 // multiplied by before the key factor: softmax scale, log2(e) and that power.
 template <int D, int COLS, int NCB>
-__device__ __forceinline__ void load_queries(const ba_kv_attend_args& a, const AtSeq& q, int kh, int group, int64_t row0, int64_t all,
+__device__ __forceinline__ void load_queries(const ba_kv_attend_args& a, const AtSeq& q, int kh, int group, int row0, int all,
                                              int n, int g, bool wide, h8 (&qf)[NCB][D * COLS / 512], float (&qc)[NCB], int (&pos)[NCB]) {
     constexpr int NG = 64 / COLS, KS = D / (8 * NG);
 #pragma unroll
     for (int c = 0; c < NCB; ++c) {
-        const int64_t r = row0 + c * COLS + n, rc = r < all ? r : all - 1;
-        const int64_t i = rc / group;
-        const int head = kh * group + (int)(rc - i * group);
-        pos[c] = q.len - q.n + (int)i;
+        const int r = row0 + c * COLS + n, rc = r < all ? r : all - 1;
+        const int i = (int)((unsigned)rc / (unsigned)group);
+        const int head = kh * group + rc - i * group;
+        pos[c] = q.len - q.n + i;
         float x[KS][8];
         uint32_t top = 0;
         const int64_t at = (q.row0 + i) * a.q_st + head * a.q_sh + g * (D / NG);
@@ -203,16 +202,17 @@ __device__ __forceinline__ void load_queries(const ba_kv_attend_args& a, const A
 
 // The result of a wave's rows, or their partial sums.
 template <int D, int COLS, int NCB, typename A>
-__device__ __forceinline__ void store_rows(const ba_kv_attend_args& a, const AtSeq& q, int kh, int group, int64_t row0, int64_t all, int sp,
+__device__ __forceinline__ void store_rows(const ba_kv_attend_args& a, const AtSeq& q, int kh, int group, int row0, int all, int sp,
                                            int n, int g, bool wide, const A (&o)[NCB][D / COLS], const float (&m)[NCB], const float (&l)[NCB]) {
     constexpr int CREG = COLS * COLS / 64, DB = D / COLS;
     typedef Mma<COLS> M;
 #pragma unroll
     for (int c = 0; c < NCB; ++c) {
-        const int64_t r = row0 + c * COLS + n;
+        const int r = row0 + c * COLS + n;
         if (r >= all) continue;
-        const int64_t i = r / group, row = q.row0 + i;
-        const int head = kh * group + (int)(r - i * group);
+        const int i = (int)((unsigned)r / (unsigned)group);
+        const int64_t row = q.row0 + i;
+        const int head = kh * group + r - i * group;
         if (a.n_splits > 1) {
             float* w = part_sum(a, row, head, sp);
 #pragma unroll
@@ -238,15 +238,15 @@ __device__ __forceinline__ void store_rows(const ba_kv_attend_args& a, const AtS
 // waves of a SIMD that the registers are to leave room for
 constexpr int at_waves(int d, int cols) { return cols == 16 ? (d <= 64 ? 4 : d <= 128 ? 2 : 1) : d <= 128 ? 2 : 1; }
 
-// Few rows: the four waves have the same COLS rows and split the blocks; every wave reads and converts its own.
+// Few rows: the waves have the same COLS rows and split the blocks; every wave reads and converts its own.
 template <int D, int KT, int COLS>
 __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_attend_args a, int n_tiles, int wide) {
     typedef Mma<COLS> M;
     typedef typename M::acc acc;
     constexpr int NG = 64 / COLS, NB = NG, CREG = COLS * COLS / 64, TPL = 64 / NG;
-    constexpr int KS = D / (8 * NG), DB = D / COLS, PS = TPL / 8, WK = AT_WAVES, NCB = 1, ROWS = COLS;
-    __shared__ float2 ref_sh[AT_WAVES * COLS * NCB];
-    __shared__ f4 sum_sh[2 * COLS * NCB * D / 4];
+    constexpr int KS = D / (8 * NG), DB = D / COLS, PS = TPL / 8, WAVES = AT_T / 64, WK = WAVES, NCB = 1, ROWS = COLS;
+    __shared__ float2 ref_sh[WAVES * COLS * NCB];
+    __shared__ f4 sum_sh[WAVES / 2 * COLS * NCB * D / 4];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = wave;
     const int n = lane % COLS, g = lane / COLS;
@@ -258,38 +258,13 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_att
     const int kh = (int)(id % (unsigned)a.heads), s = (int)(id / (unsigned)a.heads);
     const int group = a.q_heads / a.heads;
     const AtSeq q = at_seq(a, s);
-    const int64_t all = (int64_t)q.rows * group, tile0 = (int64_t)tile * ROWS;
+    const int all = q.rows * group, tile0 = tile * ROWS;
     if (tile0 >= all) return;
     int lo, hi;
     at_part(at_blocks(a, q, group, tile0, ROWS), sp, lo, hi);
     if (lo >= hi && a.n_splits > 1) return;                  // k_kv_join knows which parts there are
 
-    h8 qf[NCB][KS];
-    float qc[NCB];
-    int pos[NCB];
-    load_queries<D, COLS, NCB>(a, q, kh, group, tile0, all, n, g, wide != 0, qf, qc, pos);
-    // tokens [whole_lo, whole_hi) are seen by all rows of the wave: their blocks need no comparisons
-    const int64_t last = tile0 + ROWS < all ? tile0 + ROWS : all;
-    const int pmin = q.len - q.n + (int)(tile0 / group), pmax = q.len - q.n + (int)((last - 1) / group);
-    const int64_t window = a.window > 0 ? a.window : (int64_t)1 << 40;
-    const int whole_hi = a.causal ? pmin + 1 : q.len;
-    const int whole_lo = pmax - window + 1 > 0 ? (int)(pmax - window + 1) : 0;
     if (a.n_blocks == 0) hi = lo;
-
-    acc o[NCB][DB];
-    // weights are exp2(z + lv - m + AT_LIFT); `move`: an exponent above it moves m (any does in a row that has no m yet)
-    float m[NCB], l[NCB], move[NCB];
-#pragma unroll
-    for (int c = 0; c < NCB; ++c) {
-        m[c] = 0.0f;
-        l[c] = 0.0f;
-        move[c] = -3.0e38f;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int r = 0; r < CREG; ++r) o[c][d][r] = 0.0f;
-    }
-
     const int32_t* pages = a.pages + (int64_t)s * a.pages_stride;
     const uint8_t* kb = (const uint8_t*)a.k + (int64_t)kh * 64 * D;
     const uint8_t* vb = (const uint8_t*)a.v + (int64_t)kh * 64 * D;
@@ -334,6 +309,7 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_att
         }
     };
 
+    // the first block is under way before the queries are
     int blk = lo + wk;
     int page = page_of(blk), next = page_of(blk + WK);
     float2 f = make_float2(1.0f, 1.0f);
@@ -342,6 +318,31 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_att
         load_keys(page);
         load_values(page);
     }
+    h8 qf[NCB][KS];
+    float qc[NCB];
+    int pos[NCB];
+    load_queries<D, COLS, NCB>(a, q, kh, group, tile0, all, n, g, wide != 0, qf, qc, pos);
+    // tokens [whole_lo, whole_hi) are seen by all rows of the wave: their blocks need no comparisons
+    const int last = tile0 + ROWS < all ? tile0 + ROWS : all;
+    const int pmin = q.len - q.n + (int)((unsigned)tile0 / (unsigned)group), pmax = q.len - q.n + (int)((unsigned)(last - 1) / (unsigned)group);
+    const int64_t window = a.window > 0 ? a.window : (int64_t)1 << 40;
+    const int whole_hi = a.causal ? pmin + 1 : q.len;
+    const int whole_lo = pmax - window + 1 > 0 ? (int)(pmax - window + 1) : 0;
+
+    acc o[NCB][DB];
+    // weights are exp2(z + lv - m + AT_LIFT); `move`: an exponent above it moves m (any does in a row that has no m yet)
+    float m[NCB], l[NCB], move[NCB];
+#pragma unroll
+    for (int c = 0; c < NCB; ++c) {
+        m[c] = 0.0f;
+        l[c] = 0.0f;
+        move[c] = -3.0e38f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < CREG; ++r) o[c][d][r] = 0.0f;
+    }
+
     for (; blk < hi; blk += WK) {
         const int after = page_of(blk + 2 * WK);
         const float2 fn = factors(next);
@@ -477,10 +478,10 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_att
         __syncthreads();
 #pragma unroll
         for (int c = 0; c < NCB; ++c) {
-            float2 r[AT_WAVES];
+            float2 r[WAVES];
             float top = AT_NONE;
 #pragma unroll
-            for (int w = 0; w < AT_WAVES; ++w) {
+            for (int w = 0; w < WAVES; ++w) {
                 r[w] = ref_sh[w * COLS * NCB + c * COLS + n];
                 top = fmaxf(top, r[w].x);
             }
@@ -488,7 +489,7 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_att
             m[c] = top;
             l[c] = 0.0f;
 #pragma unroll
-            for (int w = 0; w < AT_WAVES; ++w) l[c] = fmaf(r[w].y, __builtin_amdgcn_exp2f(r[w].x - top), l[c]);
+            for (int w = 0; w < WAVES; ++w) l[c] = fmaf(r[w].y, __builtin_amdgcn_exp2f(r[w].x - top), l[c]);
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -516,14 +517,14 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_att
                         for (int k = 0; k < 4; ++k) o[c][d][r + k] += x[k];
                     }
         };
-        if (wk >= 2) put(wk - 2);
-        __syncthreads();
-        if (wk < 2) add(wk);
-        __syncthreads();
-        if (wk == 1) put(0);
-        __syncthreads();
+#pragma unroll
+        for (int w = WAVES / 2; w > 0; w /= 2) {             // halves: the upper waves' sums to the lower ones
+            if (wk >= w && wk < 2 * w) put(wk - w);
+            __syncthreads();
+            if (wk < w) add(wk);
+            if (w > 1) __syncthreads();
+        }
         if (wk != 0) return;
-        add(0);
     }
 
     store_rows<D, COLS, NCB>(a, q, kh, group, tile0, all, sp, n, g, wide != 0, o, m, l);
@@ -552,21 +553,21 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
     const int kh = (int)(id % (unsigned)a.heads), s = (int)(id / (unsigned)a.heads);
     const int group = a.q_heads / a.heads;
     const AtSeq q = at_seq(a, s);
-    const int64_t all = (int64_t)q.rows * group, tile0 = (int64_t)tile * ROWS;
+    const int all = q.rows * group, tile0 = tile * ROWS;
     if (tile0 >= all) return;
     int lo, hi;
     at_part(at_blocks(a, q, group, tile0, ROWS), sp, lo, hi);
     if (lo >= hi && a.n_splits > 1) return;                  // k_kv_join knows which parts there are
     if (a.n_blocks == 0) hi = lo;
 
-    const int64_t row0 = tile0 + wave * 32 * NCB;
+    const int row0 = tile0 + wave * 32 * NCB;
     h8 qf[NCB][KS];
     float qc[NCB];
     int pos[NCB];
     load_queries<D, 32, NCB>(a, q, kh, group, row0, all, n, g, wide != 0, qf, qc, pos);
     // tokens [whole_lo, whole_hi) are seen by all rows of the wave: their blocks need no comparisons
-    const int64_t first = row0 < all ? row0 : all - 1, last = row0 + 32 * NCB < all ? row0 + 32 * NCB : all;
-    const int pmin = q.len - q.n + (int)(first / group), pmax = q.len - q.n + (int)((last - 1) / group);
+    const int first = row0 < all ? row0 : all - 1, last = row0 + 32 * NCB < all ? row0 + 32 * NCB : all;
+    const int pmin = q.len - q.n + (int)((unsigned)first / (unsigned)group), pmax = q.len - q.n + (int)((unsigned)(last - 1) / (unsigned)group);
     const int64_t window = a.window > 0 ? a.window : (int64_t)1 << 40;
     const int whole_hi = a.causal ? pmin + 1 : q.len;
     const int whole_lo = pmax - window + 1 > 0 ? (int)(pmax - window + 1) : 0;
@@ -703,7 +704,7 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
     // products of the present one (exponents t, values v at half vb2, factors f).  The matrix unit takes a product every
     // 32 clocks; vector instructions stand between them in the order that the fences keep.  Operands are read AHEAD
     // products ahead, with `carry` through the end of the half into the second half of k, the next one's keys.
-    constexpr int AHEAD = D == 32 ? 2 : 4, READS = KS + 2 * DB, STEPS = 2 * DB;
+    constexpr int AHEAD = D == 32 ? 2 : 4, READS = KS + 2 * DB, STEPS = 2 * DB * NCB;
     h8 ring[AHEAD];
     auto key = [&](const h8* k, int b, int x) { return k[(b * KS + x) * 64 + (k_lane ^ (x / 2 << SWZ_T))]; };
     auto half = [&](acc (&t)[NCB], acc (&tn)[NCB], const h8* k, int kb2, const h8* v, int vb2, float2 f, float2 fn, auto carry, auto extra) {
@@ -735,10 +736,13 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
 #pragma unroll
         for (int x = 0; x < KS; ++x) {
 #pragma unroll
-            for (int c = 0; c < NCB; ++c) tn[c] = M::run(ring[x % AHEAD], qf[c][x], tn[c]);
-            read(x + AHEAD);
-            weigh(x * PAIRS / KS, (x + 1) * PAIRS / KS);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int c = 0; c < NCB; ++c) {                  // a product's 32 clocks are the next pairs' time
+                const int i = x * NCB + c;
+                tn[c] = M::run(ring[x % AHEAD], qf[c][x], tn[c]);
+                if (c == NCB - 1) read(x + AHEAD);
+                weigh(i * PAIRS / (KS * NCB), (i + 1) * PAIRS / (KS * NCB));
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         // weights that fp16 could not hold show in their sum: no maximum is formed until then
         bool big = false;
@@ -763,13 +767,16 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
             off[c] = lv - m[c] + AT_LIFT;
         }
 #pragma unroll
-        for (int x = 0; x < STEPS; ++x) {
+        for (int x = 0; x < 2 * DB; ++x) {
 #pragma unroll
-            for (int c = 0; c < NCB; ++c) o[c][x % DB] = M::run(ring[(KS + x) % AHEAD], pf[c][x / DB], o[c][x % DB]);
-            read(KS + x + AHEAD);
-            extra(x);
-            if (x > 0) exponents(tn, cz, off, (x - 1) * EL / (STEPS - 1), x * EL / (STEPS - 1));
-            __builtin_amdgcn_sched_barrier(0);
+            for (int c = 0; c < NCB; ++c) {
+                const int i = x * NCB + c;
+                o[c][x % DB] = M::run(ring[(KS + x) % AHEAD], pf[c][x / DB], o[c][x % DB]);
+                if (c == NCB - 1) read(KS + x + AHEAD);
+                extra(i);
+                if (i > 0) exponents(tn, cz, off, (i - 1) * EL / (STEPS - 1), i * EL / (STEPS - 1));
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     };
     auto preload = [&](const h8* k, int b) {
@@ -871,7 +878,7 @@ __global__ void __launch_bounds__(AT_T) k_kv_join(ba_kv_attend_args a, int tile_
         const int group = a.q_heads / a.heads;
         covered = i >= 0 && i < q.rows;
         if (covered) {
-            const int64_t r = i * group + head % group;
+            const int r = (int)i * group + head % group;
             const AtBlocks b = at_blocks(a, q, group, r / tile_rows * tile_rows, tile_rows);
             n = (b.hi - b.lo + b.per - 1) / b.per;
             for (int p = lane; p < n; p += lanes) top = fmaxf(top, part_ref(a, row, head, p)->x);
@@ -977,6 +984,7 @@ extern "C" int ba_kv_attend(const ba_kv_attend_args* args, void* stream) {
     const int64_t rows = a.max_rows * group;
     const AtShape v = at_shape(rows, a.dim);
     const int tile = v.rows;
+    BA_REQUIRE(rows < ((int64_t)1 << 31) - 256, "attention: too many rows for a call");
     const int64_t tiles = (rows + tile - 1) / tile;
     // a launch has less than 2^32 threads
     BA_REQUIRE(tiles <= ((int64_t)1 << 23) / a.n_seqs / a.heads / a.n_splits, "attention: too many tiles for a call (max_rows is the bound that counts)");
