@@ -116,6 +116,19 @@ __device__ __forceinline__ void load_row(const T* p, bool wide, float (&v)[V]) {
     }
 }
 
+// the codes of a values block into the tile
+template <int D>
+__device__ __forceinline__ void load_tile(const uint8_t* base, uint32_t* tile) {
+#pragma unroll
+    for (int i = 0; i < (4 * D + KV_T - 1) / KV_T; ++i) {
+        const int q = threadIdx.x + i * KV_T;
+        if (4 * D % KV_T != 0 && q >= 4 * D) break;
+        const uint4 w = ((const uint4*)base)[q];
+        uint32_t* t = tile + q / 4 * (KV_ROW / 4) + q % 4 * 4;
+        t[0] = w.x; t[1] = w.y; t[2] = w.z; t[3] = w.w;
+    }
+}
+
 // KEYS: a thread takes 8 elements of a token (UNITS times); values: 4 elements of 4 tokens.
 template <int D, int KT, typename T, bool KEYS>
 __device__ void kv_write_block(const ba_kv_args& a, const KvShare& sh, int h, bool wide, uint32_t* tile, uint32_t* red) {
@@ -213,7 +226,7 @@ __device__ void kv_write_block(const ba_kv_args& a, const KvShare& sh, int h, bo
     // through the tile: row d has the 64 tokens of element d
     const bool whole = sh.at == 0 && sh.n == 64;
     if (!whole) {
-        for (int q = tid; q < D * 16; q += KV_T) tile[q / 16 * (KV_ROW / 4) + q % 16] = ((const uint32_t*)base)[q];
+        load_tile<D>(base, tile);
         __syncthreads();
     }
 #pragma unroll
@@ -231,10 +244,13 @@ __device__ void kv_write_block(const ba_kv_args& a, const KvShare& sh, int h, bo
         }
     }
     __syncthreads();
-    for (int q = tid; q < D * 16; q += KV_T) {
-        uint32_t w = tile[q / 16 * (KV_ROW / 4) + q % 16];
-        if (again) w = kv_recode4<KT>(w, ratio, sh.at - q % 16 * 4);
-        ((uint32_t*)base)[q] = w;
+    for (int q = tid; q < D * 4; q += KV_T) {
+        const uint32_t* t = tile + q / 4 * (KV_ROW / 4) + q % 4 * 4;
+        uint32_t w[4] = {t[0], t[1], t[2], t[3]};
+        if (again)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = kv_recode4<KT>(w[j], ratio, sh.at - (q % 4 * 16 + 4 * j));
+        ((uint4*)base)[q] = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -282,38 +298,59 @@ __global__ void __launch_bounds__(KV_T) k_kv_read(ba_kv_args a, int slots, int w
     y += sh.row * st;
     const uint8_t* base = (const uint8_t*)(keys ? a.k : a.v) + (sh.page * a.heads + h) * (int64_t)(64 * D);
     const float f = a.scales[(sh.page * a.heads + h) * 2 + (keys ? 0 : 1)];
-    auto store4 = [&](T* p, const float (&v)[4]) {
+    // W elements to a store of 16 bytes where there is work for all threads
+    constexpr int W = sizeof(T) == 2 ? 8 : 4, WV = D >= 128 ? W : 4;
+    auto store = [&](T* p, const auto& v) {
+        constexpr int N = sizeof(v) / sizeof(float);
         if (wide) {
-            store_vec<T, 4>(p, v);
+            store_vec<T, N>(p, v);
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = (T)v[j];
+            for (int j = 0; j < N; ++j) p[j] = (T)v[j];
         }
     };
     if (keys) {
-        for (int q = tid; q < sh.n * (D / 4); q += KV_T) {
-            float v[4];
-            kv_values4<KT>(((const uint32_t*)base)[sh.at * (D / 4) + q], v);
+        constexpr int UNITS = (64 * (D / W) + KV_T - 1) / KV_T;
+        uint32_t w[UNITS][W / 4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] *= f;
-            store4(y + (int64_t)(q / (D / 4)) * st + q % (D / 4) * 4, v);
+        for (int i = 0; i < UNITS; ++i) {                    // all loads before the first store
+            const int q = tid + i * KV_T;
+            if (q >= sh.n * (D / W)) break;
+#pragma unroll
+            for (int j = 0; j < W / 4; ++j) w[i][j] = ((const uint32_t*)base)[(sh.at * (D / W) + q) * (W / 4) + j];
+        }
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i) {
+            const int q = tid + i * KV_T;
+            if (q >= sh.n * (D / W)) break;
+            float v[W];
+#pragma unroll
+            for (int j = 0; j < W; j += 4) {
+                float x[4];
+                kv_values4<KT>(w[i][j / 4], x);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[j + k] = x[k] * f;
+            }
+            store(y + (int64_t)(q / (D / W)) * st + q % (D / W) * W, v);
         }
         return;
     }
-    for (int q = tid; q < D * 16; q += KV_T) tile[q / 16 * (KV_ROW / 4) + q % 16] = ((const uint32_t*)base)[q];
+    load_tile<D>(base, tile);
     __syncthreads();
-    for (int u = tid; u < 16 * (D / 4); u += KV_T) {         // 4 elements of 4 tokens
-        const int e = u % (D / 4) * 4, place = u / (D / 4) * 4;
+    for (int u = tid; u < 16 * (D / WV); u += KV_T) {        // WV elements of 4 tokens
+        const int e = u % (D / WV) * WV, place = u / (D / WV) * 4;
         if (place + 4 <= sh.at || place >= sh.at + sh.n) continue;
-        float v[4][4];
+        float v[WV][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) kv_values4<KT>(tile[(e + j) * (KV_ROW / 4) + place / 4], v[j]);
+        for (int j = 0; j < WV; ++j) kv_values4<KT>(tile[(e + j) * (KV_ROW / 4) + place / 4], v[j]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int t = place + r - sh.at;
             if (t < 0 || t >= sh.n) continue;
-            const float o[4] = {v[0][r] * f, v[1][r] * f, v[2][r] * f, v[3][r] * f};
-            store4(y + (int64_t)t * st + e, o);
+            float o[WV];
+#pragma unroll
+            for (int j = 0; j < WV; ++j) o[j] = v[j][r] * f;
+            store(y + (int64_t)t * st + e, o);
         }
     }
 }
@@ -321,10 +358,9 @@ __global__ void __launch_bounds__(KV_T) k_kv_read(ba_kv_args a, int slots, int w
 template <int D, int KT, typename T>
 static int launch_kv(const ba_kv_args& a, bool write, int slots, unsigned nb, hipStream_t st) {
     const int64_t s[4] = {a.rk_st, a.rk_sh, a.rv_st, a.rv_sh};
-    // a thread's loads are 8 keys and 4 values, its stores 4 of each
-    const int kb = (write ? 8 : 4) * (int)sizeof(T), vb = 4 * (int)sizeof(T);
-    bool wide = (uintptr_t)a.rk % (kb > 16 ? 16 : kb) == 0 && (uintptr_t)a.rv % vb == 0;
-    for (int i = 0; i < 4; ++i) wide = wide && s[i] % (i < 2 && write ? 8 : 4) == 0;
+    // a thread moves 8 elements at a time at most
+    bool wide = (uintptr_t)a.rk % 16 == 0 && (uintptr_t)a.rv % 16 == 0;
+    for (int i = 0; i < 4; ++i) wide = wide && s[i] % 8 == 0;
     if (write) hipLaunchKernelGGL((k_kv_write<D, KT, T>), dim3(nb), dim3(KV_T), 0, st, a, slots, (int)wide);
     else hipLaunchKernelGGL((k_kv_read<D, KT, T>), dim3(nb), dim3(KV_T), 0, st, a, slots, (int)wide);
     BA_LAUNCHED();
