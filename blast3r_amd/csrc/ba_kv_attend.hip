@@ -3,30 +3,37 @@
 // For a row of queries q and the keys j that it sees,  o = sum_j p_j v_j / sum_j p_j,  p_j = exp(c q.k_j - m):
 // one pass over the cache with a running reference m, so that the scores never leave the registers.
 //
-// A wave takes a tile of query rows (rows that share a cache head: the tokens of a sequence times the query
-// heads of that cache head) and walks over blocks of 64 tokens.  The block's bytes go from memory to
-// registers in the layout that the matrix instructions want, without LDS:
-//   scores   S^T = K Q^T: lane (n, g) of COLS x NG holds, of every key block b, 8-element pieces of a key row;
-//            which token a key row of the product stands for is free, and is chosen so that
-//   products O^T = V^T P^T: the lane's results S are those of 64 / NG consecutive tokens for query column n,
-//            which is the layout of the second operand (P) as it stands, and the values, kept as (dim, 64),
-//            are read as consecutive bytes of a row.
-// COLS = 16 (16 x 16 x 32 products) is for at most 16 rows, COLS = 32 (32 x 32 x 16) for more, with NCB tiles
-// of 32 rows to a wave.  Codes become fp16, which holds each of them exactly; queries are scaled by a power of
-// two of their row to fp16, exactly for bf16 and fp16 queries up to 2^-28 of the row's largest element; sums
-// are fp32.
+// Rows of a wave are query rows that share a cache head (the tokens of a sequence times the query heads of that
+// cache head); it walks over blocks of 64 tokens with two matrix products each, laid out so that the weights
+// never change lanes:
+//   scores   S^T = K Q^T: lane (n, g) of COLS x NG holds 8-element pieces of key rows and of query row n.  Which
+//            token a key row of the product stands for is free, and is chosen so that
+//   products O^T = V^T P^T: the lane's scores are those of 64 / NG consecutive tokens for query row n, which is
+//            the layout of this product's second operand (P) as it stands; the values, kept as (dim, 64), are
+//            consecutive bytes.
+// Codes become fp16, which holds each of them exactly (bf16 would too, but has 8 bits for the weights); queries
+// are scaled by a power of two of their row to fp16, exactly for bf16 and fp16 queries down to 2^-28 of the
+// row's largest element; sums are fp32.
 //
 // Factors: a block's key factor goes into the constant c, its value factor into the exponent: with z = c q.k
 // and lv = log2(value factor), m follows z + lv, so that the weights exp2(z + lv - m) that meet the codes of
-// the values are at most 2^14 whatever the factors are, and the denominator adds their sums divided by the
-// value factor.  The weights of a block whose values are small beside others' may vanish in fp16 and still
-// make up the denominator, so that is summed in fp32 before the weights are rounded to fp16 (11 bits, at the
-// precision of the outputs or beyond).  m is moved only when a score passes it by 2^8; until then the products
-// need no rescaling.
+// the values fit fp16 whatever the factors are, and the denominator adds their sums divided by the value
+// factor.  The weights of a block whose values are small beside others' may vanish in fp16 and still make up
+// the denominator, so that is summed in fp32 before the weights are rounded to fp16 (11 bits, at the precision
+// of the outputs or beyond).  m is moved only when a weight nears fp16's end; until then nothing is rescaled.
 //
-// The waves of a workgroup share rows and split the blocks (few rows; joined through LDS), or share the
-// blocks and split the rows.  With few rows in all the blocks of a sequence are further cut into n_splits
-// parts, whose sums k_kv_join adds in order.
+// Two kernels:
+//   k_kv_attend       up to 32 rows: the waves of a workgroup have the same rows and split the blocks, codes go
+//                     from memory to registers without LDS, and the waves' sums are joined at the end.  Bound by
+//                     memory: a query over 192000 tokens of 16 heads of 64 (393 MB) takes 70 us, 5.6 TB/s; 48
+//                     sequences of up to 8192 tokens, 8 heads of 128 (417 MB), 89 us, 4.7 TB/s (a large copy: 4.8).
+//   k_kv_attend_tile  more rows: the waves split the rows and share blocks that are converted to fp16 once, in LDS.
+//                     Bound by the vector and matrix units together, and by power (the clock falls to 2.0 - 2.2
+//                     GHz): 2 x 2048 rows over 16384 tokens, 32 heads of 128: 1030 us, 1.0 PFLOP/s (a large fp16
+//                     matrix product on this card: 1.09); of 64: 564 us, 0.92 PFLOP/s, where the exponentials alone
+//                     take as long as half of the products.
+// Where rows are few the blocks of a sequence are further cut into n_splits parts, whose sums k_kv_join adds in
+// order (5 us for 16 rows of 24 parts, 10 us for 12288 rows of 10).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -45,7 +52,8 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16 __attribute__((ext_vector_type(16)));
 
 #define AT_T 256
-#define AT_MIN_BLOCKS 16     // a part has at least so many blocks: below that a second launch costs more than it saves
+#define AT_MIN_BLOCKS 16     // a part has at least so many blocks: below that the join costs more than it saves (a query over
+                             // 777 tokens 12 us in one part, 18 in two; over 8192 tokens 18.5 in 8 parts, 17.8 in 16)
 
 template <int COLS> struct Mma;
 template <> struct Mma<16> {
@@ -153,9 +161,9 @@ __device__ __forceinline__ void store_out4(const ba_kv_attend_args& a, int64_t r
 }
 
 #define AT_NONE -1.0e30f      // reference of a row that has seen no key
-#define AT_MOVE 8.0f          // m is moved when a score passes it by so much (log2)
+#define AT_MOVE 8.0f          // k_kv_attend moves m when a score passes it by so much (log2)
 #define AT_LIFT 6.0f          // weights at m are 2^6: with AT_MOVE at most 2^14, and fp16 is normal down to 2^-20 of m
-#define AT_MOST 32768.0f      // a lane's sum of 16 weights above it moves m too: each of them fits fp16
+#define AT_MOST 32768.0f      // k_kv_attend_tile moves it when a lane's sum of 16 weights passes this: each of them fits fp16
 
 // Query rows row0 .. of a wave (NCB tiles of COLS): their positions, their elements as fp16 (lane (n, g) holds those of
 // row n that pair with its pieces of a key) divided by a power of two of the row, and the constant that a score is
@@ -238,7 +246,9 @@ __device__ __forceinline__ void store_rows(const ba_kv_attend_args& a, const AtS
 // waves of a SIMD that the registers are to leave room for
 constexpr int at_waves(int d, int cols) { return cols == 16 ? (d <= 64 ? 4 : d <= 128 ? 2 : 1) : d <= 128 ? 2 : 1; }
 
-// Few rows: the waves have the same COLS rows and split the blocks; every wave reads and converts its own.
+// Few rows: the waves have the same COLS rows (16 x 16 x 32 products for up to 16, 32 x 32 x 16 for more) and split the
+// blocks; every wave reads and converts its own, a block ahead.  8 or 16 waves to a workgroup were no faster on short
+// sequences (777 tokens: 8.4 and 9.4 us against 8.5, most of it launch and dependent loads).
 template <int D, int KT, int COLS>
 __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_attend_args a, int n_tiles, int wide) {
     typedef Mma<COLS> M;
@@ -530,11 +540,17 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_att
     store_rows<D, COLS, NCB>(a, q, kh, group, tile0, all, sp, n, g, wide != 0, o, m, l);
 }
 
-// Many rows: the four waves have 32 * NCB rows each and share the blocks.  A block's codes are fetched once for the
-// workgroup, a block ahead, and converted into LDS in the order in which lanes read operands (16 bytes a lane, one lane
-// after the other).  Half a block (32 tokens) at a time, the scores of the next half are made while the weights of the
-// present one are: the matrix unit and the vector unit have independent work throughout.  Keys have two buffers and values
-// three, as the products with a block's second half run when others convert the next block: one barrier a block.
+// Many rows: the waves have 32 * NCB rows each and share the blocks.  A block's codes are fetched once for the
+// workgroup, a block ahead, and converted into LDS in the order in which lanes read operands (16 bytes a lane).  Half a
+// block (32 tokens) at a time, the scores of the next half are made while the weights of the present one are: the matrix
+// unit and the vector unit have independent work throughout.  Keys have two buffers and values three, as the products
+// with a block's second half run when others convert the next block: one barrier a block.
+//
+// What the steps gave, 2 x 2048 rows over 16384 tokens of 128 int8 elements, 32 heads on 8 (us): codes from memory to
+// registers, 64 rows a wave 2167; converted in LDS 1777, with 32 rows a wave so that two waves fit a SIMD 1462; the order
+// of products and vector instructions fenced 1444; conversions spread over the products and LDS slots exchanged against
+// bank conflicts 1201; 8 waves to a workgroup 1126; no maximum formed until a sum calls for it 1062; 32-bit arithmetic on
+// rows and blocks 1024.
 template <int D, int KT, int NCB, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_attend_tile(ba_kv_attend_args a, int n_tiles, int wide) {
     typedef Mma<32> M;
@@ -732,6 +748,9 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
 #pragma unroll
             for (int r = 0; r < 16; ++r) tn[c][r] = 0.0f;
         }
+        // the wave that is at its exponentials goes first: the other one's products fill the matrix unit meanwhile
+        // (2 x 2048 rows over 16384 tokens, 64 elements: 580 -> 564 us)
+        __builtin_amdgcn_s_setprio(1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int x = 0; x < KS; ++x) {
@@ -744,6 +763,7 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         // weights that fp16 could not hold show in their sum: no maximum is formed until then
         bool big = false;
 #pragma unroll
