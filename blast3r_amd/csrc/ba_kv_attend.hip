@@ -18,9 +18,13 @@
 // Factors: a block's key factor goes into the constant c, its value factor into the exponent: with z = c q.k
 // and lv = log2(value factor), m follows z + lv, so that the weights exp2(z + lv - m) that meet the codes of
 // the values fit fp16 whatever the factors are, and the denominator adds their sums divided by the value
-// factor.  The weights of a block whose values are small beside others' may vanish in fp16 and still make up
-// the denominator, so that is summed in fp32 before the weights are rounded to fp16 (11 bits, at the precision
-// of the outputs or beyond).  m is moved only when a weight nears fp16's end; until then nothing is rescaled.
+// factor.  Weights are rounded to fp16: 11 bits, an eighth of the error of rounding a bf16 output, but as much
+// as rounding an fp16 one.  For fp16 outputs (HALF) the rounded weights make up the denominator too, so that a
+// row that one key dominates is exact (errors against 64 bits 1.0 to 1.3 times those of rounding the output,
+// 1.2 to 1.4 without; 3% of the time of k_kv_attend_tile at 128 elements); for bf16 the unrounded ones do.
+// Weights of a block whose values are small beside others' (by AT_LOW) may vanish in fp16 and still count in
+// the denominator: its sums are taken before rounding in any case.  m is moved only when a weight nears
+// fp16's end; until then nothing is rescaled.
 //
 // Two kernels:
 //   k_kv_attend       up to 32 rows: the waves of a workgroup have the same rows and split the blocks, codes go
@@ -163,6 +167,7 @@ __device__ __forceinline__ void store_out4(const ba_kv_attend_args& a, int64_t r
 #define AT_NONE -1.0e30f      // reference of a row that has seen no key
 #define AT_MOVE 8.0f          // k_kv_attend moves m when a score passes it by so much (log2)
 #define AT_LIFT 6.0f          // weights at m are 2^6: with AT_MOVE at most 2^14, and fp16 is normal down to 2^-20 of m
+#define AT_LOW 0.015625f      // a value factor below 2^-6 of the largest so far
 #define AT_MOST 32768.0f      // k_kv_attend_tile moves it when a lane's sum of 16 weights passes this: each of them fits fp16
 
 // Query rows row0 .. of a wave (NCB tiles of COLS): their positions, their elements as fp16 (lane (n, g) holds those of
@@ -249,7 +254,7 @@ constexpr int at_waves(int d, int cols) { return cols == 16 ? (d <= 64 ? 4 : d <
 // Few rows: the waves have the same COLS rows (16 x 16 x 32 products for up to 16, 32 x 32 x 16 for more) and split the
 // blocks; every wave reads and converts its own, a block ahead.  8 or 16 waves to a workgroup were no faster on short
 // sequences (777 tokens: 8.4 and 9.4 us against 8.5, most of it launch and dependent loads).
-template <int D, int KT, int COLS>
+template <int D, int KT, int COLS, bool HALF>
 __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_attend_args a, int n_tiles, int wide) {
     typedef Mma<COLS> M;
     typedef typename M::acc acc;
@@ -353,6 +358,7 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_att
             for (int r = 0; r < CREG; ++r) o[c][d][r] = 0.0f;
     }
 
+    float top_f = 0.0f;                                      // the largest value factor so far
     for (; blk < hi; blk += WK) {
         const int after = page_of(blk + 2 * WK);
         const float2 fn = factors(next);
@@ -443,9 +449,11 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_att
             }
         }
         h8 pf[NCB][PS];
+        const bool low = f.y < top_f * AT_LOW;               // values small beside others': see the factors above
+        top_f = fmaxf(top_f, f.y);
 #pragma unroll
         for (int c = 0; c < NCB; ++c) {
-            float sum = 0.0f;
+            float sum = 0.0f, fine = 0.0f;
 #pragma unroll
             for (int t = 0; t < PS; ++t)
 #pragma unroll
@@ -453,10 +461,13 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_att
                     const int k = 8 * t + j;
                     const float x = __builtin_amdgcn_exp2f(sc[c][k / CREG][k % CREG]);
                     const float y = __builtin_amdgcn_exp2f(sc[c][(k + 1) / CREG][(k + 1) % CREG]);
-                    sum += x + y;                            // before rounding: see the factors above
-                    pf[c][t][j] = (_Float16)x;
-                    pf[c][t][j + 1] = (_Float16)y;
+                    const h2 p = {(_Float16)x, (_Float16)y};
+                    if (HALF) sum = __builtin_amdgcn_fdot2(p, (h2){(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+                    if (!HALF || low) fine += x + y;
+                    pf[c][t][j] = p[0];
+                    pf[c][t][j + 1] = p[1];
                 }
+            if (!HALF || low) sum = fine;
             // a row that sees nothing of a block takes nothing from a factor that is NaN
             l[c] = masked && sum == 0.0f ? l[c] : fmaf(sum, iv, l[c]);
         }
@@ -551,7 +562,7 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_att
 // of products and vector instructions fenced 1444; conversions spread over the products and LDS slots exchanged against
 // bank conflicts 1201; 8 waves to a workgroup 1126; no maximum formed until a sum calls for it 1062; 32-bit arithmetic on
 // rows and blocks 1024.
-template <int D, int KT, int NCB, int WAVES>
+template <int D, int KT, int NCB, int WAVES, bool HALF>
 __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_attend_tile(ba_kv_attend_args a, int n_tiles, int wide) {
     typedef Mma<32> M;
     typedef M::acc acc;
@@ -686,6 +697,7 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
     };
     // what most blocks do not need: tokens hidden from rows, and the first reference of a row
     bool unset = true;                                       // a row of the wave has none
+    float top_f = 0.0f;                                      // the largest value factor so far
     auto settle = [&](acc (&t)[NCB], int blk, int page, int b) {
         const int t0 = blk * 64, len = there(page) ? q.len : t0;
         const bool masked = t0 + 64 > whole_hi || t0 < whole_lo || t0 + 64 > len;
@@ -732,14 +744,18 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
         };
         h8 pf[NCB][2];
         float sum[NCB];
+        const bool low = HALF && f.y < top_f * AT_LOW;       // values small beside others': see the factors above
+        top_f = fmaxf(top_f, f.y);
         auto weigh = [&](int i0, int i1) {
 #pragma unroll
             for (int i = i0; i < i1; ++i) {
                 const int c = i % NCB, j = i / NCB * 2;
                 const float y = __builtin_amdgcn_exp2f(t[c][j]), z = __builtin_amdgcn_exp2f(t[c][j + 1]);
-                sum[c] += y + z;                             // before rounding: see the factors above
-                pf[c][j / 8][j % 8] = (_Float16)y;
-                pf[c][j / 8][j % 8 + 1] = (_Float16)z;
+                const h2 p = {(_Float16)y, (_Float16)z};
+                if (HALF) sum[c] = __builtin_amdgcn_fdot2(p, (h2){(_Float16)1.0f, (_Float16)1.0f}, sum[c], false);
+                else sum[c] += y + z;
+                pf[c][j / 8][j % 8] = p[0];
+                pf[c][j / 8][j % 8 + 1] = p[1];
             }
         };
 #pragma unroll
@@ -765,17 +781,27 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
         }
         __builtin_amdgcn_s_setprio(0);
         // weights that fp16 could not hold show in their sum: no maximum is formed until then
-        bool big = false;
+        bool rare = low, big = false;
 #pragma unroll
         for (int c = 0; c < NCB; ++c) big = big || sum[c] > AT_MOST;
-        if (__any(big)) {
+        rare = rare || big;
+        if (__any(rare)) {
+            if (__any(big)) {
 #pragma unroll
-            for (int c = 0; c < NCB; ++c) {
-                const float x = largest(t, c);
-                move_by(t, c, x > AT_LIFT ? x - AT_LIFT : 0.0f);
-                sum[c] = 0.0f;
+                for (int c = 0; c < NCB; ++c) {
+                    const float x = largest(t, c);
+                    move_by(t, c, x > AT_LIFT ? x - AT_LIFT : 0.0f);
+                    sum[c] = 0.0f;
+                }
+                weigh(0, PAIRS);
             }
-            weigh(0, PAIRS);
+            if (HALF && low)
+#pragma unroll
+                for (int c = 0; c < NCB; ++c) {
+                    sum[c] = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sum[c] += __builtin_amdgcn_exp2f(t[c][r]);
+                }
         }
         const float iv = __builtin_amdgcn_rcpf(f.y), lv = __builtin_amdgcn_logf(fn.y);
         float cz[NCB], off[NCB];
@@ -945,14 +971,21 @@ static AtShape at_shape(int64_t rows, int dim) {
     return {32, 1, 8, 256, 1};
 }
 
-template <int D, int KT>
-static int launch_attend(const ba_kv_attend_args& a, AtShape v, unsigned nb, int tiles, int wide, hipStream_t st) {
+template <int D, int KT, bool HALF>
+static void launch_attend(const ba_kv_attend_args& a, AtShape v, unsigned nb, int tiles, int wide, hipStream_t st) {
     const dim3 grid(nb), block(64 * v.waves);
-    if (v.cols == 16) hipLaunchKernelGGL((k_kv_attend<D, KT, 16>), grid, block, 0, st, a, tiles, wide);
-    else if (v.ncb == 0) hipLaunchKernelGGL((k_kv_attend<D, KT, 32>), grid, block, 0, st, a, tiles, wide);
-    else if (v.rows == 128) hipLaunchKernelGGL((k_kv_attend_tile<D, KT, 1, 4>), grid, block, 0, st, a, tiles, wide);
-    else if constexpr (D <= 64) hipLaunchKernelGGL((k_kv_attend_tile<D, KT, 2, 4>), grid, block, 0, st, a, tiles, wide);
-    else if constexpr (D <= 128) hipLaunchKernelGGL((k_kv_attend_tile<D, KT, 1, 8>), grid, block, 0, st, a, tiles, wide);
+    if (v.cols == 16) hipLaunchKernelGGL((k_kv_attend<D, KT, 16, HALF>), grid, block, 0, st, a, tiles, wide);
+    else if (v.ncb == 0) hipLaunchKernelGGL((k_kv_attend<D, KT, 32, HALF>), grid, block, 0, st, a, tiles, wide);
+    else if (v.rows == 128) hipLaunchKernelGGL((k_kv_attend_tile<D, KT, 1, 4, HALF>), grid, block, 0, st, a, tiles, wide);
+    else if constexpr (D <= 64) hipLaunchKernelGGL((k_kv_attend_tile<D, KT, 2, 4, HALF>), grid, block, 0, st, a, tiles, wide);
+    else if constexpr (D <= 128) hipLaunchKernelGGL((k_kv_attend_tile<D, KT, 1, 8, HALF>), grid, block, 0, st, a, tiles, wide);
+}
+
+template <int D>
+static int launch_attend(const ba_kv_attend_args& a, AtShape v, unsigned nb, int tiles, int wide, hipStream_t st) {
+    const bool half = a.dtype == BA_F16;
+    if (a.bits == BA_FP8) half ? launch_attend<D, BA_FP8, true>(a, v, nb, tiles, wide, st) : launch_attend<D, BA_FP8, false>(a, v, nb, tiles, wide, st);
+    else half ? launch_attend<D, BA_INT8, true>(a, v, nb, tiles, wide, st) : launch_attend<D, BA_INT8, false>(a, v, nb, tiles, wide, st);
     BA_LAUNCHED();
     return BA_OK;
 }
@@ -1017,8 +1050,7 @@ extern "C" int ba_kv_attend(const ba_kv_attend_args* args, void* stream) {
     const int wide = (uintptr_t)a.q % 16 == 0 && (uintptr_t)a.o % 8 == 0 && a.q_st % 8 == 0 && a.q_sh % 8 == 0 && a.o_st % 4 == 0 && a.o_sh % 4 == 0;
     hipStream_t st = (hipStream_t)stream;
     int rc = BA_ERR_UNSUPPORTED;
-#define BA_AT_D(D) \
-    case D: rc = a.bits == BA_FP8 ? launch_attend<D, BA_FP8>(a, v, nb, (int)tiles, wide, st) : launch_attend<D, BA_INT8>(a, v, nb, (int)tiles, wide, st); break;
+#define BA_AT_D(D) case D: rc = launch_attend<D>(a, v, nb, (int)tiles, wide, st); break;
     switch (a.dim) { BA_AT_D(32) BA_AT_D(64) BA_AT_D(96) BA_AT_D(128) BA_AT_D(256) }
 #undef BA_AT_D
     if (rc != BA_OK || a.n_splits == 1) return rc;

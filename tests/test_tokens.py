@@ -479,16 +479,17 @@ def test_attend_against_oracle(bits, dim, heads, group, lens, counts, causal, wi
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('bits', ['fp8', 'int8'])
-@pytest.mark.parametrize('counts', [[1], [3], [40], [90]])
-def test_attend_ranges(bits, counts):
-    """Factors from 2^-40 to 2^40 in neighbouring blocks, queries of very different sizes, peaked rows, a NaN block that
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('counts', [[1], [3], [12], [40], [90]])
+def test_attend_ranges(bits, counts, dtype):
+    """Factors from 2^-40 to 2^40 (to 1 where outputs are fp16) in neighbouring blocks, queries of very different sizes, peaked rows, a NaN block that
     only some rows see, NaN queries, missing blocks."""
     rng = np.random.default_rng(counts[0])
     n = 64 * 20 - 11
     c, o = _cache(22, 1, 64, bits)
     pages = _pages(rng, [20], 22, 20)
     for b in range(20):                                     # values large where keys are small and the other way round
-        e = int(rng.integers(-20, 20))
+        e = int(rng.integers(-20, 20 if dtype == torch.bfloat16 else 1))
         c.scales[int(pages[0, b]), 0] = torch.tensor([2.0 ** (-7 - abs(e) / 4), 2.0 ** (2 * e)], device=DEV)
     pages[0, 3] = -1
     pages[0, 7] = 22
@@ -496,8 +497,8 @@ def test_attend_ranges(bits, counts):
     x = rng.normal(size=(counts[0], 2, 64)) * np.exp(rng.normal(size=(counts[0], 2, 1)) * 2)
     x[0, 0] = 0.0
     x[-1, 1] *= 1e-20
-    q = torch.tensor(x, dtype=torch.float32).clamp(-8, 8).to(torch.bfloat16).to(DEV)
-    print(f'attend ranges {bits} {counts}', flush=True)
+    q = torch.tensor(x, dtype=torch.float32).clamp(-8, 8).to(dtype).to(DEV)
+    print(f'attend ranges {bits} {counts} {dtype}', flush=True)
     _check(c, o, q, pages, [n], counts)
     _check(c, o, q, pages, [n], counts, scale=0.5)
     c.scales[int(pages[0, 19]), 0, 0] = math.nan            # the newest block: rows before it do not see it
@@ -512,6 +513,23 @@ def test_attend_ranges(bits, counts):
     q[0, 1, 5] = math.nan
     o2 = _mirror(c, bits)
     _check(c, o2, q, pages, [64 * 19], counts, window=64 * 12)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', ['fp8', 'int8'])
+def test_attend_one_key(bits):
+    """A row that sees one token has its value: fp16 weights are the same in numerator and denominator, so all that is left
+    are fp32 roundings (the weight's products, a reciprocal and a factor's: 2^-21 together) and half a step."""
+    c, o = _cache(3, 2, 64, bits, seed=9)
+    lens = [1, 50, 58]                                      # with 69 rows before it each stays within two blocks
+    for n in (1, 20, 70):
+        q = torch.randn((3 * n, 4, 64), device=DEV, generator=torch.Generator(device=DEV).manual_seed(n)).half() * 3
+        got = _np(c.attend(q, _i32([[0, 1], [0, 1], [2, 1]]), _i32([n - 1 + x for x in lens]), window=1, max_new=n)).reshape(3, n, 4, 64)
+        for s, pages in enumerate(([0, 1], [0, 1], [2, 1])):
+            _, v, _ = o.sequence(pages, n - 1 + lens[s])
+            for i in range(n):
+                want = np.repeat(v[lens[s] - 1 + i], 2, 0)
+                assert np.all(np.abs(got[s, i] - want) <= (2.0 ** -21 + 2.0 ** -11) * np.abs(want) + 2.0 ** -25), (n, s, i)
 
 
 @pytest.mark.gpu
