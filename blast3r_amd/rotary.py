@@ -1,9 +1,9 @@
 """Rotary positions of a transformer's queries and keys on the device (``ba_rotary``, libba_hip.so).
 
-The depth and matching networks in front of a bundle adjustment place the patches of an image by row and column
-(src/blast3r/extensions/curope: two or three axes, each with its part of the head, members of a pair half a section
-apart); sequence models place tokens by one position, with pairs half a head apart or side by side, and may scale
-their frequencies for long contexts.  ``Rotary`` holds one such choice::
+The depth and matching networks in front of a bundle adjustment place the patches of an image by row and column (two or
+three axes, each with its part of the head; the reference has an extension for it, src/blast3r/extensions/curope, with
+which parity is unpinned); sequence models place tokens by one position, with pairs half a head apart or side by side, and
+may scale their frequencies for long contexts.  ``Rotary`` holds one such choice::
 
     rot = Rotary(64, axes=2)                    # a head of 64, rows in its first half, columns in the other
     q, k = rot(positions, q, k)                 # one launch for both; differentiable

@@ -14,6 +14,9 @@ reference algorithm (naver/blast3r), written from the reference source text:
   * ``sampling`` -- F sampling: ``bilinear_sampling`` / ``grid_sample`` and
                     ``gather_data_from_dense_tracks`` (src/blast3r/utils/geometry.py,
                     src/blast3r/inference/tracks.py), numpy fp32
+  * ``tokens``   -- rotary positions, the 8-bit key/value cache and attention over
+                    it, token by token in 64 bits (no reference counterpart but the
+                    rotation's, src/blast3r/extensions/curope)
   * ``dense``    -- brute-force dense versions (materialised J, dense normal
                     equations, dense Schur) used only to pin the above on tiny
                     problems.
@@ -23,6 +26,6 @@ Only ``tests/``, ``__graft_entry__.smoke()`` and the ``cpu_baseline`` leg of
 The product path (``blast3r_amd``) never imports, calls or falls back to it.
 
 Parity pinning of each function (what fixes it besides its own formula) is
-listed in the module docstrings and exercised by ``tests/test_oracle.py`` and
-``tests/test_sampling.py``.
+listed in the module docstrings and exercised by ``tests/test_oracle.py``,
+``tests/test_sampling.py`` and ``tests/test_tokens.py``.
 """
