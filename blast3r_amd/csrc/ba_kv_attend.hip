@@ -933,7 +933,8 @@ __global__ void __launch_bounds__(AT_T) k_kv_join(ba_kv_attend_args a, int tile_
     // one reference for the row
     den_sh[threadIdx.x] = top;
     __syncthreads();
-    for (int k = 0; k < lanes; ++k) top = fmaxf(top, den_sh[threadIdx.x + (k - lane) * quads]);
+    if (mine)                                                // threads left over have no group of their own
+        for (int k = 0; k < lanes; ++k) top = fmaxf(top, den_sh[threadIdx.x + (k - lane) * quads]);
     __syncthreads();
     for (int p = lane; p < n; p += lanes) {
         const float2 f = *part_ref(a, row, head, p);
