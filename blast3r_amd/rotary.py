@@ -57,7 +57,7 @@ def rotary_frequencies(n, base=10000.0, scaling=None):
 
 
 class _Turn(torch.autograd.Function):
-    """The rotation with its gradient, which is the opposite rotation."""
+    """The rotation with its gradient, which is the opposite rotation (and so differentiable in turn)."""
 
     @staticmethod
     def forward(ctx, rot, positions, inverse, *xs):
@@ -72,7 +72,7 @@ class _Turn(torch.autograd.Function):
         out = [None] * len(grads)
         if need:
             gs = [g if g.stride(-1) == 1 else g.contiguous() for g in (grads[i] for i in need)]
-            for i, y in zip(need, ctx.rot._run(positions, gs, None, not ctx.inverse)):
+            for i, y in zip(need, _Turn.apply(ctx.rot, positions, not ctx.inverse, *gs)):
                 out[i] = y
         return (None, None, None, *out)
 

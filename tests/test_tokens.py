@@ -281,6 +281,12 @@ def test_rotary_gradient():
     a, b = float((diff * gz.double()).sum()), float((dk.double() * u.double()).sum())
     size = float((gz.abs().double() * (k.detach().abs() + u.abs()).double()).sum())
     assert abs(a - b) <= 4e-6 * size
+    # the gradient's gradient: the map itself
+    g1 = gz.clone().requires_grad_()
+    (d1,) = torch.autograd.grad(rot(pos, x.detach().expand(2, 9, 5, 64), k)[1], (k,), (g1,), create_graph=True)
+    (d2,) = torch.autograd.grad(d1, (g1,), (u,))
+    with torch.no_grad():
+        assert torch.equal(d1, dk) and torch.equal(d2, rot(pos, u))
     # a tensor that needs no gradient beside one that does; a broadcast gradient
     q2 = mk(2, 9, 3, 64)
     y, z = rot(pos, q2, k)
