@@ -140,15 +140,15 @@ class KVCache:
         if n_rows < 0:
             raise ValueError(f'cache: {n_rows} rows')
         a = BaKvArgs.from_buffer_copy(self._args)
-        both = torch.empty((2, n_rows, self.heads, self.head_dim), dtype=dtype, device=self.device)
+        shape = (n_rows, self.heads, self.head_dim)
+        k = torch.empty(shape, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
         a.rk_st = a.rv_st = self.heads * self.head_dim
         a.rk_sh = a.rv_sh = self.head_dim
-        at = both.data_ptr()
-        a.starts, a.dtype, a.rk = starts.data_ptr(), code, at
-        a.rv = at + n_rows * self.heads * self.head_dim * both.element_size()
+        a.starts, a.dtype, a.rk, a.rv = starts.data_ptr(), code, k.data_ptr(), v.data_ptr()
         if self._fill(a, pages, starts, 'starts', offsets, n_rows, max_count):
             launch(self._lib.ba_kv_read, a, self.device)
-        return both[0], both[1]
+        return k, v
 
     def attend(self, q, pages, lengths, offsets=None, max_new=None, causal=True, window=None, scale=None, out=None,
                return_lse=False):
@@ -184,7 +184,7 @@ class KVCache:
                 raise ValueError(f'cache: scale must be positive, got {scale}')
             a.scale = scale
         if out is None:
-            out = torch.empty(shape, dtype=dtype, device=dev)
+            out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=dtype, device=dev)    # 1.1, 2.2 us
             a.o_st, a.o_sh = q_heads * dim, dim
         else:
             if out.shape != shape or out.dtype is not dtype:
