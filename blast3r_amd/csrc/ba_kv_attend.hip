@@ -97,11 +97,12 @@ __device__ __forceinline__ h8 codes8(uint2 w) {
     return r;
 }
 
-// What a sequence of the call has: its rows and its length.
+// What a sequence of the call has: its rows and its tokens.
 struct AtSeq {
     int64_t row0;
-    int n, len;
-    int rows;                // of its n rows, those within max_rows
+    int len;                 // tokens within its block list
+    int first;               // position of its first row: that of all its rows and tokens, there or not
+    int rows;                // of its rows, those within max_rows
 };
 
 __device__ __forceinline__ AtSeq at_seq(const ba_kv_attend_args& a, int s) {
@@ -111,14 +112,15 @@ __device__ __forceinline__ AtSeq at_seq(const ba_kv_attend_args& a, int s) {
         n = (int64_t)a.offsets[s + 1] - row0;
     }
     if (row0 < 0 || row0 > a.n_rows || n < 0) { row0 = 0; n = 0; }
-    n = n < a.n_rows - row0 ? n : a.n_rows - row0;
     int64_t len = a.lengths[s];
+    len = len < 0 ? 0 : len;
+    const int first = (int)(len - n);
+    n = n < a.n_rows - row0 ? n : a.n_rows - row0;
     const int64_t most = (int64_t)a.n_pages * 64;
-    len = len < 0 ? 0 : len < most ? len : most;
-    return {row0, (int)n, (int)len, (int)(n < a.max_rows ? n : a.max_rows)};
+    return {row0, (int)(len < most ? len : most), first, (int)(n < a.max_rows ? n : a.max_rows)};
 }
 
-// Blocks [lo, hi) that rows [row, row + rows) (of n * group rows) see, cut into parts of `per` blocks.
+// Blocks [lo, hi) that rows [row, row + rows) (of the sequence's rows * group) see, cut into parts of `per` blocks.
 struct AtBlocks {
     int lo, hi, per;
 };
@@ -126,8 +128,8 @@ struct AtBlocks {
 __device__ __forceinline__ AtBlocks at_blocks(const ba_kv_attend_args& a, const AtSeq& q, int group, int row, int rows) {
     const int all = q.rows * group, last = row + rows < all ? row + rows : all;
     if (row >= last) return {0, 0, 1};
-    const int p0 = q.len - q.n + (int)((unsigned)row / (unsigned)group), p1 = q.len - q.n + (int)((unsigned)(last - 1) / (unsigned)group);
-    const int keys = a.causal ? p1 + 1 : q.len;
+    const int p0 = q.first + (int)((unsigned)row / (unsigned)group), p1 = q.first + (int)((unsigned)(last - 1) / (unsigned)group);
+    const int keys = a.causal && p1 < q.len ? p1 + 1 : q.len;
     const int64_t from = a.window > 0 ? p0 - a.window + 1 : 0;
     const int first = from < 0 ? 0 : from < q.len ? (int)from : q.len;
     if (keys <= first) return {0, 0, 1};
@@ -182,7 +184,7 @@ __device__ __forceinline__ void load_queries(const ba_kv_attend_args& a, const A
         const int r = row0 + c * COLS + n, rc = r < all ? r : all - 1;
         const int i = (int)((unsigned)rc / (unsigned)group);
         const int head = kh * group + rc - i * group;
-        pos[c] = q.len - q.n + i;
+        pos[c] = q.first + i;
         float x[KS][8];
         uint32_t top = 0;
         const int64_t at = (q.row0 + i) * a.q_st + head * a.q_sh + g * (D / NG);
@@ -339,7 +341,7 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_att
     load_queries<D, COLS, NCB>(a, q, kh, group, tile0, all, n, g, wide != 0, qf, qc, pos);
     // tokens [whole_lo, whole_hi) are seen by all rows of the wave: their blocks need no comparisons
     const int last = tile0 + ROWS < all ? tile0 + ROWS : all;
-    const int pmin = q.len - q.n + (int)((unsigned)tile0 / (unsigned)group), pmax = q.len - q.n + (int)((unsigned)(last - 1) / (unsigned)group);
+    const int pmin = q.first + (int)((unsigned)tile0 / (unsigned)group), pmax = q.first + (int)((unsigned)(last - 1) / (unsigned)group);
     const int64_t window = a.window > 0 ? a.window : (int64_t)1 << 40;
     const int whole_hi = a.causal ? pmin + 1 : q.len;
     const int whole_lo = pmax - window + 1 > 0 ? (int)(pmax - window + 1) : 0;
@@ -594,7 +596,7 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
     load_queries<D, 32, NCB>(a, q, kh, group, row0, all, n, g, wide != 0, qf, qc, pos);
     // tokens [whole_lo, whole_hi) are seen by all rows of the wave: their blocks need no comparisons
     const int first = row0 < all ? row0 : all - 1, last = row0 + 32 * NCB < all ? row0 + 32 * NCB : all;
-    const int pmin = q.len - q.n + (int)((unsigned)first / (unsigned)group), pmax = q.len - q.n + (int)((unsigned)(last - 1) / (unsigned)group);
+    const int pmin = q.first + (int)((unsigned)first / (unsigned)group), pmax = q.first + (int)((unsigned)(last - 1) / (unsigned)group);
     const int64_t window = a.window > 0 ? a.window : (int64_t)1 << 40;
     const int whole_hi = a.causal ? pmin + 1 : q.len;
     const int whole_lo = pmax - window + 1 > 0 ? (int)(pmax - window + 1) : 0;
@@ -1025,7 +1027,7 @@ extern "C" int ba_kv_attend(const ba_kv_attend_args* args, void* stream) {
     BA_REQUIRE(a.bits == BA_FP8 || a.bits == BA_INT8, "attention: bits must be 0 (e4m3) or 1 (int8)");
     BA_REQUIRE(a.dtype == BA_F16 || a.dtype == BA_BF16, "attention: queries must be fp16 or bf16");
     BA_REQUIRE(a.n_rows >= 0 && a.rows_per_seq >= 0 && a.max_rows >= 0 && a.window >= 0 && a.n_rows < (int64_t)1 << 31 &&
-                   a.max_rows < (int64_t)1 << 31 && a.n_pages < 1 << 24, "attention: bad sizes");
+                   a.max_rows < (int64_t)1 << 31 && a.rows_per_seq < (int64_t)1 << 31 && a.n_pages < 1 << 24, "attention: bad sizes");
     BA_REQUIRE(a.scale > 0.0f && a.scale < 1.0e30f, "attention: scale must be positive");
     BA_REQUIRE(a.n_splits >= 1 && a.n_splits <= 65536, "attention: n_splits must be in [1, 65536]");
     if (a.n_rows == 0 || a.n_seqs == 0 || a.max_rows == 0) return BA_OK;

@@ -580,6 +580,25 @@ def test_attend_bounds():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('causal,window', [(True, None), (True, 60), (False, 150)])
+@pytest.mark.parametrize('n', [1, 20, 100, 300])
+def test_attend_positions_past_the_block_list(n, causal, window):
+    """Rows stand at the last positions of their sequence's length and row count, also where its tokens are more than its
+    block list is wide (those past it are hidden) or its rows more than the tensor has."""
+    rng = np.random.default_rng(n)
+    c, o = _cache(8, 2, 64, 'int8')
+    pages = _pages(rng, [2, 1], 8, 2)
+    lens, counts = [128 + n // 2 + 5, 60], [n, 1]
+    x = torch.tensor(rng.normal(size=(n + 1, 4, 64)), dtype=torch.float32, device=DEV).bfloat16()
+    print(f'attend past the block list {n} {causal} {window}', flush=True)
+    _check(c, o, x, pages, lens, counts, causal, window)
+    more = np.concatenate((_np(x[:n]), np.zeros((7, 4, 64))))
+    want, _, size = otok.attend(o, more, pages[:1], lens[:1], [n + 7], 0.125, causal, window)
+    got = _np(c.attend(x[:n], _i32(pages[:1]), _i32(lens[:1]), offsets=_i32([0, n + 7]), causal=causal, window=window))
+    assert np.all(np.abs(got - want[:n]) <= 1.2e-3 * size[:n] + 2.0 ** -8 * np.abs(want[:n]))
+
+
+@pytest.mark.gpu
 def test_attend_splits_join_to_one_pass():
     """Every number of parts gives the sums of one pass, to the roundings of fp32 and of the output."""
     from blast3r_amd._lib import BaKvAttendArgs, check, lib, stream_ptr
