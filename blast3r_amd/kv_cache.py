@@ -14,6 +14,7 @@ Sequences of a call have the same number of rows each, or ``offsets`` (n_seqs + 
 ``max_new`` (a host number; default: all rows) bounds the rows of one of them, and a close bound saves launches' empty
 workgroups.  Lengths, offsets and pages are device tensors, never read by the host: nothing here synchronises, and a
 call can be captured in a graph.  What they say out of range is left out (include/ba_hip.h).
+Rows of a result that no sequence has, or past ``max_new`` of one, are not written.
 """
 import math
 
