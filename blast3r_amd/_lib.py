@@ -315,6 +315,12 @@ def launch(call, args, device):
         check(status)
 
 
+def written(*tensors):
+    """Says that a kernel wrote to tensors that were there before the call: what autograd or a cache keyed by versions
+    keeps of them is out of date."""
+    torch.autograd.graph.increment_version(tensors)
+
+
 def ptr(t):
     """Raw device pointer of a tensor (None -> NULL); a host tensor raises instead of handing a
     host address to a kernel."""

@@ -20,7 +20,7 @@ import math
 
 import torch
 
-from ._lib import BaKvArgs, BaKvAttendArgs, launch, lib
+from ._lib import BaKvArgs, BaKvAttendArgs, launch, lib, written
 
 __all__ = ['KVCache', 'BLOCK']
 
@@ -131,6 +131,7 @@ class KVCache:
         a.starts, a.dtype, a.rk, a.rv = lengths.data_ptr(), code, k.data_ptr(), v.data_ptr()
         if self._fill(a, pages, lengths, 'lengths', offsets, k.shape[0], max_new):
             launch(self._lib.ba_kv_write, a, self.device)
+            written(self.k, self.v, self.scales)
 
     def read(self, pages, starts, offsets, n_rows, max_count=None, dtype=torch.bfloat16):
         """(k, v) of tokens ``starts[s]`` and on, ``offsets[s + 1] - offsets[s]`` of each sequence (n_rows / n_seqs where
@@ -184,7 +185,8 @@ class KVCache:
             if not 0.0 < scale < 1e30:
                 raise ValueError(f'cache: scale must be positive, got {scale}')
             a.scale = scale
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=dtype, device=dev)    # 1.1, 2.2 us
             a.o_st, a.o_sh = q_heads * dim, dim
         else:
@@ -207,4 +209,6 @@ class KVCache:
                 work = torch.empty(size, dtype=torch.uint8, device=dev)
                 a.workspace, a.workspace_bytes = work.data_ptr(), size
             launch(L.ba_kv_attend, a, dev)
+            if given:
+                written(out)
         return (out, lse) if return_lse else out

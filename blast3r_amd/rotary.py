@@ -14,7 +14,7 @@ import math
 
 import torch
 
-from ._lib import BaRotaryArgs, launch, lib
+from ._lib import BaRotaryArgs, launch, lib, written
 
 __all__ = ['Rotary', 'rotary_frequencies']
 
@@ -186,6 +186,8 @@ class Rotary:
             a.pos_sb = p_stride[0]
         if a.T and a.B:
             launch(self._call, a, dev)
+            if out is not None:
+                written(*ys)
         return tuple(ys)
 
     def _strides(self, t, lead, dtype):
