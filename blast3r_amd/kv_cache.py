@@ -192,6 +192,8 @@ class KVCache:
         else:
             if out.shape != shape or out.dtype is not dtype:
                 raise ValueError('cache: out must be like q')
+            if out.requires_grad and torch.is_grad_enabled():
+                raise RuntimeError('cache: attention over codes has no gradient: out must not require one')
             a.o_st, a.o_sh = self._rows(out, 'out', q_heads)
         lse = None
         if return_lse:

@@ -114,7 +114,8 @@ class Rotary:
 
         positions   int32 or int64, the tokens' shape ((T,) serves every batch), with more than one axis a last
                     dimension of ``axes``
-        out         tensors to write to, one for each x (x itself rotates in place); not differentiable
+        out         tensors to write to, one for each x (x itself rotates in place); not differentiable, and refused where
+                    gradients are recorded and one of them requires one
         inverse     rotate by the opposite angles
         """
         if not 1 <= len(xs) <= 2:
@@ -159,6 +160,8 @@ class Rotary:
             for x, y in zip(xs, ys):
                 if y.shape != x.shape or y.dtype != x.dtype or y.device != x.device or y.stride(-1) != 1:
                     raise ValueError('rotary: an output must be like its tensor, with contiguous elements of a head')
+                if y.requires_grad and torch.is_grad_enabled():
+                    raise ValueError('rotary: out must not require a gradient where gradients are recorded')
         a = BaRotaryArgs.from_buffer_copy(self._args)
         t, y = xs[0], ys[0]
         xs_, ys_ = self._strides(t, lead, dtype), y.stride()

@@ -61,3 +61,24 @@ def test_tensors_written_to_count_as_changed(host):
         rot(pos, z, out=z)
     with torch.no_grad():
         rot(pos, z, out=z)
+
+
+def test_outputs_that_require_a_gradient_are_refused(host):
+    from blast3r_amd.kv_cache import KVCache
+    from blast3r_amd.rotary import Rotary
+    rot, pos, x = Rotary(64, device='cpu'), _i32([0, 1, 2]), torch.randn(3, 2, 64)
+    leaf = torch.zeros(3, 2, 64, requires_grad=True)
+    with pytest.raises(ValueError, match='gradient'):
+        rot(pos, x, out=leaf)
+    with pytest.raises(ValueError, match='gradient'):
+        rot(pos, x, x, out=(torch.zeros_like(x), leaf))
+    c = KVCache(2, 1, 64, device='cpu')
+    q = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    out = torch.zeros_like(q).requires_grad_()
+    with pytest.raises(RuntimeError, match='gradient'):
+        c.attend(q, _i32([[0, 1]]), _i32([5]), out=out)
+    assert not host
+    with torch.no_grad():                                   # as torch's own operators take them
+        rot(pos, x, out=leaf)
+        c.attend(q, _i32([[0, 1]]), _i32([5]), out=out)
+    assert len(host) == 2 and leaf._version == 1 and out._version == 1
