@@ -10,6 +10,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'libba_hip.so')
@@ -313,6 +314,11 @@ def launch(call, args, device):
     status = call(ctypes.byref(args), stream)
     if status:
         check(status)
+
+
+def has_tangent(*tensors):
+    """Whether one of them carries a tangent of forward-mode differentiation (there are none outside a dual level)."""
+    return getattr(forward_ad, '_current_level', 0) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def written(*tensors):

@@ -14,7 +14,7 @@ import math
 
 import torch
 
-from ._lib import BaRotaryArgs, launch, lib, written
+from ._lib import BaRotaryArgs, has_tangent, launch, lib, written
 
 __all__ = ['Rotary', 'rotary_frequencies']
 
@@ -57,12 +57,14 @@ def rotary_frequencies(n, base=10000.0, scaling=None):
 
 
 class _Turn(torch.autograd.Function):
-    """The rotation with its gradient, which is the opposite rotation (and so differentiable in turn)."""
+    """The rotation with its gradient, which is the opposite rotation (and so differentiable in turn), and its
+    forward-mode derivative, which is the rotation of the tangents."""
 
     @staticmethod
     def forward(ctx, rot, positions, inverse, *xs):
-        ctx.rot, ctx.inverse = rot, inverse
+        ctx.rot, ctx.inverse, ctx.shapes = rot, inverse, [x.shape for x in xs]
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         return rot._run(positions, xs, None, inverse)
 
     @staticmethod
@@ -75,6 +77,18 @@ class _Turn(torch.autograd.Function):
             for i, y in zip(need, _Turn.apply(ctx.rot, positions, not ctx.inverse, *gs)):
                 out[i] = y
         return (None, None, None, *out)
+
+    @staticmethod
+    def jvp(ctx, rot, positions, inverse, *ts):
+        """Tangents turn as their tensors do; without one the tangent is zero."""
+        positions, = ctx.saved_tensors
+        have = [i for i, t in enumerate(ts) if t is not None]
+        like = ts[have[0]]
+        ys = _Turn.apply(ctx.rot, positions, ctx.inverse, *(ts[i] if ts[i].stride(-1) == 1 else ts[i].contiguous() for i in have))
+        out = [torch.zeros(shape, dtype=like.dtype, device=like.device) if t is None else t for t, shape in zip(ts, ctx.shapes)]
+        for i, y in zip(have, ys):
+            out[i] = y
+        return tuple(out)
 
 
 class Rotary:
@@ -120,7 +134,7 @@ class Rotary:
         """
         if not 1 <= len(xs) <= 2:
             raise ValueError(f'rotary: one or two tensors at a time, got {len(xs)}')
-        if torch.is_grad_enabled() and (xs[0].requires_grad or xs[-1].requires_grad):
+        if torch.is_grad_enabled() and (xs[0].requires_grad or xs[-1].requires_grad) or has_tangent(*xs):
             if out is not None:
                 raise ValueError('rotary: out cannot be given where gradients are recorded')
             ys = _Turn.apply(self, positions, bool(inverse), *xs)
@@ -160,8 +174,8 @@ class Rotary:
             for x, y in zip(xs, ys):
                 if y.shape != x.shape or y.dtype != x.dtype or y.device != x.device or y.stride(-1) != 1:
                     raise ValueError('rotary: an output must be like its tensor, with contiguous elements of a head')
-                if y.requires_grad and torch.is_grad_enabled():
-                    raise ValueError('rotary: out must not require a gradient where gradients are recorded')
+                if y.requires_grad and torch.is_grad_enabled() or has_tangent(y):
+                    raise ValueError('rotary: out must not require a gradient where gradients are recorded, nor have a tangent')
         a = BaRotaryArgs.from_buffer_copy(self._args)
         t, y = xs[0], ys[0]
         xs_, ys_ = self._strides(t, lead, dtype), y.stride()

@@ -82,3 +82,42 @@ def test_outputs_that_require_a_gradient_are_refused(host):
         rot(pos, x, out=leaf)
         c.attend(q, _i32([[0, 1]]), _i32([5]), out=out)
     assert len(host) == 2 and leaf._version == 1 and out._version == 1
+
+
+# ---------------------------------------------------------------------------------- forward mode
+
+def test_forward_mode_tangents_go_through_rotary(host, monkeypatch):
+    """The map is linear: a tangent is rotated as its tensor is, and one that is not there counts as zero."""
+    import ctypes
+    from torch.autograd import forward_ad
+
+    from blast3r_amd import rotary
+    from blast3r_amd.rotary import Rotary
+
+    def doubles(call, args, device):                        # stands for the rotation: y = 2 x, or x / 2 for the inverse
+        for x, y, heads in ((args.x0, args.y0, args.heads0), (args.x1, args.y1, args.heads1))[:args.n_x]:
+            src, dst = ((ctypes.c_float * (args.T * heads * args.dim)).from_address(p) for p in (x, y))
+            dst[:] = [v * (0.5 if args.inverse else 2.0) for v in src]
+
+    monkeypatch.setattr(rotary, 'launch', doubles)
+    rot, pos = Rotary(64, device='cpu'), _i32([0, 1, 2])
+    x, t, k = torch.randn(3, 2, 64), torch.randn(3, 2, 64), torch.randn(3, 1, 64)
+    for inverse in (False, True):
+        f = 0.5 if inverse else 2.0
+        for mode in (torch.no_grad, torch.enable_grad):
+            with forward_ad.dual_level(), mode():
+                dual = forward_ad.make_dual(x, t)
+                y = forward_ad.unpack_dual(rot(pos, dual, inverse=inverse))
+                assert torch.equal(y.primal, f * x) and torch.equal(y.tangent, f * t)
+                for a, b, ta, tb in ((dual, k, f * t, 0 * k), (k, dual, 0 * k, f * t)):
+                    a, b = (forward_ad.unpack_dual(r).tangent for r in rot(pos, a, b, inverse=inverse))
+                    assert torch.equal(a, ta) and torch.equal(b, tb)
+                with pytest.raises(ValueError, match='out'):
+                    rot(pos, dual, out=torch.zeros_like(x))
+                with pytest.raises(ValueError, match='out'):
+                    rot(pos, x, out=dual)
+                assert forward_ad.unpack_dual(rot(pos, x)).tangent is None
+    with forward_ad.dual_level():                           # reverse over forward
+        w = k.clone().requires_grad_()
+        y = forward_ad.unpack_dual(rot(pos, forward_ad.make_dual(w, w * 3))).tangent
+        assert torch.equal(torch.autograd.grad(y.sum(), w)[0], torch.full_like(w, 3.0 * 0.5))    # twice there, half of it back
