@@ -20,7 +20,7 @@ import math
 
 import torch
 
-from ._lib import BaKvArgs, BaKvAttendArgs, launch, lib, written
+from ._lib import BaKvArgs, BaKvAttendArgs, has_tangent, launch, lib, written
 
 __all__ = ['KVCache', 'BLOCK']
 
@@ -121,6 +121,8 @@ class KVCache:
         same block."""
         if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
             raise RuntimeError('cache: codes carry no gradient: append under torch.no_grad()')
+        if has_tangent(k, v):
+            raise RuntimeError('cache: codes carry no tangent of forward-mode differentiation')
         a = BaKvArgs.from_buffer_copy(self._args)
         a.rk_st, a.rk_sh = self._rows(k, 'k', self.heads)
         a.rv_st, a.rv_sh = self._rows(v, 'v', self.heads)
@@ -168,6 +170,8 @@ class KVCache:
         -inf where no token is seen, with which results over different tokens can be joined."""
         if q.requires_grad and torch.is_grad_enabled():
             raise RuntimeError('cache: attention over codes has no gradient: call it under torch.no_grad()')
+        if has_tangent(q) or out is not None and has_tangent(out):
+            raise RuntimeError('cache: attention over codes gives no tangent of forward-mode differentiation')
         shape = q.shape
         if len(shape) != 3 or shape[1] % self.heads or shape[1] == 0:
             raise ValueError(f'cache: q must be (tokens, a multiple of {self.heads} heads, {self.head_dim}), got {tuple(shape)}')

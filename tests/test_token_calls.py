@@ -121,3 +121,21 @@ def test_forward_mode_tangents_go_through_rotary(host, monkeypatch):
         w = k.clone().requires_grad_()
         y = forward_ad.unpack_dual(rot(pos, forward_ad.make_dual(w, w * 3))).tangent
         assert torch.equal(torch.autograd.grad(y.sum(), w)[0], torch.full_like(w, 3.0 * 0.5))    # twice there, half of it back
+
+
+def test_cache_refuses_forward_mode_tangents(host):
+    from torch.autograd import forward_ad
+
+    from blast3r_amd.kv_cache import KVCache
+    c = KVCache(2, 1, 64, device='cpu')
+    q, pages, lens = torch.zeros(1, 1, 64, dtype=torch.bfloat16), _i32([[0, 1]]), _i32([5])
+    with forward_ad.dual_level(), torch.no_grad():
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        for call in (lambda: c.attend(dual, pages, lens), lambda: c.attend(q, pages, lens, out=dual),
+                     lambda: c.append(dual, q, pages, lens), lambda: c.append(q, dual, pages, lens)):
+            with pytest.raises(RuntimeError, match='tangent'):
+                call()
+        assert not host
+        c.append(q, q, pages, lens)
+        c.attend(q, pages, lens)
+        assert len(host) == 2
