@@ -105,6 +105,15 @@ class KVCache:
         a.max_rows = most
         return most
 
+    def _no_derivative(self, *tensors):
+        """Refuses what has a gradient or a tangent, which codes cannot carry on."""
+        if torch.is_grad_enabled():
+            for t in tensors:
+                if t.requires_grad:
+                    raise RuntimeError('cache: codes carry no gradient: call it under torch.no_grad()')
+        if has_tangent(*tensors):
+            raise RuntimeError('cache: codes carry no tangent of forward-mode differentiation')
+
     def _rows(self, t, name, heads):
         shape = t.shape
         if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or t.device != self.device:
@@ -119,10 +128,7 @@ class KVCache:
         """Write the rows of k and v (tokens, heads, head_dim; fp32, fp16 or bf16) after the first ``lengths`` (n_seqs,)
         int32 tokens of their sequences.  ``lengths`` stays as it is.  No two sequences of a call may append to the
         same block."""
-        if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
-            raise RuntimeError('cache: codes carry no gradient: append under torch.no_grad()')
-        if has_tangent(k, v):
-            raise RuntimeError('cache: codes carry no tangent of forward-mode differentiation')
+        self._no_derivative(k, v, self.scales)
         a = BaKvArgs.from_buffer_copy(self._args)
         a.rk_st, a.rk_sh = self._rows(k, 'k', self.heads)
         a.rv_st, a.rv_sh = self._rows(v, 'v', self.heads)
@@ -143,6 +149,7 @@ class KVCache:
             raise ValueError(f'cache: fp32, fp16 or bf16 values, got {dtype}')
         if n_rows < 0:
             raise ValueError(f'cache: {n_rows} rows')
+        self._no_derivative(self.scales)
         a = BaKvArgs.from_buffer_copy(self._args)
         shape = (n_rows, self.heads, self.head_dim)
         k = torch.empty(shape, dtype=dtype, device=self.device)
@@ -168,10 +175,7 @@ class KVCache:
         A row that sees no token gives zeros.  q_heads is a multiple of the cache's heads; query head h reads cache
         head h // (q_heads // heads).  With ``return_lse`` also log(sum(exp(scale q k^T))) as (tokens, q_heads) fp32,
         -inf where no token is seen, with which results over different tokens can be joined."""
-        if q.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError('cache: attention over codes has no gradient: call it under torch.no_grad()')
-        if has_tangent(q) or out is not None and has_tangent(out):
-            raise RuntimeError('cache: attention over codes gives no tangent of forward-mode differentiation')
+        self._no_derivative(q, self.scales)
         shape = q.shape
         if len(shape) != 3 or shape[1] % self.heads or shape[1] == 0:
             raise ValueError(f'cache: q must be (tokens, a multiple of {self.heads} heads, {self.head_dim}), got {tuple(shape)}')
@@ -196,8 +200,7 @@ class KVCache:
         else:
             if out.shape != shape or out.dtype is not dtype:
                 raise ValueError('cache: out must be like q')
-            if out.requires_grad and torch.is_grad_enabled():
-                raise RuntimeError('cache: attention over codes has no gradient: out must not require one')
+            self._no_derivative(out)
             a.o_st, a.o_sh = self._rows(out, 'out', q_heads)
         lse = None
         if return_lse:

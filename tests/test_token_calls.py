@@ -139,3 +139,28 @@ def test_cache_refuses_forward_mode_tangents(host):
         c.append(q, q, pages, lens)
         c.attend(q, pages, lens)
         assert len(host) == 2
+
+
+def test_factors_that_require_a_gradient_are_refused(host):
+    """A wrapped cache's factors are fp32 tensors of the caller's: a gradient or tangent of them would be lost."""
+    from torch.autograd import forward_ad
+
+    from blast3r_amd.kv_cache import KVCache
+    c = KVCache(2, 1, 64, device='cpu')
+    w = KVCache.wrap(c.k, c.v, torch.ones(2, 1, 2, requires_grad=True))
+    q, pages, lens = torch.zeros(1, 1, 64, dtype=torch.bfloat16), _i32([[0, 1]]), _i32([5])
+    calls = [lambda w: w.attend(q, pages, lens), lambda w: w.read(pages, lens, None, 1), lambda w: w.append(q, q, pages, lens)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match='gradient'):
+            call(w)
+    assert not host
+    with torch.no_grad():
+        for call in calls:
+            call(w)
+        assert len(host) == 3
+        with forward_ad.dual_level():
+            d = KVCache.wrap(c.k, c.v, forward_ad.make_dual(c.scales, torch.ones_like(c.scales)))
+            for call in calls:
+                with pytest.raises(RuntimeError, match='tangent'):
+                    call(d)
+    assert len(host) == 3
