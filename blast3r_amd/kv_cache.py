@@ -30,13 +30,33 @@ BITS = {torch.float8_e4m3fn: 0, torch.int8: 1}
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
+def _tensor(name):
+    """A tensor of a cache; another one put in its place is checked, with the other two, by the next call."""
+    def put(self, t):
+        setattr(self, name, t)
+        self._at = None
+    return property(lambda self: getattr(self, name), put)
+
+
+def _given(name):
+    return property(lambda self: getattr(self, name))
+
+
 class KVCache:
     """``n_blocks`` blocks of 64 tokens for ``heads`` heads of ``head_dim`` elements.
 
     k       (n_blocks, heads, 64, head_dim), torch.float8_e4m3fn or torch.int8
     v       (n_blocks, heads, head_dim, 64): transposed, as attention reads it
     scales  (n_blocks, heads, 2) fp32: a block's factors of keys and values, value = code * factor
+
+    Other tensors may be put in the place of these three between calls (all of them for another number of blocks): the
+    next call takes them.  A captured graph goes on with the memory that it was captured with.
     """
+
+    k, v, scales = _tensor('_k'), _tensor('_v'), _tensor('_scales')
+    # of the tensors that the last call used
+    n_blocks, heads, head_dim = _given('_n_blocks'), _given('_heads'), _given('_head_dim')
+    device, dtype = _given('_device'), _given('_dtype')
 
     def __init__(self, n_blocks, heads, head_dim, dtype=torch.float8_e4m3fn, device='cuda'):
         if n_blocks < 0 or heads < 1:
@@ -71,17 +91,25 @@ class KVCache:
             raise ValueError('cache: k, v and scales must be contiguous')
         if not k.is_cuda or v.device != k.device or scales.device != k.device:
             raise RuntimeError('cache: k, v and scales must be on one GPU (the cache runs in libba_hip.so)')
-        self.k, self.v, self.scales = k, v, scales
-        self.n_blocks, self.heads, self.head_dim = n, h, d
-        self.device, self.dtype = k.device, k.dtype
+        self._k, self._v, self._scales = k, v, scales
+        self._n_blocks, self._heads, self._head_dim = n, h, d
+        self._device, self._dtype = k.device, k.dtype
         # the fields of every call
-        same = dict(k=k.data_ptr(), v=v.data_ptr(), scales=scales.data_ptr(), n_blocks=n, heads=h, dim=d, bits=BITS[k.dtype])
+        self._at = k.data_ptr(), v.data_ptr(), scales.data_ptr()
+        same = dict(zip(('k', 'v', 'scales'), self._at), n_blocks=n, heads=h, dim=d, bits=BITS[k.dtype])
         self._lib, self._args = lib(), BaKvArgs(**same)
         self._attend_args = BaKvAttendArgs(n_splits=1, scale=1.0 / math.sqrt(d), **same)
 
+    def _look(self):
+        """Every call starts with it: the fields of calls are those of the tensors held now."""
+        k, v, scales = self._k, self._v, self._scales
+        if self._at is None or (k.data_ptr(), v.data_ptr(), scales.data_ptr()) != self._at:
+            self._at = None
+            self._hold(k, v, scales)
+
     def _fill(self, a, pages, firsts, name, offsets, n_rows, max_rows):
         """The fields of a call that the arguments of every call give."""
-        dev = self.device
+        dev = self._device
         if (pages.dim() != 2 or pages.dtype is not torch.int32 or pages.device != dev or
                 pages.stride(1) != 1 and pages.shape[0] > 0 and pages.shape[1] > 1):
             raise ValueError(f'cache: pages must be (n_seqs, blocks) int32 on {dev} with contiguous rows')
@@ -116,8 +144,8 @@ class KVCache:
 
     def _rows(self, t, name, heads):
         shape = t.shape
-        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or t.device != self.device:
-            raise ValueError(f'cache: {name} must be (tokens, {heads}, {self.head_dim}) on {self.device}, got '
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self._head_dim or t.device != self._device:
+            raise ValueError(f'cache: {name} must be (tokens, {heads}, {self._head_dim}) on {self._device}, got '
                              f'{tuple(shape)} on {t.device}')
         st, sh, one = t.stride()
         if one != 1:
@@ -128,18 +156,19 @@ class KVCache:
         """Write the rows of k and v (tokens, heads, head_dim; fp32, fp16 or bf16) after the first ``lengths`` (n_seqs,)
         int32 tokens of their sequences.  ``lengths`` stays as it is.  No two sequences of a call may append to the
         same block."""
-        self._no_derivative(k, v, self.scales)
+        self._look()
+        self._no_derivative(k, v, self._scales)
         a = BaKvArgs.from_buffer_copy(self._args)
-        a.rk_st, a.rk_sh = self._rows(k, 'k', self.heads)
-        a.rv_st, a.rv_sh = self._rows(v, 'v', self.heads)
+        a.rk_st, a.rk_sh = self._rows(k, 'k', self._heads)
+        a.rv_st, a.rv_sh = self._rows(v, 'v', self._heads)
         code = DTYPES.get(k.dtype)
         if code is None or k.shape != v.shape or k.dtype is not v.dtype:
             raise ValueError(f'cache: k and v must be alike, in fp32, fp16 or bf16: got {tuple(k.shape)} {k.dtype} and '
                              f'{tuple(v.shape)} {v.dtype}')
         a.starts, a.dtype, a.rk, a.rv = lengths.data_ptr(), code, k.data_ptr(), v.data_ptr()
         if self._fill(a, pages, lengths, 'lengths', offsets, k.shape[0], max_new):
-            launch(self._lib.ba_kv_write, a, self.device)
-            written(self.k, self.v, self.scales)
+            launch(self._lib.ba_kv_write, a, self._device)
+            written(self._k, self._v, self._scales)
 
     def read(self, pages, starts, offsets, n_rows, max_count=None, dtype=torch.bfloat16):
         """(k, v) of tokens ``starts[s]`` and on, ``offsets[s + 1] - offsets[s]`` of each sequence (n_rows / n_seqs where
@@ -149,16 +178,17 @@ class KVCache:
             raise ValueError(f'cache: fp32, fp16 or bf16 values, got {dtype}')
         if n_rows < 0:
             raise ValueError(f'cache: {n_rows} rows')
-        self._no_derivative(self.scales)
+        self._look()
+        self._no_derivative(self._scales)
         a = BaKvArgs.from_buffer_copy(self._args)
-        shape = (n_rows, self.heads, self.head_dim)
-        k = torch.empty(shape, dtype=dtype, device=self.device)
+        shape = (n_rows, self._heads, self._head_dim)
+        k = torch.empty(shape, dtype=dtype, device=self._device)
         v = torch.empty_like(k)
-        a.rk_st = a.rv_st = self.heads * self.head_dim
-        a.rk_sh = a.rv_sh = self.head_dim
+        a.rk_st = a.rv_st = self._heads * self._head_dim
+        a.rk_sh = a.rv_sh = self._head_dim
         a.starts, a.dtype, a.rk, a.rv = starts.data_ptr(), code, k.data_ptr(), v.data_ptr()
         if self._fill(a, pages, starts, 'starts', offsets, n_rows, max_count):
-            launch(self._lib.ba_kv_read, a, self.device)
+            launch(self._lib.ba_kv_read, a, self._device)
         return k, v
 
     def attend(self, q, pages, lengths, offsets=None, max_new=None, causal=True, window=None, scale=None, out=None,
@@ -175,14 +205,15 @@ class KVCache:
         A row that sees no token gives zeros.  q_heads is a multiple of the cache's heads; query head h reads cache
         head h // (q_heads // heads).  With ``return_lse`` also log(sum(exp(scale q k^T))) as (tokens, q_heads) fp32,
         -inf where no token is seen, with which results over different tokens can be joined."""
-        self._no_derivative(q, self.scales)
+        self._look()
+        self._no_derivative(q, self._scales)
         shape = q.shape
-        if len(shape) != 3 or shape[1] % self.heads or shape[1] == 0:
-            raise ValueError(f'cache: q must be (tokens, a multiple of {self.heads} heads, {self.head_dim}), got {tuple(shape)}')
+        if len(shape) != 3 or shape[1] % self._heads or shape[1] == 0:
+            raise ValueError(f'cache: q must be (tokens, a multiple of {self._heads} heads, {self._head_dim}), got {tuple(shape)}')
         n_rows, q_heads, dim = shape
         a = BaKvAttendArgs.from_buffer_copy(self._attend_args)
         a.q_st, a.q_sh = self._rows(q, 'q', q_heads)
-        dtype, dev = q.dtype, self.device
+        dtype, dev = q.dtype, self._device
         if dtype is not torch.bfloat16 and dtype is not torch.float16:
             raise ValueError(f'cache: queries must be fp16 or bf16, got {dtype}')
         if window is not None:
@@ -211,7 +242,7 @@ class KVCache:
         most = self._fill(a, pages, lengths, 'lengths', offsets, n_rows, max_new)
         if most:
             L = self._lib
-            n = L.ba_kv_attend_splits(a.n_seqs, self.heads, q_heads, dim, most, a.n_pages)
+            n = L.ba_kv_attend_splits(a.n_seqs, self._heads, q_heads, dim, most, a.n_pages)
             if n > 1:                        # the partial sums live until the launches on this stream are done
                 a.n_splits = n
                 size = L.ba_kv_attend_workspace_bytes(n_rows, q_heads, dim, n)

@@ -164,3 +164,45 @@ def test_factors_that_require_a_gradient_are_refused(host):
                 with pytest.raises(RuntimeError, match='tangent'):
                     call(d)
     assert len(host) == 3
+
+
+# ---------------------------------------------------------------------------------- tensors that change hands
+
+def _calls(c, launched, blocks, heads, dim):
+    """One call of each kind, all of which have to get the cache's present tensors."""
+    q, rows = torch.zeros(1, heads, dim, dtype=torch.bfloat16), torch.zeros(1, heads, dim)
+    pages, lens = _i32([[0]]), _i32([5])
+    c.append(rows, rows, pages, lens)
+    c.read(pages, lens, None, 1)
+    c.attend(q, pages, lens)
+    for a in launched[-3:]:
+        assert (a.k, a.v, a.scales) == (c.k.data_ptr(), c.v.data_ptr(), c.scales.data_ptr())
+        assert (a.n_blocks, a.heads, a.dim) == (blocks, heads, dim) == (c.n_blocks, c.heads, c.head_dim)
+
+
+def test_cache_follows_tensors_put_in_place_of_its_own(host):
+    from blast3r_amd.kv_cache import KVCache
+    c = KVCache(2, 1, 64, device='cpu')
+    _calls(c, host, 2, 1, 64)
+    fp8 = torch.float8_e4m3fn
+    more = torch.zeros(3, 1, 64, 64, dtype=torch.uint8)
+    n = len(host)
+    c.k = torch.cat((c.k.view(torch.uint8), more)).view(fp8)               # a cache that grows
+    with pytest.raises(ValueError, match='v must be'):                      # and is not whole yet
+        c.attend(torch.zeros(1, 1, 64, dtype=torch.bfloat16), _i32([[0]]), _i32([5]))
+    c.v = torch.cat((c.v.view(torch.uint8), more)).view(fp8)
+    with pytest.raises(ValueError, match='scales must be'):
+        c.read(_i32([[0]]), _i32([5]), None, 1)
+    assert len(host) == n
+    c.scales = torch.cat((c.scales, torch.ones(3, 1, 2)))
+    _calls(c, host, 5, 1, 64)
+    for name in ('k', 'v', 'scales'):                                       # other memory behind the same tensors
+        t = getattr(c, name)
+        t.data = t.data.clone()
+    _calls(c, host, 5, 1, 64)
+    c.k, c.v, c.scales = torch.zeros(1, 2, 64, 32).char(), torch.zeros(1, 2, 32, 64).char(), torch.ones(1, 2, 2)
+    _calls(c, host, 1, 2, 32)
+    assert host[-1].bits == 1 and host[-1].scale == pytest.approx(32 ** -0.5) and c.dtype is torch.int8
+    for name in ('n_blocks', 'heads', 'head_dim', 'device', 'dtype'):       # what the tensors say
+        with pytest.raises(AttributeError):
+            setattr(c, name, getattr(c, name))
