@@ -91,6 +91,10 @@ class _Turn(torch.autograd.Function):
         return tuple(out)
 
 
+def _fixed(name):
+    return property(lambda self: getattr(self, name))
+
+
 class Rotary:
     """Rotary positions of heads of ``head_dim`` elements.
 
@@ -99,7 +103,13 @@ class Rotary:
     layout      'half': pair p of a section of n is (p, p + n/2); 'interleaved': (2p, 2p + 1)
     axes        coordinates of a position; each rotates rotary_dim / axes elements
     scaling     see ``rotary_frequencies``
+
+    These, and ``frequencies``, ``factor`` and ``turns`` that come of them, stay as they are: another choice is another
+    ``Rotary``.
     """
+
+    head_dim, rotary_dim, layout, axes = _fixed('_head_dim'), _fixed('_rotary_dim'), _fixed('_layout'), _fixed('_axes')
+    frequencies, factor, turns, device = _fixed('_frequencies'), _fixed('_factor'), _fixed('_turns'), _fixed('_device')
 
     def __init__(self, head_dim, rotary_dim=None, base=10000.0, layout='half', axes=1, scaling=None, device='cuda'):
         part = head_dim if rotary_dim is None else rotary_dim
@@ -109,17 +119,17 @@ class Rotary:
             raise ValueError(f'rotary: {part} of {head_dim} elements are not whole pairs for each of {axes} axes')
         if layout == 'interleaved' and head_dim % 2:
             raise ValueError('rotary: an interleaved head must be even')
-        self.head_dim, self.rotary_dim, self.layout, self.axes = head_dim, part, layout, axes
-        self.frequencies, self.factor = rotary_frequencies(part // axes, base, scaling)
+        self._head_dim, self._rotary_dim, self._layout, self._axes = head_dim, part, layout, axes
+        self._frequencies, self._factor = rotary_frequencies(part // axes, base, scaling)
         # turns per position in units of 2^-64 (a frequency of 2 pi or more wraps, as its angle does)
-        turns = [round(x / (2 * math.pi) * 2.0 ** 64) % (1 << 64) for x in self.frequencies]
-        self.turns = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device)
-        if not self.turns.is_cuda:
+        turns = [round(x / (2 * math.pi) * 2.0 ** 64) % (1 << 64) for x in self._frequencies]
+        self._turns = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device)
+        if not self._turns.is_cuda:
             raise RuntimeError('rotary needs a GPU (it runs in libba_hip.so)')
-        self.device = self.turns.device
+        self._device = self._turns.device
         # the fields of every call
         self._args = BaRotaryArgs(n_x=1, B=1, dim=head_dim, part=part, axes=axes, interleaved=layout == 'interleaved',
-                                  turns=self.turns.data_ptr(), factor=self.factor)
+                                  factor=self._factor)
         self._call = lib().ba_rotary
 
     def __call__(self, positions, *xs, out=None, inverse=False):
@@ -144,7 +154,7 @@ class Rotary:
 
     def _run(self, positions, xs, out, inverse):
         x = xs[0]
-        dtype, shape, dev = x.dtype, x.shape, self.device
+        dtype, shape, dev = x.dtype, x.shape, self._device
         lead = shape[:-2]
         n_lead = len(lead)
         if n_lead != 1 and n_lead != 2:
@@ -156,9 +166,9 @@ class Rotary:
         if not wide and positions.dtype is not torch.int32 or positions.device != dev:
             raise ValueError(f'rotary: positions must be int32 or int64 on {dev}')
         p_lead, p_stride = positions.shape, positions.stride()
-        if self.axes > 1:
-            if len(p_lead) < 2 or p_lead[-1] != self.axes:
-                raise ValueError(f'rotary: positions need a last dimension of {self.axes} axes, got {tuple(p_lead)}')
+        if self._axes > 1:
+            if len(p_lead) < 2 or p_lead[-1] != self._axes:
+                raise ValueError(f'rotary: positions need a last dimension of {self._axes} axes, got {tuple(p_lead)}')
             p_lead = p_lead[:-1]
         if p_lead != lead and (n_lead == 1 or p_lead != lead[1:]):
             raise ValueError(f'rotary: positions of shape {tuple(positions.shape)} for tokens {tuple(lead)}')
@@ -191,13 +201,13 @@ class Rotary:
             a.n_x = 2
             if n_lead == 2:
                 a.x_sb1, a.y_sb1 = xs_[0], ys_[0]
-        a.dtype, a.T = code, lead[-1]
+        a.dtype, a.T, a.turns = code, lead[-1], self._turns.data_ptr()
         if inverse:
             a.inverse = 1
         if wide:
             a.pos_int64 = 1
         a.positions, a.pos_st = positions.data_ptr(), p_stride[len(p_lead) - 1]
-        if self.axes > 1:
+        if self._axes > 1:
             a.pos_sa = p_stride[-1]
         if len(p_lead) == 2:
             a.pos_sb = p_stride[0]
@@ -209,9 +219,9 @@ class Rotary:
 
     def _strides(self, t, lead, dtype):
         shape, stride = t.shape, t.stride()
-        if (len(shape) != len(lead) + 2 or shape[:-2] != lead or shape[-1] != self.head_dim or shape[-2] == 0 or
-                t.dtype is not dtype or t.device != self.device):
-            raise ValueError(f'rotary: tensors must share tokens, type and device, with heads of {self.head_dim}: got '
+        if (len(shape) != len(lead) + 2 or shape[:-2] != lead or shape[-1] != self._head_dim or shape[-2] == 0 or
+                t.dtype is not dtype or t.device != self._device):
+            raise ValueError(f'rotary: tensors must share tokens, type and device, with heads of {self._head_dim}: got '
                              f'{tuple(shape)} {t.dtype} on {t.device}')
         if stride[-1] != 1:
             raise ValueError('rotary: the elements of a head must be contiguous')

@@ -206,3 +206,19 @@ def test_cache_follows_tensors_put_in_place_of_its_own(host):
     for name in ('n_blocks', 'heads', 'head_dim', 'device', 'dtype'):       # what the tensors say
         with pytest.raises(AttributeError):
             setattr(c, name, getattr(c, name))
+
+
+def test_rotary_says_what_it_was_made_with(host):
+    """The kernels get what the constructor laid out: assignments that they would not see are refused."""
+    from blast3r_amd.rotary import Rotary
+    rot, pos, x = Rotary(64, axes=2, device='cpu'), torch.zeros(3, 2, dtype=torch.int32), torch.randn(3, 2, 64)
+    for name in ('turns', 'frequencies', 'factor', 'head_dim', 'rotary_dim', 'layout', 'axes', 'device'):
+        with pytest.raises(AttributeError):
+            setattr(rot, name, getattr(rot, name))
+    assert (rot.head_dim, rot.rotary_dim, rot.layout, rot.axes, rot.factor) == (64, 64, 'half', 2, 1.0)
+    assert len(rot.frequencies) == 16 and rot.device == rot.turns.device
+    rot(pos, x)
+    assert host[-1].turns == rot.turns.data_ptr()
+    rot.turns.data = rot.turns.data.clone()                 # other memory behind the same tensor
+    rot(pos, x)
+    assert host[-1].turns == rot.turns.data_ptr()
