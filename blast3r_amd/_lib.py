@@ -301,11 +301,23 @@ def stream_ptr(device=None):
 
 
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+_tracing = getattr(torch._C, '_is_tracing', torch.jit.is_tracing)
+_modes = getattr(torch._C, '_len_torch_dispatch_stack', lambda: 1)
+
+
+def _traced():
+    """Whether a trace of torch's operations is being made, in which a launch would be missing."""
+    if _tracing():
+        return True
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    return get_proxy_mode() is not None
 
 
 def launch(call, args, device):
     """One launch of ``call(args, stream)`` on the current stream of ``device``, as tensors on it expect (the short way
     for calls whose host time counts: no stream object, no device guard where the device is the current one)."""
+    if (_tracing() or _modes()) and _traced():
+        raise RuntimeError('a trace of torch operations cannot hold this call: it is a launch of libba_hip.so')
     index = device.index
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):

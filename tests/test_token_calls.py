@@ -222,3 +222,23 @@ def test_rotary_says_what_it_was_made_with(host):
     rot.turns.data = rot.turns.data.clone()                 # other memory behind the same tensor
     rot(pos, x)
     assert host[-1].turns == rot.turns.data_ptr()
+
+
+# ---------------------------------------------------------------------------------- tracing
+
+def test_traces_are_refused(host, monkeypatch):
+    """A launch is no operation of torch's: a trace would keep the allocation of its result and nothing that fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from blast3r_amd import _lib, kv_cache, rotary
+    rot, pos, x = rotary.Rotary(64, device='cpu'), _i32([0, 1, 2]), torch.randn(3, 2, 64)
+    c = kv_cache.KVCache(2, 1, 64, device='cpu')
+    q, pages, lens = torch.zeros(1, 1, 64, dtype=torch.bfloat16), _i32([[0, 1]]), _i32([5])
+    for m in (kv_cache, rotary):
+        monkeypatch.setattr(m, 'launch', _lib.launch)       # which ends before anything of the GPU's
+    for f, args in ((lambda t: rot(pos, t), x), (lambda t: c.attend(t, pages, lens), q), (lambda t: c.append(t, t, pages, lens), q),
+                    (lambda t: c.read(pages, t, None, 1), lens)):
+        with pytest.raises(RuntimeError, match='trace'):
+            torch.jit.trace(f, (args,), check_trace=False)
+        with pytest.raises(RuntimeError, match='trace'):
+            make_fx(f)(args)
