@@ -242,3 +242,23 @@ def test_traces_are_refused(host, monkeypatch):
             torch.jit.trace(f, (args,), check_trace=False)
         with pytest.raises(RuntimeError, match='trace'):
             make_fx(f)(args)
+
+
+# ---------------------------------------------------------------------------------- addresses and strides (GPU)
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dim', [32, 64, 96, 128, 256])
+def test_append_of_fp32_rows_aligned_to_16_bytes_only(dim):
+    """Rows whose addresses are 16 bytes past a multiple of 32 are written as aligned ones are."""
+    from blast3r_amd.kv_cache import KVCache
+    gen = torch.Generator(device=DEV).manual_seed(dim)
+    base = torch.randn((2, 150 * 3 * dim + 8), device=DEV, generator=gen)
+    k, v = (b[4:-4].view(150, 3, dim)[:, 1:] for b in base)
+    assert k.data_ptr() % 32 == v.data_ptr() % 32 == 16
+    print(f'append {dim}', flush=True)
+    caches = [KVCache(4, 2, dim, torch.int8, device=DEV) for _ in range(2)]
+    pages = _i32([[2, 0, 3, 1]], DEV)
+    caches[0].append(k, v, pages, _i32([5], DEV))
+    caches[1].append(k.contiguous(), v.contiguous(), pages, _i32([5], DEV))
+    assert torch.equal(caches[0].k, caches[1].k) and torch.equal(caches[0].v, caches[1].v)
+    assert torch.equal(caches[0].scales, caches[1].scales) and bool(caches[0].k.any()) and bool(caches[0].v.any())
