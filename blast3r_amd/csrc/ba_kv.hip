@@ -381,7 +381,8 @@ static int kv_call(const ba_kv_args* args, void* stream, bool write) {
                "cache: head size must be 32, 64, 96, 128 or 256");
     BA_REQUIRE(a.bits == BA_FP8 || a.bits == BA_INT8, "cache: bits must be 0 (e4m3) or 1 (int8)");
     BA_REQUIRE(a.dtype >= 0 && a.dtype <= 2, "cache: rows must be fp32, fp16 or bf16");
-    BA_REQUIRE(a.n_rows >= 0 && a.rows_per_seq >= 0 && a.max_rows >= 0 && a.n_rows < (int64_t)1 << 31, "cache: bad sizes");
+    BA_REQUIRE(a.n_rows >= 0 && a.rows_per_seq >= 0 && a.max_rows >= 0 && a.n_rows < (int64_t)1 << 31 && a.max_rows < (int64_t)1 << 31 &&
+                   a.rows_per_seq < (int64_t)1 << 31, "cache: bad sizes");
     if (a.n_rows == 0 || a.n_seqs == 0 || a.max_rows == 0) return BA_OK;
     BA_REQUIRE(a.starts && a.rk && a.rv, "null pointer");
     BA_REQUIRE((a.n_pages == 0 || a.pages) && (a.n_blocks == 0 || (a.k && a.v && a.scales)), "null pointer");

@@ -262,3 +262,31 @@ def test_append_of_fp32_rows_aligned_to_16_bytes_only(dim):
     caches[1].append(k.contiguous(), v.contiguous(), pages, _i32([5], DEV))
     assert torch.equal(caches[0].k, caches[1].k) and torch.equal(caches[0].v, caches[1].v)
     assert torch.equal(caches[0].scales, caches[1].scales) and bool(caches[0].k.any()) and bool(caches[0].v.any())
+
+
+# ---------------------------------------------------------------------------------- limits of the C entry points (CPU)
+
+def _full(cls, **kw):
+    """Arguments that pass every check, with addresses that are only compared with each other."""
+    p = 4096
+    names = {n for n, _ in cls._fields_}
+    a = dict(k=p, v=p, scales=p, n_blocks=2, heads=2, dim=64, bits=0, n_seqs=1, pages=p, pages_stride=2, n_pages=2, dtype=2,
+             starts=p, lengths=p, offsets=p, n_rows=3, max_rows=3, rk=p, rv=p, q=p, o=p, q_heads=4, scale=1.0, n_splits=1)
+    return cls(**{**{n: x for n, x in a.items() if n in names}, **kw})
+
+
+def _refused(call, args, word):
+    import ctypes
+
+    from blast3r_amd import _lib
+    assert call(ctypes.byref(args), None) != 0 and word in _lib.lib().ba_last_error().decode(), _lib.lib().ba_last_error()
+
+
+@pytest.mark.parametrize('rows', [1 << 31, (1 << 63) - 62, (1 << 63) - 1])
+def test_cache_calls_refuse_bounds_on_rows_past_32_bits(rows):
+    """The number of blocks that a sequence may touch is rounded up from max_rows, which must not wrap."""
+    from blast3r_amd import _lib
+    L = _lib.lib()
+    for call in (L.ba_kv_write, L.ba_kv_read):
+        _refused(call, _full(_lib.BaKvArgs, max_rows=rows), 'bad sizes')
+        _refused(call, _full(_lib.BaKvArgs, max_rows=3, rows_per_seq=rows, offsets=None), 'bad sizes')
