@@ -1044,7 +1044,14 @@ extern "C" int ba_kv_attend(const ba_kv_attend_args* args, void* stream) {
     const int64_t tiles = (rows + tile - 1) / tile;
     // a launch has less than 2^32 threads
     BA_REQUIRE(tiles <= ((int64_t)1 << 23) / a.n_seqs / a.heads / a.n_splits, "attention: too many tiles for a call (max_rows is the bound that counts)");
+    // the join of the parts: those of a row are shared among threads while the chip has room for more of them
+    const int64_t jobs = a.n_rows * a.q_heads;
+    int lanes = 1, per_wg = 1;
     if (a.n_splits > 1) {
+        while (lanes < a.n_splits && 2 * lanes * (a.dim / 4) <= AT_T && jobs * (a.dim / 4) * lanes < 256 * 1024) lanes *= 2;
+        per_wg = AT_T / (a.dim / 4) / lanes;
+        // (which keeps the bytes of the workspace below 2^58 too)
+        BA_REQUIRE(jobs < (int64_t)1 << 31 && (jobs + per_wg - 1) / per_wg < (int64_t)1 << 24, "attention: too many rows for a call");
         BA_REQUIRE(a.workspace && (uintptr_t)a.workspace % 16 == 0, "null pointer");
         BA_REQUIRE(a.workspace_bytes >= ba_kv_attend_workspace_bytes(a.n_rows, a.q_heads, a.dim, a.n_splits), "attention: workspace too small");
     }
@@ -1057,12 +1064,6 @@ extern "C" int ba_kv_attend(const ba_kv_attend_args* args, void* stream) {
     switch (a.dim) { BA_AT_D(32) BA_AT_D(64) BA_AT_D(96) BA_AT_D(128) BA_AT_D(256) }
 #undef BA_AT_D
     if (rc != BA_OK || a.n_splits == 1) return rc;
-    const int64_t jobs = a.n_rows * a.q_heads;
-    // the parts of a row are shared among threads while the chip has room for more of them
-    int lanes = 1;
-    while (lanes < a.n_splits && 2 * lanes * (a.dim / 4) <= AT_T && jobs * (a.dim / 4) * lanes < 256 * 1024) lanes *= 2;
-    const int per_wg = AT_T / (a.dim / 4) / lanes;
-    BA_REQUIRE(jobs < (int64_t)1 << 31 && (jobs + per_wg - 1) / per_wg < (int64_t)1 << 24, "attention: too many rows for a call");
     hipLaunchKernelGGL(k_kv_join, dim3((unsigned)((jobs + per_wg - 1) / per_wg)), dim3(AT_T), 0, st, a, tile, lanes, wide);
     BA_LAUNCHED();
     return BA_OK;

@@ -290,3 +290,14 @@ def test_cache_calls_refuse_bounds_on_rows_past_32_bits(rows):
     for call in (L.ba_kv_write, L.ba_kv_read):
         _refused(call, _full(_lib.BaKvArgs, max_rows=rows), 'bad sizes')
         _refused(call, _full(_lib.BaKvArgs, max_rows=3, rows_per_seq=rows, offsets=None), 'bad sizes')
+
+
+def test_attention_checks_its_parts_before_it_launches():
+    """Sizes that the join of the parts cannot take are refused before the parts are made, and the room that their sums
+    need is not a number that wraps."""
+    from blast3r_amd import _lib
+    L = _lib.lib()
+    most = (1 << 63) - 1
+    for kw in (dict(n_rows=1 << 30, q_heads=2), dict(n_rows=(1 << 31) - 1, q_heads=65536, n_splits=65536)):
+        _refused(L.ba_kv_attend, _full(_lib.BaKvAttendArgs, **{**dict(n_splits=2, workspace=4096, workspace_bytes=most), **kw}), 'too many')
+        _refused(L.ba_kv_attend, _full(_lib.BaKvAttendArgs, **{**dict(n_splits=2, workspace=4096, workspace_bytes=64), **kw}), 'too many')
