@@ -1042,8 +1042,8 @@ extern "C" int ba_kv_attend(const ba_kv_attend_args* args, void* stream) {
     const int tile = v.rows;
     BA_REQUIRE(rows < ((int64_t)1 << 31) - 256, "attention: too many rows for a call");
     const int64_t tiles = (rows + tile - 1) / tile;
-    // a launch has less than 2^32 threads
-    BA_REQUIRE(tiles <= ((int64_t)1 << 23) / a.n_seqs / a.heads / a.n_splits, "attention: too many tiles for a call (max_rows is the bound that counts)");
+    // a launch has less than 2^32 threads, 512 to a workgroup
+    BA_REQUIRE(tiles <= (((int64_t)1 << 23) - 1) / a.n_seqs / a.heads / a.n_splits, "attention: too many tiles for a call (max_rows is the bound that counts)");
     // the join of the parts: those of a row are shared among threads while the chip has room for more of them
     const int64_t jobs = a.n_rows * a.q_heads;
     int lanes = 1, per_wg = 1;

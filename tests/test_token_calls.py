@@ -301,3 +301,11 @@ def test_attention_checks_its_parts_before_it_launches():
     for kw in (dict(n_rows=1 << 30, q_heads=2), dict(n_rows=(1 << 31) - 1, q_heads=65536, n_splits=65536)):
         _refused(L.ba_kv_attend, _full(_lib.BaKvAttendArgs, **{**dict(n_splits=2, workspace=4096, workspace_bytes=most), **kw}), 'too many')
         _refused(L.ba_kv_attend, _full(_lib.BaKvAttendArgs, **{**dict(n_splits=2, workspace=4096, workspace_bytes=64), **kw}), 'too many')
+
+
+def test_attention_launches_have_less_than_2_32_threads():
+    """2^23 workgroups of 512 threads are one too many."""
+    from blast3r_amd import _lib
+    a = _full(_lib.BaKvAttendArgs, dim=128, n_seqs=1 << 13, offsets=None, n_rows=1 << 18, rows_per_seq=256, max_rows=256,
+              heads=1024, q_heads=1024)
+    _refused(_lib.lib().ba_kv_attend, a, 'too many')
