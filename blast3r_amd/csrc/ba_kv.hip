@@ -58,6 +58,27 @@ __device__ __forceinline__ bool kv_share(const ba_kv_args& a, int s, int slot_of
     return true;
 }
 
+// Keys or values, head, sequence and block of the sequence's of this workgroup; slots: blocks that each sequence may touch,
+// or places of all (`packed`).
+struct KvPlace {
+    bool keys;
+    int h, s, slot;
+};
+
+__device__ __forceinline__ KvPlace kv_place(const ba_kv_args& a, int slots, int packed) {
+    unsigned id = blockIdx.x;
+    KvPlace r;
+    r.keys = (id & 1) == 0;
+    id >>= 1;
+    r.h = (int)(id % (unsigned)a.heads);
+    id /= (unsigned)a.heads;
+    r.s = (int)(id / (unsigned)slots);
+    r.slot = (int)(id % (unsigned)slots);
+    // n rows touch (n + 62) / 64 + 1 blocks at most, which is n / 64 + 2 or less
+    if (packed) r.s = seq_of_place(a.offsets, a.n_seqs, a.n_rows, 1, 64, 2, (unsigned)r.slot, r.slot);
+    return r;
+}
+
 __device__ __forceinline__ bool kv_there(const ba_kv_args& a, const KvShare& r) { return r.page >= 0 && r.page < a.n_blocks; }
 
 __device__ __forceinline__ uint32_t f32_bits(float x) { return __builtin_bit_cast(uint32_t, x); }
@@ -260,29 +281,23 @@ __device__ void kv_write_block(const ba_kv_args& a, const KvShare& sh, int h, bo
 }
 
 template <int D, int KT, typename T>
-__global__ void __launch_bounds__(KV_T) k_kv_write(ba_kv_args a, int slots, int wide) {
+__global__ void __launch_bounds__(KV_T) k_kv_write(ba_kv_args a, int slots, int packed, int wide) {
     __shared__ uint32_t tile[D * (KV_ROW / 4)];
     __shared__ uint32_t red[4];
-    unsigned id = blockIdx.x;
-    const bool keys = (id & 1) == 0;
-    id >>= 1;
-    const int h = (int)(id % (unsigned)a.heads);
-    id /= (unsigned)a.heads;
+    const KvPlace at = kv_place(a, slots, packed);
     KvShare sh;
-    if (!kv_share(a, (int)(id / (unsigned)slots), (int)(id % (unsigned)slots), sh)) return;
-    if (keys) kv_write_block<D, KT, T, true>(a, sh, h, wide != 0, tile, red);
-    else kv_write_block<D, KT, T, false>(a, sh, h, wide != 0, tile, red);
+    if (at.slot < 0 || !kv_share(a, at.s, at.slot, sh)) return;
+    if (at.keys) kv_write_block<D, KT, T, true>(a, sh, at.h, wide != 0, tile, red);
+    else kv_write_block<D, KT, T, false>(a, sh, at.h, wide != 0, tile, red);
 }
 
 template <int D, int KT, typename T>
-__global__ void __launch_bounds__(KV_T) k_kv_read(ba_kv_args a, int slots, int wide) {
+__global__ void __launch_bounds__(KV_T) k_kv_read(ba_kv_args a, int slots, int packed, int wide) {
     __shared__ uint32_t tile[D * (KV_ROW / 4)];
-    unsigned id = blockIdx.x;
-    const bool keys = (id & 1) == 0;
-    id >>= 1;
-    const int h = (int)(id % (unsigned)a.heads), tid = threadIdx.x;
-    id /= (unsigned)a.heads;
-    const int s = (int)(id / (unsigned)slots), slot = (int)(id % (unsigned)slots);
+    const KvPlace at = kv_place(a, slots, packed);
+    const bool keys = at.keys;
+    const int h = at.h, s = at.s, slot = at.slot, tid = threadIdx.x;
+    if (slot < 0) return;
     KvShare sh;
     const bool held = kv_share(a, s, slot, sh) && kv_there(a, sh);
     T* y = (T*)(keys ? a.rk : a.rv);
@@ -361,13 +376,13 @@ __global__ void __launch_bounds__(KV_T) k_kv_read(ba_kv_args a, int slots, int w
 }
 
 template <int D, int KT, typename T>
-static int launch_kv(const ba_kv_args& a, bool write, int slots, unsigned nb, hipStream_t st) {
+static int launch_kv(const ba_kv_args& a, bool write, int slots, bool packed, unsigned nb, hipStream_t st) {
     const int64_t s[4] = {a.rk_st, a.rk_sh, a.rv_st, a.rv_sh};
     // a thread moves 8 elements at a time at most
     bool wide = (uintptr_t)a.rk % 16 == 0 && (uintptr_t)a.rv % 16 == 0;
     for (int i = 0; i < 4; ++i) wide = wide && s[i] % 8 == 0;
-    if (write) hipLaunchKernelGGL((k_kv_write<D, KT, T>), dim3(nb), dim3(KV_T), 0, st, a, slots, (int)wide);
-    else hipLaunchKernelGGL((k_kv_read<D, KT, T>), dim3(nb), dim3(KV_T), 0, st, a, slots, (int)wide);
+    if (write) hipLaunchKernelGGL((k_kv_write<D, KT, T>), dim3(nb), dim3(KV_T), 0, st, a, slots, (int)packed, (int)wide);
+    else hipLaunchKernelGGL((k_kv_read<D, KT, T>), dim3(nb), dim3(KV_T), 0, st, a, slots, (int)packed, (int)wide);
     BA_LAUNCHED();
     return BA_OK;
 }
@@ -390,12 +405,18 @@ static int kv_call(const ba_kv_args* args, void* stream, bool write) {
     const int64_t strides[4] = {a.rk_st, a.rk_sh, a.rv_st, a.rv_sh};
     for (int i = 0; i < 4; ++i)
         BA_REQUIRE(strides[i] > -((int64_t)1 << 31) && strides[i] < (int64_t)1 << 31, "cache: strides of rows and heads must be below 2^31");
-    const int64_t slots = (a.max_rows + 62) / 64 + 1;
+    int64_t slots = (a.max_rows + 62) / 64 + 1, per_slot = (int64_t)a.n_seqs * a.heads;
     // a launch has less than 2^32 threads
-    BA_REQUIRE(slots <= ((int64_t)1 << 23) / a.n_seqs / a.heads - 1, "cache: too many blocks for a call (max_rows is the bound that counts)");
-    const unsigned nb = (unsigned)(slots * a.n_seqs * a.heads * 2);
+    const int64_t most = ((int64_t)1 << 23) - 1;
+    const bool packed = a.offsets && slots > most / per_slot;
+    if (packed) {
+        slots = a.n_rows / 64 + 2 * (int64_t)a.n_seqs;
+        per_slot = a.heads;
+    }
+    BA_REQUIRE(slots <= most / per_slot, "cache: too many blocks for a call");
+    const unsigned nb = (unsigned)(slots * per_slot * 2);
     hipStream_t st = (hipStream_t)stream;
-#define BA_KV_D(D, KT, T) case D: return launch_kv<D, KT, T>(a, write, (int)slots, nb, st);
+#define BA_KV_D(D, KT, T) case D: return launch_kv<D, KT, T>(a, write, (int)slots, packed, nb, st);
 #define BA_KV_ALL(KT, T) \
     switch (a.dim) { BA_KV_D(32, KT, T) BA_KV_D(64, KT, T) BA_KV_D(96, KT, T) BA_KV_D(128, KT, T) BA_KV_D(256, KT, T) }
     if (a.bits == BA_FP8) {

@@ -120,6 +120,24 @@ __device__ __forceinline__ AtSeq at_seq(const ba_kv_attend_args& a, int s) {
     return {row0, (int)(len < most ? len : most), first, (int)(n < a.max_rows ? n : a.max_rows)};
 }
 
+// The tile, part, head and sequence of this workgroup; n_tiles: tiles of each sequence, or places of all (`packed`).
+struct AtPlace {
+    int tile, sp, kh, s;
+};
+
+__device__ __forceinline__ AtPlace at_place(const ba_kv_attend_args& a, int rows, int n_tiles, int packed) {
+    unsigned id = xcd_block(blockIdx.x, gridDim.x);
+    AtPlace r;
+    r.tile = (int)(id % (unsigned)n_tiles);
+    id /= (unsigned)n_tiles;
+    r.sp = (int)(id % (unsigned)a.n_splits);
+    id /= (unsigned)a.n_splits;
+    r.kh = (int)(id % (unsigned)a.heads);
+    r.s = (int)(id / (unsigned)a.heads);
+    if (packed) r.s = seq_of_place(a.offsets, a.n_seqs, a.n_rows, a.q_heads / a.heads, rows, 1, (unsigned)r.tile, r.tile);
+    return r;
+}
+
 // Blocks [lo, hi) that rows [row, row + rows) (of the sequence's rows * group) see, cut into parts of `per` blocks.
 struct AtBlocks {
     int lo, hi, per;
@@ -257,7 +275,7 @@ constexpr int at_waves(int d, int cols) { return cols == 16 ? (d <= 64 ? 4 : d <
 // blocks; every wave reads and converts its own, a block ahead.  8 or 16 waves to a workgroup were no faster on short
 // sequences (777 tokens: 8.4 and 9.4 us against 8.5, most of it launch and dependent loads).
 template <int D, int KT, int COLS, bool HALF>
-__global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_attend_args a, int n_tiles, int wide) {
+__global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_attend_args a, int n_tiles, int packed, int wide) {
     typedef Mma<COLS> M;
     typedef typename M::acc acc;
     constexpr int NG = 64 / COLS, NB = NG, CREG = COLS * COLS / 64, TPL = 64 / NG;
@@ -267,16 +285,12 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_att
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = wave;
     const int n = lane % COLS, g = lane / COLS;
-    unsigned id = xcd_block(blockIdx.x, gridDim.x);
-    const int tile = (int)(id % (unsigned)n_tiles);
-    id /= (unsigned)n_tiles;
-    const int sp = (int)(id % (unsigned)a.n_splits);
-    id /= (unsigned)a.n_splits;
-    const int kh = (int)(id % (unsigned)a.heads), s = (int)(id / (unsigned)a.heads);
+    const AtPlace at_wg = at_place(a, ROWS, n_tiles, packed);
+    const int tile = at_wg.tile, sp = at_wg.sp, kh = at_wg.kh, s = at_wg.s;
     const int group = a.q_heads / a.heads;
     const AtSeq q = at_seq(a, s);
     const int all = q.rows * group, tile0 = tile * ROWS;
-    if (tile0 >= all) return;
+    if (tile < 0 || tile0 >= all) return;
     int lo, hi;
     at_part(at_blocks(a, q, group, tile0, ROWS), sp, lo, hi);
     if (lo >= hi && a.n_splits > 1) return;                  // k_kv_join knows which parts there are
@@ -565,7 +579,7 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_att
 // bank conflicts 1201; 8 waves to a workgroup 1126; no maximum formed until a sum calls for it 1062; 32-bit arithmetic on
 // rows and blocks 1024.
 template <int D, int KT, int NCB, int WAVES, bool HALF>
-__global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_attend_tile(ba_kv_attend_args a, int n_tiles, int wide) {
+__global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_attend_tile(ba_kv_attend_args a, int n_tiles, int packed, int wide) {
     typedef Mma<32> M;
     typedef M::acc acc;
     constexpr int KS = D / 16, DB = D / 32, T = 64 * WAVES, ROWS = WAVES * 32 * NCB, PC = (4 * D + T - 1) / T;
@@ -574,16 +588,12 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane % 32, g = lane / 32;
-    unsigned id = xcd_block(blockIdx.x, gridDim.x);
-    const int tile = (int)(id % (unsigned)n_tiles);
-    id /= (unsigned)n_tiles;
-    const int sp = (int)(id % (unsigned)a.n_splits);
-    id /= (unsigned)a.n_splits;
-    const int kh = (int)(id % (unsigned)a.heads), s = (int)(id / (unsigned)a.heads);
+    const AtPlace at_wg = at_place(a, ROWS, n_tiles, packed);
+    const int tile = at_wg.tile, sp = at_wg.sp, kh = at_wg.kh, s = at_wg.s;
     const int group = a.q_heads / a.heads;
     const AtSeq q = at_seq(a, s);
     const int all = q.rows * group, tile0 = tile * ROWS;
-    if (tile0 >= all) return;
+    if (tile < 0 || tile0 >= all) return;
     int lo, hi;
     at_part(at_blocks(a, q, group, tile0, ROWS), sp, lo, hi);
     if (lo >= hi && a.n_splits > 1) return;                  // k_kv_join knows which parts there are
@@ -975,20 +985,20 @@ static AtShape at_shape(int64_t rows, int dim) {
 }
 
 template <int D, int KT, bool HALF>
-static void launch_attend(const ba_kv_attend_args& a, AtShape v, unsigned nb, int tiles, int wide, hipStream_t st) {
+static void launch_attend(const ba_kv_attend_args& a, AtShape v, unsigned nb, int tiles, int packed, int wide, hipStream_t st) {
     const dim3 grid(nb), block(64 * v.waves);
-    if (v.cols == 16) hipLaunchKernelGGL((k_kv_attend<D, KT, 16, HALF>), grid, block, 0, st, a, tiles, wide);
-    else if (v.ncb == 0) hipLaunchKernelGGL((k_kv_attend<D, KT, 32, HALF>), grid, block, 0, st, a, tiles, wide);
-    else if (v.rows == 128) hipLaunchKernelGGL((k_kv_attend_tile<D, KT, 1, 4, HALF>), grid, block, 0, st, a, tiles, wide);
-    else if constexpr (D <= 64) hipLaunchKernelGGL((k_kv_attend_tile<D, KT, 2, 4, HALF>), grid, block, 0, st, a, tiles, wide);
-    else if constexpr (D <= 128) hipLaunchKernelGGL((k_kv_attend_tile<D, KT, 1, 8, HALF>), grid, block, 0, st, a, tiles, wide);
+    if (v.cols == 16) hipLaunchKernelGGL((k_kv_attend<D, KT, 16, HALF>), grid, block, 0, st, a, tiles, packed, wide);
+    else if (v.ncb == 0) hipLaunchKernelGGL((k_kv_attend<D, KT, 32, HALF>), grid, block, 0, st, a, tiles, packed, wide);
+    else if (v.rows == 128) hipLaunchKernelGGL((k_kv_attend_tile<D, KT, 1, 4, HALF>), grid, block, 0, st, a, tiles, packed, wide);
+    else if constexpr (D <= 64) hipLaunchKernelGGL((k_kv_attend_tile<D, KT, 2, 4, HALF>), grid, block, 0, st, a, tiles, packed, wide);
+    else if constexpr (D <= 128) hipLaunchKernelGGL((k_kv_attend_tile<D, KT, 1, 8, HALF>), grid, block, 0, st, a, tiles, packed, wide);
 }
 
 template <int D>
-static int launch_attend(const ba_kv_attend_args& a, AtShape v, unsigned nb, int tiles, int wide, hipStream_t st) {
+static int launch_attend(const ba_kv_attend_args& a, AtShape v, unsigned nb, int tiles, int packed, int wide, hipStream_t st) {
     const bool half = a.dtype == BA_F16;
-    if (a.bits == BA_FP8) half ? launch_attend<D, BA_FP8, true>(a, v, nb, tiles, wide, st) : launch_attend<D, BA_FP8, false>(a, v, nb, tiles, wide, st);
-    else half ? launch_attend<D, BA_INT8, true>(a, v, nb, tiles, wide, st) : launch_attend<D, BA_INT8, false>(a, v, nb, tiles, wide, st);
+    if (a.bits == BA_FP8) half ? launch_attend<D, BA_FP8, true>(a, v, nb, tiles, packed, wide, st) : launch_attend<D, BA_FP8, false>(a, v, nb, tiles, packed, wide, st);
+    else half ? launch_attend<D, BA_INT8, true>(a, v, nb, tiles, packed, wide, st) : launch_attend<D, BA_INT8, false>(a, v, nb, tiles, packed, wide, st);
     BA_LAUNCHED();
     return BA_OK;
 }
@@ -1041,9 +1051,15 @@ extern "C" int ba_kv_attend(const ba_kv_attend_args* args, void* stream) {
     const AtShape v = at_shape(rows, a.dim);
     const int tile = v.rows;
     BA_REQUIRE(rows < ((int64_t)1 << 31) - 256, "attention: too many rows for a call");
-    const int64_t tiles = (rows + tile - 1) / tile;
+    int64_t tiles = (rows + tile - 1) / tile, per_tile = (int64_t)a.n_seqs * a.heads * a.n_splits;
     // a launch has less than 2^32 threads, 512 to a workgroup
-    BA_REQUIRE(tiles <= (((int64_t)1 << 23) - 1) / a.n_seqs / a.heads / a.n_splits, "attention: too many tiles for a call (max_rows is the bound that counts)");
+    const int64_t most = ((int64_t)1 << 23) - 1;
+    const bool packed = a.offsets && tiles > most / per_tile;
+    if (packed) {
+        tiles = a.n_rows * group / tile + a.n_seqs;
+        per_tile = (int64_t)a.heads * a.n_splits;
+    }
+    BA_REQUIRE(tiles <= most / per_tile, "attention: too many tiles for a call");
     // the join of the parts: those of a row are shared among threads while the chip has room for more of them
     const int64_t jobs = a.n_rows * a.q_heads;
     int lanes = 1, per_wg = 1;
@@ -1055,12 +1071,12 @@ extern "C" int ba_kv_attend(const ba_kv_attend_args* args, void* stream) {
         BA_REQUIRE(a.workspace && (uintptr_t)a.workspace % 16 == 0, "null pointer");
         BA_REQUIRE(a.workspace_bytes >= ba_kv_attend_workspace_bytes(a.n_rows, a.q_heads, a.dim, a.n_splits), "attention: workspace too small");
     }
-    const unsigned nb = (unsigned)(tiles * a.n_seqs * a.heads * a.n_splits);
+    const unsigned nb = (unsigned)(tiles * per_tile);
     // loads of 8 queries, stores of 4 outputs
     const int wide = (uintptr_t)a.q % 16 == 0 && (uintptr_t)a.o % 8 == 0 && a.q_st % 8 == 0 && a.q_sh % 8 == 0 && a.o_st % 4 == 0 && a.o_sh % 4 == 0;
     hipStream_t st = (hipStream_t)stream;
     int rc = BA_ERR_UNSUPPORTED;
-#define BA_AT_D(D) case D: rc = launch_attend<D>(a, v, nb, (int)tiles, wide, st); break;
+#define BA_AT_D(D) case D: rc = launch_attend<D>(a, v, nb, (int)tiles, (int)packed, wide, st); break;
     switch (a.dim) { BA_AT_D(32) BA_AT_D(64) BA_AT_D(96) BA_AT_D(128) BA_AT_D(256) }
 #undef BA_AT_D
     if (rc != BA_OK || a.n_splits == 1) return rc;

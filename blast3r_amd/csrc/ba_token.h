@@ -56,4 +56,22 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
     }
 }
 
+// Ragged calls whose sequences may each have all rows, as far as the host knows, can be too large for a grid of so many
+// places for every one of them.  Then places are laid out by the offsets: sequence s has those from
+// floor(offsets[s] * mul / div) + s * more on, up to the next one's, which is at least its rows * mul / div, rounded up
+// (more = 1).  The sequence of place `w`, and which of its places that is (below 0: none of any sequence).
+__device__ __forceinline__ int seq_of_place(const int32_t* offsets, int n_seqs, int64_t n_rows, int mul, int div, int more, unsigned w, int& place) {
+    auto first = [&](int s) {
+        const int64_t at = offsets[s];
+        return (at < 0 ? 0 : at > n_rows ? n_rows : at) * mul / div + (int64_t)s * more;
+    };
+    int s = 0, e = n_seqs;                                   // the last s with first(s) <= w
+    while (e - s > 1) {
+        const int c = (s + e) >> 1;
+        if (first(c) <= (int64_t)w) s = c; else e = c;
+    }
+    place = (int)((int64_t)w - first(s));
+    return s;
+}
+
 }  // namespace ba

@@ -309,3 +309,61 @@ def test_attention_launches_have_less_than_2_32_threads():
     a = _full(_lib.BaKvAttendArgs, dim=128, n_seqs=1 << 13, offsets=None, n_rows=1 << 18, rows_per_seq=256, max_rows=256,
               heads=1024, q_heads=1024)
     _refused(_lib.lib().ba_kv_attend, a, 'too many')
+
+
+# ---------------------------------------------------------------------------------- many sequences without a bound on their rows
+
+def test_ragged_calls_of_many_sequences_are_not_too_large(monkeypatch):
+    """A call whose rows fit the chip many times over is no longer refused for the rows that each sequence might have:
+    what comes after the checks of its size is the launch, which fails here for want of a GPU."""
+    if torch.cuda.is_available():
+        pytest.skip('would launch on addresses that are none')
+    from blast3r_amd import _lib
+    L = _lib.lib()
+    for S in (4096, 70000):
+        n = 200 * S
+        for call, a in ((L.ba_kv_write, _full(_lib.BaKvArgs, n_seqs=S, n_rows=n, max_rows=n, heads=8)),
+                        (L.ba_kv_read, _full(_lib.BaKvArgs, n_seqs=S, n_rows=n, max_rows=n, heads=8)),
+                        (L.ba_kv_attend, _full(_lib.BaKvAttendArgs, n_seqs=S, n_rows=n, max_rows=n, heads=8, q_heads=32))):
+            import ctypes
+            assert call(ctypes.byref(a), None) != 0
+            assert b'too many' not in L.ba_last_error(), (S, L.ba_last_error())
+    # what no launch can take, in rows or in sequences
+    big = (1 << 31) - 1
+    for kw in (dict(n_rows=big, max_rows=big, heads=4096, q_heads=4096), dict(n_seqs=1 << 22, heads=8, q_heads=8)):
+        _refused(L.ba_kv_attend, _full(_lib.BaKvAttendArgs, **kw), 'too many')
+        kw.pop('q_heads')
+        _refused(L.ba_kv_write, _full(_lib.BaKvArgs, **kw), 'too many')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', [torch.float8_e4m3fn, torch.int8])
+def test_ragged_calls_of_many_sequences_without_a_bound(bits):
+    """3000 sequences: with max_new left out their rows are found by the offsets, and everything is as with a close bound."""
+    from blast3r_amd.kv_cache import KVCache
+    rng = np.random.default_rng(3)
+    S, H, G, D = 3000, 8, 2, 32
+    new = rng.integers(0, 41, S)
+    new[[0, 1, 700, S - 2]] = 0
+    new[[5, S - 1]] = 200
+    held = rng.integers(0, 200, S)
+    blocks = (held + new + 63) // 64
+    pages = np.full((S, int(blocks.max())), -1)
+    order, at = rng.permutation(int(blocks.sum())), 0
+    for s, b in enumerate(blocks):
+        pages[s, :b] = order[at:at + b]
+        at += b
+    n = int(new.sum())
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    k, v = (torch.randn((n, H, D), device=DEV, generator=gen).bfloat16() for _ in range(2))
+    q = torch.randn((n, H * G, D), device=DEV, generator=gen).bfloat16()
+    pages, held_t, lens, off = _i32(pages, DEV), _i32(held, DEV), _i32(held + new, DEV), _i32(np.concatenate(([0], np.cumsum(new))), DEV)
+    caches = [KVCache(int(blocks.sum()), H, D, bits, device=DEV) for _ in range(2)]
+    out = []
+    for c, most in zip(caches, (200, None)):
+        print(f'many sequences {bits} {most}', flush=True)
+        c.append(k, v, pages, held_t, offsets=off, max_new=most)
+        o, lse = c.attend(q, pages, lens, offsets=off, max_new=most, return_lse=True)
+        out.append((c.k.view(torch.uint8), c.v.view(torch.uint8), c.scales, o, lse, *c.read(pages, held_t, off, n, max_count=most)))
+    for a, b in zip(*out):
+        assert torch.equal(a, b) and bool(b.any())
