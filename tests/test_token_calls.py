@@ -1,8 +1,14 @@
 """What the token operators' Python side owes to autograd, to tracing and to tensors that change hands (CPU: launches are
 recorded instead of made), and calls of tests/test_tokens.py's operators that it leaves out (GPU)."""
+import ctypes
+import math
+
 import numpy as np
 import pytest
 import torch
+
+from oracle import tokens as otok
+from test_tokens import HALF_STEP, _cache, _check, _np, _pages
 
 DEV = 'cuda:0'
 
@@ -88,7 +94,6 @@ def test_outputs_that_require_a_gradient_are_refused(host):
 
 def test_forward_mode_tangents_go_through_rotary(host, monkeypatch):
     """The map is linear: a tangent is rotated as its tensor is, and one that is not there counts as zero."""
-    import ctypes
     from torch.autograd import forward_ad
 
     from blast3r_amd import rotary
@@ -276,8 +281,6 @@ def _full(cls, **kw):
 
 
 def _refused(call, args, word):
-    import ctypes
-
     from blast3r_amd import _lib
     assert call(ctypes.byref(args), None) != 0 and word in _lib.lib().ba_last_error().decode(), _lib.lib().ba_last_error()
 
@@ -325,7 +328,6 @@ def test_ragged_calls_of_many_sequences_are_not_too_large(monkeypatch):
         for call, a in ((L.ba_kv_write, _full(_lib.BaKvArgs, n_seqs=S, n_rows=n, max_rows=n, heads=8)),
                         (L.ba_kv_read, _full(_lib.BaKvArgs, n_seqs=S, n_rows=n, max_rows=n, heads=8)),
                         (L.ba_kv_attend, _full(_lib.BaKvAttendArgs, n_seqs=S, n_rows=n, max_rows=n, heads=8, q_heads=32))):
-            import ctypes
             assert call(ctypes.byref(a), None) != 0
             assert b'too many' not in L.ba_last_error(), (S, L.ba_last_error())
     # what no launch can take, in rows or in sequences
@@ -367,3 +369,138 @@ def test_ragged_calls_of_many_sequences_without_a_bound(bits):
         out.append((c.k.view(torch.uint8), c.v.view(torch.uint8), c.scales, o, lse, *c.read(pages, held_t, off, n, max_count=most)))
     for a, b in zip(*out):
         assert torch.equal(a, b) and bool(b.any())
+
+
+# ---------------------------------------------------------------------------------- attention: what test_tokens.py leaves out (GPU)
+
+def _parts(S, heads, q_heads, dim, rows, n_pages):
+    from blast3r_amd import _lib
+    return _lib.lib().ba_kv_attend_splits(S, heads, q_heads, dim, rows, n_pages)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('tokens', [500, 3000])             # in one part, and in several
+@pytest.mark.parametrize('dim,group,n', [(64, 2, 3), (128, 1, 1), (96, 3, 9), (64, 2, 50), (64, 1, 300), (128, 2, 130), (256, 1, 40)])
+def test_attend_of_unaligned_queries_and_outputs(dim, group, n, tokens, dtype):
+    """Queries and outputs at odd addresses with odd strides, the outputs' heads first: the same numbers as aligned ones, and
+    nothing else of the outputs' memory is written."""
+    heads, Hq = 2, 2 * group
+    c, _ = _cache(60, heads, dim, 'int8', seed=dim)
+    pages = _i32(_pages(np.random.default_rng(n), [(tokens + 63) // 64], 60, (tokens + 63) // 64), DEV)
+    assert (_parts(1, heads, Hq, dim, n, pages.shape[1]) > 1) == (tokens == 3000)
+    lens = _i32([tokens], DEV)
+    x = (2 * torch.randn((n, Hq, dim), generator=torch.Generator().manual_seed(n))).to(dtype).to(DEV)
+    print(f'attend unaligned {dim} {group} {n} {tokens} {dtype}', flush=True)
+    want, want_lse = c.attend(x, pages, lens, return_lse=True)
+    row = Hq * (dim + 3) + 4
+    q = torch.zeros(n * row + 1, dtype=dtype, device=DEV)[1:].as_strided((n, Hq, dim), (row, dim + 3, 1), 1)
+    q.copy_(x)
+    head = n * (dim + 1) + 2
+    base = torch.full((Hq * head + 1,), 7.0, dtype=dtype, device=DEV)
+    out = base.as_strided((n, Hq, dim), (dim + 1, head, 1), 1)
+    expect = base.clone()
+    expect.as_strided(out.shape, out.stride(), 1).copy_(want)
+    got, lse = c.attend(q, pages, lens, out=out, return_lse=True)
+    assert got is out and torch.equal(base, expect) and torch.equal(lse, want_lse)
+    base.fill_(7.0)
+    c.attend(x, pages, lens, out=out)                       # one side at a time
+    assert torch.equal(base, expect)
+    assert torch.equal(c.attend(q, pages, lens), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n,most', [(10, 7), (40, 20), (150, 40), (150, 130), (600, 300)])
+@pytest.mark.parametrize('splits', [1, 2])
+def test_attend_leaves_rows_past_the_bound_alone(n, most, splits):
+    """Rows past max_rows of their sequence keep their outputs and their lse; the others are as in a call without them."""
+    from blast3r_amd import _lib
+    L = _lib.lib()
+    heads, D, counts, lens = 2, 64, [n, 3], [3000, 1200]
+    c, o = _cache(70, heads, D, 'fp8')
+    pages = _pages(np.random.default_rng(n), [47, 19], 70, 47)
+    q = torch.randn((n + 3, heads, D), generator=torch.Generator().manual_seed(n)).bfloat16().to(DEV)
+    y, lse = torch.full_like(q, 7.0), torch.full((n + 3, heads), 5.0, device=DEV)
+    p, off, ln = _i32(pages, DEV), _i32([0, n, n + 3], DEV), _i32(lens, DEV)
+    size = L.ba_kv_attend_workspace_bytes(n + 3, heads, D, splits)
+    work = torch.full((max(size, 16),), 255, dtype=torch.uint8, device=DEV)
+    a = _lib.BaKvAttendArgs(k=c.k.data_ptr(), v=c.v.data_ptr(), scales=c.scales.data_ptr(), n_blocks=70, heads=heads, dim=D, bits=0,
+                            n_seqs=2, pages=p.data_ptr(), pages_stride=47, n_pages=47, dtype=2, lengths=ln.data_ptr(),
+                            offsets=off.data_ptr(), n_rows=n + 3, max_rows=most, q=q.data_ptr(), o=y.data_ptr(), lse=lse.data_ptr(),
+                            q_st=heads * D, q_sh=D, o_st=heads * D, o_sh=D, q_heads=heads, causal=1, scale=0.125, n_splits=splits,
+                            workspace=work.data_ptr(), workspace_bytes=size)
+    print(f'attend bound {n} {most} {splits}', flush=True)
+    _lib.check(L.ba_kv_attend(ctypes.byref(a), _lib.stream_ptr(DEV)))
+    assert bool((y[most:n] == 7.0).all()) and bool((lse[most:n] == 5.0).all())
+    want, want_lse, size = otok.attend(o, _np(q), pages, lens, counts, 0.125)
+    done = np.r_[0:most, n:n + 3]
+    assert np.all(np.abs(_np(y) - want)[done] <= 1.2e-3 * size[done] + HALF_STEP[q.dtype] * np.abs(want[done]))
+    assert np.all(np.abs(_np(lse) - want_lse)[done] <= 6e-4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', ['fp8', 'int8'])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('dim,group,n,window', [(32, 1, 70, None), (32, 2, 150, None), (32, 2, 150, 1500), (256, 1, 70, None),
+                                                (256, 2, 100, None), (256, 2, 100, 1300), (96, 1, 140, None)])
+def test_attend_of_many_rows_in_several_parts(dim, group, n, window, dtype, bits):
+    """Shared blocks (more than 32 rows) for the smallest and the largest heads, with the keys cut into parts."""
+    tokens = 2300
+    assert _parts(1, 1, group, dim, n, 36) > 1
+    c, o = _cache(37, 1, dim, bits, seed=n)
+    rng = np.random.default_rng(n)
+    pages = _pages(rng, [36], 37, 36)
+    q = torch.tensor(rng.normal(size=(n, group, dim)) * 2.0, dtype=torch.float32).to(dtype).to(DEV)
+    print(f'attend parts {bits} {dtype} {dim} {group} {n} {window}', flush=True)
+    _check(c, o, q, pages, [tokens], [n], True, window)
+    _check(c, o, q, pages, [tokens], [n], False, window)
+
+
+# ---------------------------------------------------------------------------------- derivatives, and a cache that grows (GPU)
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_rotary_in_forward_mode(dtype):
+    """The tangent is the rotation of the tangent, also of one without contiguous heads, and of the gradient's."""
+    from torch.autograd import forward_ad
+
+    from blast3r_amd.rotary import Rotary
+    rot = Rotary(64, axes=2, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    mk = lambda *s: torch.randn(s, device=DEV, generator=gen).to(dtype)  # noqa: E731
+    pos = torch.randint(0, 99, (5, 2), device=DEV, generator=gen, dtype=torch.int32)
+    q, k, t = mk(5, 4, 64), mk(5, 2, 64), mk(5, 64, 4).transpose(1, 2)
+    y, z, dy, dt = rot(pos, q), rot(pos, k), rot(pos, t.contiguous()), rot(pos, t.contiguous(), inverse=True)
+    for mode in (torch.no_grad, torch.enable_grad):
+        with forward_ad.dual_level(), mode():
+            a, b = rot(pos, forward_ad.make_dual(q, t), k)
+            a, b = forward_ad.unpack_dual(a), forward_ad.unpack_dual(b)
+            assert torch.equal(a.primal, y) and torch.equal(b.primal, z) and torch.equal(a.tangent, dy)
+            assert b.tangent is None or not b.tangent.any()
+    with forward_ad.dual_level():                           # forward over reverse
+        w = q.clone().requires_grad_()
+        (g,) = torch.autograd.grad(rot(pos, w), w, forward_ad.make_dual(q, t))
+        assert torch.equal(forward_ad.unpack_dual(g).tangent, dt)
+
+
+@pytest.mark.gpu
+def test_growing_a_cache_by_assignment():
+    from blast3r_amd.kv_cache import KVCache
+    heads, D = 2, 64
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    k, v, q = (torch.randn((200, heads, D), device=DEV, generator=gen).bfloat16() for _ in range(3))
+    lens = _i32([200], DEV)
+    big = KVCache(8, heads, D, torch.int8, device=DEV)
+    big.append(k, v, _i32([[1, 0, 6, 7]], DEV), lens - 200)
+    c = KVCache(2, heads, D, torch.int8, device=DEV)
+    c.append(k[:100], v[:100], _i32([[1, 0]], DEV), lens - 200)
+    for name, fresh in (('k', torch.zeros), ('v', torch.zeros), ('scales', torch.ones)):
+        t = getattr(c, name)
+        setattr(c, name, torch.cat((t, fresh((6, *t.shape[1:]), dtype=t.dtype, device=DEV))))
+    c.append(k[100:], v[100:], _i32([[1, 0, 6, 7]], DEV), lens - 100)
+    one, two = (x.read(_i32([[1, 0, 6, 7]], DEV), lens - 200, None, 200, dtype=torch.float32) for x in (c, big))
+    # the second block was filled in two calls, and its codes may have been made anew: one step of its factor apart at most
+    for a, b, f in zip(one, two, c.scales.unbind(-1)):
+        assert torch.equal(a[:64], b[:64]) and torch.equal(a[128:], b[128:])
+        assert bool(((a[64:128] - b[64:128]).abs() <= 1.01 * f[0][:, None]).all())
+    assert c.n_blocks == 8 and c.attend(q, _i32([[1, 0, 6, 7]], DEV), lens).isfinite().all()
