@@ -328,15 +328,19 @@ def launch(call, args, device):
         check(status)
 
 
+def dual_level():
+    """Whether forward-mode tangents can be about (there are none outside a dual level)."""
+    return getattr(forward_ad, '_current_level', 0) >= 0
+
+
 def has_tangent(*tensors):
-    """Whether one of them carries a tangent of forward-mode differentiation (there are none outside a dual level)."""
-    return getattr(forward_ad, '_current_level', 0) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    """Whether one of them carries a tangent of forward-mode differentiation."""
+    return dual_level() and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
-def written(*tensors):
-    """Says that a kernel wrote to tensors that were there before the call: what autograd or a cache keyed by versions
-    keeps of them is out of date."""
-    torch.autograd.graph.increment_version(tensors)
+# written(tensors): a kernel wrote to tensors that were there before the call, so that what autograd or a cache keyed by
+# versions keeps of them is out of date (without the public function's own 0.3 us)
+written = getattr(torch._C, '_increment_version', torch.autograd.graph.increment_version)
 
 
 def ptr(t):

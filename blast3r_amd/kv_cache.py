@@ -20,7 +20,7 @@ import math
 
 import torch
 
-from ._lib import BaKvArgs, BaKvAttendArgs, has_tangent, launch, lib, written
+from ._lib import BaKvArgs, BaKvAttendArgs, dual_level, has_tangent, launch, lib, written
 
 __all__ = ['KVCache', 'BLOCK']
 
@@ -100,12 +100,17 @@ class KVCache:
         self._lib, self._args = lib(), BaKvArgs(**same)
         self._attend_args = BaKvAttendArgs(n_splits=1, scale=1.0 / math.sqrt(d), **same)
 
-    def _look(self):
-        """Every call starts with it: the fields of calls are those of the tensors held now."""
-        k, v, scales = self._k, self._v, self._scales
-        if self._at is None or (k.data_ptr(), v.data_ptr(), scales.data_ptr()) != self._at:
+    def _begin(self, x, y):
+        """Every call starts with it: the fields of calls are those of the tensors held now, and what has a gradient or a
+        tangent, which codes cannot carry on, is refused."""
+        k, v, scales, at = self._k, self._v, self._scales, self._at
+        if at is None or k.data_ptr() != at[0] or v.data_ptr() != at[1] or scales.data_ptr() != at[2]:
             self._at = None
             self._hold(k, v, scales)
+        if (x.requires_grad or y.requires_grad or scales.requires_grad) and torch.is_grad_enabled():
+            raise RuntimeError('cache: codes carry no gradient: call it under torch.no_grad()')
+        if dual_level() and has_tangent(x, y, scales):
+            raise RuntimeError('cache: codes carry no tangent of forward-mode differentiation')
 
     def _fill(self, a, pages, firsts, name, offsets, n_rows, max_rows):
         """The fields of a call that the arguments of every call give."""
@@ -133,15 +138,6 @@ class KVCache:
         a.max_rows = most
         return most
 
-    def _no_derivative(self, *tensors):
-        """Refuses what has a gradient or a tangent, which codes cannot carry on."""
-        if torch.is_grad_enabled():
-            for t in tensors:
-                if t.requires_grad:
-                    raise RuntimeError('cache: codes carry no gradient: call it under torch.no_grad()')
-        if has_tangent(*tensors):
-            raise RuntimeError('cache: codes carry no tangent of forward-mode differentiation')
-
     def _rows(self, t, name, heads):
         shape = t.shape
         if len(shape) != 3 or shape[1] != heads or shape[2] != self._head_dim or t.device != self._device:
@@ -156,8 +152,7 @@ class KVCache:
         """Write the rows of k and v (tokens, heads, head_dim; fp32, fp16 or bf16) after the first ``lengths`` (n_seqs,)
         int32 tokens of their sequences.  ``lengths`` stays as it is.  No two sequences of a call may append to the
         same block."""
-        self._look()
-        self._no_derivative(k, v, self._scales)
+        self._begin(k, v)
         a = BaKvArgs.from_buffer_copy(self._args)
         a.rk_st, a.rk_sh = self._rows(k, 'k', self._heads)
         a.rv_st, a.rv_sh = self._rows(v, 'v', self._heads)
@@ -168,7 +163,7 @@ class KVCache:
         a.starts, a.dtype, a.rk, a.rv = lengths.data_ptr(), code, k.data_ptr(), v.data_ptr()
         if self._fill(a, pages, lengths, 'lengths', offsets, k.shape[0], max_new):
             launch(self._lib.ba_kv_write, a, self._device)
-            written(self._k, self._v, self._scales)
+            written((self._k, self._v, self._scales))
 
     def read(self, pages, starts, offsets, n_rows, max_count=None, dtype=torch.bfloat16):
         """(k, v) of tokens ``starts[s]`` and on, ``offsets[s + 1] - offsets[s]`` of each sequence (n_rows / n_seqs where
@@ -178,8 +173,7 @@ class KVCache:
             raise ValueError(f'cache: fp32, fp16 or bf16 values, got {dtype}')
         if n_rows < 0:
             raise ValueError(f'cache: {n_rows} rows')
-        self._look()
-        self._no_derivative(self._scales)
+        self._begin(self._scales, self._scales)
         a = BaKvArgs.from_buffer_copy(self._args)
         shape = (n_rows, self._heads, self._head_dim)
         k = torch.empty(shape, dtype=dtype, device=self._device)
@@ -205,8 +199,7 @@ class KVCache:
         A row that sees no token gives zeros.  q_heads is a multiple of the cache's heads; query head h reads cache
         head h // (q_heads // heads).  With ``return_lse`` also log(sum(exp(scale q k^T))) as (tokens, q_heads) fp32,
         -inf where no token is seen, with which results over different tokens can be joined."""
-        self._look()
-        self._no_derivative(q, self._scales)
+        self._begin(q, q if out is None else out)
         shape = q.shape
         if len(shape) != 3 or shape[1] % self._heads or shape[1] == 0:
             raise ValueError(f'cache: q must be (tokens, a multiple of {self._heads} heads, {self._head_dim}), got {tuple(shape)}')
@@ -231,7 +224,6 @@ class KVCache:
         else:
             if out.shape != shape or out.dtype is not dtype:
                 raise ValueError('cache: out must be like q')
-            self._no_derivative(out)
             a.o_st, a.o_sh = self._rows(out, 'out', q_heads)
         lse = None
         if return_lse:
@@ -250,5 +242,5 @@ class KVCache:
                 a.workspace, a.workspace_bytes = work.data_ptr(), size
             launch(L.ba_kv_attend, a, dev)
             if given:
-                written(out)
+                written((out,))
         return (out, lse) if return_lse else out

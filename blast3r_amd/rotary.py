@@ -14,7 +14,7 @@ import math
 
 import torch
 
-from ._lib import BaRotaryArgs, has_tangent, launch, lib, written
+from ._lib import BaRotaryArgs, dual_level, has_tangent, launch, lib, written
 
 __all__ = ['Rotary', 'rotary_frequencies']
 
@@ -144,7 +144,7 @@ class Rotary:
         """
         if not 1 <= len(xs) <= 2:
             raise ValueError(f'rotary: one or two tensors at a time, got {len(xs)}')
-        if torch.is_grad_enabled() and (xs[0].requires_grad or xs[-1].requires_grad) or has_tangent(*xs):
+        if torch.is_grad_enabled() and (xs[0].requires_grad or xs[-1].requires_grad) or dual_level() and has_tangent(*xs):
             if out is not None:
                 raise ValueError('rotary: out cannot be given where gradients are recorded')
             ys = _Turn.apply(self, positions, bool(inverse), *xs)
@@ -184,7 +184,7 @@ class Rotary:
             for x, y in zip(xs, ys):
                 if y.shape != x.shape or y.dtype != x.dtype or y.device != x.device or y.stride(-1) != 1:
                     raise ValueError('rotary: an output must be like its tensor, with contiguous elements of a head')
-                if y.requires_grad and torch.is_grad_enabled() or has_tangent(y):
+                if y.requires_grad and torch.is_grad_enabled() or dual_level() and has_tangent(y):
                     raise ValueError('rotary: out must not require a gradient where gradients are recorded, nor have a tangent')
         a = BaRotaryArgs.from_buffer_copy(self._args)
         t, y = xs[0], ys[0]
@@ -214,7 +214,7 @@ class Rotary:
         if a.T and a.B:
             launch(self._call, a, dev)
             if out is not None:
-                written(*ys)
+                written(ys)
         return tuple(ys)
 
     def _strides(self, t, lead, dtype):
