@@ -338,6 +338,14 @@ def has_tangent(*tensors):
     return dual_level() and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
+def overlaps(y, x):
+    """Whether an output y cannot be written while x, of the same shape, is read: it has one place under several elements,
+    or begins where x does with other strides.  (Views that overlap in other ways are not looked for.)"""
+    if any(n > 1 and st == 0 for n, st in zip(y.shape, y.stride())):
+        return True
+    return y.data_ptr() == x.data_ptr() and any(n > 1 and a != b for n, a, b in zip(y.shape, y.stride(), x.stride()))
+
+
 # written(tensors): a kernel wrote to tensors that were there before the call, so that what autograd or a cache keyed by
 # versions keeps of them is out of date (without the public function's own 0.3 us)
 written = getattr(torch._C, '_increment_version', torch.autograd.graph.increment_version)

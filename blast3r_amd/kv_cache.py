@@ -20,7 +20,7 @@ import math
 
 import torch
 
-from ._lib import BaKvArgs, BaKvAttendArgs, dual_level, has_tangent, launch, lib, written
+from ._lib import BaKvArgs, BaKvAttendArgs, dual_level, has_tangent, launch, lib, overlaps, written
 
 __all__ = ['KVCache', 'BLOCK']
 
@@ -195,7 +195,7 @@ class KVCache:
         causal    a row sees the tokens up to its own position (else all)
         window    it sees only tokens later than its position less ``window``
         scale     default 1 / sqrt(head_dim)
-        out       a tensor like q for the result
+        out       a tensor like q for the result (q itself, or one that does not overlap it)
         A row that sees no token gives zeros.  q_heads is a multiple of the cache's heads; query head h reads cache
         head h // (q_heads // heads).  With ``return_lse`` also log(sum(exp(scale q k^T))) as (tokens, q_heads) fp32,
         -inf where no token is seen, with which results over different tokens can be joined."""
@@ -224,6 +224,8 @@ class KVCache:
         else:
             if out.shape != shape or out.dtype is not dtype:
                 raise ValueError('cache: out must be like q')
+            if overlaps(out, q):
+                raise ValueError('cache: out overlaps itself or, not in its place, q')
             a.o_st, a.o_sh = self._rows(out, 'out', q_heads)
         lse = None
         if return_lse:

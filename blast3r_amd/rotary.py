@@ -14,7 +14,7 @@ import math
 
 import torch
 
-from ._lib import BaRotaryArgs, dual_level, has_tangent, launch, lib, written
+from ._lib import BaRotaryArgs, dual_level, has_tangent, launch, lib, overlaps, written
 
 __all__ = ['Rotary', 'rotary_frequencies']
 
@@ -138,8 +138,8 @@ class Rotary:
 
         positions   int32 or int64, the tokens' shape ((T,) serves every batch), with more than one axis a last
                     dimension of ``axes``
-        out         tensors to write to, one for each x (x itself rotates in place); not differentiable, and refused where
-                    gradients are recorded and one of them requires one
+        out         tensors to write to, one for each x (x itself rotates in place; another one may not overlap either x);
+                    not differentiable, and refused where gradients are recorded and one of them requires one
         inverse     rotate by the opposite angles
         """
         if not 1 <= len(xs) <= 2:
@@ -186,6 +186,12 @@ class Rotary:
                     raise ValueError('rotary: an output must be like its tensor, with contiguous elements of a head')
                 if y.requires_grad and torch.is_grad_enabled() or dual_level() and has_tangent(y):
                     raise ValueError('rotary: out must not require a gradient where gradients are recorded, nor have a tangent')
+                if overlaps(y, x):
+                    raise ValueError('rotary: out overlaps itself or, not in its place, the tensor that it is the rotation of')
+            if len(xs) == 2 and x.numel():
+                at = ys[0].data_ptr(), ys[1].data_ptr()
+                if at[0] == at[1] or at[0] == xs[1].data_ptr() or at[1] == xs[0].data_ptr():
+                    raise ValueError('rotary: an out overlaps the other tensor or its out')
         a = BaRotaryArgs.from_buffer_copy(self._args)
         t, y = xs[0], ys[0]
         xs_, ys_ = self._strides(t, lead, dtype), y.stride()

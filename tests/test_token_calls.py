@@ -90,6 +90,34 @@ def test_outputs_that_require_a_gradient_are_refused(host):
     assert len(host) == 2 and leaf._version == 1 and out._version == 1
 
 
+def test_outputs_that_overlap_are_refused(host):
+    """Rows are read and written in no order, so an output may be its own tensor as it stands, and otherwise neither another
+    call's operand at another place nor one place under several rows."""
+    from blast3r_amd.kv_cache import KVCache
+    from blast3r_amd.rotary import Rotary
+    rot, pos = Rotary(64, device='cpu'), _i32([0, 1, 2])
+    qkv = torch.zeros(3, 6, 64)
+    q, k = qkv[:, :2], qkv[:, 2:4]
+    other = torch.zeros(3, 2, 64).transpose(0, 1).reshape(-1).as_strided((3, 2, 64), (64, 192, 1))
+    square = torch.zeros(3, 3, 64)
+    for xs, out in (((q, k), (k, q)), ((q, q), (q, q)), ((q, k), (other, other)), ((q,), (q[:1].expand(3, 2, 64),)),
+                    ((q,), (other[:, :1].expand(3, 2, 64),)), ((square,), (square.transpose(0, 1),)), ((q, k), (k, torch.zeros_like(k)))):
+        with pytest.raises(ValueError, match='out'):
+            rot(pos, *xs, out=out)
+    c = KVCache(2, 1, 64, device='cpu')
+    x = torch.zeros(3, 3, 64, dtype=torch.bfloat16)
+    for out in (x.transpose(0, 1), x[:1].expand(3, 3, 64), x[:, :1].expand(3, 3, 64)):
+        with pytest.raises(ValueError, match='out'):
+            c.attend(x, _i32([[0, 1]]), _i32([5]), out=out)
+    assert not host
+    rot(pos, q, k, out=(q, k))                              # in place, in one buffer
+    rot(pos, q, k, out=(other, qkv[:, 4:]))
+    rot(pos[:1], q[:1], out=q[:1].as_strided((1, 2, 64), (7, 64, 1)))       # a stride that nothing uses
+    c.attend(x, _i32([[0, 1]]), _i32([5]), out=x)
+    c.attend(x, _i32([[0, 1]]), _i32([5]), out=torch.empty_like(x).transpose(0, 1))
+    assert len(host) == 5
+
+
 # ---------------------------------------------------------------------------------- forward mode
 
 def test_forward_mode_tangents_go_through_rotary(host, monkeypatch):
