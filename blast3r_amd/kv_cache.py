@@ -151,7 +151,12 @@ class KVCache:
     def append(self, k, v, pages, lengths, offsets=None, max_new=None):
         """Write the rows of k and v (tokens, heads, head_dim; fp32, fp16 or bf16) after the first ``lengths`` (n_seqs,)
         int32 tokens of their sequences.  ``lengths`` stays as it is.  No two sequences of a call may append to the
-        same block."""
+        same block.
+
+        A block that is filled by several calls has its codes made anew whenever a call outgrows its factor.  int8 codes
+        are rounded again each time: after n such calls a value is within (n + 1) / 2 steps of the factor, up to 32 steps
+        of 127 where each of 64 single tokens is a little larger than all before.  e4m3 factors at least double, which
+        loses nothing but the lowest bits of the smallest codes."""
         self._begin(k, v)
         a = BaKvArgs.from_buffer_copy(self._args)
         a.rk_st, a.rk_sh = self._rows(k, 'k', self._heads)

@@ -681,7 +681,8 @@ typedef struct {
 
 /* Rows appended to the cache at starts[s] ...  The factor of a block and head is fit(largest magnitude of its new
  * values), and not less than its present factor where the block held tokens before starts[s]; those are then recoded
- * with the new factor if it grew.  fit: e4m3: the least power of two, from 2^-60 on, with largest <= 448 * factor;
+ * with the new factor if it grew (int8: rounded anew, so that after n growths a value is within (n + 1) / 2 steps of its
+ * factor).  fit: e4m3: the least power of two, from 2^-60 on, with largest <= 448 * factor;
  * int8: max(largest / 127, 2^-60).  Codes: nearest to x * (1 / factor), ties to even.  A block with a NaN or an
  * infinity among its values (or with a factor over 2^60) gets a NaN factor and zero codes: it reads as NaN until a
  * token is written to its first place again. */

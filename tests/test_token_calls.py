@@ -532,3 +532,58 @@ def test_growing_a_cache_by_assignment():
         assert torch.equal(a[:64], b[:64]) and torch.equal(a[128:], b[128:])
         assert bool(((a[64:128] - b[64:128]).abs() <= 1.01 * f[0][:, None]).all())
     assert c.n_blocks == 8 and c.attend(q, _i32([[1, 0, 6, 7]], DEV), lens).isfinite().all()
+
+
+# ---------------------------------------------------------------------------------- factors that grow
+
+def _growing(g, n=64, heads=1, dim=32):
+    """n tokens whose largest value is g times that of the one before."""
+    x = np.random.default_rng(0).uniform(-1, 1, (n, heads, dim))
+    x[:, :, 0] = 1.0
+    return np.float32(x * (g ** np.arange(n))[:, None, None])
+
+
+@pytest.mark.parametrize('g', [1.0, 1.001, 1.0039, 1.01, 1.3, 2.5])
+def test_int8_codes_lose_half_a_step_whenever_their_factor_grows(g):
+    """The bound that the documents give: after n growths a value is within (n + 1) / 2 steps of the block's factor, and
+    slow growth comes near it; e4m3 codes of normal size, whose factors at least double, stay within their 2^-4."""
+    x = _growing(g)
+    for bits in ('int8', 'fp8'):
+        c = otok.Cache(np.zeros((1, 1, 64, 32)), np.zeros((1, 1, 64, 32)), np.ones((1, 1, 2)), bits)
+        grown, f, n = np.zeros(64), 0.0, 0
+        while n < 64:
+            c.append(x[n:n + 1], x[n:n + 1], [[0]], [n], [1])
+            before, f = f, c.scales[0, 0, 0]
+            if not f <= 2.0 ** 60:                          # past the range of factors: NaN from here on
+                assert x[n].max() > (127 if bits == 'int8' else 448) * 2.0 ** 60
+                f = before
+                break
+            grown[:n] += f > before
+            n += 1
+            k, _, _ = c.sequence([0], n)
+        grown, y = grown[:n], np.float64(x[:n])
+        err = np.abs(k - y).max((1, 2))
+        if bits == 'int8':
+            assert np.all(err <= (grown + 1) / 2 * f * (1 + 1e-5))
+            if g == 1.0039:
+                assert grown[0] == 63 and err[0] > 25 * f
+        else:
+            normal = np.abs(y) >= 2.0 ** -6 * f
+            assert np.all((np.abs(k - y) <= 2.0 ** -4 * np.abs(y))[normal])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', ['int8', 'fp8'])
+def test_append_of_single_tokens_that_grow(bits):
+    """A factor that grows with each of 64 tokens: codes and factors as the oracle's throughout."""
+    from blast3r_amd.kv_cache import KVCache
+    from test_tokens import BITS, _mirror, _same
+    x = _growing(1.0039, heads=2, dim=64)
+    c = KVCache(1, 2, 64, BITS[bits], device=DEV)
+    o = _mirror(c, bits)
+    print(f'growing {bits}', flush=True)
+    for t in range(64):
+        r = torch.tensor(x[t:t + 1], device=DEV)
+        c.append(r, r, _i32([[0]], DEV), _i32([t], DEV))
+        o.append(x[t:t + 1], x[t:t + 1], [[0]], [t], [1])
+    _same(c, o)
