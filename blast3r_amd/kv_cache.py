@@ -115,11 +115,12 @@ class KVCache:
     def _fill(self, a, pages, firsts, name, offsets, n_rows, max_rows):
         """The fields of a call that the arguments of every call give."""
         dev = self._device
-        if (pages.dim() != 2 or pages.dtype is not torch.int32 or pages.device != dev or
-                pages.stride(1) != 1 and pages.shape[0] > 0 and pages.shape[1] > 1):
+        shape, stride = pages.shape, pages.stride()
+        if (len(shape) != 2 or pages.dtype is not torch.int32 or pages.device != dev or
+                stride[1] != 1 and shape[0] > 0 and shape[1] > 1):
             raise ValueError(f'cache: pages must be (n_seqs, blocks) int32 on {dev} with contiguous rows')
-        S, a.n_pages = pages.shape
-        a.n_seqs, a.pages, a.pages_stride = S, pages.data_ptr(), pages.stride(0)
+        S, a.n_pages = shape
+        a.n_seqs, a.pages, a.pages_stride = S, pages.data_ptr(), stride[0]
         if firsts.dtype is not torch.int32 or firsts.device != dev or firsts.shape != (S,) or not firsts.is_contiguous():
             raise ValueError(f'cache: {name} must be a contiguous int32 tensor of shape {(S,)} on {dev}')
         a.n_rows = n_rows
@@ -161,12 +162,13 @@ class KVCache:
         a = BaKvArgs.from_buffer_copy(self._args)
         a.rk_st, a.rk_sh = self._rows(k, 'k', self._heads)
         a.rv_st, a.rv_sh = self._rows(v, 'v', self._heads)
-        code = DTYPES.get(k.dtype)
-        if code is None or k.shape != v.shape or k.dtype is not v.dtype:
+        n, dtype = k.shape[0], k.dtype
+        code = DTYPES.get(dtype)
+        if code is None or v.shape[0] != n or dtype is not v.dtype:
             raise ValueError(f'cache: k and v must be alike, in fp32, fp16 or bf16: got {tuple(k.shape)} {k.dtype} and '
                              f'{tuple(v.shape)} {v.dtype}')
         a.starts, a.dtype, a.rk, a.rv = lengths.data_ptr(), code, k.data_ptr(), v.data_ptr()
-        if self._fill(a, pages, lengths, 'lengths', offsets, k.shape[0], max_new):
+        if self._fill(a, pages, lengths, 'lengths', offsets, n, max_new):
             launch(self._lib.ba_kv_write, a, self._device)
             written((self._k, self._v, self._scales))
 
