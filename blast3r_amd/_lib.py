@@ -301,6 +301,7 @@ def stream_ptr(device=None):
 
 
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+_device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)       # there are tensors on it: it was started
 _tracing = getattr(torch._C, '_is_tracing', torch.jit.is_tracing)
 _modes = getattr(torch._C, '_len_torch_dispatch_stack', lambda: 1)
 
@@ -319,7 +320,7 @@ def launch(call, args, device):
     if (_tracing() or _modes()) and _traced():
         raise RuntimeError('a trace of torch operations cannot hold this call: it is a launch of libba_hip.so')
     index = device.index
-    if torch.cuda.current_device() != index:
+    if _device() != index:
         with torch.cuda.device(index):
             return check(call(ctypes.byref(args), torch.cuda.current_stream(index).cuda_stream))
     stream = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
