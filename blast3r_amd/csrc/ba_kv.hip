@@ -12,8 +12,9 @@
 // the words that a wave writes lie in different banks.
 //
 // Bound by memory: es bytes in and one out of each element (writing), the other way round (reading).  12288 tokens of
-// 16 heads of 64 (75 MB): written in 18 us, read in 13 (4.1 and 5.6 TB/s); ragged rows of 8 heads of 128 (120 MB): 24 and
-// 22 us; 131072 tokens read (805 MB): 160 us, 5.0 TB/s.  Writing is the slower one because a workgroup's stores wait for
+// 16 heads of 64 (75 MB): written in 18 us, read in 13 to 14 (4.1 and 5.6 TB/s); ragged rows of 8 heads of 128 (120 MB): 24
+// and 22 us; 131072 tokens read (805 MB): 160 us, 5.0 TB/s; one token for each of 64 sequences of 8 heads of 128: 6.2 us, 7.6
+// where every block's codes are made anew.  Writing is the slower one because a workgroup's stores wait for
 // the largest of its loads; 8 workgroups to a CU overlap.  Two workgroups of 128 threads or one of 512 in the place of
 // one of 256 were slower (32.9 and 31.2 us against 27.8 for the ragged rows).
 #include <hip/hip_runtime.h>

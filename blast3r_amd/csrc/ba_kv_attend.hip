@@ -24,18 +24,22 @@
 // 1.2 to 1.4 without; 3% of the time of k_kv_attend_tile at 128 elements); for bf16 the unrounded ones do.
 // Weights of a block whose values are small beside others' (by AT_LOW) may vanish in fp16 and still count in
 // the denominator: its sums are taken before rounding in any case.  m is moved only when a weight nears
-// fp16's end; until then nothing is rescaled.
+// fp16's end; until then nothing is rescaled.  log2 and reciprocal of a value factor are the hardware's, right to the
+// last place of fp32 or so: with |lv| up to 60 a block's weights are off by 3e-6 in all, against fp16's 5e-4 of each.
 //
 // Two kernels:
 //   k_kv_attend       up to 32 rows: the waves of a workgroup have the same rows and split the blocks, codes go
 //                     from memory to registers without LDS, and the waves' sums are joined at the end.  Bound by
-//                     memory: a query over 192000 tokens of 16 heads of 64 (393 MB) takes 70 us, 5.6 TB/s; 48
-//                     sequences of up to 8192 tokens, 8 heads of 128 (417 MB), 89 us, 4.7 TB/s (a large copy: 4.8).
+//                     memory: a query over 192000 tokens of 16 heads of 64 (393 MB) takes 70 to 74 us, 5.3 to 5.6 TB/s;
+//                     48 sequences of up to 8192 tokens, 8 heads of 128 (417 MB), 89 to 92 us, 4.6 TB/s (a large copy:
+//                     4.8); 16 sequences of 8192 tokens with 2, 5 and 32 rows (269 MB) 50, 50 and 56 us with the join.
 //   k_kv_attend_tile  more rows: the waves split the rows and share blocks that are converted to fp16 once, in LDS.
 //                     Bound by the vector and matrix units together, and by power (the clock falls to 2.0 - 2.2
-//                     GHz): 2 x 2048 rows over 16384 tokens, 32 heads of 128: 1030 us, 1.0 PFLOP/s (a large fp16
-//                     matrix product on this card: 1.09); of 64: 564 us, 0.92 PFLOP/s, where the exponentials alone
-//                     take as long as half of the products.
+//                     GHz): 2 x 2048 rows over 16384 tokens, 32 heads of 128: 1015 to 1040 us, 1.0 PFLOP/s (a large fp16
+//                     matrix product on this card: 1.09); of 64: 565 to 580 us, 0.9 PFLOP/s, where the exponentials alone
+//                     take as long as half of the products; of 32: 490 us, 0.5 PFLOP/s; of 96: 900, 0.86; 16 heads of 256:
+//                     1240, 0.83.  Where tiles are few or of different lengths workgroups are what is missing: a prompt
+//                     of 2048 rows into an empty cache takes 70 us of 32, 768 rows over 768 tokens 24 us of 2.
 // Where rows are few the blocks of a sequence are further cut into n_splits parts, whose sums k_kv_join adds in
 // order (5 us for 16 rows of 24 parts, 10 us for 12288 rows of 10).
 #include <hip/hip_runtime.h>
@@ -57,7 +61,8 @@ typedef float f16 __attribute__((ext_vector_type(16)));
 
 #define AT_T 256
 #define AT_MIN_BLOCKS 16     // a part has at least so many blocks: below that the join costs more than it saves (a query over
-                             // 777 tokens 12 us in one part, 18 in two; over 8192 tokens 18.5 in 8 parts, 17.8 in 16)
+                             // 777 tokens 12 us in one part, 18 in two; over 8192 tokens 18.5 in 8 parts, 17.8 in 16;
+                             // measured with k_kv_attend only)
 
 template <int COLS> struct Mma;
 template <> struct Mma<16> {
@@ -577,7 +582,7 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(ba_kv_att
 // registers, 64 rows a wave 2167; converted in LDS 1777, with 32 rows a wave so that two waves fit a SIMD 1462; the order
 // of products and vector instructions fenced 1444; conversions spread over the products and LDS slots exchanged against
 // bank conflicts 1201; 8 waves to a workgroup 1126; no maximum formed until a sum calls for it 1062; 32-bit arithmetic on
-// rows and blocks 1024.
+// rows and blocks 1024 (1015 to 1040 from run to run).
 template <int D, int KT, int NCB, int WAVES, bool HALF>
 __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_attend_tile(ba_kv_attend_args a, int n_tiles, int packed, int wide) {
     typedef Mma<32> M;
@@ -973,8 +978,8 @@ __global__ void __launch_bounds__(AT_T) k_kv_join(ba_kv_attend_args a, int tile_
 // The kernel for a call by the rows that share a cache head: up to 16 in 16 columns and up to 32 in 32 with the waves
 // splitting the blocks; more in workgroups of 128 rows or, from 129 on, of 256 that share the converted blocks (128 where
 // heads of 256 leave a wave registers for 32 rows only).  256 rows are 4 waves of 64 rows up to 64 elements a head, and 8
-// waves of 32 above: then two waves fit a SIMD (2 x 2048 rows over 16384 tokens: 64 elements 615 us against 690 with 8
-// waves, 128 elements 1077 us against 1375 with 4).  `fit`: workgroups that a CU holds.
+// waves of 32 above: then two waves fit a SIMD (2 x 2048 rows over 16384 tokens, before the last steps of the kernel: 64
+// elements 615 us against 690 with 8 waves, 128 elements 1077 us against 1375 with 4).  `fit`: workgroups that a CU holds.
 struct AtShape { int cols, ncb, waves, rows, fit; };
 static AtShape at_shape(int64_t rows, int dim) {
     if (rows <= 16) return {16, 0, 4, 16, dim <= 64 ? 4 : dim <= 128 ? 2 : 1};
