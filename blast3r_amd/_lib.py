@@ -169,6 +169,40 @@ class BaKvAttendArgs(ctypes.Structure):
                 ('scale', c_f), ('n_splits', c_int), ('workspace', c_p), ('workspace_bytes', c_i64)]
 
 
+class BaKvScoredArgs(BaKvAttendArgs):
+    # the header's struct begins with ba_kv_attend_args, whose size is a multiple of what follows
+    _fields_ = [('slopes', c_p), ('prefix', c_p), ('since', c_p), ('until', c_p), ('cap', c_f), ('shared', c_int),
+                ('shared_parts', c_int), ('reserved', c_int)]
+
+
+class BaKvPool(ctypes.Structure):
+    _fields_ = [('counts', c_p), ('used', c_p), ('marks', c_p), ('n_blocks', c_i64)]
+
+
+class BaKvTable(ctypes.Structure):
+    _fields_ = [('pages', c_p), ('stride', c_i64), ('n_seqs', c_int), ('n_pages', c_int)]
+
+
+class BaKvForkArgs(ctypes.Structure):
+    _fields_ = [('from_', BaKvTable), ('to', BaKvTable), ('from_lengths', c_p), ('to_lengths', c_p), ('parents', c_p),
+                ('children', c_p), ('n', c_int), ('reserved', c_int)]
+
+
+class BaKvTrimArgs(ctypes.Structure):
+    _fields_ = [('table', BaKvTable), ('first', c_p), ('last', c_p), ('rows', c_p), ('lengths', c_p), ('n_rows', c_int),
+                ('all', c_int)]
+
+
+class BaKvGrowArgs(ctypes.Structure):
+    _fields_ = [('table', BaKvTable), ('lengths', c_p), ('more', c_p), ('each', c_int), ('max_new', c_int), ('src', c_p),
+                ('dst', c_p), ('n', c_p), ('missing', c_p)]
+
+
+class BaKvCopyArgs(ctypes.Structure):
+    _fields_ = [('k', c_p), ('v', c_p), ('scales', c_p), ('n_blocks', c_i64), ('heads', c_int), ('dim', c_int), ('src', c_p),
+                ('dst', c_p), ('count', c_p), ('n', c_int), ('reserved', c_int)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     'ba_last_error': (ctypes.c_char_p, []),
@@ -249,6 +283,14 @@ _SIGS = {
     'ba_kv_attend': (c_int, [ctypes.POINTER(BaKvAttendArgs), c_p]),
     'ba_kv_attend_splits': (c_int, [c_int, c_int, c_int, c_int, c_i64, c_int]),
     'ba_kv_attend_workspace_bytes': (c_i64, [c_i64, c_int, c_int, c_int]),
+    'ba_kv_attend_scored': (c_int, [ctypes.POINTER(BaKvScoredArgs), c_p]),
+    'ba_kv_scored_parts': (None, [ctypes.POINTER(BaKvScoredArgs), ctypes.POINTER(c_int), ctypes.POINTER(c_int)]),
+    'ba_kv_pool_count': (c_int, [ctypes.POINTER(BaKvPool), ctypes.POINTER(BaKvTable), c_int, c_p]),
+    'ba_kv_pool_fork': (c_int, [ctypes.POINTER(BaKvPool), ctypes.POINTER(BaKvForkArgs), c_p]),
+    'ba_kv_pool_trim': (c_int, [ctypes.POINTER(BaKvPool), ctypes.POINTER(BaKvTrimArgs), c_p]),
+    'ba_kv_pool_grow': (c_int, [ctypes.POINTER(BaKvPool), ctypes.POINTER(BaKvGrowArgs), c_p]),
+    'ba_kv_pool_compact': (c_int, [ctypes.POINTER(BaKvPool), ctypes.POINTER(BaKvTable), c_int, c_p, c_p, c_p, c_int, c_p]),
+    'ba_kv_copy': (c_int, [ctypes.POINTER(BaKvCopyArgs), c_p]),
 }
 
 EXPORTED = tuple(_SIGS)
@@ -258,7 +300,9 @@ ABI_STRUCTS = {'ba_huber': BaHuber, 'ba_layout': BaLayout, 'ba_lin_args': BaLinA
                'ba_pcg_args': BaPcgArgs, 'ba_pcg_pairs': BaPcgPairs, 'ba_pcg_resident': BaPcgResident, 'ba_chol_args': BaCholArgs, 'ba_sample_args': BaSampleArgs,
                'ba_obs_set': BaObsSet, 'ba_gather_args': BaGatherArgs, 'ba_remove_args': BaRemoveArgs,
                'ba_tangent_args': BaTangentArgs, 'ba_rotary_args': BaRotaryArgs, 'ba_kv_args': BaKvArgs,
-               'ba_kv_attend_args': BaKvAttendArgs}
+               'ba_kv_attend_args': BaKvAttendArgs, 'ba_kv_scored_args': BaKvScoredArgs, 'ba_kv_pool': BaKvPool,
+               'ba_kv_table': BaKvTable, 'ba_kv_fork_args': BaKvForkArgs, 'ba_kv_trim_args': BaKvTrimArgs,
+               'ba_kv_grow_args': BaKvGrowArgs, 'ba_kv_copy_args': BaKvCopyArgs}
 
 
 def _check_abi(L):

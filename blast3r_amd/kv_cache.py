@@ -16,11 +16,12 @@ workgroups.  Lengths, offsets and pages are device tensors, never read by the ho
 call can be captured in a graph.  What they say out of range is left out (include/ba_hip.h).
 Rows of a result that no sequence has, or past ``max_new`` of one, are not written.
 """
+import ctypes
 import math
 
 import torch
 
-from ._lib import BaKvArgs, BaKvAttendArgs, dual_level, has_tangent, launch, lib, overlaps, written
+from ._lib import BaKvArgs, BaKvAttendArgs, BaKvCopyArgs, BaKvScoredArgs, dual_level, has_tangent, launch, lib, overlaps, written
 
 __all__ = ['KVCache', 'BLOCK']
 
@@ -99,6 +100,7 @@ class KVCache:
         same = dict(zip(('k', 'v', 'scales'), self._at), n_blocks=n, heads=h, dim=d, bits=BITS[k.dtype])
         self._lib, self._args = lib(), BaKvArgs(**same)
         self._attend_args = BaKvAttendArgs(n_splits=1, scale=1.0 / math.sqrt(d), **same)
+        self._scored_args = BaKvScoredArgs(n_splits=1, scale=1.0 / math.sqrt(d), **same)
 
     def _begin(self, x, y):
         """Every call starts with it: the fields of calls are those of the tensors held now, and what has a gradient or a
@@ -192,8 +194,34 @@ class KVCache:
             launch(self._lib.ba_kv_read, a, self._device)
         return k, v
 
+    def copy(self, src, dst, count=None):
+        """Copy blocks ``src`` to blocks ``dst`` ((n,) int32 each), codes and factors: the pairs that ``BlockPool.grow`` and
+        ``BlockPool.compact`` give, for each cache that the pool's lists are about.  count: (1,) int32, the first so many
+        pairs only.  Pairs with a number that is no block's (-1) are left out.  No block may be the destination of two pairs,
+        or of one and the source of another."""
+        self._begin(self._scales, self._scales)
+        dev, n = self._device, src.shape[0] if src.dim() == 1 else -1
+        for t, name, shape in ((src, 'src', (n,)), (dst, 'dst', (n,)), (count, 'count', (1,))):
+            if t is None and name == 'count':
+                continue
+            if t.dtype is not torch.int32 or t.device != dev or t.shape != shape or not t.is_contiguous():
+                raise ValueError(f'cache: {name} must be a contiguous int32 tensor of one dimension on {dev}, dst as long as '
+                                 'src, count of one number')
+        a = BaKvCopyArgs(k=self._at[0], v=self._at[1], scales=self._at[2], n_blocks=self._n_blocks, heads=self._heads,
+                         dim=self._head_dim, src=src.data_ptr(), dst=dst.data_ptr(), n=n)
+        if count is not None:
+            a.count = count.data_ptr()
+        if n and self._n_blocks:
+            launch(self._lib.ba_kv_copy, a, dev)
+            written((self._k, self._v, self._scales))
+
+    def _per(self, t, name, dtype, n):
+        if t.dtype is not dtype or t.device != self._device or t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f'cache: {name} must be a contiguous {dtype} tensor of shape {(n,)} on {self._device}')
+        return t.data_ptr()
+
     def attend(self, q, pages, lengths, offsets=None, max_new=None, causal=True, window=None, scale=None, out=None,
-               return_lse=False):
+               return_lse=False, cap=None, slopes=None, prefix=None, since=None, until=None, shared=0):
         """Attention of the rows of q (tokens, q_heads, head_dim; fp16 or bf16) over the cached tokens of their
         sequences: softmax(scale q k^T) v.
 
@@ -203,6 +231,14 @@ class KVCache:
         window    it sees only tokens later than its position less ``window``
         scale     default 1 / sqrt(head_dim)
         out       a tensor like q for the result (q itself, or one that does not overlap it)
+        cap       scores z become cap tanh(z / cap), cap in [1e-3, 1e3]; off by 4e-7 cap at most
+        slopes    (q_heads,) fp32, finite: then less slope |p - j| for the row's position p and token j
+        since     (tokens,) int32: a row sees only tokens from its own number on (the first token of its document)
+        until     (tokens,) int32: and only those below this one (the end of its frame, with causal=False)
+        prefix    (n_seqs,) int32: the first so many tokens of a sequence are seen by all its rows, whatever causal, window,
+                  since and until say (a prompt that is read in both directions, the first tokens beside a window)
+        shared    the first so many blocks (a host number) of every list are the same: their tokens are read once for all
+                  sequences.  Only the first list's are looked at.
         A row that sees no token gives zeros.  q_heads is a multiple of the cache's heads; query head h reads cache
         head h // (q_heads // heads).  With ``return_lse`` also log(sum(exp(scale q k^T))) as (tokens, q_heads) fp32,
         -inf where no token is seen, with which results over different tokens can be joined."""
@@ -211,7 +247,8 @@ class KVCache:
         if len(shape) != 3 or shape[1] % self._heads or shape[1] == 0:
             raise ValueError(f'cache: q must be (tokens, a multiple of {self._heads} heads, {self._head_dim}), got {tuple(shape)}')
         n_rows, q_heads, dim = shape
-        a = BaKvAttendArgs.from_buffer_copy(self._attend_args)
+        scored = bool(shared) or cap is not None or not (slopes is prefix is since is until is None)
+        a = BaKvScoredArgs.from_buffer_copy(self._scored_args) if scored else BaKvAttendArgs.from_buffer_copy(self._attend_args)
         a.q_st, a.q_sh = self._rows(q, 'q', q_heads)
         dtype, dev = q.dtype, self._device
         if dtype is not torch.bfloat16 and dtype is not torch.float16:
@@ -241,15 +278,39 @@ class KVCache:
         a.lengths, a.dtype, a.q, a.o = lengths.data_ptr(), DTYPES[dtype], q.data_ptr(), out.data_ptr()
         a.q_heads, a.causal = q_heads, 1 if causal else 0
         most = self._fill(a, pages, lengths, 'lengths', offsets, n_rows, max_new)
+        if scored:
+            if cap is not None:
+                if not 1e-3 <= cap <= 1e3:
+                    raise ValueError(f'cache: cap must be in [1e-3, 1e3], got {cap}')
+                a.cap = cap
+            if slopes is not None:
+                a.slopes = self._per(slopes, 'slopes', torch.float32, q_heads)
+                if slopes.requires_grad and torch.is_grad_enabled() or dual_level() and has_tangent(slopes):
+                    raise RuntimeError('cache: slopes carry no gradient: call it under torch.no_grad()')
+            if prefix is not None:
+                a.prefix = self._per(prefix, 'prefix', torch.int32, a.n_seqs)
+            if since is not None:
+                a.since = self._per(since, 'since', torch.int32, n_rows)
+            if until is not None:
+                a.until = self._per(until, 'until', torch.int32, n_rows)
+            if not 0 <= shared <= a.n_pages:
+                raise ValueError(f'cache: {shared} shared blocks of lists of {a.n_pages}')
+            a.shared = shared
         if most:
             L = self._lib
-            n = L.ba_kv_attend_splits(a.n_seqs, self._heads, q_heads, dim, most, a.n_pages)
+            if scored:
+                call, own, common = L.ba_kv_attend_scored, ctypes.c_int32(), ctypes.c_int32()
+                L.ba_kv_scored_parts(a, own, common)
+                a.n_splits, a.shared_parts = own.value, common.value
+                n = own.value + common.value
+            else:
+                call = L.ba_kv_attend
+                a.n_splits = n = L.ba_kv_attend_splits(a.n_seqs, self._heads, q_heads, dim, most, a.n_pages)
             if n > 1:                        # the partial sums live until the launches on this stream are done
-                a.n_splits = n
                 size = L.ba_kv_attend_workspace_bytes(n_rows, q_heads, dim, n)
                 work = torch.empty(size, dtype=torch.uint8, device=dev)
                 a.workspace, a.workspace_bytes = work.data_ptr(), size
-            launch(L.ba_kv_attend, a, dev)
+            launch(call, a, dev)
             if given:
                 written((out,))
         return (out, lse) if return_lse else out

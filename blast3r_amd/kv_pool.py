@@ -1,0 +1,178 @@
+"""The pages of an 8-bit key/value cache on the device (``ba_kv_pool_*``, libba_hip.so).
+
+A cache (``kv_cache.KVCache``) is written and read through lists of its blocks.  ``BlockPool`` keeps such lists: it knows of
+each block how many lists hold it, gives blocks to sequences that grow, lets sequences share the blocks that they begin with,
+and takes back what is no longer held.  Lists are about block numbers, so the caches of all layers of a network go by one
+pool::
+
+    pool = BlockPool(n_blocks)
+    pages = torch.full((n_seqs, width), -1, dtype=torch.int32, device='cuda')
+    moves = pool.grow(pages, lengths, n)                  # blocks for n more tokens of each sequence
+    for cache in caches:
+        cache.copy(*moves)                                # open blocks that others hold too, for their new owners
+        cache.append(k, v, pages, lengths)
+    pool.fork(pages, lengths, parents, children)          # children begin with their parents' blocks
+    pool.free(pages, lengths, rows)                       # sequences that have ended
+
+Nothing here synchronises and every call can be captured in a graph; results do not depend on the order in which threads run:
+the lowest free block is taken first, and sequences are served in their order.  What a call cannot do for want of blocks it
+counts in ``missing``.  The calls of one pool go one after the other (on one stream, or on streams that wait for each other).
+
+A table is (n_seqs, blocks) int32, -1 where a list has no block.  A block must not be written to by two lists: after a fork
+the open last block is shared, and ``grow`` is what gives each its own before new tokens are appended.
+"""
+import torch
+
+from ._lib import BaKvForkArgs, BaKvGrowArgs, BaKvPool, BaKvTable, BaKvTrimArgs, launch, lib, written
+
+__all__ = ['BlockPool']
+
+BLOCK = 64
+
+
+def _fixed(name):
+    return property(lambda self: getattr(self, name))
+
+
+class BlockPool:
+    """Who holds the ``n_blocks`` blocks of a cache.
+
+    counts   (n_blocks,) int32: the lists that hold each block (to be read; ``count`` sets it from lists)
+    missing  (1,) int32: how many blocks the last ``grow`` wanted beyond those that were free
+    """
+
+    n_blocks, device, counts, missing = _fixed('_n_blocks'), _fixed('_device'), _fixed('_counts'), _fixed('_missing')
+
+    def __init__(self, n_blocks, device='cuda'):
+        if not 0 <= n_blocks < 1 << 30:
+            raise ValueError(f'pool: bad sizes ({n_blocks} blocks)')
+        self._counts = torch.zeros(n_blocks, dtype=torch.int32, device=device)
+        if not self._counts.is_cuda:
+            raise RuntimeError('pool: needs a GPU (it runs in libba_hip.so)')
+        self._n_blocks, self._device = n_blocks, self._counts.device
+        self._used = torch.zeros((n_blocks + 31) // 32, dtype=torch.int32, device=self._device)
+        self._marks = torch.full((2 * n_blocks,), -1, dtype=torch.int32, device=self._device)
+        self._missing = torch.zeros(1, dtype=torch.int32, device=self._device)
+        self._lib = lib()
+        if n_blocks % 32:                                   # bits past the last block are set
+            self._used[-1] = -1 << n_blocks % 32
+
+    def available(self):
+        """(1,) int64 on the device: the free blocks."""
+        return (self._counts == 0).sum().view(1)
+
+    def _pool(self):
+        return BaKvPool(self._counts.data_ptr(), self._used.data_ptr(), self._marks.data_ptr(), self._n_blocks)
+
+    def _table(self, pages, name='pages'):
+        shape, stride = pages.shape, pages.stride()
+        if (len(shape) != 2 or pages.dtype is not torch.int32 or pages.device != self._device or
+                stride[1] != 1 and shape[1] > 1 or stride[0] < shape[1] and shape[0] > 1):
+            raise ValueError(f'pool: {name} must be (n_seqs, blocks) int32 on {self._device} with contiguous rows that do not '
+                             'overlap')
+        return BaKvTable(pages.data_ptr(), stride[0], shape[0], shape[1])
+
+    def _ints(self, t, name, n=None):
+        if (t.dtype is not torch.int32 or t.device != self._device or t.dim() != 1 or n is not None and t.shape[0] != n or
+                not t.is_contiguous()):
+            raise ValueError(f'pool: {name} must be a contiguous int32 tensor of shape ({"n" if n is None else n},) on {self._device}')
+        return t.data_ptr()
+
+    def _launch(self, call, args, *changed):
+        pool = self._pool()
+        launch(lambda a, stream: call(pool, a, stream), args, self._device)
+        written((self._counts, *changed))
+
+    def _tables(self, tables):
+        found = (BaKvTable * len(tables))(*(self._table(t) for t in tables))
+        at = [t.data_ptr() for t in tables if t.numel()]
+        if len(set(at)) != len(at):
+            raise ValueError('pool: a table is given twice')
+        return found
+
+    def count(self, *tables):
+        """Set the counts from tables: those of all lists that are in use.  For lists that were made or changed by hand, or
+        read from a file."""
+        found = self._tables(tables)
+        self._launch(lambda p, a, stream: self._lib.ba_kv_pool_count(p, found, len(tables), stream), found)
+
+    def grow(self, pages, lengths, new, max_new=None):
+        """Blocks for ``new`` more tokens (a number, or (n_seqs,) int32) after the first ``lengths`` of each list, written into
+        ``pages``; entries that are there already stay.  max_new (default: what lists can hold) bounds ``new``, and a close
+        bound saves time.  ``lengths`` stays as it is.
+
+        Returns (src, dst, n) for ``KVCache.copy``: where new tokens would go to a block that has tokens and that other lists
+        hold too, it is exchanged for another one in this list, and src has to be copied to dst before anything is appended
+        (and before the next call on this pool).  One list after the other, so the last holder of a block keeps it.  Lists
+        that there are no blocks left for keep -1 there, an exchanged block's place among them, and rows appended there are
+        left out; ``missing`` says how many there were."""
+        table = self._table(pages)
+        S, width = pages.shape
+        a = BaKvGrowArgs(table=table, lengths=self._ints(lengths, 'lengths', S))
+        if isinstance(new, torch.Tensor):
+            a.more = self._ints(new, 'new', S)
+            most = min(width * BLOCK, (1 << 31) - 1) if max_new is None else max_new
+        else:
+            a.each = min(int(new), (1 << 31) - 1)
+            most = a.each if max_new is None else max_new
+            if new < 0:
+                raise ValueError(f'pool: {new} new tokens')
+        if most < 0:
+            raise ValueError('pool: a negative bound on tokens')
+        a.max_new = min(int(most), (1 << 31) - 1)
+        moves = torch.empty(2 * S + 1, dtype=torch.int32, device=self._device)
+        src, dst, n = moves[:S], moves[S:2 * S], moves[2 * S:]
+        a.src, a.dst, a.n, a.missing = src.data_ptr(), dst.data_ptr(), n.data_ptr(), self._missing.data_ptr()
+        self._launch(self._lib.ba_kv_pool_grow, a, pages, self._missing)
+        return src, dst, n
+
+    def fork(self, pages, lengths, parents, children, into=None):
+        """Row children[i] becomes the list of row parents[i] ((n,) int32 each): it gives back the blocks that it held, holds
+        its parent's blocks with tokens as well, and gets its length.  into: (pages, lengths) of the children, where they are in
+        another table (which a reordering of all sequences needs).  Pairs that name a row that is not there, whose child a
+        later pair has too, or whose child is a parent in the same table, change nothing."""
+        to, to_lengths = (pages, lengths) if into is None else into
+        a = BaKvForkArgs(from_=self._table(pages), to=self._table(to), from_lengths=self._ints(lengths, 'lengths', pages.shape[0]),
+                         to_lengths=self._ints(to_lengths, "the children's lengths", to.shape[0]))
+        a.parents, a.children, a.n = self._ints(parents, 'parents'), self._ints(children, 'children', parents.shape[0]), parents.shape[0]
+        if to.shape[1] < pages.shape[1]:
+            raise ValueError("pool: children's lists must be as wide as their parents'")
+        if to is not pages and to.numel() and pages.numel() and to.data_ptr() == pages.data_ptr() and to.stride() != pages.stride():
+            raise ValueError('pool: the tables overlap')
+        if a.n:
+            self._launch(self._lib.ba_kv_pool_fork, a, to, to_lengths)
+
+    def free(self, pages, lengths, rows=None):
+        """Give back the lists ``rows`` ((n,) int32; default: all): entries become -1, lengths 0."""
+        a = BaKvTrimArgs(table=self._table(pages), lengths=self._ints(lengths, 'lengths', pages.shape[0]), all=1)
+        if rows is not None:
+            a.rows, a.n_rows = self._ints(rows, 'rows'), rows.shape[0]
+            if not a.n_rows:
+                return
+        self._launch(self._lib.ba_kv_pool_trim, a, pages, lengths)
+
+    def trim(self, pages, first=None, last=None):
+        """Give back the blocks whose tokens all lie before ``first`` (a window that has moved on) or from ``last`` on (tokens
+        that were drafted and refused); (n_seqs,) int32 each."""
+        if first is None and last is None:
+            raise ValueError('pool: trim by first, by last or by both')
+        a = BaKvTrimArgs(table=self._table(pages))
+        if first is not None:
+            a.first = self._ints(first, 'first', pages.shape[0])
+        if last is not None:
+            a.last = self._ints(last, 'last', pages.shape[0])
+        self._launch(self._lib.ba_kv_pool_trim, a, pages)
+
+    def compact(self, *tables, most=None):
+        """Move the highest used blocks to the lowest free ones, ``most`` at a time at most (default: all), so that the used
+        blocks come to be the first: ``tables`` (all that hold blocks of the pool) are changed, and (src, dst, n) is for
+        ``KVCache.copy``, before the next call on this pool."""
+        found = self._tables(tables)
+        most = self._n_blocks // 2 if most is None else min(int(most), self._n_blocks // 2)
+        if most < 0:
+            raise ValueError(f'pool: {most} moves')
+        moves = torch.empty(2 * most + 1, dtype=torch.int32, device=self._device)
+        src, dst, n = moves[:most], moves[most:2 * most], moves[2 * most:]
+        self._launch(lambda p, a, stream: self._lib.ba_kv_pool_compact(p, found, len(tables), src.data_ptr(), dst.data_ptr(),
+                                                                       n.data_ptr(), most, stream), found, *tables)
+        return src, dst, n

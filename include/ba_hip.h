@@ -727,6 +727,117 @@ int ba_kv_attend(const ba_kv_attend_args* args, void* stream);
 int32_t ba_kv_attend_splits(int32_t n_seqs, int32_t heads, int32_t q_heads, int32_t dim, int64_t max_rows, int32_t n_pages);
 int64_t ba_kv_attend_workspace_bytes(int64_t n_rows, int32_t q_heads, int32_t dim, int32_t n_splits);
 
+/* The same with formed scores, masks by row and lists that begin alike.  The score z = scale * q.k of the row at position p
+ * and token j becomes cap * tanh(z / cap) where cap is not 0 (cap in [1e-3, 1e3]; right to 4e-7 * cap), then z - slopes[h] *
+ * |p - j| where slopes (finite numbers) are given.  A row sees j < lengths[s] with j < prefix[s], or with j >= since[row], j <
+ * until[row] and what causal and window say; any of the three may be NULL.  shared: the first so many blocks of all lists are
+ * the first sequence's: they are read once for all rows.  a.n_splits counts the parts of the sequences' own blocks,
+ * shared_parts those of the shared ones (0 without any); ba_kv_scored_parts gives both.  With more than one part in all,
+ * a.workspace has ba_kv_attend_workspace_bytes for their sum. */
+typedef struct {
+    ba_kv_attend_args a;
+    const float* slopes;       /* (q_heads,) */
+    const int32_t* prefix;     /* (n_seqs,) */
+    const int32_t* since;      /* (n_rows,) */
+    const int32_t* until;      /* (n_rows,) */
+    float cap;
+    int32_t shared;
+    int32_t shared_parts;
+    int32_t reserved;
+} ba_kv_scored_args;
+
+int ba_kv_attend_scored(const ba_kv_scored_args* args, void* stream);
+void ba_kv_scored_parts(const ba_kv_scored_args* args, int32_t* own, int32_t* shared);
+
+/* Pages of the cache.  A pool knows of each block how many lists hold it: counts (n_blocks,), used ((n_blocks + 31) / 32
+ * words, a bit for each block that a list holds, bits past the last block set) and marks (2 n_blocks ints, -1 in the first
+ * half between calls), all on the device; ba_kv_pool_count sets the three.  Tables of lists have -1 (any number below 0)
+ * where there is no block; entries past the pool are left as they are.  Calls on one pool go one after the other. */
+typedef struct {
+    int32_t* counts;
+    uint32_t* used;
+    int32_t* marks;
+    int64_t n_blocks;
+} ba_kv_pool;
+
+typedef struct {
+    int32_t* pages;            /* (n_seqs, n_pages), rows `stride` entries apart */
+    int64_t stride;
+    int32_t n_seqs, n_pages;
+} ba_kv_table;
+
+/* Counts from the lists of n_tables tables (a host array): each entry counts once. */
+int ba_kv_pool_count(const ba_kv_pool* pool, const ba_kv_table* tables, int32_t n_tables, void* stream);
+
+/* Row children[i] of `to` gives back what it holds and becomes the list of row parents[i] of `from`: its blocks with tokens
+ * (below from_lengths), and its length.  A pair that names a row out of range, a child that a later pair names too, or (in one
+ * table) a child that is the parent of a pair, changes nothing. */
+typedef struct {
+    ba_kv_table from, to;      /* may be the same; `to` is at least as wide */
+    const int32_t* from_lengths;
+    int32_t* to_lengths;
+    const int32_t* parents;
+    const int32_t* children;
+    int32_t n;
+    int32_t reserved;
+} ba_kv_fork_args;
+
+int ba_kv_pool_fork(const ba_kv_pool* pool, const ba_kv_fork_args* args, void* stream);
+
+/* Blocks without a token in [first[s], last[s]) are given back (all of them where `all` is set), their entries become -1; first
+ * and last may be NULL.  rows: (n_rows,) the lists that it is done to, or NULL for every one.  lengths: set to 0, or NULL. */
+typedef struct {
+    ba_kv_table table;
+    const int32_t* first;
+    const int32_t* last;
+    const int32_t* rows;
+    int32_t* lengths;
+    int32_t n_rows;
+    int32_t all;
+} ba_kv_trim_args;
+
+int ba_kv_pool_trim(const ba_kv_pool* pool, const ba_kv_trim_args* args, void* stream);
+
+/* Blocks for more[s] (or `each`; at most max_new) tokens after the first lengths[s] of every list, taken in the order of the
+ * lists, the lowest free block first; entries that are there already stay.  Where the first of them goes to a block that has
+ * tokens and that other lists hold too, that block is exchanged for another: (src, dst)[0 .. n) are the blocks to be copied,
+ * -1 after them ((n_seqs,) ints each).  One list after the other: the last holder of a block keeps it.  missing: blocks that
+ * there were not; entries without one are -1, an exchanged one too. */
+typedef struct {
+    ba_kv_table table;
+    const int32_t* lengths;
+    const int32_t* more;
+    int32_t each, max_new;
+    int32_t* src;
+    int32_t* dst;
+    int32_t* n;
+    int32_t* missing;
+} ba_kv_grow_args;
+
+int ba_kv_pool_grow(const ba_kv_pool* pool, const ba_kv_grow_args* args, void* stream);
+
+/* The highest used blocks go to the lowest free ones, at most `most` of them: the tables and counts are changed, (src, dst)[0 ..
+ * n) are the blocks to be copied, -1 after them (`most` ints each). */
+int ba_kv_pool_compact(const ba_kv_pool* pool, const ba_kv_table* tables, int32_t n_tables, int32_t* src, int32_t* dst,
+                       int32_t* n, int32_t most, void* stream);
+
+/* Blocks src[i] copied to dst[i], codes and factors, for i < min(n, *count); pairs with a number outside [0, n_blocks) are left
+ * out.  No block may be the destination of two pairs, or of one and the source of another. */
+typedef struct {
+    void* k;
+    void* v;
+    float* scales;
+    int64_t n_blocks;
+    int32_t heads, dim;
+    const int32_t* src;
+    const int32_t* dst;
+    const int32_t* count;      /* or NULL */
+    int32_t n;
+    int32_t reserved;
+} ba_kv_copy_args;
+
+int ba_kv_copy(const ba_kv_copy_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

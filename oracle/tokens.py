@@ -131,3 +131,115 @@ def attend(cache, q, pages, lengths, counts, scale, causal=True, window=None):
                     lse[row + i, h] = np.max(z) + math.log(p.sum()) if np.isfinite(p.sum()) and not np.isnan(vs).any() else math.nan
         row += n
     return o, lse, a
+
+
+def attend_formed(cache, q, pages, lengths, counts, scale, causal=True, window=None, cap=None, slopes=None, prefix=None,
+                  since=None, until=None):
+    """``attend`` with formed scores and masks: cap tanh(z / cap), less slopes[h] |p - j|; a row sees the tokens below its
+    sequence's prefix, and of the others those from since[row] on and below until[row], causal and in the window."""
+    o, a, lse = np.zeros(q.shape), np.zeros(q.shape), np.full(q.shape[:2], -math.inf)
+    group, row = q.shape[1] // cache.k.shape[1], 0
+    for s, (length, n) in enumerate(zip(lengths, counts)):
+        k, v, there = cache.sequence(pages[s], max(0, length))
+        j = np.arange(max(0, length))
+        for i in range(n):
+            at = length - n + i
+            seen = ((j <= at) if causal else True) & ((j > at - window) if window else True) & (j >= 0)
+            if since is not None:
+                seen = seen & (j >= since[row + i])
+            if until is not None:
+                seen = seen & (j < until[row + i])
+            if prefix is not None:
+                seen = seen | (j < prefix[s])
+            seen = seen & there
+            if np.any(seen):
+                for h in range(q.shape[1]):
+                    z = scale * (k[seen, h // group] @ q[row + i, h])
+                    if cap:
+                        z = cap * np.tanh(z / cap)
+                    if slopes is not None:
+                        z = z - float(slopes[h]) * np.abs(at - j[seen])
+                    p = np.exp(z - np.max(z))
+                    vs = v[seen, h // group]
+                    o[row + i, h] = p @ vs / p.sum()
+                    a[row + i, h] = p @ np.abs(vs) / p.sum()
+                    lse[row + i, h] = np.max(z) + math.log(p.sum()) if np.isfinite(p.sum()) and not np.isnan(vs).any() else math.nan
+        row += n
+    return o, lse, a
+
+
+class Pool:
+    """Which lists hold which of n blocks, call by call and list by list."""
+
+    def __init__(self, n):
+        self.counts, self.missing = [0] * n, 0
+
+    def _held(self, b):
+        return 0 <= b < len(self.counts)
+
+    def count(self, *tables):
+        self.counts = [0] * len(self.counts)
+        for t in tables:
+            for b in np.asarray(t).flatten().tolist():
+                if self._held(b):
+                    self.counts[b] += 1
+
+    def grow(self, pages, lengths, new):
+        """The copies to be made, as [(src, dst)]; pages is changed."""
+        free = [b for b, c in enumerate(self.counts) if c == 0][::-1]
+        moves, self.missing = [], 0
+
+        def take():
+            if free:
+                self.counts[free[-1]] = 1
+                return free.pop()
+            self.missing += 1
+            return -1
+
+        for row, length, n in zip(pages, lengths, new):
+            length, n, width = max(0, int(length)), max(0, int(n)), len(row)
+            at = length // 64
+            if n and length % 64 and at < width and self._held(row[at]) and self.counts[row[at]] > 1:
+                old = int(row[at])
+                self.counts[old] -= 1
+                row[at] = take()
+                if row[at] >= 0:
+                    moves.append((old, int(row[at])))
+            for b in range((length + 63) // 64, min(width, (length + n + 63) // 64)):
+                if row[b] < 0:
+                    row[b] = take()
+        return moves
+
+    def drop(self, row, keep=lambda b: False):
+        for b in range(len(row)):
+            if row[b] >= 0 and not keep(b):
+                if self._held(row[b]) and self.counts[row[b]] > 0:
+                    self.counts[row[b]] -= 1
+                row[b] = -1
+
+    def fork(self, pages, lengths, parents, children, to, to_lengths):
+        same = to is pages
+        for i, (p, c) in enumerate(zip(parents, children)):
+            if not (0 <= p < len(pages) and 0 <= c < len(to)) or c in children[i + 1:] or same and c in parents:
+                continue
+            row = [int(b) if self._held(b) and 64 * x < lengths[p] else -1 for x, b in enumerate(pages[p])]
+            for b in row:
+                if b >= 0:
+                    self.counts[b] += 1
+            for b in to[c]:
+                if self._held(b) and self.counts[b] > 0:
+                    self.counts[b] -= 1
+            to[c] = row + [-1] * (len(to[c]) - len(row))
+            to_lengths[c] = lengths[p]
+
+    def compact(self, tables, most):
+        free = [b for b, c in enumerate(self.counts) if c == 0]
+        used = [b for b, c in enumerate(self.counts) if c > 0][::-1]
+        moves = [(a, b) for a, b in zip(used, free) if b < a][:most]
+        for a, b in moves:
+            self.counts[b], self.counts[a] = self.counts[a], 0
+        for t in tables:
+            old = t.copy()
+            for a, b in moves:
+                t[old == a] = b
+        return moves

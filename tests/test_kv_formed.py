@@ -1,0 +1,371 @@
+"""Attention over the 8-bit cache with capped scores, biases by distance, masks by row and lists that begin alike: oracle pins
+and refusals (CPU), parity with the oracle (GPU).
+
+Bars: those of tests/test_tokens.py's attention (weights in fp16, scores in fp32: 1.2e-3 sum p |v| and half a step of the output;
+6e-4 for lse), in which what is new has room: a capped score is off by 4e-7 cap at most, 2e-5 of a weight for the caps here; a
+bias that matters is below 2^6 in the exponents of 2, with three roundings of fp32, 1e-5.  Where distances are measured from
+far tokens, lse adds slope times distance once: 2^-23 of it."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import tokens as otok
+from test_tokens import HALF_STEP, _cache, _i32, _mirror, _np, _pages
+
+DEV = 'cuda:0'
+
+
+# ---------------------------------------------------------------------------------- oracle pins (CPU)
+
+def test_oracle_with_nothing_formed_is_plain_attention():
+    rng = np.random.default_rng(0)
+    c = otok.Cache(rng.normal(size=(5, 2, 64, 32)), rng.normal(size=(5, 2, 64, 32)), np.ones((5, 2, 2)), 'int8')
+    q = rng.normal(size=(9, 4, 32))
+    for kw in (dict(), dict(causal=False), dict(window=20)):
+        for x, y in zip(otok.attend(c, q, [[0, 2], [3, -1]], [100, 70], [3, 6], 0.2, **kw),
+                        otok.attend_formed(c, q, [[0, 2], [3, -1]], [100, 70], [3, 6], 0.2, cap=1e9, slopes=[0.0] * 4,
+                                           prefix=[0, -1], since=[0] * 9, until=[200] * 9, **kw)):
+            assert np.allclose(x, y, rtol=1e-9, atol=1e-12)
+
+
+def test_oracle_known_answers():
+    """Two keys of scores 3 and 1 with values 1 and 0: the weights are known."""
+    k, v = np.zeros((1, 1, 64, 32)), np.zeros((1, 1, 64, 32))
+    k[0, 0, 0, 0], k[0, 0, 1, 0], v[0, 0, 0] = 3.0, 1.0, 1.0
+    c = otok.Cache(k, v, np.ones((1, 1, 2)), 'int8')
+    q = np.zeros((1, 1, 32))
+    q[0, 0, 0] = 1.0
+    run = lambda **kw: otok.attend_formed(c, q, [[0]], [2], [1], 1.0, **kw)[0][0, 0, 0]  # noqa: E731
+    sig = lambda x: 1 / (1 + math.exp(-x))  # noqa: E731
+    assert abs(run() - sig(2.0)) < 1e-12
+    assert abs(run(cap=2.0) - sig(2 * math.tanh(1.5) - 2 * math.tanh(0.5))) < 1e-12
+    assert abs(run(slopes=[0.5]) - sig(2.0 - 0.5)) < 1e-12                 # the first key is one token away
+    assert run(since=[1]) == 0.0 and run(until=[1]) == 1.0 and run(since=[2]) == 0.0 and run(since=[1], prefix=[1]) == run()
+    assert run(window=1) == 0.0 and abs(run(window=1, prefix=[1]) - sig(2.0)) < 1e-12
+
+
+# ---------------------------------------------------------------------------------- refusals (CPU)
+
+def test_formed_entry_point_refuses_bad_arguments_without_a_gpu():
+    from blast3r_amd import _lib
+    L = _lib.lib()
+    p = 4096                                                # addresses that are only compared with each other
+    good = dict(n_blocks=2, heads=2, dim=64, bits=0, n_seqs=1, n_pages=2, pages_stride=2, dtype=2, n_rows=3, rows_per_seq=3, max_rows=3,
+                q_heads=4, scale=1.0, n_splits=1, k=p, v=p, scales=p, pages=p, lengths=p, q=p, o=p)
+    assert L.ba_kv_attend_scored(None, None) != 0
+    for word, kw in (('cap', dict(cap=-1.0)), ('cap', dict(cap=math.nan)), ('cap', dict(cap=1e4)), ('cap', dict(cap=math.inf)),
+                     ('cap', dict(cap=1e-4)), ('shared', dict(shared=3, shared_parts=1)), ('shared', dict(shared=-1)),
+                     ('shared_parts', dict(shared=1)), ('shared_parts', dict(shared_parts=1)), ('parts', dict(n_splits=65536, shared=1, shared_parts=1)),
+                     ('null pointer', dict(shared=1, shared_parts=1)), ('too small', dict(shared=1, shared_parts=1, workspace=p, workspace_bytes=64)),
+                     ('head size', dict(dim=48)), ('aligned', dict(k=p + 8)), ('null pointer', dict(q=None)), ('scale', dict(scale=0.0)),
+                     ('too many', dict(n_seqs=1 << 23)), ('too many', dict(n_rows=(1 << 31) - 1, shared=1, shared_parts=1, offsets=p)),
+                     ('fp16 or bf16', dict(dtype=0)), ('bad sizes', dict(window=-1))):
+        a = _lib.BaKvScoredArgs(**{**good, **kw})
+        assert L.ba_kv_attend_scored(ctypes.byref(a), None) != 0 and word in L.ba_last_error().decode(), (kw, L.ba_last_error())
+    assert L.ba_kv_attend_scored(ctypes.byref(_lib.BaKvScoredArgs(**{**good, 'n_rows': 0})), None) == 0
+    own, shared = ctypes.c_int32(), ctypes.c_int32()
+    for kw in (dict(), dict(shared=2), dict(shared=1, window=5), dict(n_rows=0), dict(n_seqs=0, shared=1), dict(max_rows=0), dict(n_pages=0)):
+        a = _lib.BaKvScoredArgs(**{**good, **kw})
+        L.ba_kv_scored_parts(a, own, shared)
+        assert own.value >= 1 and shared.value == (1 if a.shared else 0) or shared.value > 1
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """KVCache over host tensors; the arguments of each launch are kept."""
+    from blast3r_amd import kv_cache
+    calls = []
+    monkeypatch.setattr(torch.Tensor, 'is_cuda', True, raising=False)
+    monkeypatch.setattr(kv_cache, 'launch', lambda call, args, device: calls.append(type(args).from_buffer_copy(args)))
+    return calls
+
+
+def test_python_refuses_bad_masks_and_scores(host):
+    from torch.autograd import forward_ad
+
+    from blast3r_amd.kv_cache import KVCache
+    c = KVCache(4, 2, 64, device='cpu')
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    q, pages, lens = torch.zeros(4, 4, 64, dtype=torch.bfloat16), i32([[0, 1], [2, 3]]), i32([5, 6])
+    for kw in (dict(cap=0.0), dict(cap=-1.0), dict(cap=math.nan), dict(cap=1e9), dict(slopes=torch.zeros(2)), dict(slopes=torch.zeros(4).double()),
+               dict(slopes=torch.zeros(8)[::2]), dict(prefix=i32([1])), dict(prefix=lens.long()), dict(since=i32([1, 2])), dict(until=i32([0] * 5)),
+               dict(until=i32([[0] * 4])), dict(shared=3), dict(shared=-1)):
+        with pytest.raises(ValueError):
+            c.attend(q, pages, lens, **kw)
+    with pytest.raises(RuntimeError, match='gradient'):
+        c.attend(q, pages, lens, slopes=torch.zeros(4, requires_grad=True))
+    with forward_ad.dual_level(), torch.no_grad(), pytest.raises(RuntimeError, match='gradient'):
+        c.attend(q, pages, lens, slopes=forward_ad.make_dual(torch.zeros(4), torch.zeros(4)))
+    assert not host
+    with torch.no_grad():
+        c.attend(q, pages, lens, slopes=torch.zeros(4, requires_grad=True))
+    c.attend(q, pages, lens, cap=50.0, prefix=i32([1, 2]), since=i32([0] * 4), until=i32([9] * 4), shared=1)
+    a = host[-1]
+    assert a.cap == 50.0 and a.shared == 1 and a.shared_parts >= 1 and a.n_splits >= 1 and a.prefix and a.since and a.until and not a.slopes
+    c.attend(q, pages, lens)                                # what was there goes the way it went
+    assert type(host[-1]).__name__ == 'BaKvAttendArgs' and type(a).__name__ == 'BaKvScoredArgs'
+    for kw in (dict(cap=1.0), dict(shared=1)):
+        c.attend(q[:0], i32(np.zeros((0, 2))), i32([]), **kw)
+
+
+# ---------------------------------------------------------------------------------- parity (GPU)
+
+def _run(c, o, q, pages, lens, counts, scale=None, shared=0, uniform=False, max_new=None, bar=None, **kw):
+    """attend() and what the oracle says; rows within max_new are compared."""
+    off = None if uniform else _i32(np.concatenate(([0], np.cumsum(counts))))
+    dev = {n: (torch.tensor(np.asarray(x), dtype=torch.float32 if n == 'slopes' else torch.int32, device=DEV) if n in ('slopes', 'prefix', 'since', 'until') and x is not None else x)
+           for n, x in kw.items()}
+    got, lse = c.attend(q, _i32(pages), _i32(lens), offsets=off, max_new=max_new or max(max(counts), 1), scale=scale, return_lse=True, shared=shared, **dev)
+    want, want_lse, size = otok.attend_formed(o, _np(q), pages, lens, counts, scale or 1.0 / math.sqrt(q.shape[2]), **kw)
+    assert np.array_equal(np.isnan(_np(got)), np.isnan(want))
+    ok = ~np.isnan(want)
+    step = HALF_STEP[q.dtype] * np.abs(want) + (2.0 ** -25 if q.dtype == torch.float16 else 0.0)
+    err = np.abs(_np(got) - want)[ok]
+    assert np.all(err <= (1.2e-3 * size + step)[ok]), float(np.max(err / np.maximum((1.2e-3 * size + step)[ok], 1e-300)))
+    assert np.array_equal(_np(lse) == -math.inf, want_lse == -math.inf)
+    fine = np.isfinite(want_lse)
+    assert np.all(np.abs(_np(lse)[fine] - want_lse[fine]) <= 6e-4 + 2.0 ** -22 * np.abs(want_lse[fine]))
+    return got
+
+
+def _masks(rng, lens, counts, kind):
+    """since, until of the rows: documents in a row, frames, or anything, rows that see nothing among them."""
+    since, until = [], []
+    for length, n in zip(lens, counts):
+        length = max(length, 1)
+        edges = np.unique(np.concatenate(([0], rng.integers(0, length + 1, 1 + length // 60), [length])))
+        for i in range(n):
+            at = max(0, length - n + i)
+            e = int(np.searchsorted(edges, at, side='right'))
+            lo, hi = int(edges[e - 1]), int(edges[min(e, len(edges) - 1)])
+            if kind == 'any':
+                lo, hi = (int(x) for x in rng.integers(-5, length + 9, 2))
+            since.append(lo)
+            until.append(hi)
+    return since, until
+
+
+FORMED = [
+    # dim, heads, group, lengths, counts, options
+    (64, 2, 1, [1, 64, 65, 200], [1, 1, 1, 1], dict(cap=5.0)),
+    (64, 1, 4, [700, 3, 0, 129], [1, 2, 1, 4], dict(slopes=True, prefix=[5, 1, 3, 70])),
+    (128, 2, 8, [300, 900], [1, 1], dict(window=100, prefix=[64, 3])),
+    (128, 1, 5, [333], [6], dict(mask='documents', cap=20.0)),
+    (96, 2, 3, [100, 257], [10, 40], dict(window=37, prefix=[0, -4], slopes=True)),
+    (64, 1, 1, [5, 90], [9, 33], dict(cap=1.0, prefix=[100, 80])),         # more rows than tokens; prefix past the length
+    (32, 2, 2, [500], [70], dict(causal=False, mask='frames')),
+    (64, 1, 2, [400, 191], [150, 63], dict(mask='documents', slopes=True)),
+    (128, 1, 1, [330], [300], dict(causal=False, slopes=True)),            # tokens on both sides of a row
+    (128, 2, 2, [600, 1], [250, 1], dict(mask='any', cap=50.0)),
+    (256, 1, 2, [300], [80], dict(mask='any', causal=False, slopes=True, cap=7.0)),
+    (256, 2, 1, [650], [1], dict(slopes=True, window=200, prefix=[10])),
+    (32, 1, 16, [4000], [1], dict(window=64, prefix=[1], cap=30.0)),
+    (64, 1, 1, [3000], [3], dict(mask='any', causal=False, prefix=[130])),
+    (96, 2, 3, [190, 2500], [70, 1], dict(mask='frames', causal=False, prefix=[7, 1000])),
+    (64, 2, 1, [70, 0, 1, 2100], [70, 0, 1, 300], dict(window=200, prefix=[64, 1, 1, 65], slopes=True)),
+    (96, 1, 2, [1300], [200], dict(mask='documents', window=50)),
+    (256, 1, 4, [700], [6], dict(mask='documents', causal=False, cap=12.0)),
+    (32, 1, 2, [900], [300], dict(cap=3.0, slopes=True, causal=False, prefix=[500])),
+]
+
+
+def _case(rng, dim, heads, group, lens, counts, bits, opts, dtype, more=1):
+    blocks = [max(1, (n + 63) // 64) for n in lens]
+    c, o = _cache(sum(blocks) + 1, heads, dim, bits, seed=dim)
+    pages = _pages(rng, blocks, sum(blocks) + 1, max(blocks) + 2)
+    for s, n in enumerate(lens):                            # codes of places that hold no token yet may be anything
+        if n % 64:
+            p = int(pages[s, n // 64])
+            c.k.view(torch.uint8)[p, :, n % 64:] = 0x7f
+            c.v.view(torch.uint8)[p, :, :, n % 64:] = 0x7f
+    opts = dict(opts)
+    kind = opts.pop('mask', None)
+    if kind:
+        since, until = _masks(rng, lens, counts, kind)
+        opts.update({'documents': dict(since=since), 'frames': dict(until=until), 'any': dict(since=since, until=until)}[kind])
+    if opts.get('slopes'):
+        opts['slopes'] = [float(np.float32(2.0 ** (-8.0 * (h + 1) / (heads * group)))) for h in range(heads * group)]
+    x = torch.tensor(rng.normal(size=(sum(counts), heads * group + 1, dim)) * 2.0, dtype=torch.float32).to(dtype).to(DEV)
+    return c, o, x[:, 1:], pages, opts
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', ['fp8', 'int8'])
+@pytest.mark.parametrize('dim,heads,group,lens,counts,opts', FORMED)
+def test_formed_attention_against_oracle(bits, dim, heads, group, lens, counts, opts):
+    rng = np.random.default_rng(sum(lens))
+    for dtype in (torch.bfloat16, torch.float16):
+        c, o, q, pages, kw = _case(rng, dim, heads, group, lens, counts, bits, opts, dtype)
+        print(f'formed {bits} {dtype} {dim} {heads} {group} {lens} {counts} {opts}', flush=True)
+        _run(c, o, q, pages, lens, counts, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('counts', [[1], [3], [12], [40], [150], [300]])
+def test_formed_attention_ranges(counts):
+    """Factors far apart in neighbouring blocks, missing blocks, a NaN block that only some rows see, slopes from 2^-12 to 4 of
+    either sign, caps from 1e-3 up, scores far past the cap."""
+    rng = np.random.default_rng(counts[0])
+    n = 64 * 20 - 11
+    c, o = _cache(22, 1, 64, 'int8')
+    pages = _pages(rng, [20], 22, 20)
+    for b in range(20):
+        e = int(rng.integers(-20, 20))
+        c.scales[int(pages[0, b]), 0] = torch.tensor([2.0 ** (-7 - abs(e) / 4), 2.0 ** (2 * e)], device=DEV)
+    pages[0, 3] = -1
+    pages[0, 7] = 22
+    o = _mirror(c, 'int8')
+    x = rng.normal(size=(counts[0], 2, 64)) * np.exp(rng.normal(size=(counts[0], 2, 1)) * 2)
+    x[0, 0] = 0.0
+    q = torch.tensor(x, dtype=torch.float32).clamp(-8, 8).bfloat16().to(DEV)
+    print(f'formed ranges {counts}', flush=True)
+    for cap in (1e-3, 0.7, 40.0):
+        _run(c, o, q, pages, [n], counts, cap=cap)
+    for slopes in ([2.0 ** -12, 4.0], [-0.01, 0.25], [0.0, 1.0]):
+        _run(c, o, q, pages, [n], counts, slopes=slopes)
+        _run(c, o, q, pages, [n], counts, slopes=slopes, causal=False, cap=30.0)
+    c.scales[int(pages[0, 19]), 0, 0] = math.nan
+    c.scales[int(pages[0, 2]), 0, 1] = math.nan
+    o = _mirror(c, 'int8')
+    _run(c, o, q, pages, [n], counts, window=64 * 10, cap=9.0)
+    _run(c, o, q, pages, [n], counts, since=[64 * 3 + i % 200 for i in range(counts[0])], until=[64 * 19 + (i % 3 - 1) for i in range(counts[0])],
+         slopes=[0.1, 0.02])
+    _run(c, o, q, pages, [n], counts, since=[64 * 4] * counts[0], prefix=[64 * 2 + 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [1, 20, 100])
+def test_slopes_over_far_tokens_only(n):
+    """Rows that see nothing but tokens far away: their biases differ by little beside their size.  Distances are measured from
+    the nearest of them (with negative slopes: the farthest), so nothing is lost."""
+    rng = np.random.default_rng(n)
+    length = 64 * 400
+    c, o = _cache(40, 1, 64, 'fp8')
+    pages = np.full((1, 400), -1)
+    pages[0, :20] = np.arange(20)                           # the blocks after the first 20 are not there
+    pages[0, 380:] = 20 + np.arange(20)
+    q = torch.tensor(rng.normal(size=(n, 2, 64)), dtype=torch.float32, device=DEV).bfloat16()
+    print(f'far tokens {n}', flush=True)
+    for slopes in ([0.5, 0.01], [-0.5, -0.003]):
+        _run(c, o, q, pages, [length], [n], slopes=slopes, until=[1000 + i for i in range(n)])
+        _run(c, o, q, pages, [length], [n], slopes=slopes, since=[length] * n, prefix=[700])
+
+
+# ---------------------------------------------------------------------------------- lists that begin alike (GPU)
+
+SHARED = [
+    # dim, heads, group, shared blocks, lengths, counts, options
+    (64, 2, 1, 1, [65, 64, 200, 70], [1, 1, 1, 1], {}),
+    (128, 1, 4, 5, [700, 330, 320, 323], [1, 2, 0, 4], {}),
+    (128, 2, 2, 20, [1281 + 7 * i for i in range(40)], [1] * 40, dict(cap=20.0)),
+    (96, 2, 3, 3, [300, 457], [10, 40], dict(window=137)),
+    (64, 1, 1, 4, [100, 290, 3], [9, 33, 3], {}),                          # sequences that end within the shared blocks
+    (64, 1, 2, 10, [840, 660, 640], [150, 20, 0], dict(slopes=True)),
+    (64, 4, 1, 12, [768 + 100] * 5, [100] * 5, dict(causal=False)),
+    (256, 1, 2, 6, [500, 390], [80, 3], dict(prefix=[70, 1], window=60)),
+    (32, 1, 8, 30, [2000, 1921], [5, 1], dict(cap=10.0, slopes=True)),
+    (128, 1, 1, 9, [900, 700], [300, 90], dict(mask='any', causal=False)),
+    (64, 2, 2, 7, [448, 448], [1, 1], {}),                                 # nothing of their own
+    (128, 2, 4, 40, [2700], [1], {}),                                      # one sequence
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', ['fp8', 'int8'])
+@pytest.mark.parametrize('dim,heads,group,shared,lens,counts,opts', SHARED)
+def test_shared_blocks_against_oracle(bits, dim, heads, group, shared, lens, counts, opts):
+    rng = np.random.default_rng(sum(lens))
+    c, o, q, pages, kw = _case(rng, dim, heads, group, lens, counts, bits, opts, torch.bfloat16)
+    longest = int(np.argmax(lens))
+    pages[:, :shared] = pages[longest, :shared]
+    o = _mirror(c, bits)
+    print(f'shared {bits} {dim} {heads} {group} {shared} {lens} {counts} {opts}', flush=True)
+    uniform = len(set(counts)) == 1
+    a = _run(c, o, q, pages, lens, counts, shared=shared, uniform=uniform, **kw)
+    b = _run(c, o, q, pages, lens, counts, uniform=uniform, **kw)
+    assert float((a - b).float().abs().max()) <= 3e-3 * max(1.0, float(b.float().abs().max())) + 2.0 ** -7 * float(b.float().abs().max())
+    assert torch.equal(a, _run(c, o, q, pages, lens, counts, shared=shared, uniform=uniform, **kw))
+
+
+@pytest.mark.gpu
+def test_shared_rows_that_no_sequence_has_are_left_alone():
+    """Rows past max_new, past the last sequence or before the first are not written, nor is their lse."""
+    rng = np.random.default_rng(5)
+    c, o = _cache(8, 2, 64, 'fp8')
+    pages = np.array([[0, 1, 2, 3], [0, 1, 4, 5]])
+    for n, most in ((3, 2), (40, 30), (200, 100)):
+        lens, total = [200, 256], n + 5 + 4
+        q = torch.tensor(rng.normal(size=(total, 4, 64)), dtype=torch.float32, device=DEV).bfloat16()
+        y = torch.full_like(q, 7.0)
+        print(f'shared bounds {n}', flush=True)
+        off = _i32([2, 2 + n, 2 + n + 5])
+        _, lse = c.attend(q, _i32(pages), _i32(lens), offsets=off, max_new=most, out=y, shared=2, return_lse=True, cap=9.0)
+        rows = _np(q)[2:2 + n + 5]
+        want, _, size = otok.attend_formed(o, rows, pages, lens, [n, 5], 0.125, cap=9.0)
+        done = np.r_[0:min(n, most), n:n + min(5, most)]
+        assert np.all(np.abs(_np(y)[2:2 + n + 5] - want)[done] <= 1.2e-3 * size[done] + 2.0 ** -8 * np.abs(want[done]))
+        rest = np.setdiff1d(np.arange(total), 2 + done)
+        assert bool((y[torch.tensor(rest, device=DEV)] == 7.0).all())
+
+
+@pytest.mark.gpu
+def test_formed_calls_of_bad_lists_stay_inside():
+    """Lengths past the lists, negative ones, offsets out of order, a cache without blocks: zeros or untouched rows."""
+    from blast3r_amd.kv_cache import KVCache
+    c, o = _cache(8, 2, 64, 'int8')
+    none = KVCache(0, 2, 64, device=DEV)
+    print('formed bad lists', flush=True)
+    slopes = torch.tensor([0.1, 0.2], device=DEV)
+    for n in (2, 40, 400):
+        q = torch.randn((n, 2, 64), device=DEV).bfloat16()
+        for kw in (dict(cap=5.0), dict(slopes=slopes), dict(prefix=_i32([9, 100000])), dict(shared=2), dict(shared=3, cap=4.0)):
+            got, lse = none.attend(q, _i32(np.zeros((2, 3))), _i32([150, 20]), return_lse=True, **kw)
+            assert not got.any() and bool((lse == -math.inf).all())
+            got = c.attend(q, _i32([[0, 1, -1], [9, 99, 1 << 30]]), _i32([100000, -5]), **kw)
+            assert bool(torch.isfinite(got).all()) and not got[n // 2:].any()
+            y = torch.full_like(q, 7.0)
+            c.attend(q, _i32([[0, 1, 2]] * 2), _i32([50, 60]), offsets=_i32([n + 9, -2, n + 4]), out=y, **kw)
+            assert bool((y == 7.0).all())
+    assert not c.attend(q[:2], _i32(np.zeros((2, 0))), _i32([5, 6]), prefix=_i32([3, 4])).any()
+
+
+@pytest.mark.gpu
+def test_formed_steps_in_a_graph_and_on_a_side_stream():
+    """A step of samples that share a prompt, captured once and replayed with other inputs, lengths, masks and slopes, with
+    eager work between the replays; the same on another stream."""
+    c, _ = _cache(60, 2, 64, 'fp8')
+    S = 6
+    pages = torch.cat((_i32([list(range(20))] * S), _i32(20 + np.arange(36).reshape(6, 6))), 1)
+    q = torch.zeros((S, 8, 64), dtype=torch.bfloat16, device=DEV)
+    lens, prefix, since = _i32([1280] * S), _i32([0] * S), _i32([0] * S)
+    slopes = torch.zeros(8, device=DEV)
+
+    def step():
+        return c.attend(q, pages, lens, shared=20, cap=30.0, slopes=slopes, prefix=prefix, since=since)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step()
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    print('formed graph', flush=True)
+    for t in range(12):
+        q.copy_(torch.randn(q.shape, device=DEV, generator=gen) * 3)
+        lens.copy_(torch.randint(1, 1280 + 384, (S,), device=DEV, generator=gen))
+        prefix.copy_(torch.randint(0, 200, (S,), device=DEV, generator=gen))
+        since.copy_(torch.randint(0, 1500, (S,), device=DEV, generator=gen))
+        slopes.copy_(torch.rand(8, device=DEV, generator=gen) * 0.1)
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = step()
+        torch.cuda.synchronize()
+        assert torch.equal(y, eager) and torch.equal(y, other), t

@@ -1,0 +1,489 @@
+"""Pages of the 8-bit cache (BlockPool, KVCache.copy): refusals and what calls owe to torch (CPU); lists, counts and moves equal
+to the oracle's, block copies, and a run of all of them with the cache's other calls (GPU).  All results are whole numbers or
+copies: they are equal or wrong."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import tokens as otok
+from test_tokens import _cache, _i32, _np
+
+DEV = 'cuda:0'
+
+
+# ---------------------------------------------------------------------------------- oracle pins (CPU)
+
+def test_oracle_pool_known_answers():
+    p = otok.Pool(6)
+    rows, lens = np.full((3, 4), -1), [0, 0, 0]
+    assert p.grow(rows, lens, [65, 1, 0]) == [] and rows.tolist() == [[0, 1, -1, -1], [2, -1, -1, -1], [-1] * 4]
+    lens = [65, 1, 0]
+    table = rows.tolist()
+    p.fork(table, lens, [0, 0], [2, 1], table, lens)        # the second child gives its block back
+    assert table == [[0, 1, -1, -1]] * 3 and lens == [65, 65, 65] and p.counts == [3, 3, 0, 0, 0, 0]
+    rows = np.array(table)
+    assert p.grow(rows, lens, [1, 1, 64]) == [(1, 2), (1, 3)]              # the last holder keeps block 1
+    assert rows.tolist() == [[0, 2, -1, -1], [0, 3, -1, -1], [0, 1, 4, -1]] and p.counts == [3, 1, 1, 1, 1, 0]
+    assert p.grow(rows, [66, 66, 129], [128, 0, 64]) == [] and p.missing == 2 and rows.tolist()[0] == [0, 2, 5, -1]
+    p.drop(rows[0])
+    p.drop(rows[1])
+    assert p.counts == [1, 1, 0, 0, 1, 0]
+    assert p.compact([rows], 3) == [(4, 2)] and rows[2].tolist() == [0, 1, 2, -1] and p.counts == [1, 1, 1, 0, 0, 0]
+
+
+# ---------------------------------------------------------------------------------- refusals (CPU)
+
+def test_pool_entry_points_refuse_bad_arguments_without_a_gpu():
+    from blast3r_amd import _lib
+    L, p = _lib.lib(), 4096
+    pool = _lib.BaKvPool(p, p, p, 40)
+    table = lambda **kw: _lib.BaKvTable(**{**dict(pages=p, stride=4, n_seqs=2, n_pages=4), **kw})  # noqa: E731
+
+    def refused(call, word, *args):
+        assert call(*args, None) != 0 and word in L.ba_last_error().decode(), (word, L.ba_last_error())
+
+    for bad, word in ((_lib.BaKvPool(None, p, p, 40), 'null'), (_lib.BaKvPool(p, p, p, -1), 'bad sizes'), (_lib.BaKvPool(p, p, p, 1 << 30), 'bad sizes'),
+                      (None, 'null')):
+        refused(L.ba_kv_pool_count, word, bad, table(), 1)
+        refused(L.ba_kv_pool_grow, word, bad, _lib.BaKvGrowArgs(table=table(), lengths=p, src=p, dst=p, n=p, missing=p))
+        refused(L.ba_kv_pool_trim, word, bad, _lib.BaKvTrimArgs(table=table()))
+        refused(L.ba_kv_pool_fork, word, bad, _lib.BaKvForkArgs(from_=table(), to=table()))
+        refused(L.ba_kv_pool_compact, word, bad, table(), 1, p, p, p, 3)
+    for t, word in ((table(n_seqs=-1), 'bad sizes'), (table(n_pages=1 << 24), 'bad sizes'), (table(n_seqs=1 << 23), 'too many'), (table(pages=None), 'null')):
+        refused(L.ba_kv_pool_count, word, pool, t, 1)
+        refused(L.ba_kv_pool_grow, word, pool, _lib.BaKvGrowArgs(table=t, lengths=p, src=p, dst=p, n=p, missing=p))
+        refused(L.ba_kv_pool_trim, word, pool, _lib.BaKvTrimArgs(table=t))
+        refused(L.ba_kv_pool_fork, word, pool, _lib.BaKvForkArgs(from_=table(), to=t))
+        refused(L.ba_kv_pool_compact, word, pool, t, 1, p, p, p, 3)
+    refused(L.ba_kv_pool_count, 'null', pool, None, 1)
+    refused(L.ba_kv_pool_grow, 'bad sizes', pool, _lib.BaKvGrowArgs(table=table(), lengths=p, src=p, dst=p, n=p, missing=p, max_new=-1))
+    for name in ('lengths', 'src', 'dst', 'n', 'missing'):
+        refused(L.ba_kv_pool_grow, 'null', pool, _lib.BaKvGrowArgs(**{**dict(table=table(), lengths=p, src=p, dst=p, n=p, missing=p), name: None}))
+    fork = dict(from_=table(), to=table(), from_lengths=p, to_lengths=p, parents=p, children=p, n=2)
+    for name in ('from_lengths', 'to_lengths', 'parents', 'children'):
+        refused(L.ba_kv_pool_fork, 'null', pool, _lib.BaKvForkArgs(**{**fork, name: None}))
+    refused(L.ba_kv_pool_fork, 'narrower', pool, _lib.BaKvForkArgs(**{**fork, 'to': table(n_pages=3)}))
+    refused(L.ba_kv_pool_fork, 'bad sizes', pool, _lib.BaKvForkArgs(**{**fork, 'n': -1}))
+    assert L.ba_kv_pool_fork(pool, _lib.BaKvForkArgs(**{**fork, 'n': 0}), None) == 0
+    refused(L.ba_kv_pool_compact, 'bad sizes', pool, table(), 1, p, p, p, 41)
+    refused(L.ba_kv_pool_compact, 'null', pool, table(), 1, p, p, None, 3)
+    copy = dict(k=p, v=p, scales=p, n_blocks=3, heads=2, dim=64, src=p, dst=p, n=2)
+    for kw, word in ((dict(dim=48), 'head size'), (dict(heads=0), 'bad sizes'), (dict(n=-1), 'bad sizes'), (dict(k=p + 8), 'aligned'), (dict(dst=None), 'null')):
+        refused(L.ba_kv_copy, word, _lib.BaKvCopyArgs(**{**copy, **kw}))
+    assert L.ba_kv_copy(_lib.BaKvCopyArgs(**{**copy, 'n': 0}), None) == 0
+
+
+@pytest.fixture
+def host(monkeypatch):
+    from blast3r_amd import kv_cache, kv_pool
+    calls = []
+    monkeypatch.setattr(torch.Tensor, 'is_cuda', True, raising=False)
+    for m in (kv_cache, kv_pool):
+        monkeypatch.setattr(m, 'launch', lambda call, args, device: calls.append(args))
+    return calls
+
+
+def _ints(x):
+    return torch.tensor(np.asarray(x), dtype=torch.int32)
+
+
+def test_pool_refuses_host_tensors_and_bad_sizes():
+    from blast3r_amd.kv_pool import BlockPool
+    with pytest.raises(RuntimeError):
+        BlockPool(4, device='cpu')
+    for n in (-1, 1 << 30):
+        with pytest.raises(ValueError):
+            BlockPool(n, device='cpu')
+
+
+def test_pool_refuses_bad_arguments(host):
+    from blast3r_amd.kv_cache import KVCache
+    from blast3r_amd.kv_pool import BlockPool
+    pool = BlockPool(40, device='cpu')
+    pages, lens = torch.full((2, 6), -1, dtype=torch.int32), _ints([0, 0])
+    wide = torch.full((2, 12), -1, dtype=torch.int32)
+    for bad in (pages.long(), pages[0], pages.t(), wide[:, ::2], pages[:1].expand(2, 6)):
+        for call in (lambda: pool.count(bad), lambda: pool.grow(bad, lens, 1), lambda: pool.free(bad, lens), lambda: pool.trim(bad, first=lens),
+                     lambda: pool.compact(bad), lambda: pool.fork(bad, lens, lens, lens), lambda: pool.fork(pages, lens, lens, lens, into=(bad, lens))):
+            with pytest.raises(ValueError):
+                call()
+    for bad in (lens.long(), lens[:1], _ints([[0, 0]]), _ints([0, 0, 0, 0])[::2]):
+        for call in (lambda: pool.grow(pages, bad, 1), lambda: pool.grow(pages, lens, bad), lambda: pool.free(pages, bad), lambda: pool.trim(pages, last=bad),
+                     lambda: pool.fork(pages, bad, lens, lens), lambda: pool.fork(pages, lens, lens, bad)):
+            with pytest.raises(ValueError):
+                call()
+    for call in (lambda: pool.grow(pages, lens, -1), lambda: pool.grow(pages, lens, 1, max_new=-1), lambda: pool.trim(pages), lambda: pool.compact(pages, pages),
+                 lambda: pool.compact(pages, most=-1), lambda: pool.fork(pages, lens, lens, lens, into=(pages[:, :5], lens)),
+                 lambda: pool.fork(wide, lens, lens, lens, into=(pages, lens)), lambda: pool.fork(pages, lens, lens, lens, into=(wide[:, :6].as_strided((2, 6), (6, 1)), _ints([0])))):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(AttributeError):
+        pool.counts = pages
+    c = KVCache(4, 1, 64, device='cpu')
+    for args in ((lens.long(), lens), (lens, lens[:1]), (lens, _ints([0, 0, 0])), (lens, lens, lens), (_ints([[0]]), lens), (_ints([0, 0, 0, 0])[::2], lens)):
+        with pytest.raises(ValueError):
+            c.copy(*args)
+    assert not host
+
+
+def test_tensors_that_pool_calls_write_to_count_as_changed(host):
+    from blast3r_amd.kv_cache import KVCache
+    from blast3r_amd.kv_pool import BlockPool
+    pool = BlockPool(40, device='cpu')
+    pages, other, lens, ends = torch.full((2, 6), -1, dtype=torch.int32), torch.full((3, 6), -1, dtype=torch.int32), _ints([0, 0]), _ints([0, 0, 0])
+    c = KVCache(40, 1, 64, device='cpu')
+    calls = (
+        (lambda: pool.count(pages), (pool.counts,)), (lambda: pool.grow(pages, lens, 1), (pool.counts, pages, pool.missing)),
+        (lambda: pool.fork(pages, lens, lens, lens), (pool.counts, pages, lens)),
+        (lambda: pool.fork(pages, lens, lens, lens, into=(other, ends)), (pool.counts, other, ends)),
+        (lambda: pool.free(pages, lens), (pool.counts, pages, lens)), (lambda: pool.trim(other, first=ends), (pool.counts, other)),
+        (lambda: pool.compact(pages, other), (pool.counts, pages, other)), (lambda: c.copy(lens, lens), (c.k, c.v, c.scales)))
+    everything = (pool.counts, pool.missing, pages, other, lens, ends, c.k, c.v, c.scales)
+    for call, changed in calls:
+        before = [t._version for t in everything]
+        call()
+        for t, v in zip(everything, before):
+            assert t._version == v + (1 if any(t is u for u in changed) else 0)
+    n = len(host)
+    for call in (lambda: pool.free(pages, lens, rows=lens[:0]), lambda: pool.fork(pages, lens, lens[:0], lens[:0]), lambda: c.copy(lens[:0], lens[:0])):
+        call()
+    assert len(host) == n
+
+
+def test_copies_of_factors_with_gradients_are_refused(host):
+    from blast3r_amd.kv_cache import KVCache
+    c = KVCache(2, 1, 64, device='cpu')
+    w = KVCache.wrap(c.k, c.v, torch.ones(2, 1, 2, requires_grad=True))
+    with pytest.raises(RuntimeError, match='gradient'):
+        w.copy(_ints([0]), _ints([1]))
+    assert not host
+
+
+# ---------------------------------------------------------------------------------- parity (GPU)
+
+class Both:
+    """A pool and its oracle, and a table with its lengths."""
+
+    def __init__(self, n_blocks, n_seqs, width):
+        from blast3r_amd.kv_pool import BlockPool
+        self.pool, self.o = BlockPool(n_blocks, device=DEV), otok.Pool(n_blocks)
+        self.pages, self.lens = np.full((n_seqs, width), -1), [0] * n_seqs
+        self.t = torch.full((n_seqs, width + 3), -7, dtype=torch.int32, device=DEV)[:, :width]       # rows that are not one after the other
+        self.t.fill_(-1)
+        self.tl = torch.zeros(n_seqs, dtype=torch.int32, device=DEV)
+
+    def same(self):
+        assert self.t.tolist() == self.pages.tolist() and self.tl.tolist() == [int(x) for x in self.lens]
+        assert self.pool.counts.tolist() == self.o.counts and int(self.pool.available()) == self.o.counts.count(0)
+        used = self.pool._used.cpu().numpy().view(np.uint32)
+        bits = (used[:, None] >> np.arange(32, dtype=np.uint32) & 1).flatten()
+        assert bits[:len(self.o.counts)].tolist() == [int(c > 0) for c in self.o.counts] and bits[len(self.o.counts):].all()
+        assert bool((self.pool._marks[:len(self.o.counts)] == -1).all())
+
+    def moved(self, moves, got, size):
+        src, dst, n = got
+        assert int(n) == len(moves)
+        assert src.tolist() == [m[0] for m in moves] + [-1] * (size - len(moves)) and dst.tolist() == [m[1] for m in moves] + [-1] * (size - len(moves))
+
+    def grow(self, new, max_new=None):
+        each = isinstance(new, int)
+        got = self.pool.grow(self.t, self.tl, new if each else _i32(new), max_new=max_new)
+        counts = [new] * len(self.lens) if each else [min(x, max_new) if max_new is not None else x for x in new]
+        moves = self.o.grow(self.pages, self.lens, counts)
+        self.moved(moves, got, len(self.lens))
+        assert int(self.pool.missing) == self.o.missing
+        return counts
+
+    def advance(self, counts):
+        self.lens = [x + max(0, n) for x, n in zip(self.lens, counts)]
+        self.tl.copy_(_i32(self.lens))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n_blocks,n_seqs,width,most,seed', [
+    (1, 1, 1, 64, 0), (31, 3, 5, 70, 1), (32, 4, 8, 130, 2), (33, 40, 6, 1, 3), (200, 17, 30, 200, 4), (5000, 64, 120, 1, 5), (5000, 64, 120, 900, 6),
+    (40000, 1500, 9, 100, 7), (70001, 20, 300, 5000, 8)])
+def test_pool_against_oracle(n_blocks, n_seqs, width, most, seed):
+    """Sequences that grow, fork, give back from either end, end and are moved together, in no order, also where blocks run
+    out."""
+    rng = np.random.default_rng(seed)
+    b = Both(n_blocks, n_seqs, width)
+    print(f'pool {n_blocks} {n_seqs} {width} {most}', flush=True)
+    b.same()
+    for step in range(12 if n_seqs < 1000 else 5):
+        what = int(rng.integers(0, 6)) if step > 1 else 0
+        print(f'  step {step}: {what}', flush=True)
+        if what <= 1:
+            new = rng.integers(0, most + 1, n_seqs).tolist() if rng.random() < 0.7 else most
+            if not isinstance(new, int) and rng.random() < 0.3:
+                new[int(rng.integers(0, n_seqs))] = -3
+            counts = b.grow(new, max_new=None if isinstance(new, int) else most - int(rng.integers(0, 2)))
+            b.advance(counts)
+        elif what == 2:
+            order = rng.permutation(n_seqs)
+            k = max(1, n_seqs // 3)
+            parents, children = rng.choice(order[:k], k).tolist(), order[k:2 * k].tolist()
+            children = (children + [n_seqs, -1] * k)[:k]
+            if k > 2:
+                children[-1] = children[0]                  # the first of the two is left out
+            b.pool.fork(b.t, b.tl, _i32(parents), _i32(children))
+            rows = b.pages.tolist()
+            b.o.fork(rows, b.lens, parents, children, rows, b.lens)
+            b.pages = np.array(rows)
+        elif what == 3:
+            rows = rng.integers(-1, n_seqs + 1, max(1, n_seqs // 4)).tolist()       # some twice, some that are not there
+            b.pool.free(b.t, b.tl, _i32(rows))
+            for r in rows:
+                if 0 <= r < n_seqs:
+                    b.o.drop(b.pages[r])
+                    b.lens[r] = 0
+        elif what == 4:
+            first, last = rng.integers(-70, 200, n_seqs), np.array(b.lens) + rng.integers(-100, 100, n_seqs)
+            use = int(rng.integers(0, 3))
+            b.pool.trim(b.t, first=_i32(first) if use != 1 else None, last=_i32(last) if use != 0 else None)
+            for s in range(n_seqs):
+                lo = max(0, int(first[s])) // 64 if use != 1 else 0
+                hi = (max(0, int(last[s])) + 63) // 64 if use != 0 else 1 << 30
+                b.o.drop(b.pages[s], keep=lambda x, lo=lo, hi=hi: lo <= x < hi)
+            if use != 0:
+                b.lens = [max(0, min(x, int(y))) for x, y in zip(b.lens, last)]
+                b.tl.copy_(_i32(b.lens))
+        else:
+            some = None if rng.random() < 0.5 else int(rng.integers(0, n_blocks + 1))
+            size = n_blocks // 2 if some is None else min(some, n_blocks // 2)
+            got = b.pool.compact(b.t, most=some)
+            b.moved(b.o.compact([b.pages], size), got, size)
+        b.same()
+    b.pool.count(b.t)
+    b.o.count(b.pages)
+    b.same()
+    b.pool.free(b.t, b.tl)
+    for row in b.pages:
+        b.o.drop(row)
+    b.lens = [0] * n_seqs
+    b.same()
+    assert not any(b.o.counts)
+
+
+@pytest.mark.gpu
+def test_all_sequences_reordered_into_another_table():
+    """A step of a beam search: every row of the second table is a row of the first, whose lists then end.  Blocks that were
+    shared by rows that all write get one copy less than they have holders."""
+    b = Both(300, 8, 10)
+    print('beam', flush=True)
+    b.advance(b.grow([100, 5, 64, 0, 300, 129, 1, 63]))
+    other, ends = torch.full((9, 12), -1, dtype=torch.int32, device=DEV), torch.zeros(9, dtype=torch.int32, device=DEV)
+    rows, lens = np.full((9, 12), -1).tolist(), [0] * 9
+    for parents in ([0, 0, 0, 4, 4, 1, 2, 3], [7, 7, 7, 7, 7, 7, 7, 7], [5, 4, 3, 2, 1, 0, 0, 0]):
+        children = [8, 1, 2, 3, 4, 5, 6, 7]
+        b.pool.fork(b.t, b.tl, _i32(parents), _i32(children), into=(other, ends))
+        b.o.fork(b.pages.tolist(), b.lens, parents, children, rows, lens)
+        b.pool.free(b.t, b.tl)
+        for row in b.pages:
+            b.o.drop(row)
+        b.lens = [0] * 8
+        b.same()
+        table = np.array(rows)
+        moves = b.o.grow(table, lens, [1] * 9)
+        b.moved(moves, b.pool.grow(other, ends, 1), 9)
+        rows, lens = table.tolist(), [x + 1 for x in lens]
+        ends += 1
+        assert other.tolist() == rows
+        back = [8, 7, 6, 5, 4, 3, 2, 1]                      # and back
+        wide = torch.full((8, 12), -1, dtype=torch.int32, device=DEV)
+        b.pool.fork(other, ends, _i32(back), _i32(list(range(8))), into=(wide, b.tl))
+        mine = np.full((8, 12), -1).tolist()
+        b.o.fork(rows, lens, back, list(range(8)), mine, b.lens)
+        b.pool.free(other, ends)
+        for row in rows:
+            b.o.drop(row)
+        lens = [0] * 9
+        b.t, b.pages = wide, np.array(mine)
+        b.same()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('heads,dim,bits', [(1, 32, 'int8'), (5, 96, 'fp8'), (16, 64, 'int8'), (3, 256, 'fp8'), (8, 128, 'int8')])
+def test_copy(heads, dim, bits):
+    c, _ = _cache(20, heads, dim, bits)
+    k, v, f = c.k.view(torch.uint8).clone(), c.v.view(torch.uint8).clone(), c.scales.clone()
+    src, dst = [3, 19, -1, 7, 7, 20, 2, 4, 6], [0, 1, 5, 8, 9, 10, 2, -1, 11]
+    print(f'copy {heads} {dim} {bits}', flush=True)
+
+    def want(n):
+        for a, b in list(zip(src, dst))[:n]:
+            if 0 <= a < 20 and 0 <= b < 20:
+                k[b], v[b], f[b] = k[a], v[a], f[a]
+        assert torch.equal(c.k.view(torch.uint8), k) and torch.equal(c.v.view(torch.uint8), v) and torch.equal(c.scales, f)
+
+    c.copy(_i32(src), _i32(dst), _i32([0]))
+    want(0)
+    c.copy(_i32(src), _i32(dst), _i32([4]))
+    want(4)
+    c.copy(_i32(src), _i32(dst), _i32([-3]))
+    c.copy(_i32(src), _i32(dst), _i32([100]))
+    want(9)
+    c.k.view(torch.uint8)[3] = 1
+    k[3] = 1
+    c.copy(_i32(src), _i32(dst))
+    want(9)
+    from blast3r_amd.kv_cache import KVCache
+    KVCache(0, heads, dim, device=DEV).copy(_i32(src), _i32(dst))
+
+
+@pytest.mark.gpu
+def test_copy_past_32_bit_offsets():
+    from blast3r_amd.kv_cache import KVCache
+    n = 70_000
+    c = KVCache(n, 8, 128, torch.int8, device=DEV)
+    print('copy past 4 GB', flush=True)
+    c.k[n - 1], c.v[n - 2], c.scales[n - 1] = 5, 7, 3.0
+    c.copy(_i32([n - 1, n - 2, n - 2]), _i32([1, 2, n - 3]))
+    assert bool((c.k[1] == 5).all()) and bool((c.v[2] == 7).all()) and bool((c.v[n - 3] == 7).all()) and bool((c.scales[1] == 3.0).all())
+    assert not c.k[2].any() and not c.v[1].any() and not c.k[0].any()
+
+
+@pytest.mark.gpu
+def test_samples_of_prompts_through_the_cache():
+    """Prompts, samples forked from them, drafted tokens given back, a sequence that ends, blocks moved together: every
+    sequence attends to the tokens that it was given, with its shared blocks read once as with every list by itself; the same
+    through a captured graph."""
+    from blast3r_amd.kv_cache import KVCache
+    from blast3r_amd.kv_pool import BlockPool
+    H, G, D, S = 2, 2, 64, 6
+    rng = np.random.default_rng(0)
+    cache, pool = KVCache(90, H, D, torch.int8, device=DEV), BlockPool(90, device=DEV)
+    pages, lens = torch.full((S, 10), -1, dtype=torch.int32, device=DEV), torch.zeros(S, dtype=torch.int32, device=DEV)
+    mirror = [([], []) for _ in range(S)]                   # keys and values of each sequence
+    put = lambda x: torch.tensor(x, dtype=torch.float32, device=DEV).bfloat16()  # noqa: E731
+    print('samples', flush=True)
+
+    def append(counts):
+        k, v = (np.float64(_np(put(rng.normal(size=(sum(counts), H, D))))) for _ in range(2))
+        moves = pool.grow(pages, lens, _i32(counts), max_new=max(counts))
+        assert int(pool.missing) == 0
+        cache.copy(*moves)
+        off = _i32(np.concatenate(([0], np.cumsum(counts))))
+        cache.append(put(k), put(v), pages, lens, offsets=off, max_new=max(counts))
+        lens.add_(_i32(counts))
+        at = 0
+        for s, n in enumerate(counts):
+            mirror[s] = ([*mirror[s][0], *k[at:at + n]], [*mirror[s][1], *v[at:at + n]])
+            at += n
+
+    def check(shared=0, **kw):
+        """Rows over codes against attention over the values that were appended.  int8 keeps a normal number to half of 1/127
+        of its block's largest, 0.015 (0.0084 in the mean square); a block that grows token by token is recoded a few times:
+        0.08 at most, 0.025.  Queries have length 1, so scores move by 0.025, 0.1 at most, and results by that times a value's
+        distance from their mean, 0.8 on the average: 0.16 in all."""
+        q = torch.nn.functional.normalize(put(rng.normal(size=(S, H * G, D))).float(), dim=-1).bfloat16()
+        got = cache.attend(q, pages, lens, shared=shared, scale=1.0, **kw)
+        for s in range(S):
+            k, v = (np.array(x) for x in mirror[s])
+            for h in range(H * G):
+                if not len(k):
+                    assert not got[s, h].any()
+                    continue
+                z = k[:, h // G] @ _np(q)[s, h]
+                p = np.exp(z - z.max())
+                assert np.abs(_np(got)[s, h] - p @ v[:, h // G] / p.sum()).max() < 0.2, (s, h)
+        return q, got
+
+    append([200, 0, 0, 70, 0, 0])
+    check()
+    pool.fork(pages, lens, _i32([0, 0, 3, 0]), _i32([1, 2, 4, 5]))
+    for a, b in ((0, 1), (0, 2), (3, 4), (0, 5)):
+        mirror[b] = (list(mirror[a][0]), list(mirror[a][1]))
+    check()
+    append([1, 1, 1, 1, 0, 1])                               # four samples of the first prompt: three copies
+    assert int((pool.counts > 0).sum()) == 4 + 3 + 2 + 1 and pages[4, 1] != pages[3, 1]
+    q, got = check()
+    # rows of the first prompt alone: they share three blocks
+    rows = torch.tensor([0, 1, 2, 5], device=DEV)
+    alone = cache.attend(q[rows], pages[rows], lens[rows], scale=1.0)
+    joint = cache.attend(q[rows], pages[rows], lens[rows], scale=1.0, shared=3)
+    assert torch.equal(alone, got[rows]) and float((alone - joint).float().abs().max()) < 0.02
+    pool.grow(pages, lens, 130)                              # drafted and refused
+    pool.trim(pages, last=lens)
+    check()
+    append([64, 3, 1, 1, 5, 200])
+    check()
+    pool.free(pages, lens, _i32([0, 3]))
+    mirror[0] = mirror[3] = ([], [])
+    q, got = check()
+    moves = pool.compact(pages)
+    cache.copy(*moves)
+    used = int((pool.counts > 0).sum())
+    assert int(moves[2]) > 0 and int(pages.max()) == used - 1
+    assert torch.equal(cache.attend(q, pages, lens, scale=1.0), got)
+    append([30, 1, 1, 64, 1, 1])
+    check()
+    # a step captured: the blocks that it takes depend on what the pool holds at each replay
+    new = torch.zeros((S, H, D), dtype=torch.bfloat16, device=DEV)
+
+    def step():
+        cache.copy(*pool.grow(pages, lens, 1))
+        cache.append(new, new, pages, lens)
+        lens.add_(1)
+        return cache.attend(q, pages, lens, scale=1.0, cap=40.0)
+
+    state = [t.clone() for t in (pages, lens, pool.counts, pool._used, pool._marks, cache.k, cache.v, cache.scales)]
+
+    def reset():
+        for t, x in zip((pages, lens, pool._counts, pool._used, pool._marks, cache.k, cache.v, cache.scales), state):
+            t.copy_(x)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    reset()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step()
+    outs = []
+    for t in range(70):
+        new.copy_(put(rng.normal(size=(S, H, D))))
+        if t == 20:
+            pool.free(pages, lens, _i32([1]))               # eager work between the replays
+        graph.replay()
+        torch.cuda.synchronize()
+        outs.append((y.clone(), new.clone()))
+    end = pages.tolist(), lens.tolist(), pool.counts.tolist()
+    reset()
+    for t, (y, n) in enumerate(outs):
+        new.copy_(n)
+        if t == 20:
+            pool.free(pages, lens, _i32([1]))
+        assert torch.equal(step(), y), t
+    assert end == (pages.tolist(), lens.tolist(), pool.counts.tolist())
+
+
+@pytest.mark.gpu
+def test_pool_calls_of_nothing():
+    """No blocks, no lists, lists without places."""
+    from blast3r_amd.kv_pool import BlockPool
+    none = torch.full((0, 4), -1, dtype=torch.int32, device=DEV)
+    thin = torch.full((3, 0), -1, dtype=torch.int32, device=DEV)
+    some = torch.full((3, 4), -1, dtype=torch.int32, device=DEV)
+    print('pool of nothing', flush=True)
+    for n in (0, 5):
+        pool = BlockPool(n, device=DEV)
+        for pages in (none, thin, some.clone()):
+            lens = torch.zeros(pages.shape[0], dtype=torch.int32, device=DEV)
+            pool.count(pages)
+            src, dst, m = pool.grow(pages, lens, 100)
+            assert src.tolist() == dst.tolist() == [-1] * len(lens) and int(m) == 0
+            assert int(pool.missing) == (max(0, 6 - n) if pages.numel() else 0)
+            pool.fork(pages, lens, _i32([0, 1]), _i32([1, 2]))
+            pool.trim(pages, first=lens, last=lens)
+            assert not pool.counts.any()
+            src, dst, m = pool.compact(pages)
+            assert int(m) == 0 and src.tolist() == [-1] * (n // 2)
+            pool.free(pages, lens)
+            pool.free(pages, lens, _i32([0, 7, -1, 0]))
+            assert not pool.counts.any() and int(pool.available()) == n
