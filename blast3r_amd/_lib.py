@@ -172,7 +172,7 @@ class BaKvAttendArgs(ctypes.Structure):
 class BaKvScoredArgs(BaKvAttendArgs):
     # the header's struct begins with ba_kv_attend_args, whose size is a multiple of what follows
     _fields_ = [('slopes', c_p), ('prefix', c_p), ('since', c_p), ('until', c_p), ('cap', c_f), ('shared', c_int),
-                ('shared_parts', c_int), ('reserved', c_int)]
+                ('shared_parts', c_int), ('tile', c_int), ('shared_tile', c_int), ('reserved', c_int)]
 
 
 class BaKvPool(ctypes.Structure):
@@ -284,7 +284,7 @@ _SIGS = {
     'ba_kv_attend_splits': (c_int, [c_int, c_int, c_int, c_int, c_i64, c_int]),
     'ba_kv_attend_workspace_bytes': (c_i64, [c_i64, c_int, c_int, c_int]),
     'ba_kv_attend_scored': (c_int, [ctypes.POINTER(BaKvScoredArgs), c_p]),
-    'ba_kv_scored_parts': (None, [ctypes.POINTER(BaKvScoredArgs), ctypes.POINTER(c_int), ctypes.POINTER(c_int)]),
+    'ba_kv_scored_plan': (None, [ctypes.POINTER(BaKvScoredArgs)]),
     'ba_kv_pool_count': (c_int, [ctypes.POINTER(BaKvPool), ctypes.POINTER(BaKvTable), c_int, c_p]),
     'ba_kv_pool_fork': (c_int, [ctypes.POINTER(BaKvPool), ctypes.POINTER(BaKvForkArgs), c_p]),
     'ba_kv_pool_trim': (c_int, [ctypes.POINTER(BaKvPool), ctypes.POINTER(BaKvTrimArgs), c_p]),

@@ -12,7 +12,8 @@ CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libba_hip.so')
 SOURCES = ['ba_compat.hip', 'ba_schur.hip', 'ba_pcg.hip', 'ba_chol.hip', 'ba_update.hip', 'ba_sample.hip', 'ba_tracks.hip', 'ba_tangent.hip',
            'ba_pmplan.hip', 'ba_rotary.hip', 'ba_kv.hip', 'ba_kv_attend.hip', 'ba_kv_scored.hip',
-           'ba_kv_sloped.hip', 'ba_kv_capped.hip', 'ba_kv_pool.hip', 'ba_plan.cpp']
+           'ba_kv_form_masks.hip', 'ba_kv_form_slopes.hip', 'ba_kv_form_capped.hip', 'ba_kv_form_both.hip', 'ba_kv_form_any.hip',
+           'ba_kv_pool.hip', 'ba_plan.cpp']
 ARCH = os.environ.get('BA_OFFLOAD_ARCH', 'gfx950')
 
 HIPCC_FLAGS = ['-O3', '-std=c++17', '-fPIC', f'--offload-arch={ARCH}',
@@ -23,7 +24,8 @@ HIPCC_FLAGS = ['-O3', '-std=c++17', '-fPIC', f'--offload-arch={ARCH}',
 SOURCE_FLAGS = {
     # products in the general registers: the compiler's own choice moves sums to and fro between the register files
     # (attention of 2 x 2048 rows over 16384 tokens, 64 rows a wave: 1665 -> 1427 us)
-    f'ba_kv_{name}.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form=1'] for name in ('attend', 'scored', 'sloped', 'capped')
+    f'ba_kv_{name}.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form=1']
+    for name in ('attend', 'form_masks', 'form_slopes', 'form_capped', 'form_both', 'form_any')
 }
 
 

@@ -81,13 +81,18 @@ template <> struct Mma<32> {
     static __device__ __forceinline__ int row(int g, int r) { return 8 * (r >> 2) + 4 * g + (r & 3); }
 };
 
-// What a kernel does with scores and with what rows see:
+// What a kernel does with scores and with what rows see.  Few rows are bound by memory, and one form decides as it runs; the
+// tiles' exponents stand between matrix products, instruction by instruction, and each has a kernel of its own.
 //   AT_PLAIN   softmax(scale q.k) over the tokens up to a row's own (causal) and in its window
 //   AT_MASKS   a row's tokens are [lo, hi) and those below pre (AtRow); a launch may take some of the lists' blocks only, and
 //              the rows of all sequences together
 //   AT_SLOPES  the same, less slope |position - token| in each score
-//   AT_CAPPED  the same, with cap tanh(score / cap) in the place of each score first
-enum { AT_PLAIN = 0, AT_MASKS = 1, AT_SLOPES = 2, AT_CAPPED = 3 };
+//   AT_CAPPED  the same as AT_MASKS, with cap tanh(score / cap) in the place of each score
+//   AT_BOTH    capped, then less the slopes' part
+//   AT_ANY     what the call asks for
+enum { AT_PLAIN = 0, AT_MASKS = 1, AT_SLOPES = 2, AT_CAPPED = 3, AT_BOTH = 4, AT_ANY = 5 };
+constexpr bool at_slopes(int mode) { return mode == AT_SLOPES || mode == AT_BOTH || mode == AT_ANY; }
+constexpr bool at_caps(int mode) { return mode == AT_CAPPED || mode == AT_BOTH || mode == AT_ANY; }
 
 // of a launch that is not plain
 struct AtMore {
@@ -98,6 +103,7 @@ struct AtMore {
     float cap;
     int blk_lo, blk_hi;      // the blocks of the lists that it takes
     int part0, parts;        // it writes the parts [part0, part0 + parts) of the n_splits
+    int least;               // blocks of a part at least
     int stacked;             // its rows are those of all sequences, and the list is the first sequence's
 };
 
@@ -171,6 +177,7 @@ __device__ __forceinline__ AtPlace at_place(const AtArgs<MODE>& x, int rows, int
     id /= parts;
     r.kh = (int)(id % (unsigned)a.heads);
     r.s = (int)(id / (unsigned)a.heads);
+    if (MODE != AT_PLAIN) r.tile = n_tiles - 1 - r.tile;     // later rows see more: the longest tiles first
     if (packed) r.s = seq_of_place(a.offsets, a.n_seqs, a.n_rows, a.q_heads / a.heads, rows, 1, (unsigned)r.tile, r.tile);
     return r;
 }
@@ -284,6 +291,18 @@ __device__ __forceinline__ AtSpan at_span(const AtRow (&r)[N]) {
     return {one(s.lo0), one(s.lo1), one(s.hi0), one(s.hi1), one(s.pre0), one(s.pre1), one(s.pos0), one(s.pos1)};
 }
 
+// The same of rows i0 .. i1 of a sequence, whose bounds rise with them where neither since nor until says otherwise (rows that
+// see nothing widen it, which costs blocks at most).
+template <int MODE>
+__device__ __forceinline__ AtSpan at_span_of(const AtArgs<MODE>& x, const AtSeq& q, int s, int i0, int i1) {
+    const ba_kv_attend_args& a = x.a;
+    const int64_t p0 = (int64_t)q.first + i0, p1 = (int64_t)q.first + i1, w = a.window > 0 ? a.window : (int64_t)1 << 40;
+    auto at_least0 = [](int64_t v) { return v < 0 ? 0 : (int)v; };
+    auto end = [&](int64_t pos) { return a.causal && pos < q.len ? at_least0(pos + 1) : q.len; };
+    const int pre = x.m.prefix ? x.m.prefix[s] : 0, p = pre < 0 ? 0 : pre < q.len ? pre : q.len;
+    return {at_least0(p0 - w + 1), at_least0(p1 - w + 1), end(p0), end(p1), p, p, (int)p0, (int)p1};
+}
+
 // The blocks that a workgroup's rows see in a launch: the first na from a0 on, then those from c0 on, n in all.  Places in
 // that row of blocks are what parts are cut by.
 struct AtWalk {
@@ -309,9 +328,9 @@ __device__ __forceinline__ AtSeq at_rows(const AtArgs<MODE>& x, int s) {
     return at_seq(x.a, s);
 }
 
-__device__ __forceinline__ AtBlocks at_cut(const AtWalk& w, int parts) {
-    const int per = (w.n + parts - 1) / parts;
-    return {0, w.n, per < AT_MIN_BLOCKS ? AT_MIN_BLOCKS : per};
+__device__ __forceinline__ AtBlocks at_cut(const AtWalk& w, const AtMore& m) {
+    const int per = (w.n + m.parts - 1) / m.parts;
+    return {0, w.n, per < m.least ? m.least : per};
 }
 
 // cap tanh(z / cap), as off - 2 cap / (exp(2 z / cap) + 1) with off = cap; `in` brings a score to the exponent of 2.  Off by
@@ -394,7 +413,7 @@ __device__ __forceinline__ void load_queries(const ba_kv_attend_args& a, const A
 // What biases take from the logarithm of a row's sum, as its distances are measured from the anchor.
 template <int MODE>
 __device__ __forceinline__ float lse_shift(const AtArgs<MODE>& x, const AtRow& r, int head) {
-    if (MODE < AT_SLOPES || !x.m.slopes) return 0.0f;
+    if (!at_slopes(MODE) || !x.m.slopes) return 0.0f;
     const float slope = x.m.slopes[head];
     return slope * (float)at_anchor(r, slope);
 }
@@ -434,7 +453,7 @@ __device__ __forceinline__ void store_rows(const AtArgs<MODE>& x, const AtSeq& q
                            (f4){o[c][d][k] * inv, o[c][d][k + 1] * inv, o[c][d][k + 2] * inv, o[c][d][k + 3] * inv}, wide);
         if (a.lse && g == 0) {
             float lse = l[c] == 0.0f ? -__builtin_inff() : 0.693147180559945309f * (m[c] - AT_LIFT + __builtin_amdgcn_logf(l[c]));
-            if constexpr (MODE >= AT_SLOPES) lse -= lse_shift(x, at_row(x, q, s, i), head);
+            if constexpr (at_slopes(MODE)) lse -= lse_shift(x, at_row(x, q, s, i), head);
             a.lse[row * a.q_heads + head] = lse;
         }
     }
@@ -493,9 +512,14 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(AtArgs<MO
             const int r = tile0 + c * COLS + n;
             row[c] = at_row(x, q, s, (int)((unsigned)(r < all ? r : all - 1) / (unsigned)group));
         }
-        span = at_span<NCB, COLS>(row);
+        if (x.m.since || x.m.until || x.m.stacked) {
+            span = at_span<NCB, COLS>(row);
+        } else {
+            const int end = tile0 + ROWS < all ? tile0 + ROWS : all;
+            span = at_span_of(x, q, s, (int)((unsigned)tile0 / (unsigned)group), (int)((unsigned)(end - 1) / (unsigned)group));
+        }
         walk = at_walk(x.m, span.lo0, span.hi1, span.pre1);
-        at_part(at_cut(walk, x.m.parts), sp, lo, hi);
+        at_part(at_cut(walk, x.m), sp, lo, hi);
     }
     const bool none = lo >= hi;
     if (a.n_blocks == 0) hi = lo;
@@ -559,10 +583,13 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(AtArgs<MO
     load_queries<D, COLS, NCB>(a, q, kh, group, tile0, all, n, g, wide != 0, qf, qc, pos);
     float slope[NCB];
     int anchor[NCB];
-    if constexpr (MODE >= AT_SLOPES) load_slopes<MODE, COLS, NCB>(x, kh, group, tile0, all, n, row, slope, anchor);
+    if constexpr (at_slopes(MODE)) load_slopes<MODE, COLS, NCB>(x, kh, group, tile0, all, n, row, slope, anchor);
+    bool caps = false, slopes = false;
     float cap_in = 0.0f, cap_out = 0.0f;                     // exp2 of cap_in times a score, and 2 cap in units of the exponents
-    if constexpr (MODE == AT_CAPPED) {
-        cap_in = 2.0f / x.m.cap;
+    if constexpr (MODE == AT_ANY) {
+        caps = x.m.cap != 0.0f;
+        slopes = x.m.slopes != nullptr;
+        if (caps) cap_in = 2.0f / x.m.cap;
         cap_out = 2.0f * 1.44269504088896341f * x.m.cap;
     }
     // tokens [whole_lo, whole_hi) are seen by all rows of the wave: their blocks need no comparisons
@@ -629,8 +656,13 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(AtArgs<MO
         float top[NCB];
 #pragma unroll
         for (int c = 0; c < NCB; ++c) {
-            const float cz = f.x * qc[c], off = lv - m[c] + AT_LIFT;
-            if constexpr (MODE == AT_CAPPED) {
+            const float cz = f.x * qc[c];
+            float off = lv - m[c] + AT_LIFT;
+            // biases of tokens before all rows rise from token to token; around the rows' own they are made one by one
+            const int at = MODE == AT_ANY ? row[c].pos - (t0 + g * TPL) : 0;
+            const bool past = MODE == AT_ANY && slopes && t0 + 63 <= span.pos0;
+            if (past) off = fmaf(-slope[c], (float)(at - anchor[c]), off);
+            if (caps) {
                 const float cy = cz * cap_in, oc = off + 0.5f * cap_out;
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
@@ -642,8 +674,10 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(AtArgs<MO
 #pragma unroll
                     for (int r = 0; r < CREG; ++r) sc[c][b][r] = fmaf(sc[c][b][r], cz, off);
             }
-            if constexpr (MODE >= AT_SLOPES) {
-                const int at = row[c].pos - (t0 + g * TPL);
+            if (past) {
+#pragma unroll
+                for (int t = 1; t < TPL; ++t) sc[c][t / CREG][t % CREG] = fmaf(slope[c], (float)t, sc[c][t / CREG][t % CREG]);
+            } else if (slopes) {
 #pragma unroll
                 for (int t = 0; t < TPL; ++t)
                     sc[c][t / CREG][t % CREG] = fmaf(-slope[c], (float)((at < t ? t - at : at - t) - anchor[c]), sc[c][t / CREG][t % CREG]);
@@ -849,16 +883,27 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
             const int r = row0 + c * 32 + n;
             row[c] = at_row(x, q, s, (int)((unsigned)(r < all ? r : all - 1) / (unsigned)group));
         }
-        span = at_span<NCB, 32>(row);
-        if (lane == 0) span_sh[wave] = make_int3(span.lo0, span.hi1, span.pre1);
-        __syncthreads();
-        int3 r = span_sh[0];
+        int3 r;                                              // of all waves
+        if (x.m.since || x.m.until || x.m.stacked) {
+            span = at_span<NCB, 32>(row);
+            if (lane == 0) span_sh[wave] = make_int3(span.lo0, span.hi1, span.pre1);
+            __syncthreads();
+            r = span_sh[0];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) r = make_int3(min(r.x, span_sh[w].x), max(r.y, span_sh[w].y), max(r.z, span_sh[w].z));
-        r = make_int3(__builtin_amdgcn_readfirstlane(r.x), __builtin_amdgcn_readfirstlane(r.y), __builtin_amdgcn_readfirstlane(r.z));
+            for (int w = 1; w < WAVES; ++w) r = make_int3(min(r.x, span_sh[w].x), max(r.y, span_sh[w].y), max(r.z, span_sh[w].z));
+            r = make_int3(__builtin_amdgcn_readfirstlane(r.x), __builtin_amdgcn_readfirstlane(r.y), __builtin_amdgcn_readfirstlane(r.z));
+        } else {
+            auto of = [&](int r0, int rows) {
+                const int r1 = r0 + rows < all ? r0 + rows : all;
+                return at_span_of(x, q, s, (int)((unsigned)(r0 < all ? r0 : all - 1) / (unsigned)group), (int)((unsigned)(r1 - 1) / (unsigned)group));
+            };
+            span = of(row0, 32 * NCB);
+            const AtSpan w = of(tile0, ROWS);
+            r = make_int3(w.lo0, w.hi1, w.pre1);
+        }
         walk = at_walk(x.m, r.x, r.y, r.z);
         seen_end = max(r.y, r.z);
-        at_part(at_cut(walk, x.m.parts), sp, lo, hi);
+        at_part(at_cut(walk, x.m), sp, lo, hi);
     }
     const bool none = lo >= hi;
     if (a.n_blocks == 0) hi = lo;
@@ -870,9 +915,9 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
     load_queries<D, 32, NCB>(a, q, kh, group, row0, all, n, g, wide != 0, qf, qc, pos);
     float slope[NCB];
     int anchor[NCB];
-    if constexpr (MODE >= AT_SLOPES) load_slopes<MODE, 32, NCB>(x, kh, group, row0, all, n, row, slope, anchor);
+    if constexpr (at_slopes(MODE)) load_slopes<MODE, 32, NCB>(x, kh, group, row0, all, n, row, slope, anchor);
     float cap_in = 0.0f, cap_out = 0.0f;                     // exp2 of cap_in times a score, and 2 cap in units of the exponents
-    if constexpr (MODE == AT_CAPPED) {
+    if constexpr (at_caps(MODE)) {
         cap_in = 2.0f / x.m.cap;
         cap_out = 2.0f * 1.44269504088896341f * x.m.cap;
     }
@@ -969,11 +1014,11 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
             r.cz[c] = f.x * qc[c];
             r.off[c] = lv - m[c] + AT_LIFT;
             r.rise[c] = 0.0f;
-            if constexpr (MODE == AT_CAPPED) {
+            if constexpr (at_caps(MODE)) {
                 r.cz[c] *= cap_in;
                 r.off[c] += 0.5f * cap_out;
             }
-            if constexpr (MODE >= AT_SLOPES) {
+            if constexpr (at_slopes(MODE)) {
                 const int at = row[c].pos - (blk * 64 + 32 * g + 16 * b);
                 r.rise[c] = at > 0 ? slope[c] : -slope[c];
                 r.off[c] = fmaf(-slope[c], (float)((at > 0 ? at : -at) - anchor[c]), r.off[c]);
@@ -986,9 +1031,9 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
 #pragma unroll
         for (int e = e0; e < e1; ++e) {
             float y = t[e / 16][e % 16];
-            if constexpr (MODE == AT_CAPPED) y = capped(y, r.cz[e / 16], cap_out, r.off[e / 16]);
+            if constexpr (at_caps(MODE)) y = capped(y, r.cz[e / 16], cap_out, r.off[e / 16]);
             else y = fmaf(y, r.cz[e / 16], r.off[e / 16]);
-            if constexpr (MODE >= AT_SLOPES) y = fmaf(r.rise[e / 16], (float)(e % 16), y);
+            if constexpr (at_slopes(MODE)) y = fmaf(r.rise[e / 16], (float)(e % 16), y);
             t[e / 16][e % 16] = y;
         }
     };
@@ -1018,12 +1063,12 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
         const bool gone = MODE != AT_PLAIN && !there(page);
         const bool masked = MODE == AT_PLAIN ? t0 + 64 > whole_hi || t0 < whole_lo || t0 + 64 > len
                                              : gone || !(t0 + 64 <= span.pre0 || (t0 >= span.lo1 && t0 + 64 <= span.hi0));
-        const bool both = MODE >= AT_SLOPES && t0 + 64 > span.pos0 && t0 <= span.pos1;       // sides of a row's position
+        const bool both = at_slopes(MODE) && t0 + 64 > span.pos0 && t0 <= span.pos1;       // sides of a row's position
         if (!masked && !unset && !both) return;
         bool none = false;
 #pragma unroll
         for (int c = 0; c < NCB; ++c) {
-            if constexpr (MODE >= AT_SLOPES)
+            if constexpr (at_slopes(MODE))
                 if (both) {
                     const int at = row[c].pos - (t0 + 32 * g + 16 * b);
 #pragma unroll
@@ -1301,13 +1346,14 @@ __global__ void __launch_bounds__(AT_T) k_kv_join(AtArgs<MODE> x, int tile_rows,
 // waves of 32 above: then two waves fit a SIMD (2 x 2048 rows over 16384 tokens, before the last steps of the kernel: 64
 // elements 615 us against 690 with 8 waves, 128 elements 1077 us against 1375 with 4).  `fit`: workgroups that a CU holds.
 struct AtShape { int cols, ncb, waves, rows, fit; };
-static inline AtShape at_shape(int64_t rows, int dim) {
-    if (rows <= 16) return {16, 0, 4, 16, dim <= 64 ? 4 : dim <= 128 ? 2 : 1};
-    if (rows <= 32) return {32, 0, 4, 32, dim <= 128 ? 2 : 1};
-    if (rows <= 128 || dim > 128) return {32, 1, 4, 128, dim <= 64 ? 3 : dim <= 128 ? 2 : 1};
+static inline AtShape at_tile(int rows, int dim) {
+    if (rows == 16) return {16, 0, 4, 16, dim <= 64 ? 4 : dim <= 128 ? 2 : 1};
+    if (rows == 32) return {32, 0, 4, 32, dim <= 128 ? 2 : 1};
+    if (rows == 128 || dim > 128) return {32, 1, 4, 128, dim <= 64 ? 3 : dim <= 128 ? 2 : 1};
     if (dim <= 64) return {32, 2, 4, 256, 2};
     return {32, 1, 8, 256, 1};
 }
+static inline AtShape at_shape(int64_t rows, int dim) { return at_tile(rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 128 ? 128 : 256, dim); }
 
 // The checks and sizes of every attention call (ba_kv_attend.hip).
 struct AtGrid { unsigned nb; int tiles, packed; };
@@ -1317,36 +1363,44 @@ int attend_grid(const ba_kv_attend_args& a, int64_t rows, int64_t n_seqs, int pa
 int attend_join(const ba_kv_attend_args& a, AtJoin& j);
 int attend_wide(const ba_kv_attend_args& a);
 
+// Launches of the kernels for few rows and of those for tiles; each mode's are made in a source of their own.
 template <int MODE, int D, int KT, bool HALF>
-static void launch_attend(const AtArgs<MODE>& x, AtShape v, unsigned nb, int tiles, int packed, int wide, hipStream_t st) {
-    const dim3 grid(nb), block(64 * v.waves);
-    if (v.cols == 16) hipLaunchKernelGGL((k_kv_attend<MODE, D, KT, 16, HALF>), grid, block, 0, st, x, tiles, packed, wide);
-    else if (v.ncb == 0) hipLaunchKernelGGL((k_kv_attend<MODE, D, KT, 32, HALF>), grid, block, 0, st, x, tiles, packed, wide);
-    else if (v.rows == 128) hipLaunchKernelGGL((k_kv_attend_tile<MODE, D, KT, 1, 4, HALF>), grid, block, 0, st, x, tiles, packed, wide);
-    else if constexpr (D <= 64) hipLaunchKernelGGL((k_kv_attend_tile<MODE, D, KT, 2, 4, HALF>), grid, block, 0, st, x, tiles, packed, wide);
-    else if constexpr (D <= 128) hipLaunchKernelGGL((k_kv_attend_tile<MODE, D, KT, 1, 8, HALF>), grid, block, 0, st, x, tiles, packed, wide);
+static void launch_few(const AtArgs<MODE>& x, const AtShape& v, const AtGrid& g, int wide, hipStream_t st) {
+    const dim3 grid(g.nb), block(64 * v.waves);
+    if (v.cols == 16) hipLaunchKernelGGL((k_kv_attend<MODE, D, KT, 16, HALF>), grid, block, 0, st, x, g.tiles, g.packed, wide);
+    else hipLaunchKernelGGL((k_kv_attend<MODE, D, KT, 32, HALF>), grid, block, 0, st, x, g.tiles, g.packed, wide);
 }
 
-template <int MODE, int D>
-static int launch_attend(const AtArgs<MODE>& x, AtShape v, unsigned nb, int tiles, int packed, int wide, hipStream_t st) {
-    const bool half = x.a.dtype == BA_F16;
-    if (x.a.bits == BA_FP8) half ? launch_attend<MODE, D, BA_FP8, true>(x, v, nb, tiles, packed, wide, st) : launch_attend<MODE, D, BA_FP8, false>(x, v, nb, tiles, packed, wide, st);
-    else half ? launch_attend<MODE, D, BA_INT8, true>(x, v, nb, tiles, packed, wide, st) : launch_attend<MODE, D, BA_INT8, false>(x, v, nb, tiles, packed, wide, st);
-    BA_LAUNCHED();
-    return BA_OK;
+template <int MODE, int D, int KT, bool HALF>
+static void launch_tiles(const AtArgs<MODE>& x, const AtShape& v, const AtGrid& g, int wide, hipStream_t st) {
+    const dim3 grid(g.nb), block(64 * v.waves);
+    if (v.rows == 128) hipLaunchKernelGGL((k_kv_attend_tile<MODE, D, KT, 1, 4, HALF>), grid, block, 0, st, x, g.tiles, g.packed, wide);
+    else if constexpr (D <= 64) hipLaunchKernelGGL((k_kv_attend_tile<MODE, D, KT, 2, 4, HALF>), grid, block, 0, st, x, g.tiles, g.packed, wide);
+    else if constexpr (D <= 128) hipLaunchKernelGGL((k_kv_attend_tile<MODE, D, KT, 1, 8, HALF>), grid, block, 0, st, x, g.tiles, g.packed, wide);
 }
 
-// A launch of the kernels of one mode, each mode's made in a source of its own.
-template <int MODE>
-int launch_attend(const AtArgs<MODE>& x, AtShape v, unsigned nb, int tiles, int packed, int wide, hipStream_t st) {
-    switch (x.a.dim) {
-        case 32: return launch_attend<MODE, 32>(x, v, nb, tiles, packed, wide, st);
-        case 64: return launch_attend<MODE, 64>(x, v, nb, tiles, packed, wide, st);
-        case 96: return launch_attend<MODE, 96>(x, v, nb, tiles, packed, wide, st);
-        case 128: return launch_attend<MODE, 128>(x, v, nb, tiles, packed, wide, st);
-        case 256: return launch_attend<MODE, 256>(x, v, nb, tiles, packed, wide, st);
+#define AT_LAUNCH(NAME)                                                                                                   \
+    template <int MODE, int D>                                                                                            \
+    static int NAME##_of(const AtArgs<MODE>& x, const AtShape& v, const AtGrid& g, int wide, hipStream_t st) {            \
+        const bool half = x.a.dtype == BA_F16;                                                                            \
+        if (x.a.bits == BA_FP8) half ? NAME<MODE, D, BA_FP8, true>(x, v, g, wide, st) : NAME<MODE, D, BA_FP8, false>(x, v, g, wide, st);   \
+        else half ? NAME<MODE, D, BA_INT8, true>(x, v, g, wide, st) : NAME<MODE, D, BA_INT8, false>(x, v, g, wide, st);   \
+        BA_LAUNCHED();                                                                                                    \
+        return BA_OK;                                                                                                     \
+    }                                                                                                                     \
+    template <int MODE>                                                                                                   \
+    int NAME(const AtArgs<MODE>& x, const AtShape& v, const AtGrid& g, int wide, hipStream_t st) {                        \
+        switch (x.a.dim) {                                                                                                \
+            case 32: return NAME##_of<MODE, 32>(x, v, g, wide, st);                                                       \
+            case 64: return NAME##_of<MODE, 64>(x, v, g, wide, st);                                                       \
+            case 96: return NAME##_of<MODE, 96>(x, v, g, wide, st);                                                       \
+            case 128: return NAME##_of<MODE, 128>(x, v, g, wide, st);                                                     \
+            case 256: return NAME##_of<MODE, 256>(x, v, g, wide, st);                                                     \
+        }                                                                                                                 \
+        return BA_ERR_UNSUPPORTED;                                                                                        \
     }
-    return BA_ERR_UNSUPPORTED;
-}
+AT_LAUNCH(launch_few)
+AT_LAUNCH(launch_tiles)
+#undef AT_LAUNCH
 
 }  // namespace ba

@@ -99,7 +99,7 @@ extern "C" int ba_kv_attend(const ba_kv_attend_args* args, void* stream) {
     const int wide = attend_wide(a);
     hipStream_t st = (hipStream_t)stream;
     const AtArgs<AT_PLAIN> x = {a};
-    rc = launch_attend<AT_PLAIN>(x, v, g.nb, g.tiles, g.packed, wide, st);
+    rc = v.ncb ? launch_tiles<AT_PLAIN>(x, v, g, wide, st) : launch_few<AT_PLAIN>(x, v, g, wide, st);
     if (rc != BA_OK || a.n_splits == 1) return rc;
     hipLaunchKernelGGL(k_kv_join<AT_PLAIN>, dim3(j.nb), dim3(AT_T), 0, st, x, v.rows, j.lanes, wide);
     BA_LAUNCHED();

@@ -1,0 +1,8 @@
+// The kernels of attention that AT_CAPPED names (ba_kv_attend.h), in a source of their own because of the time that they take to build.
+#include "ba_kv_attend.h"
+
+namespace ba {
+
+template int launch_tiles<AT_CAPPED>(const AtArgs<AT_CAPPED>&, const AtShape&, const AtGrid&, int, hipStream_t);
+
+}  // namespace ba

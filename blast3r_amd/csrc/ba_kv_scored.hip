@@ -14,67 +14,136 @@
 
 namespace ba {
 
-extern template int launch_attend<AT_SLOPES>(const AtArgs<AT_SLOPES>&, AtShape, unsigned, int, int, int, hipStream_t);
-extern template int launch_attend<AT_CAPPED>(const AtArgs<AT_CAPPED>&, AtShape, unsigned, int, int, int, hipStream_t);
+#define SC_MIN_BLOCKS 4      // blocks of a part of a tile at least
 
-template <int MODE>
+#define AT_ELSEWHERE(NAME, MODE) extern template int NAME<MODE>(const AtArgs<MODE>&, const AtShape&, const AtGrid&, int, hipStream_t);
+AT_ELSEWHERE(launch_few, AT_ANY)
+AT_ELSEWHERE(launch_tiles, AT_MASKS)
+AT_ELSEWHERE(launch_tiles, AT_SLOPES)
+AT_ELSEWHERE(launch_tiles, AT_CAPPED)
+AT_ELSEWHERE(launch_tiles, AT_BOTH)
+#undef AT_ELSEWHERE
+
+static int launch_formed(const ba_kv_attend_args& a, const AtMore& m, const AtShape& v, const AtGrid& g, int wide, hipStream_t st) {
+    if (!v.ncb) return launch_few(AtArgs<AT_ANY>{a, m}, v, g, wide, st);
+    if (m.cap != 0.0f) return m.slopes ? launch_tiles(AtArgs<AT_BOTH>{a, m}, v, g, wide, st) : launch_tiles(AtArgs<AT_CAPPED>{a, m}, v, g, wide, st);
+    return m.slopes ? launch_tiles(AtArgs<AT_SLOPES>{a, m}, v, g, wide, st) : launch_tiles(AtArgs<AT_MASKS>{a, m}, v, g, wide, st);
+}
+
 static int attend_scored(const ba_kv_scored_args& s, hipStream_t st) {
-    AtArgs<MODE> x;
-    x.a = s.a;
-    x.a.n_splits = s.a.n_splits + s.shared_parts;
-    const int group = s.a.q_heads / s.a.heads;
-    const int64_t rows = s.a.max_rows * group, all = s.a.n_rows * group;
-    const AtShape v = at_shape(rows, s.a.dim), w = at_shape(all, s.a.dim);
+    ba_kv_attend_args a = s.a;
+    a.n_splits = s.a.n_splits + s.shared_parts;
+    const int group = a.q_heads / a.heads;
+    const int64_t rows = a.max_rows * group, all = a.n_rows * group;
+    const AtShape v = s.tile ? at_tile(s.tile, a.dim) : at_shape(rows, a.dim), w = s.shared_tile ? at_tile(s.shared_tile, a.dim) : at_shape(all, a.dim);
+    auto least = [](const AtShape& x) { return x.ncb ? SC_MIN_BLOCKS : AT_MIN_BLOCKS; };
     AtGrid g, h;
     AtJoin j;
-    int rc = attend_grid(x.a, rows, s.a.n_seqs, s.a.n_splits, v, g);
-    if (rc == BA_OK && s.shared) rc = attend_grid(x.a, all, 1, s.shared_parts, w, h);
-    if (rc == BA_OK) rc = attend_join(x.a, j);
+    int rc = attend_grid(a, rows, a.n_seqs, s.a.n_splits, v, g);
+    if (rc == BA_OK && s.shared) rc = attend_grid(a, all, 1, s.shared_parts, w, h);
+    if (rc == BA_OK) rc = attend_join(a, j);
     if (rc != BA_OK) return rc;
-    const int wide = attend_wide(s.a);
-    x.m = {s.slopes, s.prefix, s.since, s.until, s.cap, 0, s.shared, 0, s.shared_parts, 1};
-    if (s.shared) rc = launch_attend<MODE>(x, w, h.nb, h.tiles, h.packed, wide, st);
+    const int wide = attend_wide(a);
+    if (s.shared) rc = launch_formed(a, {s.slopes, s.prefix, s.since, s.until, s.cap, 0, s.shared, 0, s.shared_parts, least(w), 1}, w, h, wide, st);
     if (rc != BA_OK) return rc;
-    x.m.blk_lo = s.shared;
-    x.m.blk_hi = s.a.n_pages;
-    x.m.part0 = s.shared_parts;
-    x.m.parts = s.a.n_splits;
-    x.m.stacked = 0;
-    rc = launch_attend<MODE>(x, v, g.nb, g.tiles, g.packed, wide, st);
-    if (rc != BA_OK || x.a.n_splits == 1) return rc;
-    hipLaunchKernelGGL(k_kv_join<MODE>, dim3(j.nb), dim3(AT_T), 0, st, x, v.rows, j.lanes, wide);
+    const AtMore m = {s.slopes, s.prefix, s.since, s.until, s.cap, s.shared, a.n_pages, s.shared_parts, s.a.n_splits, least(v), 0};
+    rc = launch_formed(a, m, v, g, wide, st);
+    if (rc != BA_OK || a.n_splits == 1) return rc;
+    hipLaunchKernelGGL(k_kv_join<AT_ANY>, dim3(j.nb), dim3(AT_T), 0, st, AtArgs<AT_ANY>{a, m}, v.rows, j.lanes, wide);
     BA_LAUNCHED();
     return BA_OK;
 }
 
-// Parts for a launch of `base` workgroups that may have `blocks` blocks each: as for the plain form.
-static int parts_of(int64_t base, int64_t blocks, const AtShape& v, int least) {
-    const int64_t most = (blocks + AT_MIN_BLOCKS - 1) / AT_MIN_BLOCKS;
-    int64_t n = v.ncb ? 256 * v.fit / base : (384 + base - 1) / base;
-    if (v.ncb == 0 && n < least) n = least;
-    n = n < most ? n : most;
-    return (int)(n < 1 ? 1 : n);
+// What a launch is expected to take (us), which shapes and parts are chosen by.  Tiles: rounds of workgroups that the CUs hold at
+// a time, each with its blocks and as much as SC_START blocks to begin and end with; per block what 2 x 2048 rows over 16384
+// tokens take by the block (32 elements a head 2.0 us, 64 2.3, 96 and 128 1.8 and 2.0, 256 2.5; tiles of 128 rows, of which a
+// CU holds more, 1.8, 1.8 and 2.2).  Few rows: the bytes of the blocks at 4.8 TB/s, or the blocks of a wave in series.  Partial
+// sums are written and read once, with a launch of 4 us.
+#define SC_START 4
+
+struct Guess {
+    AtShape v;
+    int parts;
+    double us;
+};
+
+static double launch_us(const AtShape& v, int dim, int64_t base, int64_t blocks, int parts) {
+    const int64_t per = (blocks + parts - 1) / parts;
+    if (!v.ncb) {
+        const double bytes = (double)base * blocks * 128.0 * dim / 4.8e6, chain = ((per + 3) / 4) * 1.0;
+        return 6.0 + (bytes > chain ? bytes : chain);
+    }
+    const double block = v.rows == 256 ? (dim == 64 ? 2.3 : dim == 96 ? 1.8 : 2.0) : dim == 256 ? 2.5 : dim <= 64 ? 1.8 : 2.2;
+    const int64_t rounds = (base * parts + 256 * v.fit - 1) / (256 * v.fit);
+    return 4.0 + rounds * (per + SC_START) * block;
+}
+
+// The best shape and number of parts for the rows of n_seqs sequences that may see `blocks` blocks each; join: time that a part
+// more of all rows costs; joined: there is a join anyway.
+static Guess guess(int64_t rows, int64_t n_seqs, int heads, int dim, int64_t blocks, double join, bool joined, bool brief) {
+    Guess best = {at_shape(rows, dim), 1, 0.0};
+    if (blocks < 1) blocks = 1;
+    if (!best.v.ncb) {                                       // one and a half workgroups per CU, two parts for unequal lengths
+        const int64_t base = n_seqs * heads, most = (blocks + AT_MIN_BLOCKS - 1) / AT_MIN_BLOCKS;
+        int64_t n = (384 + base - 1) / base;
+        n = n < 2 && !joined ? 2 : n;
+        n = n < most ? n : most;
+        best.parts = (int)(n < 1 ? 1 : n);
+        best.us = launch_us(best.v, dim, base, blocks, best.parts) + (best.parts > 1 || joined ? join * best.parts : 0.0) + (best.parts > 1 && !joined ? 4.0 : 0.0);
+        return best;
+    }
+    // documents are short beside their sequence: small tiles, whole (8192 tokens of documents of 50 to 2000: 164 us, 174 with
+    // tiles of 256 rows, 251 in two parts)
+    if (brief) return {at_tile(128, dim), 1, launch_us(at_tile(128, dim), dim, n_seqs * heads * ((rows + 127) / 128), blocks, 1)};
+    static const int some[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 40, 48, 64};
+    best.us = 1.0e30;
+    for (int tile = 128; tile <= 256; tile += 128) {
+        if (tile == 256 && (dim > 128 || rows <= 128)) break;
+        const AtShape v = at_tile(tile, dim);
+        const int64_t base = n_seqs * heads * ((rows + tile - 1) / tile);
+        for (int p : some) {
+            if (p > 1 && p * SC_MIN_BLOCKS > blocks) break;
+            const double us = launch_us(v, dim, base, blocks, p) + (p > 1 || joined ? join * p : 0.0) + (p > 1 && !joined ? 4.0 : 0.0);
+            if (us < best.us) best = {v, p, us};
+        }
+    }
+    return best;
 }
 
 }  // namespace ba
 
 using namespace ba;
 
-extern "C" void ba_kv_scored_parts(const ba_kv_scored_args* args, int32_t* own, int32_t* shared) {
-    const ba_kv_attend_args& a = args->a;
-    *own = 1;
-    *shared = args->shared > 0 ? 1 : 0;
-    if (a.n_seqs < 1 || a.heads < 1 || a.q_heads < a.heads || a.max_rows < 1 || a.n_rows < 1 || args->shared < 0) return;
+extern "C" void ba_kv_scored_plan(ba_kv_scored_args* args) {
+    ba_kv_attend_args& a = args->a;
+    a.n_splits = 1;
+    args->shared_parts = args->shared > 0 ? 1 : 0;
+    args->tile = args->shared_tile = 0;
+    if (a.n_seqs < 1 || a.heads < 1 || a.q_heads < a.heads || a.max_rows < 1 || a.n_rows < 1 || args->shared < 0 || args->shared > a.n_pages) return;
     const int group = a.q_heads / a.heads;
     const int64_t rows = a.max_rows * group, all = a.n_rows * group;
-    const AtShape v = at_shape(rows, a.dim), w = at_shape(all, a.dim);
-    int64_t blocks = a.n_pages - args->shared;
+    const double join = 8.0 * a.n_rows * a.q_heads * (a.dim + 2) / 4.5e6;
+    const bool brief = args->since != nullptr;
+    int64_t blocks = a.n_pages;
     if (a.window > 0 && !args->prefix) {                     // what a tile's rows can see
-        const int64_t tile = v.rows / group < a.max_rows ? v.rows / group + 1 : a.max_rows, seen = (a.window + tile + 62) / 64 + 1;
+        const int64_t at_once = 256 / group < a.max_rows ? 256 / group + 1 : a.max_rows, seen = (a.window + at_once + 62) / 64 + 1;
         blocks = seen < blocks ? seen : blocks;
     }
-    *own = parts_of((int64_t)a.n_seqs * a.heads * ((rows + v.rows - 1) / v.rows), blocks, v, 2);
-    if (args->shared > 0) *shared = parts_of((int64_t)a.heads * ((all + w.rows - 1) / w.rows), args->shared, w, 1);
+    Guess own = guess(rows, a.n_seqs, a.heads, a.dim, blocks, join, false, brief);
+    if (args->shared > 0) {
+        const Guess common = guess(all, 1, a.heads, a.dim, args->shared, join, true, false);
+        const int64_t rest = a.n_pages - args->shared;
+        const Guess left = guess(rows, a.n_seqs, a.heads, a.dim, rest < blocks ? rest : blocks, join, true, brief);
+        if (common.us + left.us + 4.0 < own.us) {
+            own = left;
+            args->shared_parts = common.parts;
+            args->shared_tile = common.v.rows;
+        } else {
+            args->shared = args->shared_parts = 0;
+        }
+    }
+    a.n_splits = own.parts;
+    args->tile = own.v.rows;
 }
 
 extern "C" int ba_kv_attend_scored(const ba_kv_scored_args* args, void* stream) {
@@ -88,8 +157,8 @@ extern "C" int ba_kv_attend_scored(const ba_kv_scored_args* args, void* stream) 
     BA_REQUIRE(s.shared >= 0 && s.shared <= s.a.n_pages, "attention: shared blocks past the lists");
     BA_REQUIRE(s.shared ? s.shared_parts >= 1 && s.shared_parts <= 65536 : s.shared_parts == 0, "attention: bad shared_parts");
     BA_REQUIRE(s.a.n_splits + s.shared_parts <= 65536, "attention: too many parts");
+    for (const int tile : {s.tile, s.shared_tile})
+        BA_REQUIRE(tile == 0 || tile == 16 || tile == 32 || tile == 128 || (tile == 256 && s.a.dim <= 128), "attention: tiles have 16, 32, 128 or (up to heads of 128) 256 rows");
     if (nothing) return BA_OK;
-    hipStream_t st = (hipStream_t)stream;
-    if (s.cap != 0.0f) return attend_scored<AT_CAPPED>(s, st);
-    return s.slopes ? attend_scored<AT_SLOPES>(s, st) : attend_scored<AT_MASKS>(s, st);
+    return attend_scored(s, (hipStream_t)stream);
 }

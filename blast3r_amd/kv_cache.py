@@ -16,7 +16,6 @@ workgroups.  Lengths, offsets and pages are device tensors, never read by the ho
 call can be captured in a graph.  What they say out of range is left out (include/ba_hip.h).
 Rows of a result that no sequence has, or past ``max_new`` of one, are not written.
 """
-import ctypes
 import math
 
 import torch
@@ -299,10 +298,9 @@ class KVCache:
         if most:
             L = self._lib
             if scored:
-                call, own, common = L.ba_kv_attend_scored, ctypes.c_int32(), ctypes.c_int32()
-                L.ba_kv_scored_parts(a, own, common)
-                a.n_splits, a.shared_parts = own.value, common.value
-                n = own.value + common.value
+                call = L.ba_kv_attend_scored
+                L.ba_kv_scored_plan(a)
+                n = a.n_splits + a.shared_parts
             else:
                 call = L.ba_kv_attend
                 a.n_splits = n = L.ba_kv_attend_splits(a.n_seqs, self._heads, q_heads, dim, most, a.n_pages)

@@ -732,8 +732,10 @@ int64_t ba_kv_attend_workspace_bytes(int64_t n_rows, int32_t q_heads, int32_t di
  * |p - j| where slopes (finite numbers) are given.  A row sees j < lengths[s] with j < prefix[s], or with j >= since[row], j <
  * until[row] and what causal and window say; any of the three may be NULL.  shared: the first so many blocks of all lists are
  * the first sequence's: they are read once for all rows.  a.n_splits counts the parts of the sequences' own blocks,
- * shared_parts those of the shared ones (0 without any); ba_kv_scored_parts gives both.  With more than one part in all,
- * a.workspace has ba_kv_attend_workspace_bytes for their sum. */
+ * shared_parts those of the shared ones (0 without any); tile and shared_tile are rows of a workgroup (16, 32, 128, 256; 0: by
+ * their number).  ba_kv_scored_plan sets the four from everything else but pointers to rows and workspace, and sets shared to
+ * 0 where reading each list by itself is expected to be faster.  With more than one part in all, a.workspace has
+ * ba_kv_attend_workspace_bytes for their sum. */
 typedef struct {
     ba_kv_attend_args a;
     const float* slopes;       /* (q_heads,) */
@@ -743,11 +745,12 @@ typedef struct {
     float cap;
     int32_t shared;
     int32_t shared_parts;
+    int32_t tile, shared_tile;
     int32_t reserved;
 } ba_kv_scored_args;
 
 int ba_kv_attend_scored(const ba_kv_scored_args* args, void* stream);
-void ba_kv_scored_parts(const ba_kv_scored_args* args, int32_t* own, int32_t* shared);
+void ba_kv_scored_plan(ba_kv_scored_args* args);
 
 /* Pages of the cache.  A pool knows of each block how many lists hold it: counts (n_blocks,), used ((n_blocks + 31) / 32
  * words, a bit for each block that a list holds, bits past the last block set) and marks (2 n_blocks ints, -1 in the first

@@ -66,11 +66,16 @@ def test_formed_entry_point_refuses_bad_arguments_without_a_gpu():
         a = _lib.BaKvScoredArgs(**{**good, **kw})
         assert L.ba_kv_attend_scored(ctypes.byref(a), None) != 0 and word in L.ba_last_error().decode(), (kw, L.ba_last_error())
     assert L.ba_kv_attend_scored(ctypes.byref(_lib.BaKvScoredArgs(**{**good, 'n_rows': 0})), None) == 0
-    own, shared = ctypes.c_int32(), ctypes.c_int32()
-    for kw in (dict(), dict(shared=2), dict(shared=1, window=5), dict(n_rows=0), dict(n_seqs=0, shared=1), dict(max_rows=0), dict(n_pages=0)):
+    for kw in (dict(), dict(shared=2), dict(shared=1, window=5), dict(n_rows=0), dict(n_seqs=0, shared=1), dict(max_rows=0), dict(n_pages=0),
+               dict(n_seqs=64, n_rows=64, rows_per_seq=1, max_rows=1, n_pages=300, shared=256), dict(n_rows=9000, max_rows=9000, n_pages=900, dim=256),
+               dict(n_rows=9000, max_rows=9000, n_pages=900, since=p), dict(n_rows=(1 << 31) - 1, max_rows=(1 << 31) - 1, n_pages=(1 << 24) - 1)):
         a = _lib.BaKvScoredArgs(**{**good, **kw})
-        L.ba_kv_scored_parts(a, own, shared)
-        assert own.value >= 1 and shared.value == (1 if a.shared else 0) or shared.value > 1
+        L.ba_kv_scored_plan(a)
+        assert 1 <= a.n_splits <= 64 or a.max_rows == 1 and a.n_splits <= 384
+        assert a.shared_parts >= 1 if a.shared else a.shared_parts == 0
+        assert a.tile in (0, 16, 32, 128, 256) and a.shared_tile in (0, 16, 32, 128, 256) and not (a.dim == 256 and a.tile == 256)
+    assert L.ba_kv_attend_scored(ctypes.byref(_lib.BaKvScoredArgs(**{**good, 'tile': 64})), None) != 0 and 'tiles' in L.ba_last_error().decode()
+    assert L.ba_kv_attend_scored(ctypes.byref(_lib.BaKvScoredArgs(**{**good, 'shared_tile': 256, 'dim': 256})), None) != 0
 
 
 @pytest.fixture
@@ -104,7 +109,11 @@ def test_python_refuses_bad_masks_and_scores(host):
         c.attend(q, pages, lens, slopes=torch.zeros(4, requires_grad=True))
     c.attend(q, pages, lens, cap=50.0, prefix=i32([1, 2]), since=i32([0] * 4), until=i32([9] * 4), shared=1)
     a = host[-1]
-    assert a.cap == 50.0 and a.shared == 1 and a.shared_parts >= 1 and a.n_splits >= 1 and a.prefix and a.since and a.until and not a.slopes
+    assert a.cap == 50.0 and a.n_splits >= 1 and a.prefix and a.since and a.until and not a.slopes
+    assert a.shared == a.shared_parts == 0                  # two blocks are not worth another launch
+    many, long = torch.zeros(64, 4, 64, dtype=torch.bfloat16), torch.zeros(64, 300, dtype=torch.int32)
+    c.attend(many, long, torch.zeros(64, dtype=torch.int32), shared=256)
+    assert host[-1].shared == 256 and host[-1].shared_parts >= 1
     c.attend(q, pages, lens)                                # what was there goes the way it went
     assert type(host[-1]).__name__ == 'BaKvAttendArgs' and type(a).__name__ == 'BaKvScoredArgs'
     for kw in (dict(cap=1.0), dict(shared=1)):
@@ -112,6 +121,22 @@ def test_python_refuses_bad_masks_and_scores(host):
 
 
 # ---------------------------------------------------------------------------------- parity (GPU)
+
+class Planned:
+    """The library with a plan of the test's choosing: parts and tiles of the sequences' own blocks and of the shared ones."""
+
+    def __init__(self, shared, own=1, common=1, tile=0, shared_tile=0):
+        from blast3r_amd import _lib
+        self.lib, self.plan = _lib.lib(), (shared, own, common, tile, shared_tile)
+
+    def __getattr__(self, name):
+        return getattr(self.lib, name)
+
+    def ba_kv_scored_plan(self, a):
+        a.shared, a.n_splits, a.shared_parts, a.tile, a.shared_tile = self.plan
+        if not a.shared:
+            a.shared_parts = 0
+
 
 def _run(c, o, q, pages, lens, counts, scale=None, shared=0, uniform=False, max_new=None, bar=None, **kw):
     """attend() and what the oracle says; rows within max_new are compared."""
@@ -284,10 +309,29 @@ def test_shared_blocks_against_oracle(bits, dim, heads, group, shared, lens, cou
     o = _mirror(c, bits)
     print(f'shared {bits} {dim} {heads} {group} {shared} {lens} {counts} {opts}', flush=True)
     uniform = len(set(counts)) == 1
-    a = _run(c, o, q, pages, lens, counts, shared=shared, uniform=uniform, **kw)
-    b = _run(c, o, q, pages, lens, counts, uniform=uniform, **kw)
-    assert float((a - b).float().abs().max()) <= 3e-3 * max(1.0, float(b.float().abs().max())) + 2.0 ** -7 * float(b.float().abs().max())
-    assert torch.equal(a, _run(c, o, q, pages, lens, counts, shared=shared, uniform=uniform, **kw))
+    _run(c, o, q, pages, lens, counts, shared=shared, uniform=uniform, **kw)             # as it is planned
+    real = c._lib
+    for plan in ((), (1, 1, 16, 128), (2, 3, 32, 32), (3, 2, 128, 16), (1, 7, 0, 256 if dim < 256 else 128)):
+        print(f'  plan {plan}', flush=True)
+        c._lib = Planned(shared, *plan)
+        a = _run(c, o, q, pages, lens, counts, shared=shared, uniform=uniform, **kw)
+        assert torch.equal(a, _run(c, o, q, pages, lens, counts, shared=shared, uniform=uniform, **kw))
+    c._lib = real
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dim,heads,group,lens,counts,opts', [
+    (64, 1, 2, [900, 191], [200, 63], dict(slopes=True)), (128, 2, 1, [1500], [300], dict(cap=9.0)), (256, 1, 1, [800], [150], dict(mask='any')),
+    (96, 1, 3, [1200], [5], dict(prefix=[200], window=300)), (32, 1, 1, [700, 650], [300, 1], dict(mask='frames', causal=False))])
+def test_every_plan_gives_the_result(dim, heads, group, lens, counts, opts):
+    """Tiles of every size, and parts without blocks among them."""
+    rng = np.random.default_rng(sum(lens))
+    c, o, q, pages, kw = _case(rng, dim, heads, group, lens, counts, 'fp8', opts, torch.float16)
+    for tile in (16, 32, 128, 256):
+        for parts in (1, 2, 5, 40):
+            print(f'plan {dim} {tile} {parts}', flush=True)
+            c._lib = Planned(0, parts, 0, tile if dim < 256 else min(tile, 128))
+            _run(c, o, q, pages, lens, counts, **kw)
 
 
 @pytest.mark.gpu
@@ -302,6 +346,7 @@ def test_shared_rows_that_no_sequence_has_are_left_alone():
         y = torch.full_like(q, 7.0)
         print(f'shared bounds {n}', flush=True)
         off = _i32([2, 2 + n, 2 + n + 5])
+        c._lib = Planned(2, 2, 2)
         _, lse = c.attend(q, _i32(pages), _i32(lens), offsets=off, max_new=most, out=y, shared=2, return_lse=True, cap=9.0)
         rows = _np(q)[2:2 + n + 5]
         want, _, size = otok.attend_formed(o, rows, pages, lens, [n, 5], 0.125, cap=9.0)
@@ -322,6 +367,7 @@ def test_formed_calls_of_bad_lists_stay_inside():
     for n in (2, 40, 400):
         q = torch.randn((n, 2, 64), device=DEV).bfloat16()
         for kw in (dict(cap=5.0), dict(slopes=slopes), dict(prefix=_i32([9, 100000])), dict(shared=2), dict(shared=3, cap=4.0)):
+            none._lib = c._lib = Planned(kw.get('shared', 0), 1, 2)
             got, lse = none.attend(q, _i32(np.zeros((2, 3))), _i32([150, 20]), return_lse=True, **kw)
             assert not got.any() and bool((lse == -math.inf).all())
             got = c.attend(q, _i32([[0, 1, -1], [9, 99, 1 << 30]]), _i32([100000, -5]), **kw)
@@ -329,6 +375,7 @@ def test_formed_calls_of_bad_lists_stay_inside():
             y = torch.full_like(q, 7.0)
             c.attend(q, _i32([[0, 1, 2]] * 2), _i32([50, 60]), offsets=_i32([n + 9, -2, n + 4]), out=y, **kw)
             assert bool((y == 7.0).all())
+    c._lib = c._lib.lib
     assert not c.attend(q[:2], _i32(np.zeros((2, 0))), _i32([5, 6]), prefix=_i32([3, 4])).any()
 
 
@@ -338,6 +385,7 @@ def test_formed_steps_in_a_graph_and_on_a_side_stream():
     eager work between the replays; the same on another stream."""
     c, _ = _cache(60, 2, 64, 'fp8')
     S = 6
+    c._lib = Planned(20, 2, 2)
     pages = torch.cat((_i32([list(range(20))] * S), _i32(20 + np.arange(36).reshape(6, 6))), 1)
     q = torch.zeros((S, 8, 64), dtype=torch.bfloat16, device=DEV)
     lens, prefix, since = _i32([1280] * S), _i32([0] * S), _i32([0] * S)
