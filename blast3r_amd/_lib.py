@@ -183,19 +183,28 @@ class BaKvTable(ctypes.Structure):
     _fields_ = [('pages', c_p), ('stride', c_i64), ('n_seqs', c_int), ('n_pages', c_int)]
 
 
+class BaKvCountArgs(ctypes.Structure):
+    _fields_ = [('pool', BaKvPool), ('tables', ctypes.POINTER(BaKvTable)), ('n_tables', c_int), ('reserved', c_int)]
+
+
 class BaKvForkArgs(ctypes.Structure):
-    _fields_ = [('from_', BaKvTable), ('to', BaKvTable), ('from_lengths', c_p), ('to_lengths', c_p), ('parents', c_p),
-                ('children', c_p), ('n', c_int), ('reserved', c_int)]
+    _fields_ = [('pool', BaKvPool), ('from_', BaKvTable), ('to', BaKvTable), ('from_lengths', c_p), ('to_lengths', c_p),
+                ('parents', c_p), ('children', c_p), ('n', c_int), ('reserved', c_int)]
 
 
 class BaKvTrimArgs(ctypes.Structure):
-    _fields_ = [('table', BaKvTable), ('first', c_p), ('last', c_p), ('rows', c_p), ('lengths', c_p), ('n_rows', c_int),
-                ('all', c_int)]
+    _fields_ = [('pool', BaKvPool), ('table', BaKvTable), ('first', c_p), ('last', c_p), ('rows', c_p), ('lengths', c_p),
+                ('n_rows', c_int), ('all', c_int)]
 
 
 class BaKvGrowArgs(ctypes.Structure):
-    _fields_ = [('table', BaKvTable), ('lengths', c_p), ('more', c_p), ('each', c_int), ('max_new', c_int), ('src', c_p),
-                ('dst', c_p), ('n', c_p), ('missing', c_p)]
+    _fields_ = [('pool', BaKvPool), ('table', BaKvTable), ('lengths', c_p), ('more', c_p), ('each', c_int), ('max_new', c_int),
+                ('src', c_p), ('dst', c_p), ('n', c_p), ('missing', c_p)]
+
+
+class BaKvCompactArgs(ctypes.Structure):
+    _fields_ = [('pool', BaKvPool), ('tables', ctypes.POINTER(BaKvTable)), ('n_tables', c_int), ('most', c_int), ('src', c_p),
+                ('dst', c_p), ('n', c_p)]
 
 
 class BaKvCopyArgs(ctypes.Structure):
@@ -285,11 +294,11 @@ _SIGS = {
     'ba_kv_attend_workspace_bytes': (c_i64, [c_i64, c_int, c_int, c_int]),
     'ba_kv_attend_scored': (c_int, [ctypes.POINTER(BaKvScoredArgs), c_p]),
     'ba_kv_scored_plan': (None, [ctypes.POINTER(BaKvScoredArgs)]),
-    'ba_kv_pool_count': (c_int, [ctypes.POINTER(BaKvPool), ctypes.POINTER(BaKvTable), c_int, c_p]),
-    'ba_kv_pool_fork': (c_int, [ctypes.POINTER(BaKvPool), ctypes.POINTER(BaKvForkArgs), c_p]),
-    'ba_kv_pool_trim': (c_int, [ctypes.POINTER(BaKvPool), ctypes.POINTER(BaKvTrimArgs), c_p]),
-    'ba_kv_pool_grow': (c_int, [ctypes.POINTER(BaKvPool), ctypes.POINTER(BaKvGrowArgs), c_p]),
-    'ba_kv_pool_compact': (c_int, [ctypes.POINTER(BaKvPool), ctypes.POINTER(BaKvTable), c_int, c_p, c_p, c_p, c_int, c_p]),
+    'ba_kv_pool_count': (c_int, [ctypes.POINTER(BaKvCountArgs), c_p]),
+    'ba_kv_pool_fork': (c_int, [ctypes.POINTER(BaKvForkArgs), c_p]),
+    'ba_kv_pool_trim': (c_int, [ctypes.POINTER(BaKvTrimArgs), c_p]),
+    'ba_kv_pool_grow': (c_int, [ctypes.POINTER(BaKvGrowArgs), c_p]),
+    'ba_kv_pool_compact': (c_int, [ctypes.POINTER(BaKvCompactArgs), c_p]),
     'ba_kv_copy': (c_int, [ctypes.POINTER(BaKvCopyArgs), c_p]),
 }
 
@@ -302,7 +311,8 @@ ABI_STRUCTS = {'ba_huber': BaHuber, 'ba_layout': BaLayout, 'ba_lin_args': BaLinA
                'ba_tangent_args': BaTangentArgs, 'ba_rotary_args': BaRotaryArgs, 'ba_kv_args': BaKvArgs,
                'ba_kv_attend_args': BaKvAttendArgs, 'ba_kv_scored_args': BaKvScoredArgs, 'ba_kv_pool': BaKvPool,
                'ba_kv_table': BaKvTable, 'ba_kv_fork_args': BaKvForkArgs, 'ba_kv_trim_args': BaKvTrimArgs,
-               'ba_kv_grow_args': BaKvGrowArgs, 'ba_kv_copy_args': BaKvCopyArgs}
+               'ba_kv_grow_args': BaKvGrowArgs, 'ba_kv_copy_args': BaKvCopyArgs, 'ba_kv_count_args': BaKvCountArgs,
+               'ba_kv_compact_args': BaKvCompactArgs}
 
 
 def _check_abi(L):

@@ -25,6 +25,7 @@ namespace ba {
 
 #define PL_T 256
 #define PL_ONE 1024          // threads of the kernels that run in one workgroup
+#define PL_FEW 16384         // blocks that one workgroup counts (64 KB), and half of the entries
 
 // what other threads of this launch change by atomics is read past the first cache
 __device__ __forceinline__ int32_t fresh(const int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -72,9 +73,34 @@ __global__ void __launch_bounds__(PL_T) k_pool_bits(ba_kv_pool p) {
     p.used[w] = bits;
 }
 
+// The same of one table in one launch, where that is little: counts are made in LDS.
+__global__ void __launch_bounds__(PL_ONE) k_pool_count_one(ba_kv_pool p, ba_kv_table t) {
+    extern __shared__ int32_t counts_sh[];
+    const int blocks = (int)p.n_blocks, n = t.n_seqs * t.n_pages;
+    for (int i = threadIdx.x; i < blocks; i += PL_ONE) counts_sh[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += PL_ONE) {
+        const int s = (int)((unsigned)i / (unsigned)t.n_pages);
+        const int32_t b = t.pages[s * t.stride + (i - s * t.n_pages)];
+        if (held(p, b)) atomicAdd(counts_sh + b, 1);
+    }
+    __syncthreads();
+    // a lane to a block, a ballot to two words
+    for (int i = threadIdx.x; i < (blocks + 63) / 64 * 64; i += PL_ONE) {
+        const int c = i < blocks ? counts_sh[i] : 1;
+        if (i < blocks) {
+            p.counts[i] = c;
+            p.marks[i] = -1;
+        }
+        const unsigned long long bits = __ballot(c > 0);
+        if ((i & 31) == 0 && i < (blocks + 31) / 32 * 32) p.used[i / 32] = (uint32_t)(i & 32 ? bits >> 32 : bits);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ lists forked, blocks given back
 
-__global__ void __launch_bounds__(PL_T) k_pool_fork(ba_kv_pool p, ba_kv_fork_args a, int same) {
+__global__ void __launch_bounds__(PL_T) k_pool_fork(ba_kv_fork_args a, int same) {
+    const ba_kv_pool& p = a.pool;
     const int i = blockIdx.x;
     const int32_t from = a.parents[i], to = a.children[i];
     if (from < 0 || from >= a.from.n_seqs || to < 0 || to >= a.to.n_seqs) return;
@@ -100,7 +126,8 @@ __global__ void __launch_bounds__(PL_T) k_pool_fork(ba_kv_pool p, ba_kv_fork_arg
 }
 
 // Rows of a table (those of the list `rows`, or all): what lies outside the tokens [first, last) is given back.
-__global__ void __launch_bounds__(PL_T) k_pool_trim(ba_kv_pool p, ba_kv_trim_args a) {
+__global__ void __launch_bounds__(PL_T) k_pool_trim(ba_kv_trim_args a) {
+    const ba_kv_pool& p = a.pool;
     const int32_t s = a.rows ? a.rows[blockIdx.x] : (int32_t)blockIdx.x;
     if (s < 0 || s >= a.table.n_seqs) return;
     const int32_t first = a.first ? a.first[s] : 0, last = a.last ? a.last[s] : 0x7fffffff;
@@ -140,33 +167,58 @@ __device__ __forceinline__ int scan_before(int v, int* red, int& all) {
     return before;
 }
 
-// The first `most` blocks that are free (want = false: ascending) or used (descending), in `list`; how many there are of them.
-template <bool USED>
-__device__ int pool_list(const ba_kv_pool& p, int32_t* list, int most, int* red) {
+// Words of bits are looked through a thread each, then 32 threads take the bits of one (a thread that wrote all of its word's
+// blocks was most of the time of a pool of 5000 of them: 19 us for the plan of its moves).  each(word, used bits, used blocks
+// before it) in the order of the words, by 32 threads a word, until it has seen `enough` used (USED) or free blocks.
+template <bool USED, typename F>
+__device__ __forceinline__ void pool_words(const ba_kv_pool& p, int enough, int* red, uint2* words_sh, F each) {
     const int words = (int)((p.n_blocks + 31) / 32);
-    int found = 0;
-    for (int base = 0; base < words && found < most; base += PL_ONE) {
-        const int i = base + (int)threadIdx.x, w = USED ? words - 1 - i : i;
+    int used = 0;
+    for (int base = 0; base < words && (USED ? used : base * 32 - used) < enough; base += PL_ONE) {
+        const int w = base + (int)threadIdx.x;
         uint32_t bits = 0;
-        if (i < words) {
+        if (w < words) {
             bits = p.used[w];
-            if (!USED) bits = ~bits;
-            else if (w == words - 1 && p.n_blocks % 32) bits &= (1u << (p.n_blocks % 32)) - 1u;
+            if (w == words - 1 && p.n_blocks % 32) bits &= (1u << (p.n_blocks % 32)) - 1u;
         }
-        int all, at = found + scan_before(__popc(bits), red, all);
-        while (bits && at < most) {
-            const int b = USED ? 31 - __clz(bits) : __ffs(bits) - 1;
-            bits &= ~(1u << b);
-            list[at++] = w * 32 + b;
+        int all;
+        const int at = used + scan_before(__popc(bits), red, all);
+        words_sh[threadIdx.x] = make_uint2(bits, (uint32_t)at);      // (the scan has barriers: nobody reads the last round's)
+        __syncthreads();
+        const int here = min(words - base, PL_ONE);
+        for (int k = threadIdx.x >> 5; k < here; k += PL_ONE / 32) {
+            const uint2 x = words_sh[k];
+            if ((USED ? (int)x.y : (base + k) * 32 - (int)x.y) >= enough) break;
+            each(base + k, x.x, (int)x.y);
         }
-        found += all;
+        used += all;
     }
-    return found < most ? found : most;
+}
+
+// The first `most` free blocks in `list`; how many there are of them.
+__device__ int pool_free(const ba_kv_pool& p, int32_t* list, int most, int* red, uint2* words_sh, int* found_sh) {
+    if (threadIdx.x == 0) *found_sh = 0;
+    const int bit = threadIdx.x & 31;
+    int found = 0;
+    __syncthreads();
+    pool_words<false>(p, most, red, words_sh, [&](int w, uint32_t used, int before) {
+        const int64_t block = (int64_t)w * 32 + bit;
+        const int at = w * 32 - before + __popc(~used & ((1u << bit) - 1u));
+        if ((used >> bit & 1u) || block >= p.n_blocks || at >= most) return;
+        list[at] = (int32_t)block;
+        found = at + 1;
+    });
+    if (found) atomicMax(found_sh, found);
+    __syncthreads();
+    return *found_sh;
 }
 
 // Sequences of a round have 1 << shift threads each, which take their new blocks side by side.
-__global__ void __launch_bounds__(PL_ONE) k_pool_grow(ba_kv_pool p, ba_kv_grow_args a, int shift, int most) {
+__global__ void __launch_bounds__(PL_ONE) k_pool_grow(ba_kv_grow_args a, int shift, int most) {
+    const ba_kv_pool& p = a.pool;
     __shared__ int red[PL_ONE / 64];
+    __shared__ uint2 words_sh[PL_ONE];
+    __shared__ int found_sh;
     const int tid = threadIdx.x, lanes = 1 << shift, l = tid & (lanes - 1), lead = (tid & 63) & ~(lanes - 1), per = PL_ONE >> shift;
     int32_t* list = p.marks + p.n_blocks;
     struct Seq {
@@ -204,8 +256,7 @@ __global__ void __launch_bounds__(PL_ONE) k_pool_grow(ba_kv_pool p, ba_kv_grow_a
             if (r.open >= 0 && fresh(p.marks + r.open) >= 0) atomicSub(p.counts + r.open, 1);
         }
     }
-    const int free = pool_list<false>(p, list, most, red);
-    __syncthreads();
+    const int free = pool_free(p, list, most, red, words_sh, &found_sh);
     int base = 0, moves = 0;
     for (int s0 = 0; s0 < a.table.n_seqs; s0 += per) {
         const int s = s0 + (tid >> shift);
@@ -242,6 +293,7 @@ __global__ void __launch_bounds__(PL_ONE) k_pool_grow(ba_kv_pool p, ba_kv_grow_a
                     const int32_t block = list[k];
                     r.row[b + l] = block;
                     p.counts[block] = 1;
+                    p.marks[block] = -1;
                     atomicOr(p.used + (block >> 5), 1u << (block & 31));
                 } else if (r.row[b + l] != -1) {
                     r.row[b + l] = -1;
@@ -262,6 +314,7 @@ __global__ void __launch_bounds__(PL_ONE) k_pool_grow(ba_kv_pool p, ba_kv_grow_a
                 a.src[m] = r.open;
                 a.dst[m] = got;
                 p.counts[got] = 1;
+                p.marks[got] = -1;
                 atomicOr(p.used + (got >> 5), 1u << (got & 31));
             }
         }
@@ -278,9 +331,13 @@ __global__ void __launch_bounds__(PL_ONE) k_pool_grow(ba_kv_pool p, ba_kv_grow_a
 
 // The k-th highest used block is to go to the k-th lowest free one while that is lower: as many pairs as there are used blocks
 // past the number of used ones.
-__global__ void __launch_bounds__(PL_ONE) k_pool_plan(ba_kv_pool p, int32_t* src, int32_t* dst, int32_t* n, int most) {
+__global__ void __launch_bounds__(PL_ONE) k_pool_plan(ba_kv_compact_args c) {
+    const ba_kv_pool& p = c.pool;
+    int32_t *src = c.src, *dst = c.dst;
+    const int most = c.most;
     __shared__ int red[PL_ONE / 64];
-    const int tid = threadIdx.x, words = (int)((p.n_blocks + 31) / 32), spare = (int)((int64_t)words * 32 - p.n_blocks);
+    __shared__ uint2 words_sh[PL_ONE];
+    const int tid = threadIdx.x, bit = tid & 31, words = (int)((p.n_blocks + 31) / 32), spare = (int)((int64_t)words * 32 - p.n_blocks);
     int v = 0, total, above;
     for (int w = tid; w < words; w += PL_ONE) v += __popc(p.used[w]);
     if (tid == 0) v -= spare;
@@ -294,8 +351,15 @@ __global__ void __launch_bounds__(PL_ONE) k_pool_plan(ba_kv_pool p, int32_t* src
     if (tid == 0) v -= spare;                                // its word is among them if there are any
     scan_before(v, red, above);
     const int pairs = above < most ? above : most;
-    pool_list<false>(p, dst, pairs, red);
-    pool_list<true>(p, src, pairs, red);
+    if (pairs)
+        pool_words<true>(p, total, red, words_sh, [&](int w, uint32_t used, int before) {
+            const int64_t block = (int64_t)w * 32 + bit;
+            const uint32_t below = (1u << bit) - 1u;
+            if (block >= p.n_blocks) return;
+            const bool full = used >> bit & 1u;
+            const int at = full ? total - 1 - before - __popc(used & below) : w * 32 - before + __popc(~used & below);
+            if (at < pairs) (full ? src : dst)[at] = (int32_t)block;
+        });
     __syncthreads();
     for (int k = tid; k < most; k += PL_ONE) {
         if (k >= pairs) {
@@ -306,29 +370,25 @@ __global__ void __launch_bounds__(PL_ONE) k_pool_plan(ba_kv_pool p, int32_t* src
         const int32_t a = src[k], b = dst[k];
         p.counts[b] = p.counts[a];
         p.counts[a] = 0;
-        p.marks[a] = b;
+        p.marks[a] = b;                                      // a is free now, b is not
+        p.marks[b] = -1;
         atomicOr(p.used + (b >> 5), 1u << (b & 31));
         atomicAnd(p.used + (a >> 5), ~(1u << (a & 31)));
     }
-    if (tid == 0) *n = pairs;
+    if (tid == 0) *c.n = pairs;
 }
 
-// entries of lists whose block moves
+// entries of lists whose block moves: it has become free
 __global__ void __launch_bounds__(PL_T) k_pool_move(ba_kv_pool p, ba_kv_table t) {
     const int64_t n = (int64_t)t.n_seqs * t.n_pages;
     for (int64_t i = (int64_t)blockIdx.x * PL_T + threadIdx.x; i < n; i += (int64_t)gridDim.x * PL_T) {
         const int64_t s = i / t.n_pages;
         int32_t* e = t.pages + s * t.stride + (i - s * t.n_pages);
         const int32_t b = *e;
-        if (!held(p, b)) continue;
+        if (!held(p, b) || p.counts[b] > 0) continue;
         const int32_t to = p.marks[b];
-        if (to >= 0) *e = to;
+        if (held(p, to)) *e = to;
     }
-}
-
-__global__ void __launch_bounds__(PL_T) k_pool_unmark(ba_kv_pool p, const int32_t* src, int most) {
-    const int k = blockIdx.x * PL_T + threadIdx.x;
-    if (k < most && src[k] >= 0) p.marks[src[k]] = -1;
 }
 
 // ------------------------------------------------------------------------------------------------ blocks copied
@@ -342,6 +402,7 @@ __global__ void __launch_bounds__(PL_T) k_kv_copy(ba_kv_copy_args a, int units, 
         const int c = *a.count;
         n = c < n ? c : n;
     }
+    typedef uint32_t v4 __attribute__((ext_vector_type(4)));
     const int per = 2 * chunks;
     for (int64_t item = blockIdx.x; item < (int64_t)n * per; item += gridDim.x) {
         const int pair = (int)(item / per), part = (int)(item - (int64_t)pair * per), chunk = part >> 1;
@@ -361,10 +422,15 @@ __global__ void __launch_bounds__(PL_T) k_kv_copy(ba_kv_copy_args a, int units, 
 #pragma unroll
         for (int i = 0; i < CP_UNITS / PL_T; ++i) {
             const int u = chunk * CP_UNITS + i * PL_T + (int)threadIdx.x;
-            if (u < units) y[u] = w[i];
+            if (u < units) {                                 // not read soon: 228 MB in 48 us (4.8 TB/s; a copy of as many bytes 46), 50.5 otherwise
+                const v4 x4 = {w[i].x, w[i].y, w[i].z, w[i].w};
+                __builtin_nontemporal_store(x4, (v4*)y + u);
+            }
         }
     }
 }
+
+#define POOL_TRY(call) do { const int rc_ = (call); if (rc_ != BA_OK) return rc_; } while (0)
 
 static int pool_check(const ba_kv_pool& p) {
     BA_REQUIRE(p.n_blocks >= 0 && p.n_blocks < (int64_t)1 << 30, "pool: bad sizes");
@@ -388,60 +454,75 @@ static unsigned entry_grid(const ba_kv_table& t) {
 
 using namespace ba;
 
-#define POOL_TRY(call) do { const int rc_ = (call); if (rc_ != BA_OK) return rc_; } while (0)
+static int tables_check(const ba_kv_table* tables, int n) {
+    BA_REQUIRE(n >= 0 && (n == 0 || tables), "pool: bad tables");
+    for (int i = 0; i < n; ++i) POOL_TRY(table_check(tables[i]));
+    return BA_OK;
+}
 
-extern "C" int ba_kv_pool_count(const ba_kv_pool* pool, const ba_kv_table* tables, int32_t n_tables, void* stream) {
+extern "C" int ba_kv_pool_count(const ba_kv_count_args* args, void* stream) {
     clear_error();
-    BA_REQUIRE(pool != nullptr && n_tables >= 0 && (n_tables == 0 || tables), "null args");
-    POOL_TRY(pool_check(*pool));
-    for (int i = 0; i < n_tables; ++i) POOL_TRY(table_check(tables[i]));
-    if (pool->n_blocks == 0) return BA_OK;
+    BA_REQUIRE(args != nullptr, "null args");
+    const ba_kv_pool p = args->pool;
+    const ba_kv_table* tables = args->tables;
+    const int n_tables = args->n_tables;
+    POOL_TRY(pool_check(p));
+    POOL_TRY(tables_check(tables, n_tables));
+    if (p.n_blocks == 0) return BA_OK;
     hipStream_t st = (hipStream_t)stream;
-    const ba_kv_pool p = *pool;
+    if (n_tables == 1 && p.n_blocks <= PL_FEW && (int64_t)tables[0].n_seqs * tables[0].n_pages <= 2 * PL_FEW) {
+        hipLaunchKernelGGL(k_pool_count_one, dim3(1), dim3(PL_ONE), (size_t)p.n_blocks * 4, st, p, tables[0]);
+        BA_LAUNCHED();
+        return BA_OK;
+    }
     const unsigned nb = (unsigned)((p.n_blocks + PL_T - 1) / PL_T);
     hipLaunchKernelGGL(k_pool_clear, dim3(nb), dim3(PL_T), 0, st, p);
-    for (int i = 0; i < n_tables; ++i)
-        if (tables[i].n_seqs && tables[i].n_pages) hipLaunchKernelGGL(k_pool_count, dim3(entry_grid(tables[i])), dim3(PL_T), 0, st, p, tables[i]);
+    BA_LAUNCHED();
+    for (int i = 0; i < n_tables; ++i) {
+        if (tables[i].n_seqs == 0 || tables[i].n_pages == 0) continue;
+        hipLaunchKernelGGL(k_pool_count, dim3(entry_grid(tables[i])), dim3(PL_T), 0, st, p, tables[i]);
+        BA_LAUNCHED();
+    }
     hipLaunchKernelGGL(k_pool_bits, dim3((nb + 31) / 32), dim3(PL_T), 0, st, p);
     BA_LAUNCHED();
     return BA_OK;
 }
 
-extern "C" int ba_kv_pool_fork(const ba_kv_pool* pool, const ba_kv_fork_args* args, void* stream) {
+extern "C" int ba_kv_pool_fork(const ba_kv_fork_args* args, void* stream) {
     clear_error();
-    BA_REQUIRE(pool && args, "null args");
+    BA_REQUIRE(args != nullptr, "null args");
     const ba_kv_fork_args& a = *args;
-    POOL_TRY(pool_check(*pool));
+    POOL_TRY(pool_check(a.pool));
     POOL_TRY(table_check(a.from));
     POOL_TRY(table_check(a.to));
     BA_REQUIRE(a.n >= 0 && a.n < 1 << 23, "pool: bad sizes");
     BA_REQUIRE(a.to.n_pages >= a.from.n_pages, "pool: children's lists are narrower than their parents'");
     if (a.n == 0 || a.from.n_seqs == 0 || a.to.n_seqs == 0) return BA_OK;
     BA_REQUIRE(a.parents && a.children && a.from_lengths && a.to_lengths, "null pointer");
-    hipLaunchKernelGGL(k_pool_fork, dim3((unsigned)a.n), dim3(PL_T), 0, (hipStream_t)stream, *pool, a, (int)(a.from.pages == a.to.pages));
+    hipLaunchKernelGGL(k_pool_fork, dim3((unsigned)a.n), dim3(PL_T), 0, (hipStream_t)stream, a, (int)(a.from.pages == a.to.pages));
     BA_LAUNCHED();
     return BA_OK;
 }
 
-extern "C" int ba_kv_pool_trim(const ba_kv_pool* pool, const ba_kv_trim_args* args, void* stream) {
+extern "C" int ba_kv_pool_trim(const ba_kv_trim_args* args, void* stream) {
     clear_error();
-    BA_REQUIRE(pool && args, "null args");
+    BA_REQUIRE(args != nullptr, "null args");
     const ba_kv_trim_args& a = *args;
-    POOL_TRY(pool_check(*pool));
+    POOL_TRY(pool_check(a.pool));
     POOL_TRY(table_check(a.table));
     BA_REQUIRE(a.n_rows >= 0 && a.n_rows < 1 << 23, "pool: bad sizes");
     const int n = a.rows ? a.n_rows : a.table.n_seqs;
     if (n == 0 || a.table.n_seqs == 0) return BA_OK;
-    hipLaunchKernelGGL(k_pool_trim, dim3((unsigned)n), dim3(PL_T), 0, (hipStream_t)stream, *pool, a);
+    hipLaunchKernelGGL(k_pool_trim, dim3((unsigned)n), dim3(PL_T), 0, (hipStream_t)stream, a);
     BA_LAUNCHED();
     return BA_OK;
 }
 
-extern "C" int ba_kv_pool_grow(const ba_kv_pool* pool, const ba_kv_grow_args* args, void* stream) {
+extern "C" int ba_kv_pool_grow(const ba_kv_grow_args* args, void* stream) {
     clear_error();
-    BA_REQUIRE(pool && args, "null args");
+    BA_REQUIRE(args != nullptr, "null args");
     const ba_kv_grow_args& a = *args;
-    POOL_TRY(pool_check(*pool));
+    POOL_TRY(pool_check(a.pool));
     POOL_TRY(table_check(a.table));
     BA_REQUIRE(a.max_new >= 0, "pool: bad sizes");
     BA_REQUIRE(a.n && a.missing && (a.table.n_seqs == 0 || (a.lengths && a.src && a.dst)), "null pointer");
@@ -451,28 +532,27 @@ extern "C" int ba_kv_pool_grow(const ba_kv_pool* pool, const ba_kv_grow_args* ar
     int shift = 0;
     while (shift < 6 && (1 << shift) < slots) ++shift;
     const int64_t most = (slots + 1) * a.table.n_seqs;
-    hipLaunchKernelGGL(k_pool_grow, dim3(1), dim3(PL_ONE), 0, (hipStream_t)stream, *pool, a, shift, (int)(most < pool->n_blocks ? most : pool->n_blocks));
+    hipLaunchKernelGGL(k_pool_grow, dim3(1), dim3(PL_ONE), 0, (hipStream_t)stream, a, shift, (int)(most < a.pool.n_blocks ? most : a.pool.n_blocks));
     BA_LAUNCHED();
     return BA_OK;
 }
 
-extern "C" int ba_kv_pool_compact(const ba_kv_pool* pool, const ba_kv_table* tables, int32_t n_tables, int32_t* src, int32_t* dst,
-                                  int32_t* n, int32_t most, void* stream) {
+extern "C" int ba_kv_pool_compact(const ba_kv_compact_args* args, void* stream) {
     clear_error();
-    BA_REQUIRE(pool != nullptr && n_tables >= 0 && (n_tables == 0 || tables), "null args");
-    POOL_TRY(pool_check(*pool));
-    for (int i = 0; i < n_tables; ++i) POOL_TRY(table_check(tables[i]));
-    BA_REQUIRE(most >= 0 && most <= pool->n_blocks, "pool: bad sizes");
-    BA_REQUIRE(n && (most == 0 || (src && dst)), "null pointer");
+    BA_REQUIRE(args != nullptr, "null args");
+    const ba_kv_compact_args& a = *args;
+    POOL_TRY(pool_check(a.pool));
+    POOL_TRY(tables_check(a.tables, a.n_tables));
+    BA_REQUIRE(a.most >= 0 && a.most <= a.pool.n_blocks, "pool: bad sizes");
+    BA_REQUIRE(a.n && (a.most == 0 || (a.src && a.dst)), "null pointer");
     hipStream_t st = (hipStream_t)stream;
-    const ba_kv_pool p = *pool;
-    hipLaunchKernelGGL(k_pool_plan, dim3(1), dim3(PL_ONE), 0, st, p, src, dst, n, most);
-    if (most) {
-        for (int i = 0; i < n_tables; ++i)
-            if (tables[i].n_seqs && tables[i].n_pages) hipLaunchKernelGGL(k_pool_move, dim3(entry_grid(tables[i])), dim3(PL_T), 0, st, p, tables[i]);
-        hipLaunchKernelGGL(k_pool_unmark, dim3((unsigned)((most + PL_T - 1) / PL_T)), dim3(PL_T), 0, st, p, src, most);
-    }
+    hipLaunchKernelGGL(k_pool_plan, dim3(1), dim3(PL_ONE), 0, st, a);
     BA_LAUNCHED();
+    for (int i = 0; i < a.n_tables && a.most; ++i) {
+        if (a.tables[i].n_seqs == 0 || a.tables[i].n_pages == 0) continue;
+        hipLaunchKernelGGL(k_pool_move, dim3(entry_grid(a.tables[i])), dim3(PL_T), 0, st, a.pool, a.tables[i]);
+        BA_LAUNCHED();
+    }
     return BA_OK;
 }
 

@@ -23,7 +23,8 @@ the open last block is shared, and ``grow`` is what gives each its own before ne
 """
 import torch
 
-from ._lib import BaKvForkArgs, BaKvGrowArgs, BaKvPool, BaKvTable, BaKvTrimArgs, launch, lib, written
+from ._lib import (BaKvCompactArgs, BaKvCountArgs, BaKvForkArgs, BaKvGrowArgs, BaKvPool, BaKvTable, BaKvTrimArgs, launch, lib,
+                   written)
 
 __all__ = ['BlockPool']
 
@@ -53,7 +54,7 @@ class BlockPool:
         self._used = torch.zeros((n_blocks + 31) // 32, dtype=torch.int32, device=self._device)
         self._marks = torch.full((2 * n_blocks,), -1, dtype=torch.int32, device=self._device)
         self._missing = torch.zeros(1, dtype=torch.int32, device=self._device)
-        self._lib = lib()
+        self._lib, self._at = lib(), None
         if n_blocks % 32:                                   # bits past the last block are set
             self._used[-1] = -1 << n_blocks % 32
 
@@ -61,40 +62,49 @@ class BlockPool:
         """(1,) int64 on the device: the free blocks."""
         return (self._counts == 0).sum().view(1)
 
-    def _pool(self):
-        return BaKvPool(self._counts.data_ptr(), self._used.data_ptr(), self._marks.data_ptr(), self._n_blocks)
+    def _args(self, kind):
+        """The arguments of a call, with the pool's own."""
+        at = self._counts.data_ptr()
+        if at != self._at:
+            self._at = at
+            pool = BaKvPool(at, self._used.data_ptr(), self._marks.data_ptr(), self._n_blocks)
+            self._kinds = {k: k(pool=pool) for k in (BaKvCountArgs, BaKvForkArgs, BaKvTrimArgs, BaKvGrowArgs, BaKvCompactArgs)}
+        return kind.from_buffer_copy(self._kinds[kind])
 
-    def _table(self, pages, name='pages'):
+    def _table(self, a, pages, name='pages'):
         shape, stride = pages.shape, pages.stride()
         if (len(shape) != 2 or pages.dtype is not torch.int32 or pages.device != self._device or
                 stride[1] != 1 and shape[1] > 1 or stride[0] < shape[1] and shape[0] > 1):
             raise ValueError(f'pool: {name} must be (n_seqs, blocks) int32 on {self._device} with contiguous rows that do not '
                              'overlap')
-        return BaKvTable(pages.data_ptr(), stride[0], shape[0], shape[1])
+        a.pages, a.stride, a.n_seqs, a.n_pages = pages.data_ptr(), stride[0], shape[0], shape[1]
+        return shape
 
     def _ints(self, t, name, n=None):
-        if (t.dtype is not torch.int32 or t.device != self._device or t.dim() != 1 or n is not None and t.shape[0] != n or
+        shape = t.shape
+        if (t.dtype is not torch.int32 or t.device != self._device or len(shape) != 1 or n is not None and shape[0] != n or
                 not t.is_contiguous()):
             raise ValueError(f'pool: {name} must be a contiguous int32 tensor of shape ({"n" if n is None else n},) on {self._device}')
         return t.data_ptr()
 
-    def _launch(self, call, args, *changed):
-        pool = self._pool()
-        launch(lambda a, stream: call(pool, a, stream), args, self._device)
+    def _launch(self, call, a, *changed):
+        launch(call, a, self._device)
         written((self._counts, *changed))
 
-    def _tables(self, tables):
-        found = (BaKvTable * len(tables))(*(self._table(t) for t in tables))
+    def _tables(self, a, tables):
+        a.tables, a.n_tables = (BaKvTable * len(tables))(), len(tables)
+        for i, t in enumerate(tables):
+            self._table(a.tables[i], t)
         at = [t.data_ptr() for t in tables if t.numel()]
         if len(set(at)) != len(at):
             raise ValueError('pool: a table is given twice')
-        return found
 
     def count(self, *tables):
         """Set the counts from tables: those of all lists that are in use.  For lists that were made or changed by hand, or
         read from a file."""
-        found = self._tables(tables)
-        self._launch(lambda p, a, stream: self._lib.ba_kv_pool_count(p, found, len(tables), stream), found)
+        a = self._args(BaKvCountArgs)
+        self._tables(a, tables)
+        self._launch(self._lib.ba_kv_pool_count, a)
 
     def grow(self, pages, lengths, new, max_new=None):
         """Blocks for ``new`` more tokens (a number, or (n_seqs,) int32) after the first ``lengths`` of each list, written into
@@ -106,25 +116,26 @@ class BlockPool:
         (and before the next call on this pool).  One list after the other, so the last holder of a block keeps it.  Lists
         that there are no blocks left for keep -1 there, an exchanged block's place among them, and rows appended there are
         left out; ``missing`` says how many there were."""
-        table = self._table(pages)
-        S, width = pages.shape
-        a = BaKvGrowArgs(table=table, lengths=self._ints(lengths, 'lengths', S))
+        a = self._args(BaKvGrowArgs)
+        S, width = self._table(a.table, pages)
+        a.lengths = self._ints(lengths, 'lengths', S)
         if isinstance(new, torch.Tensor):
             a.more = self._ints(new, 'new', S)
-            most = min(width * BLOCK, (1 << 31) - 1) if max_new is None else max_new
+            most = width * BLOCK if max_new is None else max_new
         else:
-            a.each = min(int(new), (1 << 31) - 1)
-            most = a.each if max_new is None else max_new
             if new < 0:
                 raise ValueError(f'pool: {new} new tokens')
+            a.each = most = min(int(new), (1 << 31) - 1)
+            if max_new is not None:
+                most = max_new
         if most < 0:
             raise ValueError('pool: a negative bound on tokens')
         a.max_new = min(int(most), (1 << 31) - 1)
-        moves = torch.empty(2 * S + 1, dtype=torch.int32, device=self._device)
-        src, dst, n = moves[:S], moves[S:2 * S], moves[2 * S:]
-        a.src, a.dst, a.n, a.missing = src.data_ptr(), dst.data_ptr(), n.data_ptr(), self._missing.data_ptr()
-        self._launch(self._lib.ba_kv_pool_grow, a, pages, self._missing)
-        return src, dst, n
+        moves = torch.empty(2 * S + 1, dtype=torch.int32, device=self._device).split_with_sizes((S, S, 1))
+        at, missing = moves[2].data_ptr() - 8 * S, self._missing
+        a.src, a.dst, a.n, a.missing = at, at + 4 * S, at + 8 * S, missing.data_ptr()
+        self._launch(self._lib.ba_kv_pool_grow, a, pages, missing)
+        return moves
 
     def fork(self, pages, lengths, parents, children, into=None):
         """Row children[i] becomes the list of row parents[i] ((n,) int32 each): it gives back the blocks that it held, holds
@@ -132,10 +143,12 @@ class BlockPool:
         another table (which a reordering of all sequences needs).  Pairs that name a row that is not there, whose child a
         later pair has too, or whose child is a parent in the same table, change nothing."""
         to, to_lengths = (pages, lengths) if into is None else into
-        a = BaKvForkArgs(from_=self._table(pages), to=self._table(to), from_lengths=self._ints(lengths, 'lengths', pages.shape[0]),
-                         to_lengths=self._ints(to_lengths, "the children's lengths", to.shape[0]))
+        a = self._args(BaKvForkArgs)
+        S, width = self._table(a.from_, pages)
+        T, wide = self._table(a.to, to)
+        a.from_lengths, a.to_lengths = self._ints(lengths, 'lengths', S), self._ints(to_lengths, "the children's lengths", T)
         a.parents, a.children, a.n = self._ints(parents, 'parents'), self._ints(children, 'children', parents.shape[0]), parents.shape[0]
-        if to.shape[1] < pages.shape[1]:
+        if wide < width:
             raise ValueError("pool: children's lists must be as wide as their parents'")
         if to is not pages and to.numel() and pages.numel() and to.data_ptr() == pages.data_ptr() and to.stride() != pages.stride():
             raise ValueError('pool: the tables overlap')
@@ -144,7 +157,9 @@ class BlockPool:
 
     def free(self, pages, lengths, rows=None):
         """Give back the lists ``rows`` ((n,) int32; default: all): entries become -1, lengths 0."""
-        a = BaKvTrimArgs(table=self._table(pages), lengths=self._ints(lengths, 'lengths', pages.shape[0]), all=1)
+        a = self._args(BaKvTrimArgs)
+        S, _ = self._table(a.table, pages)
+        a.lengths, a.all = self._ints(lengths, 'lengths', S), 1
         if rows is not None:
             a.rows, a.n_rows = self._ints(rows, 'rows'), rows.shape[0]
             if not a.n_rows:
@@ -156,23 +171,25 @@ class BlockPool:
         that were drafted and refused); (n_seqs,) int32 each."""
         if first is None and last is None:
             raise ValueError('pool: trim by first, by last or by both')
-        a = BaKvTrimArgs(table=self._table(pages))
+        a = self._args(BaKvTrimArgs)
+        S, _ = self._table(a.table, pages)
         if first is not None:
-            a.first = self._ints(first, 'first', pages.shape[0])
+            a.first = self._ints(first, 'first', S)
         if last is not None:
-            a.last = self._ints(last, 'last', pages.shape[0])
+            a.last = self._ints(last, 'last', S)
         self._launch(self._lib.ba_kv_pool_trim, a, pages)
 
     def compact(self, *tables, most=None):
         """Move the highest used blocks to the lowest free ones, ``most`` at a time at most (default: all), so that the used
         blocks come to be the first: ``tables`` (all that hold blocks of the pool) are changed, and (src, dst, n) is for
         ``KVCache.copy``, before the next call on this pool."""
-        found = self._tables(tables)
+        a = self._args(BaKvCompactArgs)
+        self._tables(a, tables)
         most = self._n_blocks // 2 if most is None else min(int(most), self._n_blocks // 2)
         if most < 0:
             raise ValueError(f'pool: {most} moves')
-        moves = torch.empty(2 * most + 1, dtype=torch.int32, device=self._device)
-        src, dst, n = moves[:most], moves[most:2 * most], moves[2 * most:]
-        self._launch(lambda p, a, stream: self._lib.ba_kv_pool_compact(p, found, len(tables), src.data_ptr(), dst.data_ptr(),
-                                                                       n.data_ptr(), most, stream), found, *tables)
-        return src, dst, n
+        moves = torch.empty(2 * most + 1, dtype=torch.int32, device=self._device).split_with_sizes((most, most, 1))
+        at = moves[2].data_ptr() - 8 * most
+        a.most, a.src, a.dst, a.n = most, at, at + 4 * most, at + 8 * most
+        self._launch(self._lib.ba_kv_pool_compact, a, *tables)
+        return moves

@@ -753,8 +753,8 @@ int ba_kv_attend_scored(const ba_kv_scored_args* args, void* stream);
 void ba_kv_scored_plan(ba_kv_scored_args* args);
 
 /* Pages of the cache.  A pool knows of each block how many lists hold it: counts (n_blocks,), used ((n_blocks + 31) / 32
- * words, a bit for each block that a list holds, bits past the last block set) and marks (2 n_blocks ints, -1 in the first
- * half between calls), all on the device; ba_kv_pool_count sets the three.  Tables of lists have -1 (any number below 0)
+ * words, a bit for each block that a list holds, bits past the last block set) and marks (2 n_blocks ints, between calls -1
+ * for used blocks and anything for others), all on the device; ba_kv_pool_count sets the three.  Tables of lists have -1 (any number below 0)
  * where there is no block; entries past the pool are left as they are.  Calls on one pool go one after the other. */
 typedef struct {
     int32_t* counts;
@@ -769,13 +769,21 @@ typedef struct {
     int32_t n_seqs, n_pages;
 } ba_kv_table;
 
-/* Counts from the lists of n_tables tables (a host array): each entry counts once. */
-int ba_kv_pool_count(const ba_kv_pool* pool, const ba_kv_table* tables, int32_t n_tables, void* stream);
+/* Counts from the lists of n_tables tables (a host array, read by the call): each entry counts once. */
+typedef struct {
+    ba_kv_pool pool;
+    const ba_kv_table* tables;
+    int32_t n_tables;
+    int32_t reserved;
+} ba_kv_count_args;
+
+int ba_kv_pool_count(const ba_kv_count_args* args, void* stream);
 
 /* Row children[i] of `to` gives back what it holds and becomes the list of row parents[i] of `from`: its blocks with tokens
  * (below from_lengths), and its length.  A pair that names a row out of range, a child that a later pair names too, or (in one
  * table) a child that is the parent of a pair, changes nothing. */
 typedef struct {
+    ba_kv_pool pool;
     ba_kv_table from, to;      /* may be the same; `to` is at least as wide */
     const int32_t* from_lengths;
     int32_t* to_lengths;
@@ -785,11 +793,12 @@ typedef struct {
     int32_t reserved;
 } ba_kv_fork_args;
 
-int ba_kv_pool_fork(const ba_kv_pool* pool, const ba_kv_fork_args* args, void* stream);
+int ba_kv_pool_fork(const ba_kv_fork_args* args, void* stream);
 
 /* Blocks without a token in [first[s], last[s]) are given back (all of them where `all` is set), their entries become -1; first
  * and last may be NULL.  rows: (n_rows,) the lists that it is done to, or NULL for every one.  lengths: set to 0, or NULL. */
 typedef struct {
+    ba_kv_pool pool;
     ba_kv_table table;
     const int32_t* first;
     const int32_t* last;
@@ -799,7 +808,7 @@ typedef struct {
     int32_t all;
 } ba_kv_trim_args;
 
-int ba_kv_pool_trim(const ba_kv_pool* pool, const ba_kv_trim_args* args, void* stream);
+int ba_kv_pool_trim(const ba_kv_trim_args* args, void* stream);
 
 /* Blocks for more[s] (or `each`; at most max_new) tokens after the first lengths[s] of every list, taken in the order of the
  * lists, the lowest free block first; entries that are there already stay.  Where the first of them goes to a block that has
@@ -807,6 +816,7 @@ int ba_kv_pool_trim(const ba_kv_pool* pool, const ba_kv_trim_args* args, void* s
  * -1 after them ((n_seqs,) ints each).  One list after the other: the last holder of a block keeps it.  missing: blocks that
  * there were not; entries without one are -1, an exchanged one too. */
 typedef struct {
+    ba_kv_pool pool;
     ba_kv_table table;
     const int32_t* lengths;
     const int32_t* more;
@@ -817,12 +827,21 @@ typedef struct {
     int32_t* missing;
 } ba_kv_grow_args;
 
-int ba_kv_pool_grow(const ba_kv_pool* pool, const ba_kv_grow_args* args, void* stream);
+int ba_kv_pool_grow(const ba_kv_grow_args* args, void* stream);
 
-/* The highest used blocks go to the lowest free ones, at most `most` of them: the tables and counts are changed, (src, dst)[0 ..
- * n) are the blocks to be copied, -1 after them (`most` ints each). */
-int ba_kv_pool_compact(const ba_kv_pool* pool, const ba_kv_table* tables, int32_t n_tables, int32_t* src, int32_t* dst,
-                       int32_t* n, int32_t most, void* stream);
+/* The highest used blocks go to the lowest free ones, at most `most` of them: the n_tables tables (a host array, read by the
+ * call) and the counts are changed, (src, dst)[0 .. n) are the blocks to be copied, -1 after them (`most` ints each). */
+typedef struct {
+    ba_kv_pool pool;
+    const ba_kv_table* tables;
+    int32_t n_tables;
+    int32_t most;
+    int32_t* src;
+    int32_t* dst;
+    int32_t* n;
+} ba_kv_compact_args;
+
+int ba_kv_pool_compact(const ba_kv_compact_args* args, void* stream);
 
 /* Blocks src[i] copied to dst[i], codes and factors, for i < min(n, *count); pairs with a number outside [0, n_blocks) are left
  * out.  No block may be the destination of two pairs, or of one and the source of another. */

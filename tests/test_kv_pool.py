@@ -41,38 +41,40 @@ def test_pool_entry_points_refuse_bad_arguments_without_a_gpu():
     L, p = _lib.lib(), 4096
     pool = _lib.BaKvPool(p, p, p, 40)
     table = lambda **kw: _lib.BaKvTable(**{**dict(pages=p, stride=4, n_seqs=2, n_pages=4), **kw})  # noqa: E731
+    calls = {
+        'count': (_lib.BaKvCountArgs, lambda t: dict(tables=ctypes.pointer(t), n_tables=1)),
+        'grow': (_lib.BaKvGrowArgs, lambda t: dict(table=t, lengths=p, src=p, dst=p, n=p, missing=p)),
+        'trim': (_lib.BaKvTrimArgs, lambda t: dict(table=t)),
+        'fork': (_lib.BaKvForkArgs, lambda t: dict(from_=table(), to=t, from_lengths=p, to_lengths=p, parents=p, children=p, n=2)),
+        'compact': (_lib.BaKvCompactArgs, lambda t: dict(tables=ctypes.pointer(t), n_tables=1, src=p, dst=p, n=p, most=3))}
 
-    def refused(call, word, *args):
-        assert call(*args, None) != 0 and word in L.ba_last_error().decode(), (word, L.ba_last_error())
+    def refused(name, word, pool=pool, t=None, **kw):
+        kind, fields = calls[name]
+        call = getattr(L, 'ba_kv_pool_' + name)
+        assert call(kind(pool=pool, **{**fields(t if t is not None else table()), **kw}), None) != 0 and word in L.ba_last_error().decode(), (name, word, L.ba_last_error())
 
-    for bad, word in ((_lib.BaKvPool(None, p, p, 40), 'null'), (_lib.BaKvPool(p, p, p, -1), 'bad sizes'), (_lib.BaKvPool(p, p, p, 1 << 30), 'bad sizes'),
-                      (None, 'null')):
-        refused(L.ba_kv_pool_count, word, bad, table(), 1)
-        refused(L.ba_kv_pool_grow, word, bad, _lib.BaKvGrowArgs(table=table(), lengths=p, src=p, dst=p, n=p, missing=p))
-        refused(L.ba_kv_pool_trim, word, bad, _lib.BaKvTrimArgs(table=table()))
-        refused(L.ba_kv_pool_fork, word, bad, _lib.BaKvForkArgs(from_=table(), to=table()))
-        refused(L.ba_kv_pool_compact, word, bad, table(), 1, p, p, p, 3)
-    for t, word in ((table(n_seqs=-1), 'bad sizes'), (table(n_pages=1 << 24), 'bad sizes'), (table(n_seqs=1 << 23), 'too many'), (table(pages=None), 'null')):
-        refused(L.ba_kv_pool_count, word, pool, t, 1)
-        refused(L.ba_kv_pool_grow, word, pool, _lib.BaKvGrowArgs(table=t, lengths=p, src=p, dst=p, n=p, missing=p))
-        refused(L.ba_kv_pool_trim, word, pool, _lib.BaKvTrimArgs(table=t))
-        refused(L.ba_kv_pool_fork, word, pool, _lib.BaKvForkArgs(from_=table(), to=t))
-        refused(L.ba_kv_pool_compact, word, pool, t, 1, p, p, p, 3)
-    refused(L.ba_kv_pool_count, 'null', pool, None, 1)
-    refused(L.ba_kv_pool_grow, 'bad sizes', pool, _lib.BaKvGrowArgs(table=table(), lengths=p, src=p, dst=p, n=p, missing=p, max_new=-1))
+    for name in calls:
+        assert getattr(L, 'ba_kv_pool_' + name)(None, None) != 0
+        for bad, word in ((_lib.BaKvPool(None, p, p, 40), 'null'), (_lib.BaKvPool(p, p, p, -1), 'bad sizes'), (_lib.BaKvPool(p, p, p, 1 << 30), 'bad sizes')):
+            refused(name, word, pool=bad)
+        for t, word in ((table(n_seqs=-1), 'bad sizes'), (table(n_pages=1 << 24), 'bad sizes'), (table(n_seqs=1 << 23), 'too many'), (table(pages=None), 'null')):
+            refused(name, word, t=t)
+    refused('count', 'bad tables', tables=None)
+    refused('compact', 'bad tables', n_tables=-1)
+    refused('grow', 'bad sizes', max_new=-1)
     for name in ('lengths', 'src', 'dst', 'n', 'missing'):
-        refused(L.ba_kv_pool_grow, 'null', pool, _lib.BaKvGrowArgs(**{**dict(table=table(), lengths=p, src=p, dst=p, n=p, missing=p), name: None}))
-    fork = dict(from_=table(), to=table(), from_lengths=p, to_lengths=p, parents=p, children=p, n=2)
+        refused('grow', 'null', **{name: None})
     for name in ('from_lengths', 'to_lengths', 'parents', 'children'):
-        refused(L.ba_kv_pool_fork, 'null', pool, _lib.BaKvForkArgs(**{**fork, name: None}))
-    refused(L.ba_kv_pool_fork, 'narrower', pool, _lib.BaKvForkArgs(**{**fork, 'to': table(n_pages=3)}))
-    refused(L.ba_kv_pool_fork, 'bad sizes', pool, _lib.BaKvForkArgs(**{**fork, 'n': -1}))
-    assert L.ba_kv_pool_fork(pool, _lib.BaKvForkArgs(**{**fork, 'n': 0}), None) == 0
-    refused(L.ba_kv_pool_compact, 'bad sizes', pool, table(), 1, p, p, p, 41)
-    refused(L.ba_kv_pool_compact, 'null', pool, table(), 1, p, p, None, 3)
+        refused('fork', 'null', **{name: None})
+    refused('fork', 'narrower', t=table(n_pages=3))
+    refused('fork', 'bad sizes', n=-1)
+    assert L.ba_kv_pool_fork(_lib.BaKvForkArgs(pool=pool, from_=table(), to=table()), None) == 0
+    refused('compact', 'bad sizes', most=41)
+    refused('compact', 'null', n=None)
+    refused('trim', 'bad sizes', n_rows=-1)
     copy = dict(k=p, v=p, scales=p, n_blocks=3, heads=2, dim=64, src=p, dst=p, n=2)
     for kw, word in ((dict(dim=48), 'head size'), (dict(heads=0), 'bad sizes'), (dict(n=-1), 'bad sizes'), (dict(k=p + 8), 'aligned'), (dict(dst=None), 'null')):
-        refused(L.ba_kv_copy, word, _lib.BaKvCopyArgs(**{**copy, **kw}))
+        assert L.ba_kv_copy(_lib.BaKvCopyArgs(**{**copy, **kw}), None) != 0 and word in L.ba_last_error().decode(), (kw, L.ba_last_error())
     assert L.ba_kv_copy(_lib.BaKvCopyArgs(**{**copy, 'n': 0}), None) == 0
 
 
@@ -181,7 +183,7 @@ class Both:
         used = self.pool._used.cpu().numpy().view(np.uint32)
         bits = (used[:, None] >> np.arange(32, dtype=np.uint32) & 1).flatten()
         assert bits[:len(self.o.counts)].tolist() == [int(c > 0) for c in self.o.counts] and bits[len(self.o.counts):].all()
-        assert bool((self.pool._marks[:len(self.o.counts)] == -1).all())
+        assert bool(((self.pool._marks[:len(self.o.counts)] == -1) | (self.pool.counts == 0)).all())
 
     def moved(self, moves, got, size):
         src, dst, n = got
