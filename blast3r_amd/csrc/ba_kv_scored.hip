@@ -54,12 +54,12 @@ static int attend_scored(const ba_kv_scored_args& s, hipStream_t st) {
     return BA_OK;
 }
 
-// What a launch is expected to take (us), which shapes and parts are chosen by.  Tiles: rounds of workgroups that the CUs hold at
-// a time, each with its blocks and as much as SC_START blocks to begin and end with; per block what 2 x 2048 rows over 16384
-// tokens take by the block (32 elements a head 2.0 us, 64 2.3, 96 and 128 1.8 and 2.0, 256 2.5; tiles of 128 rows, of which a
-// CU holds more, 1.8, 1.8 and 2.2).  Few rows: the bytes of the blocks at 4.8 TB/s, or the blocks of a wave in series.  Partial
-// sums are written and read once, with a launch of 4 us.
-#define SC_START 4
+// What a launch is expected to take (us), which shapes and parts are chosen by.  Tiles: a CU holds `fit` workgroups at a time
+// and takes its share of all of them in turns of so many; a workgroup's time is its blocks' and that of SC_START more to begin
+// and end with, and a block's (us, by how many workgroups share the CU) what calls of 2 x 2048 rows over 16384 tokens, of 6144
+// over 12288 and of documents of 64 tokens took.  Few rows: the bytes of the blocks at 4.8 TB/s, or the blocks of a wave in
+// series.  Partial sums are written and read once, with a launch of 4 us.
+#define SC_START 5
 
 struct Guess {
     AtShape v;
@@ -70,12 +70,15 @@ struct Guess {
 static double launch_us(const AtShape& v, int dim, int64_t base, int64_t blocks, int parts) {
     const int64_t per = (blocks + parts - 1) / parts;
     if (!v.ncb) {
-        const double bytes = (double)base * blocks * 128.0 * dim / 4.8e6, chain = ((per + 3) / 4) * 1.0;
+        const double bytes = (double)base * blocks * 128.0 * dim / 4.8e6, chain = (double)((per + 3) / 4);
         return 6.0 + (bytes > chain ? bytes : chain);
     }
-    const double block = v.rows == 256 ? (dim == 64 ? 2.3 : dim == 96 ? 1.8 : 2.0) : dim == 256 ? 2.5 : dim <= 64 ? 1.8 : 2.2;
-    const int64_t rounds = (base * parts + 256 * v.fit - 1) / (256 * v.fit);
-    return 4.0 + rounds * (per + SC_START) * block;
+    static const double small[5][3] = {{0.6, 0.5, 0.43}, {1.0, 0.66, 0.6}, {1.2, 0.93, 0.0}, {1.36, 1.09, 0.0}, {2.45, 0.0, 0.0}};
+    static const double large[4][2] = {{1.4, 0.94}, {1.6, 1.13}, {1.78, 0.0}, {2.03, 0.0}};
+    const int d = dim <= 96 ? dim / 32 - 1 : dim == 128 ? 3 : 4;
+    const double* block = v.rows == 256 ? large[d] : small[d];
+    const int64_t each = (base * parts + 255) / 256, full = each / v.fit, rest = each % v.fit;
+    return 4.0 + (per + SC_START) * (full * v.fit * block[v.fit - 1] + (rest ? rest * block[rest - 1] : 0.0));
 }
 
 // The best shape and number of parts for the rows of n_seqs sequences that may see `blocks` blocks each; join: time that a part
