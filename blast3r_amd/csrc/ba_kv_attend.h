@@ -104,7 +104,7 @@ struct AtMore {
     int blk_lo, blk_hi;      // the blocks of the lists that it takes
     int part0, parts;        // it writes the parts [part0, part0 + parts) of the n_splits
     int least;               // blocks of a part at least
-    int stacked;             // its rows are those of all sequences, and the list is the first sequence's
+    int stacked;             // its rows are those of all sequences, and a workgroup's list is that of its row that sees furthest
 };
 
 template <int MODE> struct AtArgs {
@@ -223,6 +223,7 @@ __device__ __forceinline__ void at_part(const AtBlocks& b, int sp, int& lo, int&
 // What a row sees when it is not plain: tokens below pre, and [lo, hi) where that is not empty (else lo is AT_NEVER and hi 0).
 struct AtRow {
     int pos, lo, hi, pre;
+    int seq;                 // its sequence
 };
 #define AT_NEVER 0x7fffffff
 
@@ -235,14 +236,14 @@ __device__ __forceinline__ AtRow at_row(const AtArgs<MODE>& x, AtSeq q, int s, i
         s = seq_of_row(a, row);
         q = at_seq(a, s);
         i = row - q.row0;
-        if (i < 0 || i >= q.rows) return {0, AT_NEVER, 0, 0};
+        if (i < 0 || i >= q.rows) return {0, AT_NEVER, 0, 0, s};
     }
     const int64_t pos = (int64_t)q.first + i, since = x.m.since ? x.m.since[row] : 0, until = x.m.until ? x.m.until[row] : q.len;
     const int64_t from = a.window > 0 ? pos - a.window + 1 : 0, end = a.causal ? pos + 1 : q.len;
     const int64_t lo = since > from ? since : from, hi = until < end ? until : end;
     const int l = (int)(lo < 0 ? 0 : lo), h = (int)(hi < q.len ? hi : q.len);
     const int pre = x.m.prefix ? x.m.prefix[s] : 0;
-    return {(int)pos, h > l ? l : AT_NEVER, h > l ? h : 0, pre < 0 ? 0 : pre < q.len ? pre : q.len};
+    return {(int)pos, h > l ? l : AT_NEVER, h > l ? h : 0, pre < 0 ? 0 : pre < q.len ? pre : q.len, s};
 }
 
 // Distance that a row's biases are measured from: that of the token it sees whose bias is the largest.  Far tokens' biases
@@ -289,6 +290,24 @@ __device__ __forceinline__ AtSpan at_span(const AtRow (&r)[N]) {
              __shfl_xor(s.pre1, k), __shfl_xor(s.pos0, k), __shfl_xor(s.pos1, k));
     auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
     return {one(s.lo0), one(s.lo1), one(s.hi0), one(s.hi1), one(s.pre0), one(s.pre1), one(s.pos0), one(s.pos1)};
+}
+
+// The sequence of the row that sees the furthest token, of a wave's rows where these are stacked: it has all blocks that the
+// others see of the shared ones (the first sequence may be an empty place of the batch).  Furthest token above, sequence below.
+template <int N, int COLS>
+__device__ __forceinline__ int64_t at_furthest(const AtRow (&r)[N]) {
+    int64_t best = -1;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        const int64_t key = (int64_t)max(r[c].hi, r[c].pre) << 32 | (uint32_t)r[c].seq;
+        best = key > best ? key : best;
+    }
+#pragma unroll
+    for (int k = 1; k < COLS; k <<= 1) {
+        const int64_t key = (int64_t)__shfl_xor((long long)best, k);
+        best = key > best ? key : best;
+    }
+    return best;
 }
 
 // The same of rows i0 .. i1 of a sequence, whose bounds rise with them where neither since nor until says otherwise (rows that
@@ -558,6 +577,7 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(AtArgs<MO
     AtRow row[NCB];
     AtSpan span = {};
     AtWalk walk = {};
+    int list = s;                                            // whose list
     auto find_rows = [&] {
         if constexpr (MODE != AT_PLAIN)
 #pragma unroll
@@ -573,6 +593,7 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(AtArgs<MO
         if (x.m.since || x.m.until || x.m.stacked) {
             find_rows();
             span = at_span<NCB, COLS>(row);
+            if (x.m.stacked) list = __builtin_amdgcn_readfirstlane((int)at_furthest<NCB, COLS>(row));
         } else {
             const int end = tile0 + ROWS < all ? tile0 + ROWS : all;
             span = at_span_of(x, q, s, (int)((unsigned)tile0 / (unsigned)group), (int)((unsigned)(end - 1) / (unsigned)group));
@@ -587,7 +608,7 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(AtArgs<MO
     bool last_first = false;
     if constexpr (MODE == AT_ANY) last_first = x.m.slopes != nullptr;
     auto block = [&](int v) { return MODE == AT_PLAIN ? v : walk.block(last_first ? walk.n - 1 - v : v); };
-    const int32_t* pages = a.pages + (int64_t)s * a.pages_stride;
+    const int32_t* pages = a.pages + (int64_t)list * a.pages_stride;
     const uint8_t* kb = (const uint8_t*)a.k + (int64_t)kh * 64 * D;
     const uint8_t* vb = (const uint8_t*)a.v + (int64_t)kh * 64 * D;
     const int64_t step = (int64_t)a.heads * 64 * D;
@@ -938,6 +959,7 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
     AtSpan span = {};
     AtWalk walk = {};
     uint4 raw[NCB][KS];
+    int list = s;                                            // whose list
     auto find_rows = [&] {
         if constexpr (MODE != AT_PLAIN)
 #pragma unroll
@@ -952,13 +974,24 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
         if (lo >= hi && a.n_splits > 1) return;              // k_kv_join knows which parts there are
     } else {
         int3* span_sh = (int3*)k_sh[1];                      // free until the first block has been converted by all
+        int64_t* far_sh = (int64_t*)k_sh[1] + 16;
         if (x.m.since || x.m.until || x.m.stacked) find_rows();
         fetch_queries<D, 32, NCB>(a, q, kh, group, row0, all, n, g, wide != 0, raw);
         int3 r;                                              // of all waves
         if (x.m.since || x.m.until || x.m.stacked) {
             span = at_span<NCB, 32>(row);
-            if (lane == 0) span_sh[wave] = make_int3(span.lo0, span.hi1, span.pre1);
+            const int64_t far = x.m.stacked ? at_furthest<NCB, 32>(row) : 0;
+            if (lane == 0) {
+                span_sh[wave] = make_int3(span.lo0, span.hi1, span.pre1);
+                far_sh[wave] = far;
+            }
             __syncthreads();
+            if (x.m.stacked) {
+                int64_t f = far_sh[0];
+#pragma unroll
+                for (int w = 1; w < WAVES; ++w) f = far_sh[w] > f ? far_sh[w] : f;
+                list = __builtin_amdgcn_readfirstlane((int)f);
+            }
             r = span_sh[0];
 #pragma unroll
             for (int w = 1; w < WAVES; ++w) r = make_int3(min(r.x, span_sh[w].x), max(r.y, span_sh[w].y), max(r.z, span_sh[w].z));
@@ -1014,7 +1047,7 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
             for (int r = 0; r < 16; ++r) o[c][d][r] = 0.0f;
     }
 
-    const int32_t* pages = a.pages + (int64_t)s * a.pages_stride;
+    const int32_t* pages = a.pages + (int64_t)list * a.pages_stride;
     const uint8_t* kb = (const uint8_t*)a.k + (int64_t)kh * 64 * D;
     const uint8_t* vb = (const uint8_t*)a.v + (int64_t)kh * 64 * D;
     const int64_t step = (int64_t)a.heads * 64 * D;

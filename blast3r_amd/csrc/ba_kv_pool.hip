@@ -495,7 +495,8 @@ extern "C" int ba_kv_pool_fork(const ba_kv_fork_args* args, void* stream) {
     POOL_TRY(pool_check(a.pool));
     POOL_TRY(table_check(a.from));
     POOL_TRY(table_check(a.to));
-    BA_REQUIRE(a.n >= 0 && a.n < 1 << 23, "pool: bad sizes");
+    BA_REQUIRE(a.n >= 0, "pool: bad sizes");
+    BA_REQUIRE(a.n <= 65536, "pool: too many pairs for a call");         // each is compared with all others
     BA_REQUIRE(a.to.n_pages >= a.from.n_pages, "pool: children's lists are narrower than their parents'");
     if (a.n == 0 || a.from.n_seqs == 0 || a.to.n_seqs == 0) return BA_OK;
     BA_REQUIRE(a.parents && a.children && a.from_lengths && a.to_lengths, "null pointer");

@@ -35,6 +35,21 @@ def _fixed(name):
     return property(lambda self: getattr(self, name))
 
 
+def _overlap(x, y):
+    """Whether two tables have an entry in common."""
+    if x.numel() == 0 or y.numel() == 0:
+        return False
+    if y.data_ptr() < x.data_ptr():
+        x, y = y, x
+    (rows, width), stride = x.shape, x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    off = (y.data_ptr() - x.data_ptr()) // 4
+    if off >= (rows - 1) * stride + width:
+        return False
+    if y.shape[0] > 1 and rows > 1 and y.stride(0) != stride:
+        return True                                          # rows of other lengths: not looked at more closely
+    return off % stride < width or off % stride + y.shape[1] > stride and off // stride + 1 < rows
+
+
 class BlockPool:
     """Who holds the ``n_blocks`` blocks of a cache.
 
@@ -95,9 +110,8 @@ class BlockPool:
         a.tables, a.n_tables = (BaKvTable * len(tables))(), len(tables)
         for i, t in enumerate(tables):
             self._table(a.tables[i], t)
-        at = [t.data_ptr() for t in tables if t.numel()]
-        if len(set(at)) != len(at):
-            raise ValueError('pool: a table is given twice')
+        if any(_overlap(x, y) for i, x in enumerate(tables) for y in tables[:i]):
+            raise ValueError('pool: tables overlap')
 
     def count(self, *tables):
         """Set the counts from tables: those of all lists that are in use.  For lists that were made or changed by hand, or
@@ -150,7 +164,7 @@ class BlockPool:
         a.parents, a.children, a.n = self._ints(parents, 'parents'), self._ints(children, 'children', parents.shape[0]), parents.shape[0]
         if wide < width:
             raise ValueError("pool: children's lists must be as wide as their parents'")
-        if to is not pages and to.numel() and pages.numel() and to.data_ptr() == pages.data_ptr() and to.stride() != pages.stride():
+        if to is not pages and (to.data_ptr() != pages.data_ptr() or to.stride() != pages.stride()) and _overlap(to, pages):
             raise ValueError('pool: the tables overlap')
         if a.n:
             self._launch(self._lib.ba_kv_pool_fork, a, to, to_lengths)

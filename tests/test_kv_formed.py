@@ -68,7 +68,8 @@ def test_formed_entry_point_refuses_bad_arguments_without_a_gpu():
     assert L.ba_kv_attend_scored(ctypes.byref(_lib.BaKvScoredArgs(**{**good, 'n_rows': 0})), None) == 0
     for kw in (dict(), dict(shared=2), dict(shared=1, window=5), dict(n_rows=0), dict(n_seqs=0, shared=1), dict(max_rows=0), dict(n_pages=0),
                dict(n_seqs=64, n_rows=64, rows_per_seq=1, max_rows=1, n_pages=300, shared=256), dict(n_rows=9000, max_rows=9000, n_pages=900, dim=256),
-               dict(n_rows=9000, max_rows=9000, n_pages=900, since=p), dict(n_rows=(1 << 31) - 1, max_rows=(1 << 31) - 1, n_pages=(1 << 24) - 1)):
+               dict(n_rows=9000, max_rows=9000, n_pages=900, since=p), dict(n_seqs=(1 << 31) - 1, heads=65536, q_heads=65536, n_rows=(1 << 31) - 1, max_rows=(1 << 31) - 1),
+               dict(n_rows=(1 << 31) - 1, max_rows=(1 << 31) - 1, n_pages=(1 << 24) - 1)):
         a = _lib.BaKvScoredArgs(**{**good, **kw})
         L.ba_kv_scored_plan(a)
         assert 1 <= a.n_splits <= 64 or a.max_rows == 1 and a.n_splits <= 384
@@ -317,6 +318,22 @@ def test_shared_blocks_against_oracle(bits, dim, heads, group, shared, lens, cou
         a = _run(c, o, q, pages, lens, counts, shared=shared, uniform=uniform, **kw)
         assert torch.equal(a, _run(c, o, q, pages, lens, counts, shared=shared, uniform=uniform, **kw))
     c._lib = real
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('counts', [[1] * 5, [40] * 5, [0, 3, 0, 90, 1]])
+def test_shared_blocks_of_a_batch_with_empty_places(counts):
+    """Places of the batch without a sequence (no tokens, no blocks) among others, the first one too."""
+    rng = np.random.default_rng(sum(counts))
+    lens = [0, 700, 0, 650, 500]
+    c, o, q, pages, _ = _case(rng, 64, 2, 2, lens, counts, 'int8', {}, torch.bfloat16)
+    pages[:, :7] = pages[1, :7]
+    pages[0], pages[2] = -1, -1
+    for plan in ((2, 2, 0, 0), (1, 1, 32, 128)):
+        print(f'empty places {counts} {plan}', flush=True)
+        c._lib = Planned(7, *plan)
+        _run(c, o, q, pages, lens, counts, shared=7, uniform=len(set(counts)) == 1, max_new=max(counts))
+        _run(c, o, q, pages, lens, counts, shared=7, uniform=len(set(counts)) == 1, cap=20.0, slopes=[0.1, 0.01, 0.2, 0.0])
 
 
 @pytest.mark.gpu

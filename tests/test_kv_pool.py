@@ -68,6 +68,7 @@ def test_pool_entry_points_refuse_bad_arguments_without_a_gpu():
         refused('fork', 'null', **{name: None})
     refused('fork', 'narrower', t=table(n_pages=3))
     refused('fork', 'bad sizes', n=-1)
+    refused('fork', 'too many', n=65537)
     assert L.ba_kv_pool_fork(_lib.BaKvForkArgs(pool=pool, from_=table(), to=table()), None) == 0
     refused('compact', 'bad sizes', most=41)
     refused('compact', 'null', n=None)
@@ -122,6 +123,15 @@ def test_pool_refuses_bad_arguments(host):
                  lambda: pool.fork(wide, lens, lens, lens, into=(pages, lens)), lambda: pool.fork(pages, lens, lens, lens, into=(wide[:, :6].as_strided((2, 6), (6, 1)), _ints([0])))):
         with pytest.raises(ValueError):
             call()
+    both = torch.full((6, 12), -1, dtype=torch.int32)         # tables in one buffer
+    four = _ints([0] * 4)
+    for x, y in ((both[:4], both[2:]), (both[:4], both[3:5]), (both[:, :7], both[:, 6:]), (both[:4, 3:], both[1:3, :4]), (both, both[2:3, 5:6]),
+                 (both[2:3, 5:6], both), (both.view(12, 6), both[3:]), (both[:, 4:], both.view(-1)[8:68].view(5, 12)[:, 2:])):
+        with pytest.raises(ValueError, match='overlap'):
+            pool.compact(x, y)
+        if y.shape[1] >= x.shape[1]:
+            with pytest.raises(ValueError, match='overlap'):
+                pool.fork(x, _ints([0] * len(x)), four, four, into=(y, _ints([0] * len(y))))
     with pytest.raises(AttributeError):
         pool.counts = pages
     c = KVCache(4, 1, 64, device='cpu')
@@ -143,12 +153,17 @@ def test_tensors_that_pool_calls_write_to_count_as_changed(host):
         (lambda: pool.fork(pages, lens, lens, lens, into=(other, ends)), (pool.counts, other, ends)),
         (lambda: pool.free(pages, lens), (pool.counts, pages, lens)), (lambda: pool.trim(other, first=ends), (pool.counts, other)),
         (lambda: pool.compact(pages, other), (pool.counts, pages, other)), (lambda: c.copy(lens, lens), (c.k, c.v, c.scales)))
+    both = torch.full((6, 12), -1, dtype=torch.int32)
     everything = (pool.counts, pool.missing, pages, other, lens, ends, c.k, c.v, c.scales)
     for call, changed in calls:
         before = [t._version for t in everything]
         call()
         for t, v in zip(everything, before):
             assert t._version == v + (1 if any(t is u for u in changed) else 0)
+    for x, y in ((both[:3], both[3:]), (both[:, :6], both[:, 6:]), (both[:, 3:8], both[:5, 8:]), (both[:0], both), (both[2:3], both[3:4])):
+        pool.compact(x, y)
+        if y.shape[1] >= x.shape[1]:
+            pool.fork(x, _ints([0] * len(x)), lens, lens, into=(y, _ints([0] * len(y))))
     n = len(host)
     for call in (lambda: pool.free(pages, lens, rows=lens[:0]), lambda: pool.fork(pages, lens, lens[:0], lens[:0]), lambda: c.copy(lens[:0], lens[:0])):
         call()
