@@ -56,11 +56,12 @@ static int attend_scored(const ba_kv_scored_args& s, hipStream_t st) {
     return BA_OK;
 }
 
-// What a launch is expected to take (us), which shapes and parts are chosen by.  Tiles: a CU holds `fit` workgroups at a time
-// and takes its share of all of them in turns of so many; a workgroup's time is its blocks' and that of SC_START more to begin
-// and end with, and a block's (us, by how many workgroups share the CU) what calls of 2 x 2048 rows over 16384 tokens, of 6144
-// over 12288 and of documents of 64 tokens took.  Few rows: the bytes of the blocks at 4.8 TB/s, or the blocks of a wave in
-// series.  Partial sums are written and read once, with a launch of 4 us.
+// What a launch is expected to take (us), which shapes and parts are chosen by.  A CU holds `fit` workgroups at a time and takes
+// its share of all of them in turns of so many; a workgroup's time is its blocks' and that of SC_START more to begin and end
+// with, and a block's (us, by how many workgroups share the CU) what calls of 2 x 2048 rows over 16384 tokens, of 6144 over
+// 12288, of documents of 64 tokens and of 64 to 512 rows over 4096 to 32000 took.  Rows of one tile of 16 or 32 are bound by
+// memory: the bytes of the blocks at 4.8 TB/s, or the blocks of a wave in series.  Partial sums add a launch, and their bytes
+// go through the caches.  `share`: that of the bound on blocks that tiles see on the average, where each CU has several.
 #define SC_START 5
 
 struct Guess {
@@ -69,26 +70,31 @@ struct Guess {
     double us;
 };
 
-static double launch_us(const AtShape& v, int dim, double base, int64_t blocks, int parts) {
-    const int64_t per = (blocks + parts - 1) / parts;
-    if (!v.ncb) {
-        const double bytes = base * blocks * 128.0 * dim / 4.8e6, chain = (double)((per + 3) / 4);
-        return 6.0 + (bytes > chain ? bytes : chain);
-    }
-    static const double small[5][3] = {{0.6, 0.5, 0.43}, {1.0, 0.66, 0.6}, {1.2, 0.93, 0.0}, {1.36, 1.09, 0.0}, {2.45, 0.0, 0.0}};
-    static const double large[4][2] = {{1.4, 0.94}, {1.6, 1.13}, {1.78, 0.0}, {2.03, 0.0}};
+static double launch_us(const AtShape& v, int dim, double base, int64_t blocks, int parts, double share) {
+    const double per = (double)((blocks + parts - 1) / parts);
+    static const double rows32[5][2] = {{0.4, 0.2}, {0.5, 0.28}, {0.65, 0.35}, {0.75, 0.41}, {1.5, 0.0}};
+    static const double rows128[5][3] = {{0.7, 0.5, 0.43}, {1.2, 0.66, 0.6}, {1.5, 0.93, 0.0}, {1.7, 1.09, 0.0}, {2.45, 0.0, 0.0}};
+    static const double rows256[4][2] = {{1.4, 0.94}, {1.6, 1.13}, {1.78, 0.0}, {2.03, 0.0}};
     const int d = dim <= 96 ? dim / 32 - 1 : dim == 128 ? 3 : 4;
-    const double* block = v.rows == 256 ? large[d] : small[d];
+    const double* block = v.rows == 256 ? rows256[d] : v.rows == 128 ? rows128[d] : rows32[d];
     const double each = ceil(base * parts / 256.0), full = floor(each / v.fit);
     const int rest = (int)(each - full * v.fit);
-    return 4.0 + (per + SC_START) * (full * v.fit * block[v.fit - 1] + (rest ? rest * block[rest - 1] : 0.0));
+    return 4.0 + ((each >= 2.0 ? per * share : per) + (v.rows == 256 ? SC_START + 2 : SC_START)) * (full * v.fit * block[v.fit - 1] + (rest ? rest * block[rest - 1] : 0.0));
+}
+
+static double few_us(int dim, double base, int64_t blocks, int parts) {
+    const double bytes = base * blocks * 128.0 * dim / 4.8e6, chain = (double)(((blocks + parts - 1) / parts + 3) / 4);
+    return 6.0 + (bytes > chain ? bytes : chain);
 }
 
 // The best shape and number of parts for the rows of n_seqs sequences that may see `blocks` blocks each; join: time that a part
-// more of all rows costs; joined: there is a join anyway.
-static Guess guess(int64_t rows, int64_t n_seqs, int heads, int dim, int64_t blocks, double join, bool joined, bool brief) {
+// more of all rows costs; joined: there is a join anyway; brief: rows see a short part of their lists.
+static Guess guess(int64_t rows, int64_t n_seqs, int heads, int dim, int64_t blocks, double join, bool joined, bool brief, double share) {
     Guess best = {at_shape(rows, dim), 1, 0.0};
     if (blocks < 1) blocks = 1;
+    // (partial sums of large tiles end their workgroups later than the model's blocks say: 64 rows over 16000 tokens, heads of 64,
+    // 40 us in 32 parts of 128 rows, 32 in 8 of 32)
+    auto parted = [&](int p, bool large) { return p > 1 || joined ? join * p + (large ? 14.0 : 6.0) + (joined ? 0.0 : 4.0) : 0.0; };
     if (!best.v.ncb) {                                       // one and a half workgroups per CU, two parts for unequal lengths
         // (a list of less than two parts stays whole: 8 x 5 rows over 1100 tokens 10.9 us, 13.9 in two)
         const int64_t base = n_seqs * heads, most = blocks / AT_MIN_BLOCKS;
@@ -96,21 +102,22 @@ static Guess guess(int64_t rows, int64_t n_seqs, int heads, int dim, int64_t blo
         n = n < 2 && !joined ? 2 : n;
         n = n < most ? n : most;
         best.parts = (int)(n < 1 ? 1 : n);
-        best.us = launch_us(best.v, dim, (double)base, blocks, best.parts) + (best.parts > 1 || joined ? join * best.parts : 0.0) + (best.parts > 1 && !joined ? 4.0 : 0.0);
+        best.us = few_us(dim, (double)base, blocks, best.parts) + parted(best.parts, false);
         return best;
     }
     // documents are short beside their sequence: small tiles, whole (8192 tokens of documents of 50 to 2000: 164 us, 174 with
     // tiles of 256 rows, 251 in two parts)
-    if (brief) return {at_tile(128, dim), 1, launch_us(at_tile(128, dim), dim, (double)n_seqs * heads * ((rows + 127) / 128), blocks, 1)};
+    if (brief) return {at_tile(128, dim), 1, launch_us(at_tile(128, dim), dim, (double)n_seqs * heads * ((rows + 127) / 128), blocks, 1, 1.0)};
     static const int some[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 40, 48, 64};
     best.us = 1.0e30;
-    for (int tile = 128; tile <= 256; tile += 128) {
+    for (const int tile : {32, 128, 256}) {
         if (tile == 256 && (dim > 128 || rows <= 128)) break;
         const AtShape v = at_tile(tile, dim);
+        const int least = v.ncb ? SC_MIN_BLOCKS : AT_MIN_BLOCKS;
         const double base = (double)n_seqs * heads * ((rows + tile - 1) / tile);
-        for (int p : some) {
-            if (p > 1 && p * SC_MIN_BLOCKS > blocks) break;
-            const double us = launch_us(v, dim, base, blocks, p) + (p > 1 || joined ? join * p : 0.0) + (p > 1 && !joined ? 4.0 : 0.0);
+        for (const int p : some) {
+            if (p > 1 && (int64_t)p * least > blocks) break;
+            const double us = launch_us(v, dim, base, blocks, p, share) + parted(p, v.ncb != 0);
             if (us < best.us) best = {v, p, us};
         }
     }
@@ -129,18 +136,20 @@ extern "C" void ba_kv_scored_plan(ba_kv_scored_args* args) {
     if (a.n_seqs < 1 || a.heads < 1 || a.q_heads < a.heads || a.max_rows < 1 || a.n_rows < 1 || args->shared < 0 || args->shared > a.n_pages) return;
     const int group = a.q_heads / a.heads;
     const int64_t rows = a.max_rows * group, all = a.n_rows * group;
-    const double join = 8.0 * a.n_rows * a.q_heads * (a.dim + 2) / 4.5e6;
+    const double join = 8.0 * a.n_rows * a.q_heads * (a.dim + 2) / 9.0e6;        // mostly in the caches
     const bool brief = args->since != nullptr;
     int64_t blocks = a.n_pages;
     if (a.window > 0 && !args->prefix) {                     // what a tile's rows can see
         const int64_t at_once = 256 / group < a.max_rows ? 256 / group + 1 : a.max_rows, seen = (a.window + at_once + 62) / 64 + 1;
         blocks = seen < blocks ? seen : blocks;
     }
-    Guess own = guess(rows, a.n_seqs, a.heads, a.dim, blocks, join, false, brief);
+    // causal tiles of a prompt see half of what is new on the average
+    const double fresh = (double)a.max_rows / (64.0 * (blocks < 1 ? 1 : blocks)), share = a.causal ? 1.0 - 0.5 * (fresh < 1.0 ? fresh : 1.0) : 1.0;
+    Guess own = guess(rows, a.n_seqs, a.heads, a.dim, blocks, join, false, brief, share);
     if (args->shared > 0) {
-        const Guess common = guess(all, 1, a.heads, a.dim, args->shared, join, true, false);
+        const Guess common = guess(all, 1, a.heads, a.dim, args->shared, join, true, false, 1.0);
         const int64_t rest = a.n_pages - args->shared;
-        const Guess left = guess(rows, a.n_seqs, a.heads, a.dim, rest < blocks ? rest : blocks, join, true, brief);
+        const Guess left = guess(rows, a.n_seqs, a.heads, a.dim, rest < blocks ? rest : blocks, join, true, brief, 1.0);
         if (common.us + left.us + 4.0 < own.us) {
             own = left;
             args->shared_parts = common.parts;
