@@ -11,6 +11,7 @@ and, for the networks whose answers the adjustment reads:
 
   * ``blast3r_amd.rotary``     -- rotary positions of queries and keys
   * ``blast3r_amd.kv_cache``   -- an 8-bit key/value cache and attention over it
+  * ``blast3r_amd.kv_pool``    -- the cache's pages: blocks taken, shared, given back and moved
 
 All compute runs in ``libba_hip.so`` (C ABI, include/ba_hip.h), built in-tree by
 ``blast3r_amd.build``.

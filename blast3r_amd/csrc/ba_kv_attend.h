@@ -27,7 +27,7 @@
 // fp16's end; until then nothing is rescaled.  log2 and reciprocal of a value factor are the hardware's, right to the
 // last place of fp32 or so: with |lv| up to 60 a block's weights are off by 3e-6 in all, against fp16's 5e-4 of each.
 //
-// Two kernels:
+// Two kernels (figures of the plain form; what the other forms add and take is in ba_kv_scored.hip):
 //   k_kv_attend       up to 32 rows: the waves of a workgroup have the same rows and split the blocks, codes go
 //                     from memory to registers without LDS, and the waves' sums are joined at the end.  Bound by
 //                     memory: a query over 192000 tokens of 16 heads of 64 (393 MB) takes 70 to 74 us, 5.3 to 5.6 TB/s;

@@ -14,7 +14,9 @@
 //
 // All but copy are a few thousand integers: their time is launches and dependent loads (lengths, lists, counts).  grow and
 // the plan of compact run in one workgroup, where a barrier takes the place of a launch; bits in the place of counts make
-// what it has to look through short (a million blocks are 128 KB).
+// what it has to look through short (a million blocks are 128 KB).  For 64 to 128 sequences and 5000 blocks: count 4 us, fork
+// 5.5, trim 3, grow 6 (9.5 where 120 open blocks are exchanged), the plan of 870 moves 18 and the lists 4.  copy is bound by
+// memory: 870 blocks of 131 KB (228 MB read and written) 42 us, 5.4 TB/s, as a large copy.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -131,7 +131,8 @@ class BlockPool:
         that there are no blocks left for keep -1 there, an exchanged block's place among them, and rows appended there are
         left out; ``missing`` says how many there were."""
         a = self._args(BaKvGrowArgs)
-        S, width = self._table(a.table, pages)
+        self._table(a.table, pages)
+        S, width = a.table.n_seqs, a.table.n_pages
         a.lengths = self._ints(lengths, 'lengths', S)
         if isinstance(new, torch.Tensor):
             a.more = self._ints(new, 'new', S)

@@ -323,6 +323,46 @@ def test_all_sequences_reordered_into_another_table():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('n_blocks', [100, 16384, 16385, 50000])
+def test_lists_of_several_tables_counted_and_moved(n_blocks):
+    """Two tables, one of them a part of a wider one, of more and fewer blocks than one workgroup counts; entries that are no
+    block's; on another stream than the tensors were made on, and under inference mode."""
+    from blast3r_amd.kv_pool import BlockPool
+    rng = np.random.default_rng(n_blocks)
+    pool, o = BlockPool(n_blocks, device=DEV), otok.Pool(n_blocks)
+    one, two = rng.integers(-3, n_blocks + 3, (7, 9)), rng.integers(n_blocks // 2, n_blocks, (40, 33))
+    one[0, 0], one[1, 1] = (1 << 31) - 1, -(1 << 31)
+    a, wide = _i32(one), torch.full((40, 70), 7, dtype=torch.int32, device=DEV)
+    b = wide[:, 30:63]
+    b.copy_(_i32(two))
+    print(f'tables {n_blocks}', flush=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.inference_mode():
+        pool.count(a)
+    torch.cuda.synchronize()
+    o.count(one)
+    assert pool.counts.tolist() == o.counts
+    pool.count(a, b)
+    o.count(one, two)
+    assert pool.counts.tolist() == o.counts
+    for most in (5, None):
+        moves = o.compact([one, two], n_blocks // 2 if most is None else most)
+        src, dst, n = pool.compact(a, b, most=most)
+        assert int(n) == len(moves) and list(zip(src[:len(moves)].tolist(), dst[:len(moves)].tolist())) == moves
+        assert bool((src[len(moves):] == -1).all()) and bool((dst[len(moves):] == -1).all())
+        assert pool.counts.tolist() == o.counts and a.tolist() == one.tolist() and b.tolist() == two.tolist()
+    assert bool((wide[:, :30] == 7).all()) and bool((wide[:, 63:] == 7).all())
+    src, dst, n = pool.compact(a, b)
+    assert int(n) == 0
+    used = sum(x > 0 for x in o.counts)
+    pages, lens = torch.full((3, 4), -1, dtype=torch.int32, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV)
+    pool.grow(pages, lens, 65)                               # what was free is at the end now
+    free = n_blocks - used
+    assert pages.flatten().tolist() == [used + 2 * (i // 4) + i % 4 if i % 4 < 2 and 2 * (i // 4) + i % 4 < free else -1 for i in range(12)]
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('heads,dim,bits', [(1, 32, 'int8'), (5, 96, 'fp8'), (16, 64, 'int8'), (3, 256, 'fp8'), (8, 128, 'int8')])
 def test_copy(heads, dim, bits):
     c, _ = _cache(20, heads, dim, bits)
