@@ -15,7 +15,7 @@
 // All but copy are a few thousand integers: their time is launches and dependent loads (lengths, lists, counts).  grow and
 // the plan of compact run in one workgroup, where a barrier takes the place of a launch; bits in the place of counts make
 // what it has to look through short (a million blocks are 128 KB).  For 64 to 128 sequences and 5000 blocks: count 4 us, fork
-// 5.5, trim 3, grow 6 (9.5 where 120 open blocks are exchanged), the plan of 870 moves 18 and the lists 4.  copy is bound by
+// 5.5, trim 3, grow 6 (9 where 120 open blocks are exchanged), the plan of 870 moves 6 and the lists 3.  copy is bound by
 // memory: 870 blocks of 131 KB (228 MB read and written) 42 us, 5.4 TB/s, as a large copy.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -244,18 +244,24 @@ __global__ void __launch_bounds__(PL_ONE) k_pool_grow(ba_kv_grow_args a, int shi
         return r;
     };
     // open blocks that other lists hold too: marked with the last sequence that is to write there, and given back by all
+    auto shared = [&](int s) {                               // the one of a sequence, or -1 (before any is given back)
+        const int32_t open = seq(s).open;
+        return open >= 0 && fresh(p.counts + open) > 1 ? open : -1;
+    };
+    const int32_t first = shared(tid);                       // of the first PL_ONE sequences it is not looked up again
     int any = 0;
     for (int s = tid; s < a.table.n_seqs; s += PL_ONE) {
-        const Seq r = seq(s);
-        if (r.open < 0 || fresh(p.counts + r.open) < 2) continue;
-        atomicMax(p.marks + r.open, s);
+        const int32_t open = s == tid ? first : shared(s);
+        if (open < 0) continue;
+        atomicMax(p.marks + open, s);
         any = 1;
     }
     any = __syncthreads_or(any);
     if (any) {
-        for (int s = tid; s < a.table.n_seqs; s += PL_ONE) {
-            const Seq r = seq(s);
-            if (r.open >= 0 && fresh(p.marks + r.open) >= 0) atomicSub(p.counts + r.open, 1);
+        if (first >= 0) atomicSub(p.counts + first, 1);
+        for (int s = tid + PL_ONE; s < a.table.n_seqs; s += PL_ONE) {
+            const int32_t open = seq(s).open;
+            if (open >= 0 && fresh(p.marks + open) >= 0) atomicSub(p.counts + open, 1);
         }
     }
     const int free = pool_free(p, list, most, red, words_sh, &found_sh);
@@ -357,10 +363,13 @@ __global__ void __launch_bounds__(PL_ONE) k_pool_plan(ba_kv_compact_args c) {
         pool_words<true>(p, total, red, words_sh, [&](int w, uint32_t used, int before) {
             const int64_t block = (int64_t)w * 32 + bit;
             const uint32_t below = (1u << bit) - 1u;
-            if (block >= p.n_blocks) return;
-            const bool full = used >> bit & 1u;
+            const bool full = used >> bit & 1u, there = block < p.n_blocks;
             const int at = full ? total - 1 - before - __popc(used & below) : w * 32 - before + __popc(~used & below);
-            if (at < pairs) (full ? src : dst)[at] = (int32_t)block;
+            const bool moves = there && at < pairs;
+            if (moves) (full ? src : dst)[at] = (int32_t)block;
+            // the word afterwards (one store; an atomic for each of its blocks took as long as all else)
+            const unsigned long long now = __ballot(!there || full != moves);
+            if (bit == 0) p.used[w] = (uint32_t)(tid & 32 ? now >> 32 : now);
         });
     __syncthreads();
     for (int k = tid; k < most; k += PL_ONE) {
@@ -374,8 +383,6 @@ __global__ void __launch_bounds__(PL_ONE) k_pool_plan(ba_kv_compact_args c) {
         p.counts[a] = 0;
         p.marks[a] = b;                                      // a is free now, b is not
         p.marks[b] = -1;
-        atomicOr(p.used + (b >> 5), 1u << (b & 31));
-        atomicAnd(p.used + (a >> 5), ~(1u << (a & 31)));
     }
     if (tid == 0) *c.n = pairs;
 }
