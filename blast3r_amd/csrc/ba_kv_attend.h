@@ -104,6 +104,7 @@ struct AtMore {
     int blk_lo, blk_hi;      // the blocks of the lists that it takes
     int part0, parts;        // it writes the parts [part0, part0 + parts) of the n_splits
     int least;               // blocks of a part at least
+    int mix;                 // rows of tiles (a head, a part) that each XCD has whole, 0 where it has none so, -1: tiles are alike
     int stacked;             // its rows are those of all sequences, and a workgroup's list is that of its row that sees furthest
 };
 
@@ -165,11 +166,31 @@ struct AtPlace {
     int tile, sp, kh, s;
 };
 
+// Later rows see more (their tiles come first below), and workgroups of one CU should see as much together as those of another:
+// tiles of all heads that an XCD has go by their length, and every other 32 of them, which its CUs take in turn, from the
+// shortest (6144 rows of frames over 12288 tokens, 16 heads of 64: 312 -> 289 us; prompts of 2048 for 4 sequences into an empty
+// cache, 32 heads on 8: 149 -> 131; 8 of 768 after as many 126 -> 115).  Tiles that are alike, and few rows, are better off in
+// their own order, where those of one head read the same blocks at the same time (391 against 400, 80 against 94).
+__device__ __forceinline__ unsigned at_turn(int mix, int n_tiles) {
+    const unsigned nb = gridDim.x, x = blockIdx.x % BA_N_XCD, q = nb / BA_N_XCD, r = nb % BA_N_XCD;
+    const unsigned n = q + (x < r ? 1u : 0u), first = x * q + (x < r ? x : r);
+    unsigned k = blockIdx.x / BA_N_XCD;
+    if ((k & 32u) && (k | 31u) < n) k ^= 31u;
+    if (mix > 1) {
+        const unsigned rank = k / (unsigned)mix;
+        k = (k - rank * (unsigned)mix) * (unsigned)n_tiles + rank;
+    }
+    return first + k;
+}
+
 template <int MODE>
 __device__ __forceinline__ AtPlace at_place(const AtArgs<MODE>& x, int rows, int n_tiles, int packed) {
     const ba_kv_attend_args& a = x.a;
     unsigned id = xcd_block(blockIdx.x, gridDim.x), parts = (unsigned)a.n_splits;
-    if constexpr (MODE != AT_PLAIN) parts = (unsigned)x.m.parts;
+    if constexpr (MODE != AT_PLAIN) {
+        parts = (unsigned)x.m.parts;
+        if (x.m.mix >= 0) id = at_turn(x.m.mix, n_tiles);
+    }
     AtPlace r;
     r.tile = (int)(id % (unsigned)n_tiles);
     id /= (unsigned)n_tiles;

@@ -55,10 +55,12 @@ static int attend_scored(const ba_kv_scored_args& s, hipStream_t st) {
     if (rc == BA_OK && s.shared) rc = attend_grid(a, all, 1, s.shared_parts, w, h);
     if (rc == BA_OK) rc = attend_join(a, j);
     if (rc != BA_OK) return rc;
+    const unsigned at_once = BA_N_XCD * (unsigned)g.tiles;
+    const int mix = !v.ncb || !(a.causal || s.until) ? -1 : g.nb % at_once == 0 ? (int)(g.nb / at_once) : 0;
     const int wide = attend_wide(a);
-    if (s.shared) rc = launch_formed(a, {s.slopes, s.prefix, s.since, s.until, s.cap, 0, s.shared, 0, s.shared_parts, least(w), 1}, w, h, wide, st);
+    if (s.shared) rc = launch_formed(a, {s.slopes, s.prefix, s.since, s.until, s.cap, 0, s.shared, 0, s.shared_parts, least(w), -1, 1}, w, h, wide, st);
     if (rc != BA_OK) return rc;
-    const AtMore m = {s.slopes, s.prefix, s.since, s.until, s.cap, s.shared, a.n_pages, s.shared_parts, s.a.n_splits, least(v), 0};
+    const AtMore m = {s.slopes, s.prefix, s.since, s.until, s.cap, s.shared, a.n_pages, s.shared_parts, s.a.n_splits, least(v), mix, 0};
     rc = launch_formed(a, m, v, g, wide, st);
     if (rc != BA_OK || a.n_splits == 1) return rc;
     hipLaunchKernelGGL(k_kv_join<AT_ANY>, dim3(j.nb), dim3(AT_T), 0, st, AtArgs<AT_ANY>{a, m}, v.rows, j.lanes, wide);
