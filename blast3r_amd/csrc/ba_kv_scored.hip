@@ -56,7 +56,9 @@ static int attend_scored(const ba_kv_scored_args& s, hipStream_t st) {
     if (rc == BA_OK) rc = attend_join(a, j);
     if (rc != BA_OK) return rc;
     const unsigned at_once = BA_N_XCD * (unsigned)g.tiles;
-    const int mix = !v.ncb || !(a.causal || s.until) ? -1 : g.nb % at_once == 0 ? (int)(g.nb / at_once) : 0;
+    // unequal: what a tile sees grows with its place by a quarter of the longest's at least (2048 rows over 16384 tokens 1219 us, 1236 dealt out)
+    const bool unequal = v.ncb && ((a.causal && !s.since) || s.until) && 4 * a.max_rows >= 64 * (int64_t)a.n_pages;
+    const int mix = !unequal ? -1 : g.nb % at_once == 0 ? (int)(g.nb / at_once) : 0;
     const int wide = attend_wide(a);
     if (s.shared) rc = launch_formed(a, {s.slopes, s.prefix, s.since, s.until, s.cap, 0, s.shared, 0, s.shared_parts, least(w), -1, 1}, w, h, wide, st);
     if (rc != BA_OK) return rc;
