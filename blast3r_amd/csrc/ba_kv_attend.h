@@ -94,6 +94,16 @@ enum { AT_PLAIN = 0, AT_MASKS = 1, AT_SLOPES = 2, AT_CAPPED = 3, AT_BOTH = 4, AT
 constexpr bool at_slopes(int mode) { return mode == AT_SLOPES || mode == AT_BOTH || mode == AT_ANY; }
 constexpr bool at_caps(int mode) { return mode == AT_CAPPED || mode == AT_BOTH || mode == AT_ANY; }
 
+// what differs between the workgroups of a launch that is not plain
+struct AtPart {
+    int blk_lo, blk_hi;      // the blocks of the lists that they take
+    int part0, parts;        // they write the parts [part0, part0 + parts) of the n_splits
+    int least;               // blocks of a part at least
+    int stacked;             // their rows are those of all sequences, and a workgroup's list is that of its row that sees furthest
+    int tiles, packed;       // their grid (AtGrid), and
+    unsigned first, wgs;     // which of the launch's they are
+};
+
 // of a launch that is not plain
 struct AtMore {
     const float* slopes;     // of the query heads, or NULL
@@ -101,11 +111,8 @@ struct AtMore {
     const int32_t* since;    // of the rows, or NULL
     const int32_t* until;
     float cap;
-    int blk_lo, blk_hi;      // the blocks of the lists that it takes
-    int part0, parts;        // it writes the parts [part0, part0 + parts) of the n_splits
-    int least;               // blocks of a part at least
     int mix;                 // rows of tiles (a head, a part) that each XCD has whole, 0 where it has none so, -1: tiles are alike
-    int stacked;             // its rows are those of all sequences, and a workgroup's list is that of its row that sees furthest
+    AtPart p;
 };
 
 template <int MODE> struct AtArgs {
@@ -115,6 +122,30 @@ template <int MODE> struct AtArgs {
 template <> struct AtArgs<AT_PLAIN> {
     ba_kv_attend_args a;
 };
+// Few rows: shared blocks and the sequences' own are one launch, whose later workgroups (`after`) run beside the others where
+// these leave the CUs room (64 tokens over 16384 shared and up to 512 of their own 60 -> 52 us, 16 over 8192 and 1000 39 -> 26).
+template <> struct AtArgs<AT_ANY> {
+    ba_kv_attend_args a;
+    AtMore m;
+    AtPart after;
+};
+
+// the arguments of this workgroup
+template <int MODE>
+__device__ __forceinline__ decltype(auto) at_args(const AtArgs<MODE>& x) {
+    if constexpr (MODE == AT_ANY) {
+        // each field chosen by itself: of a copied struct the compiler chooses addresses, and loads wait for loads (0.4 us a call)
+        const AtPart &l = x.m.p, &r = x.after;
+        const bool after = blockIdx.x >= l.wgs;
+        AtArgs<MODE> y = x;
+        y.m.p = {after ? r.blk_lo : l.blk_lo, after ? r.blk_hi : l.blk_hi, after ? r.part0 : l.part0, after ? r.parts : l.parts,
+                 after ? r.least : l.least, after ? r.stacked : l.stacked, after ? r.tiles : l.tiles, after ? r.packed : l.packed,
+                 after ? r.first : l.first, after ? r.wgs : l.wgs};
+        return y;
+    } else {
+        return (x);
+    }
+}
 
 // 8 codes to fp16
 template <int KT>
@@ -187,8 +218,13 @@ template <int MODE>
 __device__ __forceinline__ AtPlace at_place(const AtArgs<MODE>& x, int rows, int n_tiles, int packed) {
     const ba_kv_attend_args& a = x.a;
     unsigned id = xcd_block(blockIdx.x, gridDim.x), parts = (unsigned)a.n_splits;
-    if constexpr (MODE != AT_PLAIN) {
-        parts = (unsigned)x.m.parts;
+    if constexpr (MODE == AT_ANY) {
+        n_tiles = x.m.p.tiles;
+        packed = x.m.p.packed;
+        id = xcd_block(blockIdx.x - x.m.p.first, x.m.p.wgs);
+        parts = (unsigned)x.m.p.parts;
+    } else if constexpr (MODE != AT_PLAIN) {
+        parts = (unsigned)x.m.p.parts;
         if (x.m.mix >= 0) id = at_turn(x.m.mix, n_tiles);
     }
     AtPlace r;
@@ -253,7 +289,7 @@ template <int MODE>
 __device__ __forceinline__ AtRow at_row(const AtArgs<MODE>& x, AtSeq q, int s, int64_t i) {
     const ba_kv_attend_args& a = x.a;
     const int64_t row = q.row0 + i;
-    if (x.m.stacked) {
+    if (x.m.p.stacked) {
         s = seq_of_row(a, row);
         q = at_seq(a, s);
         i = row - q.row0;
@@ -350,7 +386,7 @@ struct AtWalk {
     __device__ __forceinline__ int block(int v) const { return v < na ? a0 + v : c0 + (v - na); }
 };
 
-__device__ __forceinline__ AtWalk at_walk(const AtMore& m, int lo, int hi, int pre) {
+__device__ __forceinline__ AtWalk at_walk(const AtPart& m, int lo, int hi, int pre) {
     AtWalk w;
     w.a0 = m.blk_lo;
     const int a1 = min((int)(((int64_t)pre + 63) / 64), m.blk_hi), c1 = min((int)(((int64_t)hi + 63) / 64), m.blk_hi);
@@ -364,11 +400,11 @@ __device__ __forceinline__ AtWalk at_walk(const AtMore& m, int lo, int hi, int p
 template <int MODE>
 __device__ __forceinline__ AtSeq at_rows(const AtArgs<MODE>& x, int s) {
     if constexpr (MODE != AT_PLAIN)
-        if (x.m.stacked) return {0, 0, 0, (int)x.a.n_rows};
+        if (x.m.p.stacked) return {0, 0, 0, (int)x.a.n_rows};
     return at_seq(x.a, s);
 }
 
-__device__ __forceinline__ AtBlocks at_cut(const AtWalk& w, const AtMore& m) {
+__device__ __forceinline__ AtBlocks at_cut(const AtWalk& w, const AtPart& m) {
     const int per = (w.n + m.parts - 1) / m.parts;
     return {0, w.n, per < m.least ? m.least : per};
 }
@@ -520,7 +556,7 @@ __device__ __forceinline__ void store_rows(const AtArgs<MODE>& x, const AtSeq& q
     constexpr int CREG = COLS * COLS / 64, DB = D / COLS;
     typedef Mma<COLS> M;
     const ba_kv_attend_args& a = x.a;
-    if constexpr (MODE != AT_PLAIN) sp += x.m.part0;
+    if constexpr (MODE != AT_PLAIN) sp += x.m.p.part0;
 #pragma unroll
     for (int c = 0; c < NCB; ++c) {
         const int r = row0 + c * COLS + n;
@@ -577,7 +613,8 @@ constexpr int at_waves(int d, int cols) { return cols == 16 ? (d <= 64 ? 4 : d <
 // blocks; every wave reads and converts its own, a block ahead.  8 or 16 waves to a workgroup were no faster on short
 // sequences (777 tokens: 8.4 and 9.4 us against 8.5, most of it launch and dependent loads).
 template <int MODE, int D, int KT, int COLS, bool HALF>
-__global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(AtArgs<MODE> x, int n_tiles, int packed, int wide) {
+__global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(AtArgs<MODE> args, int n_tiles, int packed, int wide) {
+    const auto& x = at_args(args);
     const ba_kv_attend_args& a = x.a;
     typedef Mma<COLS> M;
     typedef typename M::acc acc;
@@ -611,16 +648,16 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(AtArgs<MO
         at_part(at_blocks(a, q, group, tile0, ROWS), sp, lo, hi);
         if (lo >= hi && a.n_splits > 1) return;              // k_kv_join knows which parts there are
     } else {
-        if (x.m.since || x.m.until || x.m.stacked) {
+        if (x.m.since || x.m.until || x.m.p.stacked) {
             find_rows();
             span = at_span<NCB, COLS>(row);
-            if (x.m.stacked) list = __builtin_amdgcn_readfirstlane((int)at_furthest<NCB, COLS>(row));
+            if (x.m.p.stacked) list = __builtin_amdgcn_readfirstlane((int)at_furthest<NCB, COLS>(row));
         } else {
             const int end = tile0 + ROWS < all ? tile0 + ROWS : all;
             span = at_span_of(x, q, s, (int)((unsigned)tile0 / (unsigned)group), (int)((unsigned)(end - 1) / (unsigned)group));
         }
-        walk = at_walk(x.m, span.lo0, span.hi1, span.pre1);
-        at_part(at_cut(walk, x.m), sp, lo, hi);
+        walk = at_walk(x.m.p, span.lo0, span.hi1, span.pre1);
+        at_part(at_cut(walk, x.m.p), sp, lo, hi);
     }
     const bool none = lo >= hi;
     if (a.n_blocks == 0) hi = lo;
@@ -687,7 +724,7 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(AtArgs<MO
     int pos[NCB];
     load_queries<D, COLS, NCB>(a, q, kh, group, tile0, all, n, g, wide != 0, qf, qc, pos);
     if constexpr (MODE != AT_PLAIN)                          // while the block is under way, where its number did not need them
-        if (!(x.m.since || x.m.until || x.m.stacked)) find_rows();
+        if (!(x.m.since || x.m.until || x.m.p.stacked)) find_rows();
     float slope[NCB];
     int anchor[NCB];
     if constexpr (at_slopes(MODE)) load_slopes<MODE, COLS, NCB>(x, kh, group, tile0, all, n, row, slope, anchor);
@@ -996,18 +1033,18 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
     } else {
         int3* span_sh = (int3*)k_sh[1];                      // free until the first block has been converted by all
         int64_t* far_sh = (int64_t*)k_sh[1] + 16;
-        if (x.m.since || x.m.until || x.m.stacked) find_rows();
+        if (x.m.since || x.m.until || x.m.p.stacked) find_rows();
         fetch_queries<D, 32, NCB>(a, q, kh, group, row0, all, n, g, wide != 0, raw);
         int3 r;                                              // of all waves
-        if (x.m.since || x.m.until || x.m.stacked) {
+        if (x.m.since || x.m.until || x.m.p.stacked) {
             span = at_span<NCB, 32>(row);
-            const int64_t far = x.m.stacked ? at_furthest<NCB, 32>(row) : 0;
+            const int64_t far = x.m.p.stacked ? at_furthest<NCB, 32>(row) : 0;
             if (lane == 0) {
                 span_sh[wave] = make_int3(span.lo0, span.hi1, span.pre1);
                 far_sh[wave] = far;
             }
             __syncthreads();
-            if (x.m.stacked) {
+            if (x.m.p.stacked) {
                 int64_t f = far_sh[0];
 #pragma unroll
                 for (int w = 1; w < WAVES; ++w) f = far_sh[w] > f ? far_sh[w] : f;
@@ -1026,10 +1063,10 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
             const AtSpan w = of(tile0, ROWS);
             r = make_int3(w.lo0, w.hi1, w.pre1);
         }
-        walk = at_walk(x.m, r.x, r.y, r.z);
+        walk = at_walk(x.m.p, r.x, r.y, r.z);
         seen_end = max(r.y, r.z);
-        if (!(x.m.since || x.m.until || x.m.stacked)) find_rows();
-        at_part(at_cut(walk, x.m), sp, lo, hi);
+        if (!(x.m.since || x.m.until || x.m.p.stacked)) find_rows();
+        at_part(at_cut(walk, x.m.p), sp, lo, hi);
     }
     const bool none = lo >= hi;
     if (a.n_blocks == 0) hi = lo;

@@ -8,8 +8,8 @@
 // blocks that any of its rows sees (AtWalk): a window behind a prefix, or a document in a long prompt, costs its own blocks.
 //
 // shared: the first so many blocks of all lists that have tokens there are the same.  One launch takes the rows of all sequences
-// over these blocks as if they were one sequence's (AtMore.stacked), another each sequence's own blocks, and both leave partial
-// sums for one join: the shared tokens are read, and converted, once for up to 256 rows instead of once for each sequence.
+// over these blocks as if they were one sequence's (AtPart.stacked), another, or the rest of the same, each sequence's own
+// blocks, and both leave partial sums for one join: the shared tokens are read, and converted, once for up to 256 rows instead of once for each sequence.
 //
 // Measured (heads of 128 int8, 32 on 8, unless said otherwise):
 //   memory   48 sequences of up to 8192 tokens, a token each, slopes: 91 us (4.6 TB/s) + join 5, as without slopes; 16 of 65000
@@ -37,9 +37,13 @@ AT_ELSEWHERE(launch_tiles, AT_BOTH)
 #undef AT_ELSEWHERE
 
 static int launch_formed(const ba_kv_attend_args& a, const AtMore& m, const AtShape& v, const AtGrid& g, int wide, hipStream_t st) {
-    if (!v.ncb) return launch_few(AtArgs<AT_ANY>{a, m}, v, g, wide, st);
+    if (!v.ncb) return launch_few(AtArgs<AT_ANY>{a, m, {}}, v, g, wide, st);
     if (m.cap != 0.0f) return m.slopes ? launch_tiles(AtArgs<AT_BOTH>{a, m}, v, g, wide, st) : launch_tiles(AtArgs<AT_CAPPED>{a, m}, v, g, wide, st);
     return m.slopes ? launch_tiles(AtArgs<AT_SLOPES>{a, m}, v, g, wide, st) : launch_tiles(AtArgs<AT_MASKS>{a, m}, v, g, wide, st);
+}
+
+static bool joint_shape(const AtShape& own, const AtShape& common, double wgs) {
+    return !own.ncb && !common.ncb && (own.rows >= common.rows || wgs <= 1024.0);
 }
 
 static int attend_scored(const ba_kv_scored_args& s, hipStream_t st) {
@@ -47,7 +51,11 @@ static int attend_scored(const ba_kv_scored_args& s, hipStream_t st) {
     a.n_splits = s.a.n_splits + s.shared_parts;
     const int group = a.q_heads / a.heads;
     const int64_t rows = a.max_rows * group, all = a.n_rows * group;
-    const AtShape v = s.tile ? at_tile(s.tile, a.dim) : at_shape(rows, a.dim), w = s.shared_tile ? at_tile(s.shared_tile, a.dim) : at_shape(all, a.dim);
+    AtShape v = s.tile ? at_tile(s.tile, a.dim) : at_shape(rows, a.dim), w = s.shared_tile ? at_tile(s.shared_tile, a.dim) : at_shape(all, a.dim);
+    // both in one launch, where that takes the sequences' own no larger tile or they are few (2048 workgroups of tokens over 164
+    // tokens in tiles of 16 rows: 50 us, 63 in tiles of 32)
+    const bool joint = s.shared && joint_shape(v, w, (double)a.n_seqs * a.heads);
+    if (joint) v = w = v.rows > w.rows ? v : w;
     auto least = [](const AtShape& x) { return x.ncb ? SC_MIN_BLOCKS : AT_MIN_BLOCKS; };
     AtGrid g, h;
     AtJoin j;
@@ -55,17 +63,26 @@ static int attend_scored(const ba_kv_scored_args& s, hipStream_t st) {
     if (rc == BA_OK && s.shared) rc = attend_grid(a, all, 1, s.shared_parts, w, h);
     if (rc == BA_OK) rc = attend_join(a, j);
     if (rc != BA_OK) return rc;
+    BA_REQUIRE(!joint || g.nb < (1u << 23) - h.nb, "attention: too many tiles for a call");
     const unsigned at_once = BA_N_XCD * (unsigned)g.tiles;
     // unequal: what a tile sees grows with its place by a quarter of the longest's at least (2048 rows over 16384 tokens 1219 us, 1236 dealt out)
     const bool unequal = v.ncb && ((a.causal && !s.since) || s.until) && 4 * a.max_rows >= 64 * (int64_t)a.n_pages;
     const int mix = !unequal ? -1 : g.nb % at_once == 0 ? (int)(g.nb / at_once) : 0;
     const int wide = attend_wide(a);
-    if (s.shared) rc = launch_formed(a, {s.slopes, s.prefix, s.since, s.until, s.cap, 0, s.shared, 0, s.shared_parts, least(w), -1, 1}, w, h, wide, st);
-    if (rc != BA_OK) return rc;
-    const AtMore m = {s.slopes, s.prefix, s.since, s.until, s.cap, s.shared, a.n_pages, s.shared_parts, s.a.n_splits, least(v), mix, 0};
-    rc = launch_formed(a, m, v, g, wide, st);
+    AtMore m = {s.slopes, s.prefix, s.since, s.until, s.cap, mix, {s.shared, a.n_pages, s.shared_parts, s.a.n_splits, least(v), 0, g.tiles, g.packed, 0, g.nb}};
+    if (s.shared) {
+        const AtMore common = {s.slopes, s.prefix, s.since, s.until, s.cap, -1, {0, s.shared, 0, s.shared_parts, least(w), 1, h.tiles, h.packed, 0, h.nb}};
+        if (joint) {
+            m.p.first = h.nb;
+            rc = launch_few(AtArgs<AT_ANY>{a, common, m.p}, v, {h.nb + g.nb, 0, 0}, wide, st);
+        } else {
+            rc = launch_formed(a, common, w, h, wide, st);
+        }
+        if (rc != BA_OK) return rc;
+    }
+    if (!joint) rc = launch_formed(a, m, v, g, wide, st);
     if (rc != BA_OK || a.n_splits == 1) return rc;
-    hipLaunchKernelGGL(k_kv_join<AT_ANY>, dim3(j.nb), dim3(AT_T), 0, st, AtArgs<AT_ANY>{a, m}, v.rows, j.lanes, wide);
+    hipLaunchKernelGGL(k_kv_join<AT_ANY>, dim3(j.nb), dim3(AT_T), 0, st, AtArgs<AT_ANY>{a, m, {}}, v.rows, j.lanes, wide);
     BA_LAUNCHED();
     return BA_OK;
 }
@@ -86,7 +103,7 @@ struct Guess {
 
 static double launch_us(const AtShape& v, int dim, double base, int64_t blocks, int parts, double share) {
     const double per = (double)((blocks + parts - 1) / parts);
-    static const double rows32[5][2] = {{0.4, 0.2}, {0.5, 0.28}, {0.65, 0.35}, {0.75, 0.41}, {1.5, 0.0}};
+    static const double rows32[5][2] = {{0.33, 0.2}, {0.42, 0.28}, {0.52, 0.35}, {0.6, 0.41}, {1.2, 0.0}};
     static const double rows128[5][3] = {{0.7, 0.5, 0.43}, {1.2, 0.66, 0.6}, {1.5, 0.93, 0.0}, {1.7, 1.09, 0.0}, {2.45, 0.0, 0.0}};
     static const double rows256[4][2] = {{1.4, 0.94}, {1.6, 1.13}, {1.78, 0.0}, {2.03, 0.0}};
     const int d = dim <= 96 ? dim / 32 - 1 : dim == 128 ? 3 : 4;
@@ -102,8 +119,15 @@ static double few_us(int dim, double base, int64_t blocks, int parts) {
 }
 
 // The best shape and number of parts for the rows of n_seqs sequences that may see `blocks` blocks each; join: time that a part
-// more of all rows costs; joined: there is a join anyway; brief: rows see a short part of their lists.
-static Guess guess(int64_t rows, int64_t n_seqs, int heads, int dim, int64_t blocks, double join, bool joined, bool brief, double share) {
+// more of all rows costs; joined: there is a join anyway; brief: rows see a short part of their lists; beside: another launch
+// of the call, which few rows take in where the CUs have room for both.
+static Guess guess(int64_t rows, int64_t n_seqs, int heads, int dim, int64_t blocks, double join, bool joined, bool brief, double share,
+                   const Guess* beside = nullptr, double beside_wgs = 0.0) {
+    auto with = [&](const AtShape& v, double wgs, double us) {
+        if (!beside) return us;
+        if (!joint_shape(beside->v, v, beside_wgs)) return us + beside->us + 4.0;
+        return us + (wgs > 256.0 * (v.fit - 1) || beside->us > us ? beside->us : 2.0);
+    };
     Guess best = {at_shape(rows, dim), 1, 0.0};
     if (blocks < 1) blocks = 1;
     // (partial sums of large tiles end their workgroups later than the model's blocks say: 64 rows over 16000 tokens, heads of 64,
@@ -116,7 +140,7 @@ static Guess guess(int64_t rows, int64_t n_seqs, int heads, int dim, int64_t blo
         n = n < 2 && !joined ? 2 : n;
         n = n < most ? n : most;
         best.parts = (int)(n < 1 ? 1 : n);
-        best.us = few_us(dim, (double)base, blocks, best.parts) + parted(best.parts, false);
+        best.us = with(best.v, (double)base * best.parts, few_us(dim, (double)base, blocks, best.parts) + parted(best.parts, false));
         return best;
     }
     // documents are short beside their sequence: small tiles, whole (8192 tokens of documents of 50 to 2000: 164 us, 174 with
@@ -131,7 +155,7 @@ static Guess guess(int64_t rows, int64_t n_seqs, int heads, int dim, int64_t blo
         const double base = (double)n_seqs * heads * ((rows + tile - 1) / tile);
         for (const int p : some) {
             if (p > 1 && (int64_t)p * least > blocks) break;
-            const double us = launch_us(v, dim, base, blocks, p, share) + parted(p, v.ncb != 0);
+            const double us = with(v, base * p, launch_us(v, dim, base, blocks, p, share) + parted(p, v.ncb != 0));
             if (us < best.us) best = {v, p, us};
         }
     }
@@ -161,10 +185,10 @@ extern "C" void ba_kv_scored_plan(ba_kv_scored_args* args) {
     const double fresh = (double)a.max_rows / (64.0 * (blocks < 1 ? 1 : blocks)), share = a.causal ? 1.0 - 0.5 * (fresh < 1.0 ? fresh : 1.0) : 1.0;
     Guess own = guess(rows, a.n_seqs, a.heads, a.dim, blocks, join, false, brief, share);
     if (args->shared > 0) {
-        const Guess common = guess(all, 1, a.heads, a.dim, args->shared, join, true, false, 1.0);
         const int64_t rest = a.n_pages - args->shared;
         const Guess left = guess(rows, a.n_seqs, a.heads, a.dim, rest < blocks ? rest : blocks, join, true, brief, 1.0);
-        if (common.us + left.us + 4.0 < own.us) {
+        const Guess common = guess(all, 1, a.heads, a.dim, args->shared, join, true, false, 1.0, &left, (double)a.n_seqs * a.heads);
+        if (common.us < own.us) {
             own = left;
             args->shared_parts = common.parts;
             args->shared_tile = common.v.rows;

@@ -319,7 +319,7 @@ def test_shared_blocks_against_oracle(bits, dim, heads, group, shared, lens, cou
     uniform = len(set(counts)) == 1
     _run(c, o, q, pages, lens, counts, shared=shared, uniform=uniform, **kw)             # as it is planned
     real = c._lib
-    for plan in ((), (1, 1, 16, 128), (2, 3, 32, 32), (3, 2, 128, 16), (1, 7, 0, 256 if dim < 256 else 128)):
+    for plan in ((), (1, 1, 16, 128), (2, 3, 32, 32), (2, 3, 16, 32), (3, 1, 32, 16), (3, 2, 128, 16), (1, 7, 0, 256 if dim < 256 else 128)):
         print(f'  plan {plan}', flush=True)
         c._lib = Planned(shared, *plan)
         a = _run(c, o, q, pages, lens, counts, shared=shared, uniform=uniform, **kw)
