@@ -9,7 +9,8 @@
 //
 // shared: the first so many blocks of all lists that have tokens there are the same.  One launch takes the rows of all sequences
 // over these blocks as if they were one sequence's (AtPart.stacked), another, or the rest of the same, each sequence's own
-// blocks, and both leave partial sums for one join: the shared tokens are read, and converted, once for up to 256 rows instead of once for each sequence.
+// blocks, and both leave partial sums for one join: the shared tokens are read, and converted, once for up to 256 rows instead
+// of once for each sequence.
 //
 // Measured (heads of 128 int8, 32 on 8, unless said otherwise):
 //   memory   48 sequences of up to 8192 tokens, a token each, slopes: 91 us (4.6 TB/s) + join 5, as without slopes; 16 of 65000
@@ -18,8 +19,8 @@
 //   units    capped (matrix unit busy 35%, vector units 64%: two more transcendentals a score), 1180 both
 //   latency  8192 tokens of documents of 50 to 2000: 160 us, where their products would take 65 (documents of 64, one block a tile:
 //            54, in four turns of two tiles a CU: that is what a tile takes to begin and end)
-//   shared   64 tokens over 16384 shared and 1 to 512 of their own: 41 + 16 + 7 us; read by each, 460
-//   16 heads of 64, e4m3: 6144 rows of frames over 12288 tokens 312 us (0.77 PFLOP/s), 4608 rows of six frames over 16128 391 us
+//   shared   64 tokens over 16384 shared and 1 to 512 of their own: 45 + 6 us (41 + 16 + 6 as two launches); read by each, 460
+//   16 heads of 64, e4m3: 6144 rows of frames over 12288 tokens 290 us (0.83 PFLOP/s), 4608 rows of six frames over 16128 391 us
 #include <math.h>
 
 #include "ba_kv_attend.h"
