@@ -542,6 +542,7 @@ extern "C" int ba_kv_pool_grow(const ba_kv_grow_args* args, void* stream) {
     int shift = 0;
     while (shift < 6 && (1 << shift) < slots) ++shift;
     const int64_t most = (slots + 1) * a.table.n_seqs;
+    BA_REQUIRE(most < (int64_t)1 << 31, "pool: too many blocks for a call");     // they are counted in 32 bits
     hipLaunchKernelGGL(k_pool_grow, dim3(1), dim3(PL_ONE), 0, (hipStream_t)stream, a, shift, (int)(most < a.pool.n_blocks ? most : a.pool.n_blocks));
     BA_LAUNCHED();
     return BA_OK;

@@ -62,6 +62,7 @@ def test_pool_entry_points_refuse_bad_arguments_without_a_gpu():
     refused('count', 'bad tables', tables=None)
     refused('compact', 'bad tables', n_tables=-1)
     refused('grow', 'bad sizes', max_new=-1)
+    refused('grow', 'too many blocks', t=table(n_seqs=1 << 20, n_pages=2047, stride=2047), max_new=1 << 30)
     for name in ('lengths', 'src', 'dst', 'n', 'missing'):
         refused('grow', 'null', **{name: None})
     for name in ('from_lengths', 'to_lengths', 'parents', 'children'):
