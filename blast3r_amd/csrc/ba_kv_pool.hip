@@ -509,6 +509,9 @@ extern "C" int ba_kv_pool_fork(const ba_kv_fork_args* args, void* stream) {
     BA_REQUIRE(a.to.n_pages >= a.from.n_pages, "pool: children's lists are narrower than their parents'");
     if (a.n == 0 || a.from.n_seqs == 0 || a.to.n_seqs == 0) return BA_OK;
     BA_REQUIRE(a.parents && a.children && a.from_lengths && a.to_lengths, "null pointer");
+    // (lengths of parents in another table are read while children's are written)
+    BA_REQUIRE((a.from.pages == a.to.pages && a.from_lengths == a.to_lengths) || a.from_lengths + a.from.n_seqs <= a.to_lengths ||
+                   a.to_lengths + a.to.n_seqs <= a.from_lengths, "pool: the children's lengths overlap the parents'");
     hipLaunchKernelGGL(k_pool_fork, dim3((unsigned)a.n), dim3(PL_T), 0, (hipStream_t)stream, a, (int)(a.from.pages == a.to.pages));
     BA_LAUNCHED();
     return BA_OK;

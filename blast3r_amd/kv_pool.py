@@ -155,7 +155,7 @@ class BlockPool:
     def fork(self, pages, lengths, parents, children, into=None):
         """Row children[i] becomes the list of row parents[i] ((n,) int32 each): it gives back the blocks that it held, holds
         its parent's blocks with tokens as well, and gets its length.  into: (pages, lengths) of the children, where they are in
-        another table (which a reordering of all sequences needs).  Pairs that name a row that is not there, whose child a
+        another table (which a reordering of all sequences needs), with lengths of its own.  Pairs that name a row that is not there, whose child a
         later pair has too, or whose child is a parent in the same table, change nothing."""
         to, to_lengths = (pages, lengths) if into is None else into
         a = self._args(BaKvForkArgs)
@@ -167,6 +167,10 @@ class BlockPool:
             raise ValueError("pool: children's lists must be as wide as their parents'")
         if to is not pages and (to.data_ptr() != pages.data_ptr() or to.stride() != pages.stride()) and _overlap(to, pages):
             raise ValueError('pool: the tables overlap')
+        # (lengths of parents in another table are read while children's are written)
+        same = to.data_ptr() == pages.data_ptr() and a.from_lengths == a.to_lengths
+        if S and T and not same and a.from_lengths < a.to_lengths + 4 * T and a.to_lengths < a.from_lengths + 4 * S:
+            raise ValueError("pool: the children's lengths overlap the parents'")
         if a.n:
             self._launch(self._lib.ba_kv_pool_fork, a, to, to_lengths)
 

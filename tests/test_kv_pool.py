@@ -70,6 +70,9 @@ def test_pool_entry_points_refuse_bad_arguments_without_a_gpu():
     refused('fork', 'narrower', t=table(n_pages=3))
     refused('fork', 'bad sizes', n=-1)
     refused('fork', 'too many', n=65537)
+    for at in (p, p + 4, p - 4):                             # lengths that are read and written, of tables of their own
+        refused('fork', 'overlap', t=table(pages=1 << 20), to_lengths=at)
+    refused('fork', 'overlap', to_lengths=p + 4)
     assert L.ba_kv_pool_fork(_lib.BaKvForkArgs(pool=pool, from_=table(), to=table()), None) == 0
     refused('compact', 'bad sizes', most=41)
     refused('compact', 'null', n=None)
@@ -133,6 +136,10 @@ def test_pool_refuses_bad_arguments(host):
         if y.shape[1] >= x.shape[1]:
             with pytest.raises(ValueError, match='overlap'):
                 pool.fork(x, _ints([0] * len(x)), four, four, into=(y, _ints([0] * len(y))))
+    other = torch.full((2, 6), -1, dtype=torch.int32)         # lengths in one buffer
+    for to, x, y in ((other, lens, lens), (other, four[:2], four[1:3]), (pages, four[1:3], four[:2])):
+        with pytest.raises(ValueError, match='lengths overlap'):
+            pool.fork(pages, x, lens, lens, into=(to, y))
     with pytest.raises(AttributeError):
         pool.counts = pages
     c = KVCache(4, 1, 64, device='cpu')
