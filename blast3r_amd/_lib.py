@@ -187,6 +187,10 @@ class BaKvCountArgs(ctypes.Structure):
     _fields_ = [('pool', BaKvPool), ('tables', ctypes.POINTER(BaKvTable)), ('n_tables', c_int), ('reserved', c_int)]
 
 
+class BaKvFreeArgs(ctypes.Structure):
+    _fields_ = [('pool', BaKvPool), ('free', c_p)]
+
+
 class BaKvForkArgs(ctypes.Structure):
     _fields_ = [('pool', BaKvPool), ('from_', BaKvTable), ('to', BaKvTable), ('from_lengths', c_p), ('to_lengths', c_p),
                 ('parents', c_p), ('children', c_p), ('n', c_int), ('reserved', c_int)]
@@ -295,6 +299,7 @@ _SIGS = {
     'ba_kv_attend_scored': (c_int, [ctypes.POINTER(BaKvScoredArgs), c_p]),
     'ba_kv_scored_plan': (None, [ctypes.POINTER(BaKvScoredArgs)]),
     'ba_kv_pool_count': (c_int, [ctypes.POINTER(BaKvCountArgs), c_p]),
+    'ba_kv_pool_free': (c_int, [ctypes.POINTER(BaKvFreeArgs), c_p]),
     'ba_kv_pool_fork': (c_int, [ctypes.POINTER(BaKvForkArgs), c_p]),
     'ba_kv_pool_trim': (c_int, [ctypes.POINTER(BaKvTrimArgs), c_p]),
     'ba_kv_pool_grow': (c_int, [ctypes.POINTER(BaKvGrowArgs), c_p]),
@@ -312,7 +317,7 @@ ABI_STRUCTS = {'ba_huber': BaHuber, 'ba_layout': BaLayout, 'ba_lin_args': BaLinA
                'ba_kv_attend_args': BaKvAttendArgs, 'ba_kv_scored_args': BaKvScoredArgs, 'ba_kv_pool': BaKvPool,
                'ba_kv_table': BaKvTable, 'ba_kv_fork_args': BaKvForkArgs, 'ba_kv_trim_args': BaKvTrimArgs,
                'ba_kv_grow_args': BaKvGrowArgs, 'ba_kv_copy_args': BaKvCopyArgs, 'ba_kv_count_args': BaKvCountArgs,
-               'ba_kv_compact_args': BaKvCompactArgs}
+               'ba_kv_compact_args': BaKvCompactArgs, 'ba_kv_free_args': BaKvFreeArgs}
 
 
 def _check_abi(L):

@@ -197,6 +197,16 @@ __device__ __forceinline__ void pool_words(const ba_kv_pool& p, int enough, int*
     }
 }
 
+__global__ void __launch_bounds__(PL_ONE) k_pool_available(ba_kv_free_args a) {
+    const ba_kv_pool& p = a.pool;
+    __shared__ int red[PL_ONE / 64];
+    const int words = (int)((p.n_blocks + 31) / 32);
+    int v = 0, total;
+    for (int w = threadIdx.x; w < words; w += PL_ONE) v += __popc(~p.used[w]);       // bits past the last block are set
+    scan_before(v, red, total);
+    if (threadIdx.x == 0) *a.free = total;
+}
+
 // The first `most` free blocks in `list`; how many there are of them.
 __device__ int pool_free(const ba_kv_pool& p, int32_t* list, int most, int* red, uint2* words_sh, int* found_sh) {
     if (threadIdx.x == 0) *found_sh = 0;
@@ -493,6 +503,16 @@ extern "C" int ba_kv_pool_count(const ba_kv_count_args* args, void* stream) {
         BA_LAUNCHED();
     }
     hipLaunchKernelGGL(k_pool_bits, dim3((nb + 31) / 32), dim3(PL_T), 0, st, p);
+    BA_LAUNCHED();
+    return BA_OK;
+}
+
+extern "C" int ba_kv_pool_free(const ba_kv_free_args* args, void* stream) {
+    clear_error();
+    BA_REQUIRE(args != nullptr, "null args");
+    POOL_TRY(pool_check(args->pool));
+    BA_REQUIRE(args->free != nullptr, "null pointer");
+    hipLaunchKernelGGL(k_pool_available, dim3(1), dim3(PL_ONE), 0, (hipStream_t)stream, *args);
     BA_LAUNCHED();
     return BA_OK;
 }

@@ -748,6 +748,7 @@ extern "C" int64_t ba_abi_sizeof(const char* name) {
     BA_SZ(ba_tangent_args); BA_SZ(ba_rotary_args); BA_SZ(ba_kv_args); BA_SZ(ba_kv_attend_args);
     BA_SZ(ba_kv_scored_args); BA_SZ(ba_kv_pool); BA_SZ(ba_kv_table); BA_SZ(ba_kv_fork_args); BA_SZ(ba_kv_trim_args);
     BA_SZ(ba_kv_grow_args); BA_SZ(ba_kv_copy_args); BA_SZ(ba_kv_count_args); BA_SZ(ba_kv_compact_args);
+    BA_SZ(ba_kv_free_args);
 #undef BA_SZ
     return -1;
 }

@@ -23,8 +23,8 @@ the open last block is shared, and ``grow`` is what gives each its own before ne
 """
 import torch
 
-from ._lib import (BaKvCompactArgs, BaKvCountArgs, BaKvForkArgs, BaKvGrowArgs, BaKvPool, BaKvTable, BaKvTrimArgs, launch, lib,
-                   written)
+from ._lib import (BaKvCompactArgs, BaKvCountArgs, BaKvForkArgs, BaKvFreeArgs, BaKvGrowArgs, BaKvPool, BaKvTable, BaKvTrimArgs,
+                   launch, lib, written)
 
 __all__ = ['BlockPool']
 
@@ -75,7 +75,11 @@ class BlockPool:
 
     def available(self):
         """(1,) int64 on the device: the free blocks."""
-        return (self._counts == 0).sum().view(1)
+        free = torch.empty(1, dtype=torch.int64, device=self._device)
+        a = self._args(BaKvFreeArgs)
+        a.free = free.data_ptr()
+        launch(self._lib.ba_kv_pool_free, a, self._device)
+        return free
 
     def _args(self, kind):
         """The arguments of a call, with the pool's own."""
@@ -83,7 +87,8 @@ class BlockPool:
         if at != self._at:
             self._at = at
             pool = BaKvPool(at, self._used.data_ptr(), self._marks.data_ptr(), self._n_blocks)
-            self._kinds = {k: k(pool=pool) for k in (BaKvCountArgs, BaKvForkArgs, BaKvTrimArgs, BaKvGrowArgs, BaKvCompactArgs)}
+            self._kinds = {k: k(pool=pool) for k in (BaKvCountArgs, BaKvFreeArgs, BaKvForkArgs, BaKvTrimArgs, BaKvGrowArgs,
+                                                     BaKvCompactArgs)}
         return kind.from_buffer_copy(self._kinds[kind])
 
     def _table(self, a, pages, name='pages'):

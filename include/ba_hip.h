@@ -779,6 +779,14 @@ typedef struct {
 
 int ba_kv_pool_count(const ba_kv_count_args* args, void* stream);
 
+/* *free (device): the blocks that no list holds. */
+typedef struct {
+    ba_kv_pool pool;
+    int64_t* free;
+} ba_kv_free_args;
+
+int ba_kv_pool_free(const ba_kv_free_args* args, void* stream);
+
 /* Row children[i] of `to` gives back what it holds and becomes the list of row parents[i] of `from`: its blocks with tokens
  * (below from_lengths), and its length.  The two arrays of lengths are one, for one table, or do not overlap.  A pair that
  * names a row out of range, a child that a later pair names too, or (in one table) a child that is the parent of a pair, changes

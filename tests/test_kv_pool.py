@@ -59,6 +59,9 @@ def test_pool_entry_points_refuse_bad_arguments_without_a_gpu():
             refused(name, word, pool=bad)
         for t, word in ((table(n_seqs=-1), 'bad sizes'), (table(n_pages=1 << 24), 'bad sizes'), (table(n_seqs=1 << 23), 'too many'), (table(pages=None), 'null')):
             refused(name, word, t=t)
+    for bad, at, word in ((_lib.BaKvPool(None, p, p, 40), p, 'null'), (pool, None, 'null'), (_lib.BaKvPool(p, p, p, -1), p, 'bad sizes')):
+        assert L.ba_kv_pool_free(_lib.BaKvFreeArgs(bad, at), None) != 0 and word in L.ba_last_error().decode()
+    assert L.ba_kv_pool_free(None, None) != 0
     refused('count', 'bad tables', tables=None)
     refused('compact', 'bad tables', n_tables=-1)
     refused('grow', 'bad sizes', max_new=-1)
@@ -552,3 +555,28 @@ def test_pool_calls_of_nothing():
             pool.free(pages, lens)
             pool.free(pages, lens, _i32([0, 7, -1, 0]))
             assert not pool.counts.any() and int(pool.available()) == n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n_blocks', [1, 31, 32, 33, 5000, 100_000])
+def test_free_blocks_counted_in_a_graph(n_blocks):
+    """What ``available`` says is that of the present counts, at each replay."""
+    from blast3r_amd.kv_pool import BlockPool
+    print(f'free blocks of {n_blocks}', flush=True)
+    pool = BlockPool(n_blocks, device=DEV)
+    assert pool.available().tolist() == [n_blocks]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        free = pool.available()
+    pages = torch.full((2, n_blocks // 2 + 1), -1, dtype=torch.int32, device=DEV)
+    lens = torch.zeros(2, dtype=torch.int32, device=DEV)
+    left = n_blocks
+    for n in (64, 0, 640, 64 * (n_blocks // 2)):
+        pool.grow(pages, lens, n)
+        lens += n
+        left = n_blocks - int((pages >= 0).sum())
+        g.replay()
+        assert free.tolist() == pool.available().tolist() == [left] == [int((pool.counts == 0).sum())]
+    pool.free(pages, lens)
+    g.replay()
+    assert free.tolist() == [n_blocks]
