@@ -236,8 +236,9 @@ class KVCache:
         until     (tokens,) int32: and only those below this one (the end of its frame, with causal=False)
         prefix    (n_seqs,) int32: the first so many tokens of a sequence are seen by all its rows, whatever causal, window,
                   since and until say (a prompt that is read in both directions, the first tokens beside a window)
-        shared    the first so many blocks (a host number) of all lists that have tokens there are the same: they are read
-                  once for all sequences, where that is expected to be faster than reading each list by itself
+        shared    the first so many blocks (a host number) of all lists are the same as far as their tokens go (none that was
+                  given back is among them): they are read once for all sequences, where that is expected to be faster than
+                  reading each list by itself
         A row that sees no token gives zeros.  q_heads is a multiple of the cache's heads; query head h reads cache
         head h // (q_heads // heads).  With ``return_lse`` also log(sum(exp(scale q k^T))) as (tokens, q_heads) fp32,
         -inf where no token is seen, with which results over different tokens can be joined."""

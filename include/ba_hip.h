@@ -730,8 +730,8 @@ int64_t ba_kv_attend_workspace_bytes(int64_t n_rows, int32_t q_heads, int32_t di
 /* The same with formed scores, masks by row and lists that begin alike.  The score z = scale * q.k of the row at position p
  * and token j becomes cap * tanh(z / cap) where cap is not 0 (cap in [1e-3, 1e3]; right to 4e-7 * cap), then z - slopes[h] *
  * |p - j| where slopes (finite numbers) are given.  A row sees j < lengths[s] with j < prefix[s], or with j >= since[row], j <
- * until[row] and what causal and window say; any of the three may be NULL.  shared: the first so many blocks of all lists that
- * have tokens there are the same: they are read once for all rows.  a.n_splits counts the parts of the sequences' own blocks,
+ * until[row] and what causal and window say; any of the three may be NULL.  shared: the first so many blocks of all lists are
+ * the same as far as their tokens go, and none of them is missing: they are read once for all rows.  a.n_splits counts the parts of the sequences' own blocks,
  * shared_parts those of the shared ones (0 without any); tile and shared_tile are rows of a workgroup (16, 32, 128, 256; 0: by
  * their number).  ba_kv_scored_plan sets the four from everything else but pointers to rows and workspace, and sets shared to
  * 0 where reading each list by itself is expected to be faster.  With more than one part in all, a.workspace has

@@ -75,6 +75,11 @@ def test_formed_entry_point_refuses_bad_arguments_without_a_gpu():
         assert 1 <= a.n_splits <= 64 or a.max_rows == 1 and a.n_splits <= 384
         assert a.shared_parts >= 1 if a.shared else a.shared_parts == 0
         assert a.tile in (0, 16, 32, 128, 256) and a.shared_tile in (0, 16, 32, 128, 256) and not (a.dim == 256 and a.tile == 256)
+    plans = []                                               # a window wider than any list is none
+    for window in (0, 1 << 35, (1 << 63) - 1):
+        plans.append(_lib.BaKvScoredArgs(**{**good, 'window': window, 'n_pages': 300, 'max_rows': 1, 'rows_per_seq': 1, 'n_rows': 1}))
+        L.ba_kv_scored_plan(plans[-1])
+    assert plans[0].n_splits > 1 and len({(a.n_splits, a.tile) for a in plans}) == 1
     assert L.ba_kv_attend_scored(ctypes.byref(_lib.BaKvScoredArgs(**{**good, 'tile': 64})), None) != 0 and 'tiles' in L.ba_last_error().decode()
     assert L.ba_kv_attend_scored(ctypes.byref(_lib.BaKvScoredArgs(**{**good, 'shared_tile': 256, 'dim': 256})), None) != 0
 
@@ -516,3 +521,17 @@ def test_formed_steps_in_a_graph_and_on_a_side_stream():
             other = step()
         torch.cuda.synchronize()
         assert torch.equal(y, eager) and torch.equal(y, other), t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [1, 200])
+def test_windows_wider_than_64_bits_hold(n):
+    """The widest window there is, with rows whose positions are negative among others: as without one."""
+    c, _ = _cache(12, 2, 64, 'int8')
+    q = torch.randn((2 * n, 4, 64), device=DEV).bfloat16()
+    pages, lens = _i32(np.arange(12).reshape(2, 6)), _i32([380, n // 2])
+    print(f'widest window {n}', flush=True)
+    for causal in (True, False):
+        for kw in (dict(cap=9.0), dict(slopes=torch.rand(4, device=DEV)), dict(prefix=_i32([70, 5]))):
+            want = c.attend(q, pages, lens, causal=causal, **kw)
+            assert torch.equal(c.attend(q, pages, lens, causal=causal, window=(1 << 63) - 1, **kw), want)
