@@ -321,6 +321,17 @@ __device__ __forceinline__ int at_anchor(const AtRow& r, float slope) {
     return d;
 }
 
+// The tokens [at, at + 32) that a row sees, a bit each; a score whose bit is not set is hidden (two instructions a score where
+// comparisons take five).
+__device__ __forceinline__ uint32_t at_bits(const AtRow& r, int at) {
+    auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
+    return below(r.pre - at) | (below(r.hi - at) & ~below(r.lo - at));
+}
+__device__ __forceinline__ float at_hidden(float score, uint32_t bits, int t) {
+    const uint32_t keep = (uint32_t)((int32_t)(bits << (31 - t)) >> 31);
+    return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, score) & keep) | (0xff800000u & ~keep));
+}
+
 // the smallest and largest of what rows see
 struct AtSpan {
     int lo0, lo1, hi0, hi1, pre0, pre1, pos0, pos1;
@@ -830,10 +841,9 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(AtArgs<MO
         if (MODE != AT_PLAIN && masked) {
 #pragma unroll
             for (int c = 0; c < NCB; ++c) {
-                const int base = t0 + g * TPL, pre = gone ? 0 : row[c].pre - base, from = row[c].lo - base, end = gone ? 0 : row[c].hi - base;
+                const uint32_t bits = at_bits(row[c], t0 + g * TPL) & (gone ? 0u : ~0u);
 #pragma unroll
-                for (int t = 0; t < TPL; ++t)
-                    if (!(t < pre || (t >= from && t < end))) sc[c][t / CREG][t % CREG] = -__builtin_inff();
+                for (int t = 0; t < TPL; ++t) sc[c][t / CREG][t % CREG] = at_hidden(sc[c][t / CREG][t % CREG], bits, t);
             }
         }
         if (MODE == AT_PLAIN && masked) {
@@ -1233,17 +1243,15 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
         for (int c = 0; c < NCB; ++c) {
             if constexpr (at_slopes(MODE))
                 if (both) {
-                    const int at = row[c].pos - (t0 + 32 * g + 16 * b);
+                    const int at = row[c].pos - (t0 + 32 * g + 16 * b), from = at > 0 ? at : 16;
 #pragma unroll
-                    for (int r = 1; r < 16; ++r)
-                        if (at > 0 && r > at) t[c][r] = fmaf(-2.0f * slope[c], (float)(r - at), t[c][r]);
+                    for (int r = 2; r < 16; ++r) t[c][r] = fmaf(-2.0f * slope[c], (float)max(r - from, 0), t[c][r]);
                 }
             if constexpr (MODE != AT_PLAIN)
                 if (masked) {
-                    const int base = t0 + 32 * g + 16 * b, pre = gone ? 0 : row[c].pre - base, from = row[c].lo - base, end = gone ? 0 : row[c].hi - base;
+                    const uint32_t bits = at_bits(row[c], t0 + 32 * g + 16 * b) & (gone ? 0u : ~0u);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (!(r < pre || (r >= from && r < end))) t[c][r] = -__builtin_inff();
+                    for (int r = 0; r < 16; ++r) t[c][r] = at_hidden(t[c][r], bits, r);
                 }
             if (MODE == AT_PLAIN && masked) {                                    // the lane's tokens that the row sees
                 const int base = t0 + 32 * g + 16 * b;
