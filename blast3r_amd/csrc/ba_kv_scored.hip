@@ -17,10 +17,10 @@
 //            that see 64 + 4096 tokens, e4m3: 32 us (4.3 TB/s) + 5
 //   vector   2 x 2048 rows over 16384 tokens: 1030 us with masks, 960 with slopes (far weights vanish, and power with them), 1200
 //   units    capped (matrix unit busy 35%, vector units 64%: two more transcendentals a score), 1180 both
-//   latency  8192 tokens of documents of 50 to 2000: 160 us, where their products would take 65 (documents of 64, one block a tile:
+//   latency  8192 tokens of documents of 50 to 2000: 149 us, where their products would take 65 (documents of 64, one block a tile:
 //            54, in four turns of two tiles a CU: that is what a tile takes to begin and end)
 //   shared   64 tokens over 16384 shared and 1 to 512 of their own: 45 + 6 us (41 + 16 + 6 as two launches); read by each, 460
-//   16 heads of 64, e4m3: 6144 rows of frames over 12288 tokens 290 us (0.83 PFLOP/s), 4608 rows of six frames over 16128 391 us
+//   16 heads of 64, e4m3: 6144 rows of frames over 12288 tokens 288 us (0.83 PFLOP/s), 4608 rows of six frames over 16128 391 us
 #include <math.h>
 
 #include "ba_kv_attend.h"
@@ -147,8 +147,8 @@ static Guess guess(int64_t rows, int64_t n_seqs, int heads, int dim, int64_t blo
         best.us = with(best.v, (double)base * best.parts, few_us(dim, (double)base, blocks, best.parts) + parted(best.parts, false));
         return best;
     }
-    // documents are short beside their sequence: small tiles, whole (8192 tokens of documents of 50 to 2000: 164 us, 174 with
-    // tiles of 256 rows, 251 in two parts)
+    // documents are short beside their sequence: small tiles, whole (8192 tokens of documents of 50 to 2000: 143 us, 146 with
+    // tiles of 256 rows, 263 in two parts)
     if (brief) return {at_tile(128, dim), 1, launch_us(at_tile(128, dim), dim, (double)n_seqs * heads * ((rows + 127) / 128), blocks, 1, 1.0)};
     static const int some[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 40, 48, 64};
     best.us = 1.0e30;
