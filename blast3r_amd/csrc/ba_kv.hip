@@ -300,7 +300,11 @@ __global__ void __launch_bounds__(KV_T) k_kv_read(ba_kv_args a, int slots, int p
     const int h = at.h, s = at.s, slot = at.slot, tid = threadIdx.x;
     if (slot < 0) return;
     KvShare sh;
-    const bool held = kv_share(a, s, slot, sh) && kv_there(a, sh);
+    bool held = kv_share(a, s, slot, sh);
+    if (held) {
+        sh.page = kv_block((int32_t)sh.page);
+        held = kv_there(a, sh);
+    }
     T* y = (T*)(keys ? a.rk : a.rv);
     const int st = (int)(keys ? a.rk_st : a.rv_st);         // below 2^31: a row's address is one multiply-add
     y += h * (keys ? a.rk_sh : a.rv_sh);
@@ -392,7 +396,7 @@ static int kv_call(const ba_kv_args* args, void* stream, bool write) {
     clear_error();
     BA_REQUIRE(args != nullptr, "null args");
     const ba_kv_args& a = *args;
-    BA_REQUIRE(a.n_blocks >= 0 && a.heads >= 1 && a.heads <= 65536 && a.n_seqs >= 0 && a.n_pages >= 0, "cache: bad sizes");
+    BA_REQUIRE(a.n_blocks >= 0 && a.n_blocks <= KV_KEPT && a.heads >= 1 && a.heads <= 65536 && a.n_seqs >= 0 && a.n_pages >= 0, "cache: bad sizes");
     BA_REQUIRE(a.dim == 32 || a.dim == 64 || a.dim == 96 || a.dim == 128 || a.dim == 256,
                "cache: head size must be 32, 64, 96, 128 or 256");
     BA_REQUIRE(a.bits == BA_FP8 || a.bits == BA_INT8, "cache: bits must be 0 (e4m3) or 1 (int8)");

@@ -683,7 +683,7 @@ __global__ void __launch_bounds__(AT_T, at_waves(D, COLS)) k_kv_attend(AtArgs<MO
     const int64_t step = (int64_t)a.heads * 64 * D;
     uint2 kr[NB][KS], vr[DB][PS];
     // a block that is not there is read as block 0 and hidden
-    auto page_of = [&](int v) { return v < hi ? pages[block(v)] : 0; };
+    auto page_of = [&](int v) { return v < hi ? kv_block(pages[block(v)]) : 0; };
     auto there = [&](int p) { return p >= 0 && p < a.n_blocks; };
     auto factors = [&](int p) {
         const float2 f = *(const float2*)(a.scales + ((int64_t)(there(p) ? p : 0) * a.heads + kh) * 2);
@@ -1120,7 +1120,7 @@ __global__ void __launch_bounds__(64 * WAVES, D * NCB <= 128 ? 2 : 1) k_kv_atten
     const uint8_t* vb = (const uint8_t*)a.v + (int64_t)kh * 64 * D;
     const int64_t step = (int64_t)a.heads * 64 * D;
     // a block that is not there is read as block 0 and hidden
-    auto page_of = [&](int v) { return v < hi ? pages[block(v)] : 0; };
+    auto page_of = [&](int v) { return v < hi ? kv_block(pages[block(v)]) : 0; };
     auto there = [&](int p) { return p >= 0 && p < a.n_blocks; };
     auto factors = [&](int p) {
         const float2 f = *(const float2*)(a.scales + ((int64_t)(there(p) ? p : 0) * a.heads + kh) * 2);

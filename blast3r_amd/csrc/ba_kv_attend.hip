@@ -25,7 +25,7 @@ extern "C" int64_t ba_kv_attend_workspace_bytes(int64_t n_rows, int32_t q_heads,
 // What every attention call is checked for, before anything is launched; `nothing`: it has no rows.
 int ba::attend_check(const ba_kv_attend_args& a, bool& nothing) {
     nothing = false;
-    BA_REQUIRE(a.n_blocks >= 0 && a.heads >= 1 && a.heads <= 65536 && a.n_seqs >= 0 && a.n_pages >= 0, "attention: bad sizes");
+    BA_REQUIRE(a.n_blocks >= 0 && a.n_blocks <= KV_KEPT && a.heads >= 1 && a.heads <= 65536 && a.n_seqs >= 0 && a.n_pages >= 0, "attention: bad sizes");
     BA_REQUIRE(a.dim == 32 || a.dim == 64 || a.dim == 96 || a.dim == 128 || a.dim == 256,
                "attention: head size must be 32, 64, 96, 128 or 256");
     BA_REQUIRE(a.q_heads >= 1 && a.q_heads <= 65536 && a.q_heads % a.heads == 0, "attention: query heads must be a multiple of the cache's");

@@ -7,7 +7,8 @@
 //   count    counts from the lists
 //   fork     children get their parents' lists: counts rise, nothing is copied
 //   grow     blocks for new tokens.  An open last block that other lists hold too is exchanged for a block of one's own, with
-//            the pair (old, new) to be copied; sequence after sequence, so that the last of its holders keeps it.
+//            the pair (old, new) to be copied; sequence after sequence, so that the last of its holders keeps it.  Without
+//            a block to exchange it for it stays, marked (KV_KEPT): its tokens are seen, and nothing is written there.
 //   trim     blocks outside a range of tokens are given back
 //   compact  the highest used blocks go to the lowest free ones
 //   copy     blocks' codes and factors, pair by pair
@@ -22,6 +23,7 @@
 
 #include "ba_error.h"
 #include "ba_hip.h"
+#include "ba_token.h"
 
 namespace ba {
 
@@ -57,7 +59,7 @@ __global__ void __launch_bounds__(PL_T) k_pool_count(ba_kv_pool p, ba_kv_table t
     const int64_t n = (int64_t)t.n_seqs * t.n_pages;
     for (int64_t i = (int64_t)blockIdx.x * PL_T + threadIdx.x; i < n; i += (int64_t)gridDim.x * PL_T) {
         const int64_t s = i / t.n_pages;
-        const int32_t b = t.pages[s * t.stride + (i - s * t.n_pages)];
+        const int32_t b = kv_block(t.pages[s * t.stride + (i - s * t.n_pages)]);
         if (held(p, b)) atomicAdd(p.counts + b, 1);
     }
 }
@@ -83,7 +85,7 @@ __global__ void __launch_bounds__(PL_ONE) k_pool_count_one(ba_kv_pool p, ba_kv_t
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += PL_ONE) {
         const int s = (int)((unsigned)i / (unsigned)t.n_pages);
-        const int32_t b = t.pages[s * t.stride + (i - s * t.n_pages)];
+        const int32_t b = kv_block(t.pages[s * t.stride + (i - s * t.n_pages)]);
         if (held(p, b)) atomicAdd(counts_sh + b, 1);
     }
     __syncthreads();
@@ -117,11 +119,11 @@ __global__ void __launch_bounds__(PL_T) k_pool_fork(ba_kv_fork_args a, int same)
     const int32_t* src = a.from.pages + from * a.from.stride;
     int32_t* dst = a.to.pages + to * a.to.stride;
     for (int b = threadIdx.x; b < a.to.n_pages; b += PL_T) {
-        const int32_t old = dst[b];
+        const int32_t old = dst[b], given = kv_block(old);
         int32_t now = b < a.from.n_pages && (int64_t)b * 64 < len ? src[b] : -1;
-        if (held(p, now)) hold(p, now);
+        if (held(p, kv_block(now))) hold(p, kv_block(now));
         else now = -1;
-        if (held(p, old)) give_back(p, old);
+        if (held(p, given)) give_back(p, given);
         if (now != old) dst[b] = now;
     }
     if (threadIdx.x == 0) a.to_lengths[to] = len;
@@ -138,7 +140,7 @@ __global__ void __launch_bounds__(PL_T) k_pool_trim(ba_kv_trim_args a) {
     for (int b = threadIdx.x; b < a.table.n_pages; b += PL_T) {
         if (b >= lo && b < hi) continue;
         if (row[b] < 0) continue;
-        const int32_t old = atomicExch(row + b, -1);         // a row that is named twice gives back once
+        const int32_t old = kv_block(atomicExch(row + b, -1));         // a row that is named twice gives back once
         if (held(p, old)) give_back(p, old);
     }
     if (a.lengths && threadIdx.x == 0) a.lengths[s] = 0;
@@ -236,10 +238,11 @@ __global__ void __launch_bounds__(PL_ONE) k_pool_grow(ba_kv_grow_args a, int shi
     struct Seq {
         int len, filled, end;                                // blocks [filled, end) are those of new tokens alone
         int32_t open;                                        // the block that holds tokens and gets new ones, or -1
+        bool marked;                                         // its entry is
         int32_t* row;
     };
     auto seq = [&](int s) {
-        Seq r = {0, 0, 0, -1, nullptr};
+        Seq r = {0, 0, 0, -1, false, nullptr};
         if (s >= a.table.n_seqs) return r;
         const int64_t len = a.lengths[s] < 0 ? 0 : a.lengths[s];
         int64_t n = a.more ? a.more[s] : a.each;
@@ -250,13 +253,20 @@ __global__ void __launch_bounds__(PL_ONE) k_pool_grow(ba_kv_grow_args a, int shi
         r.end = (int)(end < a.table.n_pages ? end : a.table.n_pages);
         r.filled = (int)(filled < r.end ? filled : r.end);
         if (n > 0 && len % 64 && len / 64 < a.table.n_pages) r.open = r.row[len / 64];
+        r.marked = r.open >= KV_KEPT;
+        r.open = kv_block(r.open);
         if (!held(p, r.open)) r.open = -1;
         return r;
     };
-    // open blocks that other lists hold too: marked with the last sequence that is to write there, and given back by all
+    // open blocks that other lists hold too: their marks are the last sequence that is to write there, and all give them back
     auto shared = [&](int s) {                               // the one of a sequence, or -1 (before any is given back)
-        const int32_t open = seq(s).open;
-        return open >= 0 && fresh(p.counts + open) > 1 ? open : -1;
+        const Seq r = seq(s);
+        if (r.open < 0) return -1;
+        const int32_t n = fresh(p.counts + r.open);
+        if (n > 1) return r.open;
+        if (n < 1) p.marks[r.open] = -1;                     // of no list that the pool knows: its mark may be an old one
+        if (r.marked) r.row[r.len / 64] = r.open;            // the others have ended: it may be written again
+        return -1;
     };
     const int32_t first = shared(tid);                       // of the first PL_ONE sequences it is not looked up again
     int any = 0;
@@ -324,18 +334,33 @@ __global__ void __launch_bounds__(PL_ONE) k_pool_grow(ba_kv_grow_args a, int shi
         const int m = moves + scan_before(l == 0 && got >= 0 ? 1 : 0, red, made);
         moves += made;
         // (all threads of the round have read marks and counts before the scans)
-        if (l == 0 && final) p.marks[r.open] = -1;
-        if (l == 0 && keeps) p.counts[r.open] = 1;
-        if (l == 0 && own) {
-            r.row[r.len / 64] = got;
-            if (got >= 0) {
-                a.src[m] = r.open;
-                a.dst[m] = got;
-                p.counts[got] = 1;
-                p.marks[got] = -1;
-                atomicOr(p.used + (got >> 5), 1u << (got & 31));
-            }
+        const bool enough = base <= free;                    // all before it, and this round's, got theirs
+        if (l == 0 && final && (own ? got >= 0 : enough)) p.marks[r.open] = -1;
+        if (l == 0 && keeps && enough) {
+            p.counts[r.open] = 1;
+            if (r.marked) r.row[r.len / 64] = r.open;
         }
+        if (l == 0 && got >= 0) {
+            r.row[r.len / 64] = got;
+            a.src[m] = r.open;
+            a.dst[m] = got;
+            p.counts[got] = 1;
+            p.marks[got] = -1;
+            atomicOr(p.used + (got >> 5), 1u << (got & 31));
+        }
+    }
+    if (any && base > free) {                                // those that got none hold their open block as before
+        auto kept = [&](auto f) {
+            __syncthreads();
+            for (int s = tid; s < a.table.n_seqs; s += PL_ONE) {
+                const Seq r = seq(s);
+                if (r.open >= 0 && fresh(p.marks + r.open) >= 0) f(r);
+            }
+        };
+        kept([&](const Seq& r) { atomicAdd(p.counts + r.open, 1); });
+        // and none of them may write there while another does not let go, not the last one either
+        kept([&](const Seq& r) { r.row[r.len / 64] = fresh(p.counts + r.open) > 1 ? r.open | KV_KEPT : r.open; });
+        kept([&](const Seq& r) { p.marks[r.open] = -1; });
     }
     for (int m = moves + tid; m < a.table.n_seqs; m += PL_ONE) {
         a.src[m] = -1;
@@ -403,10 +428,10 @@ __global__ void __launch_bounds__(PL_T) k_pool_move(ba_kv_pool p, ba_kv_table t)
     for (int64_t i = (int64_t)blockIdx.x * PL_T + threadIdx.x; i < n; i += (int64_t)gridDim.x * PL_T) {
         const int64_t s = i / t.n_pages;
         int32_t* e = t.pages + s * t.stride + (i - s * t.n_pages);
-        const int32_t b = *e;
+        const int32_t entry = *e, b = kv_block(entry);
         if (!held(p, b) || p.counts[b] > 0) continue;
         const int32_t to = p.marks[b];
-        if (held(p, to)) *e = to;
+        if (held(p, to)) *e = entry < KV_KEPT ? to : to | KV_KEPT;
     }
 }
 

@@ -12,6 +12,12 @@ enum { BA_F32 = 0, BA_F16 = 1, BA_BF16 = 2 };
 // what `bits` says of a cache
 enum { BA_FP8 = 0, BA_INT8 = 1 };
 
+// The block of a list's entry, below 0 where it has none.  A block that other lists hold too, and that must therefore not be
+// written for this one, may be marked (ba_kv_pool_grow): it is read like any other, while rows appended there are left out, as
+// those of a number that is no block's.
+#define KV_KEPT (1 << 30)
+__device__ __forceinline__ int32_t kv_block(int32_t entry) { return entry & ~KV_KEPT; }
+
 // V consecutive elements as floats, in loads of 16 bytes or what they are if less, and aligned to that
 template <typename T, int V>
 __device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {

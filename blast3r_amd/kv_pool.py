@@ -132,9 +132,12 @@ class BlockPool:
 
         Returns (src, dst, n) for ``KVCache.copy``: where new tokens would go to a block that has tokens and that other lists
         hold too, it is exchanged for another one in this list, and src has to be copied to dst before anything is appended
-        (and before the next call on this pool).  One list after the other, so the last holder of a block keeps it.  Lists
-        that there are no blocks left for keep -1 there, an exchanged block's place among them, and rows appended there are
-        left out; ``missing`` says how many there were."""
+        (and before the next call on this pool).  One list after the other, so the last holder of a block keeps it.
+
+        ``missing`` says how many blocks there were not.  Lists that there were none left for have -1 at the places of their
+        new tokens; one whose shared block there was no other for holds it as before, with 2^30 added to its number.  Its
+        tokens are seen and read as ever, and rows appended to either are left out (``lengths`` must not count them).  When
+        blocks have been given back, the same call again gives such lists what they lacked."""
         a = self._args(BaKvGrowArgs)
         self._table(a.table, pages)
         S, width = a.table.n_seqs, a.table.n_pages

@@ -659,7 +659,8 @@ int ba_rotary(const ba_rotary_args* args, void* stream);
  * 128 or 256.  Sequence s of a call has the rows offsets[s] .. offsets[s + 1] of the row tensors (n_rows rows in
  * all), or rows_per_seq rows each where offsets is NULL; max_rows bounds the rows of a sequence: what is over it is
  * left out.  Entries of pages outside [0, n_blocks), tokens past the width of pages and rows past n_rows are left
- * out too: not written, read as zeros, hidden from queries. */
+ * out too: not written, read as zeros, hidden from queries.  An entry of 2^30 and a block's number (ba_kv_pool_grow) is that
+ * block for what is read, and none for what is written. */
 typedef struct {
     void* k;
     void* v;
@@ -755,7 +756,8 @@ void ba_kv_scored_plan(ba_kv_scored_args* args);
 /* Pages of the cache.  A pool knows of each block how many lists hold it: counts (n_blocks,), used ((n_blocks + 31) / 32
  * words, a bit for each block that a list holds, bits past the last block set) and marks (2 n_blocks ints, between calls -1
  * for used blocks and anything for others), all on the device; ba_kv_pool_count sets the three.  Tables of lists have -1 (any number below 0)
- * where there is no block; entries past the pool are left as they are.  Calls on one pool go one after the other. */
+ * where there is no block, and a block's number + 2^30 where the list holds it and must not write to it (ba_kv_pool_grow);
+ * entries past the pool are left as they are.  Calls on one pool go one after the other. */
 typedef struct {
     int32_t* counts;
     uint32_t* used;
@@ -823,7 +825,9 @@ int ba_kv_pool_trim(const ba_kv_trim_args* args, void* stream);
  * lists, the lowest free block first; entries that are there already stay.  Where the first of them goes to a block that has
  * tokens and that other lists hold too, that block is exchanged for another: (src, dst)[0 .. n) are the blocks to be copied,
  * -1 after them ((n_seqs,) ints each).  One list after the other: the last holder of a block keeps it.  missing: blocks that
- * there were not; entries without one are -1, an exchanged one too. */
+ * there were not; entries of new tokens without one are -1, and a block for which there was no other stays where it is, marked
+ * (its number + 2^30) in all lists that were to write there and hold it still: it is read, rows appended to it are left out,
+ * and a later call exchanges it or, when no other list holds it any more, takes the mark away. */
 typedef struct {
     ba_kv_pool pool;
     ba_kv_table table;

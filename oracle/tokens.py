@@ -102,8 +102,8 @@ class Cache:
         k, v, there = np.zeros((length, H, D)), np.zeros((length, H, D)), np.zeros(length, bool)
         for b in range((length + 63) // 64):
             n = min(64, length - 64 * b)
-            if b < len(pages) and 0 <= pages[b] < len(self.k):
-                p = pages[b]
+            if b < len(pages) and 0 <= block(pages[b]) < len(self.k):
+                p = block(pages[b])
                 k[64 * b:64 * b + n] = (self.k[p, :, :n] * self.scales[p, :, 0][:, None, None]).transpose(1, 0, 2)
                 v[64 * b:64 * b + n] = (self.v[p, :, :n] * self.scales[p, :, 1][:, None, None]).transpose(1, 0, 2)
                 there[64 * b:64 * b + n] = True
@@ -168,6 +168,13 @@ def attend_formed(cache, q, pages, lengths, counts, scale, causal=True, window=N
     return o, lse, a
 
 
+KEPT = 1 << 30       # added to the number of a block that a list holds and must not write to
+
+
+def block(entry):
+    return int(entry) - KEPT if entry >= KEPT else int(entry)
+
+
 class Pool:
     """Which lists hold which of n blocks, call by call and list by list."""
 
@@ -181,13 +188,15 @@ class Pool:
         self.counts = [0] * len(self.counts)
         for t in tables:
             for b in np.asarray(t).flatten().tolist():
-                if self._held(b):
-                    self.counts[b] += 1
+                if self._held(block(b)):
+                    self.counts[block(b)] += 1
 
     def grow(self, pages, lengths, new):
         """The copies to be made, as [(src, dst)]; pages is changed."""
         free = [b for b, c in enumerate(self.counts) if c == 0][::-1]
         moves, self.missing = [], 0
+        left = dict()                    # holders of an open block that have not been asked to part with it
+        stay = []                        # lists whose open block is the one that it was
 
         def take():
             if free:
@@ -199,22 +208,32 @@ class Pool:
         for row, length, n in zip(pages, lengths, new):
             length, n, width = max(0, int(length)), max(0, int(n)), len(row)
             at = length // 64
-            if n and length % 64 and at < width and self._held(row[at]) and self.counts[row[at]] > 1:
-                old = int(row[at])
-                self.counts[old] -= 1
-                row[at] = take()
-                if row[at] >= 0:
-                    moves.append((old, int(row[at])))
+            if n and length % 64 and at < width and self._held(block(row[at])):
+                old = block(row[at])
+                got = -1
+                if left.setdefault(old, self.counts[old]) > 1:
+                    left[old] -= 1
+                    got = take()
+                if got >= 0:
+                    self.counts[old] -= 1
+                    row[at] = got
+                    moves.append((old, got))
+                else:
+                    stay.append((row, at))
             for b in range((length + 63) // 64, min(width, (length + n + 63) // 64)):
                 if row[b] < 0:
                     row[b] = take()
+        for row, at in stay:
+            b = block(row[at])
+            row[at] = b + KEPT if self.counts[b] > 1 else b
         return moves
 
     def drop(self, row, keep=lambda b: False):
         for b in range(len(row)):
             if row[b] >= 0 and not keep(b):
-                if self._held(row[b]) and self.counts[row[b]] > 0:
-                    self.counts[row[b]] -= 1
+                old = block(row[b])
+                if self._held(old) and self.counts[old] > 0:
+                    self.counts[old] -= 1
                 row[b] = -1
 
     def fork(self, pages, lengths, parents, children, to, to_lengths):
@@ -222,13 +241,13 @@ class Pool:
         for i, (p, c) in enumerate(zip(parents, children)):
             if not (0 <= p < len(pages) and 0 <= c < len(to)) or c in children[i + 1:] or same and c in parents:
                 continue
-            row = [int(b) if self._held(b) and 64 * x < lengths[p] else -1 for x, b in enumerate(pages[p])]
+            row = [int(b) if self._held(block(b)) and 64 * x < lengths[p] else -1 for x, b in enumerate(pages[p])]
             for b in row:
                 if b >= 0:
-                    self.counts[b] += 1
+                    self.counts[block(b)] += 1
             for b in to[c]:
-                if self._held(b) and self.counts[b] > 0:
-                    self.counts[b] -= 1
+                if self._held(block(b)) and self.counts[block(b)] > 0:
+                    self.counts[block(b)] -= 1
             to[c] = row + [-1] * (len(to[c]) - len(row))
             to_lengths[c] = lengths[p]
 
@@ -242,4 +261,5 @@ class Pool:
             old = t.copy()
             for a, b in moves:
                 t[old == a] = b
+                t[old == a + KEPT] = b + KEPT
         return moves

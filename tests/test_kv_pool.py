@@ -580,3 +580,176 @@ def test_free_blocks_counted_in_a_graph(n_blocks):
     pool.free(pages, lens)
     g.replay()
     assert free.tolist() == [n_blocks]
+
+
+# ---------------------------------------------------------------------------------- blocks that run out
+
+KEPT = 1 << 30
+
+
+def test_oracle_keeps_shared_blocks_that_there_is_no_other_for():
+    p = otok.Pool(4)
+    p.counts = [1, 3, 1, 0]
+    rows = np.array([[1, -1], [1, -1], [1, -1]])
+    assert p.grow(rows, [5, 5, 5], [1, 1, 1]) == [(1, 3)] and p.missing == 1       # the third cannot have it alone
+    assert rows[:, 0].tolist() == [3, 1 + KEPT, 1 + KEPT] and p.counts == [1, 2, 1, 1]
+    assert p.grow(rows, [6, 5, 5], [1, 1, 0]) == [] and p.missing == 1 and rows[:, 0].tolist() == [3, 1 + KEPT, 1 + KEPT]
+    p.drop(rows[0])
+    assert p.counts == [1, 2, 1, 0] and p.grow(rows, [0, 5, 5], [0, 1, 1]) == [(1, 3)] and p.missing == 0
+    assert rows[:, 0].tolist() == [-1, 3, 1] and p.counts == [1, 1, 1, 1]
+    rows[1, 0], p.counts[3] = 2 + KEPT, 0
+    assert p.grow(rows, [0, 5, 5], [0, 1, 1]) == [] and rows[1, 0] == 2            # no list beside it any more
+    rows[1, 0] = 2 + KEPT
+    table, lens = rows.tolist(), [0, 5, 5]
+    p.fork(table, lens, [1], [0], table, lens)
+    assert table[0][0] == 2 + KEPT and p.counts == [1, 1, 2, 0]
+    rows = np.array(table)
+    p.count(rows)
+    assert p.counts == [0, 1, 2, 0] and p.compact([rows], 4) == [(2, 0)] and rows[:, 0].tolist() == [KEPT, KEPT, 1]
+    p.drop(rows[0])
+    assert p.counts == [1, 1, 0, 0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n_seqs', [1, 2, 5, 64, 1500])
+@pytest.mark.parametrize('spare', [0, 1, 3, 700])
+@pytest.mark.parametrize('new', [1, 70, 200])
+def test_shared_blocks_stay_where_there_is_no_other(n_seqs, spare, new):
+    """Forks of a few sequences that all grow, with fewer free blocks than that takes, others than those that grow among the
+    holders: lists, counts and moves as the oracle's; again after some have ended; lists counted, forked and moved with marks."""
+    rng = np.random.default_rng(n_seqs * 7 + spare)
+    print(f'out of blocks {n_seqs} {spare} {new}', flush=True)
+    most = -(-n_seqs // 5)
+    b = Both(most * 3 + spare, n_seqs, 6)
+    b.advance(b.grow([int(rng.integers(64, 190)) if s < most else 0 for s in range(n_seqs)]))
+    b.same()
+
+    def fork(parents, children):
+        b.pool.fork(b.t, b.tl, _i32(parents), _i32(children))
+        rows = b.pages.tolist()
+        b.o.fork(rows, b.lens, parents, children, rows, b.lens)
+        b.pages = np.array(rows)
+
+    if n_seqs > most:
+        fork(rng.integers(0, most, n_seqs - most).tolist(), list(range(most, n_seqs)))
+    b.same()
+    seen = False
+    for step in range(6):
+        counts = [0 if rng.random() < 0.2 else int(rng.integers(1, new + 1)) for _ in range(n_seqs)]
+        b.grow(counts, max_new=new)
+        b.same()
+        seen = seen or bool((b.pages >= KEPT).any())
+        # lists that got all that they asked for have the tokens
+        fine = [all(0 <= x < KEPT for x in row[length // 64:-(-(length + n) // 64)]) and length + n <= 6 * 64 for row, length, n in zip(b.pages, b.lens, counts)]
+        b.advance([n if f else 0 for n, f in zip(counts, fine)])
+        if step == 1 and n_seqs > 4:                        # a child of a marked list, in the place of another
+            marked = np.flatnonzero((b.pages >= KEPT).any(1))
+            if len(marked) > 1:
+                fork([int(marked[0])], [int(marked[-1])])
+                b.same()
+        if step == 2:
+            b.pool.count(b.t)
+            b.o.count(b.pages)
+            b.same()
+        if step == 3:
+            size = len(b.o.counts) // 2
+            b.moved(b.o.compact([b.pages], size), b.pool.compact(b.t), size)
+            b.same()
+        rows = rng.permutation(n_seqs)[:max(1, n_seqs // 4)].tolist()
+        b.pool.free(b.t, b.tl, _i32(rows))
+        for r in rows:
+            b.o.drop(b.pages[r])
+            b.lens[r] = 0
+        b.same()
+    assert seen or n_seqs < 64 or spare > 3
+    for s in range(n_seqs):                                 # the last one has its blocks for itself
+        if s != n_seqs - 1:
+            b.o.drop(b.pages[s])
+    b.pool.trim(b.t, last=_i32([0] * (n_seqs - 1) + [6 * 64]))
+    b.lens = [0] * (n_seqs - 1) + b.lens[-1:]
+    b.tl.copy_(_i32(b.lens))
+    b.grow([0] * (n_seqs - 1) + [1])
+    b.same()
+    assert not (b.pages >= KEPT).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('seed', range(4))
+def test_tokens_of_every_list_through_a_cache_that_runs_full(seed):
+    """Every sequence reads back, token by token, what it was given, while lists are forked, cut, ended and moved in a pool that
+    is often too small: a step that had no blocks is not counted, is appended all the same, and is done again later.  Rows hold
+    127, which makes the factor 1, so that whole numbers are kept exactly.  Attention sees the tokens of marked blocks: a query
+    along one token's key gives its value."""
+    from blast3r_amd.kv_cache import KVCache
+    from blast3r_amd.kv_pool import BlockPool
+    rng = np.random.default_rng(seed)
+    S, D, n_blocks = 7, 32, 16
+    cache, pool = KVCache(n_blocks, 1, D, torch.int8, device=DEV), BlockPool(n_blocks, device=DEV)
+    pages, lens = torch.full((S, 6), -1, dtype=torch.int32, device=DEV), torch.zeros(S, dtype=torch.int32, device=DEV)
+    tokens = [[] for _ in range(S)]                          # their numbers
+    last, short, marked = 0, 0, 0
+
+    def rows(ids):
+        x = np.zeros((len(ids), 1, D))
+        x[:, 0, 0] = 127
+        for d in range(12):                                  # the number's bits, as +-100: keys point different ways
+            x[:, 0, 1 + d] = np.where(np.asarray(ids, int) >> d & 1, 100, -100)
+        return x
+
+    def check():
+        counts = [len(t) for t in tokens]
+        off = _i32(np.concatenate(([0], np.cumsum(counts))))
+        assert lens.tolist() == counts
+        if not sum(counts):
+            return
+        got = cache.read(pages, torch.zeros_like(lens), off, sum(counts), max_count=max(counts), dtype=torch.float32)
+        want = rows(sum(tokens, []))
+        for x in got:
+            assert np.array_equal(_np(x), want)
+        # one token of each, its 12 bits against others': a score of 12e4 of 0.01 against 10e4 at most
+        pick = [t[int(rng.integers(0, len(t)))] if t else 0 for t in tokens]
+        q = rows(pick)
+        q[:, 0, 0] = 0
+        for kw in (dict(), dict(cap=900.0)):
+            o = _np(cache.attend(torch.tensor(q, device=DEV).half(), pages, lens, causal=False, scale=0.005, **kw))
+            for s in range(S):
+                assert np.array_equal(o[s], rows([pick[s]])[0] if tokens[s] else np.zeros((1, D))), s
+
+    print(f'full cache {seed}', flush=True)
+    # at first four lists share an open block, and a fifth one takes all but one of the others
+    first = {0: [100, 0, 0, 0, 0, 0, 0], 2: [0] * 4 + [384, 384, 64], 3: [1] * 7, 4: [1] * 7, 6: [1] * 7}
+    for step in range(40):
+        what = int(rng.integers(0, 8)) if step > 6 else {1: 5, 5: 6}.get(step, 0)
+        if what < 5:
+            counts = first[step] if step in first else [int(rng.integers(0, 3)) if rng.random() < 0.6 else int(rng.integers(0, 80)) for _ in range(S)]
+            counts = [min(n, 6 * 64 - len(t)) for n, t in zip(counts, tokens)]
+            if sum(counts):
+                cache.copy(*pool.grow(pages, lens, _i32(counts), max_new=max(counts)))
+                ids = [[last + sum(counts[:s]) + i for i in range(n)] for s, n in enumerate(counts)]
+                last = (last + sum(counts)) % 3000
+                x = torch.tensor(rows(sum(ids, [])), dtype=torch.float32, device=DEV)
+                cache.append(x, x, pages, lens, offsets=_i32(np.concatenate(([0], np.cumsum(counts)))), max_new=max(counts))
+                table = pages.tolist()
+                for s, n in enumerate(counts):
+                    if all(0 <= b < KEPT for b in table[s][len(tokens[s]) // 64:-(-(len(tokens[s]) + n) // 64)]):
+                        tokens[s] = tokens[s] + ids[s]
+                    else:
+                        short += 1
+                marked += sum(b >= KEPT for row in table for b in row)
+                lens.copy_(_i32([len(t) for t in tokens]))
+        elif what == 5:
+            order = rng.permutation(S).tolist() if step > 6 else list(range(S))
+            pool.fork(pages, lens, _i32([order[0]] * 3), _i32(order[1:4]))
+            for c in order[1:4]:
+                tokens[c] = list(tokens[order[0]])
+        elif what == 6:
+            gone = [int(rng.integers(0, S))] if step > 6 else [6]
+            pool.free(pages, lens, _i32(gone))
+            tokens[gone[0]] = []
+        else:
+            tokens = [t[:max(0, len(t) - int(rng.integers(0, 70)))] if rng.random() < 0.5 else t for t in tokens]
+            lens.copy_(_i32([len(t) for t in tokens]))
+            pool.trim(pages, last=lens)
+            cache.copy(*pool.compact(pages))
+        check()
+    assert short > 3 and marked > 0, (short, marked)
