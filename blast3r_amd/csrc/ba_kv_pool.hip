@@ -268,8 +268,39 @@ __global__ void __launch_bounds__(PL_ONE) k_pool_grow(ba_kv_grow_args a, int shi
         if (r.marked) r.row[r.len / 64] = r.open;            // the others have ended: it may be written again
         return -1;
     };
-    const int32_t first = shared(tid);                       // of the first PL_ONE sequences it is not looked up again
+    // blocks past a list's tokens that other lists hold too are not to be written either (tokens that it has no more, and others
+    // have): it gives them back and takes others.  By the counts that the call begins with, so in three passes
+    auto past = [&](auto f) {
+        for (int s = tid >> shift; s < a.table.n_seqs; s += per) {
+            const Seq r = seq(s);
+            for (int b = r.filled + l; b < r.end; b += lanes) f(r.row[b]);
+        }
+    };
     int any = 0;
+    past([&](int32_t& e) {
+        const int32_t b = kv_block(e);
+        if (!held(p, b)) return;
+        const int32_t n = fresh(p.counts + b);
+        if (n > 1) any = 1;
+        if (n > 1 || n < 1) p.marks[b] = n > 1 ? 0 : -1;
+        else if (e != b) e = b;
+    });
+    int32_t first = shared(tid);                             // of the first PL_ONE sequences it is not looked up again
+    if (__syncthreads_or(any)) {
+        past([&](int32_t& e) {
+            const int32_t b = kv_block(e);
+            if (!held(p, b) || fresh(p.marks + b) < 0) return;
+            give_back(p, b);
+            e = -2 - b;                                      // wanted, and whose mark it was
+        });
+        __syncthreads();
+        past([&](int32_t& e) {
+            if (held(p, -2 - e)) p.marks[-2 - e] = -1;
+        });
+        __syncthreads();
+        first = shared(tid);
+    }
+    any = 0;
     for (int s = tid; s < a.table.n_seqs; s += PL_ONE) {
         const int32_t open = s == tid ? first : shared(s);
         if (open < 0) continue;

@@ -127,7 +127,7 @@ class BlockPool:
 
     def grow(self, pages, lengths, new, max_new=None):
         """Blocks for ``new`` more tokens (a number, or (n_seqs,) int32) after the first ``lengths`` of each list, written into
-        ``pages``; entries that are there already stay.  max_new (default: what lists can hold) bounds ``new``, and a close
+        ``pages``; blocks that are there already stay, unless other lists hold them too.  max_new (default: what lists can hold) bounds ``new``, and a close
         bound saves time.  ``lengths`` stays as it is.
 
         Returns (src, dst, n) for ``KVCache.copy``: where new tokens would go to a block that has tokens and that other lists

@@ -822,7 +822,8 @@ typedef struct {
 int ba_kv_pool_trim(const ba_kv_trim_args* args, void* stream);
 
 /* Blocks for more[s] (or `each`; at most max_new) tokens after the first lengths[s] of every list, taken in the order of the
- * lists, the lowest free block first; entries that are there already stay.  Where the first of them goes to a block that has
+ * lists, the lowest free block first; entries that are there already stay, but for those past the list's tokens whose
+ * block other lists hold too (tokens that this one has no more): it is given back.  Where the first of them goes to a block that has
  * tokens and that other lists hold too, that block is exchanged for another: (src, dst)[0 .. n) are the blocks to be copied,
  * -1 after them ((n_seqs,) ints each).  One list after the other: the last holder of a block keeps it.  missing: blocks that
  * there were not; entries of new tokens without one are -1, and a block for which there was no other stays where it is, marked

@@ -193,6 +193,16 @@ class Pool:
 
     def grow(self, pages, lengths, new):
         """The copies to be made, as [(src, dst)]; pages is changed."""
+        past = []                        # blocks past the tokens of lists that grow, which other lists hold too
+        for row, length, n in zip(pages, lengths, new):
+            length, n = max(0, int(length)), max(0, int(n))
+            for b in range((length + 63) // 64, min(len(row), (length + n + 63) // 64)) if n else ():
+                if self._held(block(row[b])):
+                    row[b] = row[b] if self.counts[block(row[b])] > 1 else block(row[b])
+                    past += [(row, b)] if self.counts[block(row[b])] > 1 else []
+        for row, b in past:
+            self.counts[block(row[b])] -= 1
+            row[b] = -1
         free = [b for b, c in enumerate(self.counts) if c == 0][::-1]
         moves, self.missing = [], 0
         left = dict()                    # holders of an open block that have not been asked to part with it

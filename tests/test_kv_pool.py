@@ -753,3 +753,64 @@ def test_tokens_of_every_list_through_a_cache_that_runs_full(seed):
             cache.copy(*pool.compact(pages))
         check()
     assert short > 3 and marked > 0, (short, marked)
+
+
+def test_oracle_gives_back_shared_blocks_past_the_tokens():
+    p = otok.Pool(6)
+    p.counts = [1, 2, 2, 1, 0, 0]
+    rows = np.array([[0, 1, 2], [3, 1, 2]])
+    assert p.grow(rows, [64, 192], [64, 0]) == [] and rows.tolist() == [[0, 4, 2], [3, 1, 2]] and p.counts == [1, 1, 2, 1, 1, 0]
+    assert p.grow(rows, [64, 64], [128, 128]) == [] and p.missing == 0     # nobody has tokens in block 2
+    assert rows.tolist() == [[0, 4, 2], [3, 1, 5]] and p.counts == [1, 1, 1, 1, 1, 1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n_blocks,n_seqs,width,new', [(40, 3, 6, 64), (300, 9, 20, 200), (300, 9, 20, 1300), (4000, 700, 6, 130), (6000, 1500, 5, 300)])
+def test_lists_cut_short_give_up_what_others_hold(n_blocks, n_seqs, width, new):
+    """Forks whose lengths are set back without a trim, and that grow again: blocks that the others still hold are exchanged
+    without a copy, those of one's own stay."""
+    rng = np.random.default_rng(new)
+    print(f'cut short {n_blocks} {n_seqs} {new}', flush=True)
+    b = Both(n_blocks, n_seqs, width)
+    b.advance(b.grow([int(rng.integers(64, 64 * width)) if s < max(1, n_seqs // 4) else 0 for s in range(n_seqs)]))
+    for step in range(5):
+        parents = rng.integers(0, max(1, n_seqs // 4), n_seqs - max(1, n_seqs // 4)).tolist()
+        children = list(range(max(1, n_seqs // 4), n_seqs))
+        b.pool.fork(b.t, b.tl, _i32(parents), _i32(children))
+        rows = b.pages.tolist()
+        b.o.fork(rows, b.lens, parents, children, rows, b.lens)
+        b.pages = np.array(rows)
+        for k in range(2):
+            b.lens = [int(rng.integers(0, x + 1)) if rng.random() < 0.7 else x for x in b.lens]
+            b.tl.copy_(_i32(b.lens))
+            b.grow([0 if rng.random() < 0.2 else int(rng.integers(1, new + 1)) for _ in range(n_seqs)], max_new=new)
+            b.same()
+    b.pool.trim(b.t, last=b.tl)
+    for s in range(n_seqs):
+        b.o.drop(b.pages[s], keep=lambda x, s=s: 64 * x < b.lens[s])
+    b.same()
+
+
+@pytest.mark.gpu
+def test_tokens_of_others_stay_when_a_list_is_cut_short():
+    """A child that takes back tokens down to the middle of what it shares, and appends others."""
+    from blast3r_amd.kv_cache import KVCache
+    from blast3r_amd.kv_pool import BlockPool
+    cache, pool = KVCache(12, 1, 32, torch.int8, device=DEV), BlockPool(12, device=DEV)
+    pages, lens = torch.full((2, 6), -1, dtype=torch.int32, device=DEV), _i32([0, 0])
+    rng = np.random.default_rng(0)
+    x, y = (torch.tensor(rng.integers(-126, 127, (n, 1, 32)), dtype=torch.float32, device=DEV) for n in (300, 200))
+    x[:, :, 0], y[:, :, 0] = 127, 127                        # the factor is 1, and whole numbers are kept
+    print('cut short, through the cache', flush=True)
+    pool.grow(pages, lens, _i32([300, 0]))
+    cache.append(x, x, pages, lens, offsets=_i32([0, 300, 300]))
+    lens[0] = 300
+    pool.fork(pages, lens, _i32([0]), _i32([1]))
+    for cut in (128, 70, 0):
+        lens[1] = cut
+        cache.copy(*pool.grow(pages, lens, _i32([0, 200])))
+        cache.append(y, y, pages, lens, offsets=_i32([0, 0, 200]))
+        lens[1] += 200
+        k, v = cache.read(pages, _i32([0, 0]), _i32([0, 300, 500 + cut]), 500 + cut, dtype=torch.float32)
+        for got in (k, v):
+            assert torch.equal(got[:300], x) and torch.equal(got[300:300 + cut], x[:cut]) and torch.equal(got[300 + cut:], y)
