@@ -49,25 +49,44 @@ static bool joint_shape(const AtShape& own, const AtShape& common, double wgs) {
 
 #define SC_WINDOW ((int64_t)1 << 40)      // wider ones are no narrower to any position, and sums with them pass 64 bits
 
+// The launches of a call: of the sequences' own blocks, of the shared ones, and the join's.
+struct ScoredShape {
+    AtShape v, w;
+    AtGrid g, h;
+    AtJoin j;
+    bool joint;
+};
+
+// a: the call's, with all of its parts.  Errors are those of sizes and of the workspace.
+static int scored_shape(const ba_kv_scored_args& s, const ba_kv_attend_args& a, ScoredShape& r) {
+    const int group = a.q_heads / a.heads;
+    const int64_t rows = a.max_rows * group, all = a.n_rows * group;
+    r.v = s.tile ? at_tile(s.tile, a.dim) : at_shape(rows, a.dim);
+    r.w = s.shared_tile ? at_tile(s.shared_tile, a.dim) : at_shape(all, a.dim);
+    // both in one launch, where that takes the sequences' own no larger tile or they are few (2048 workgroups of tokens over 164
+    // tokens in tiles of 16 rows: 50 us, 63 in tiles of 32)
+    r.joint = s.shared && joint_shape(r.v, r.w, (double)a.n_seqs * a.heads);
+    if (r.joint) r.v = r.w = r.v.rows > r.w.rows ? r.v : r.w;
+    int rc = attend_grid(a, rows, a.n_seqs, s.a.n_splits, r.v, r.g);
+    if (rc == BA_OK && s.shared) rc = attend_grid(a, all, 1, s.shared_parts, r.w, r.h);
+    if (rc == BA_OK) rc = attend_join(a, r.j);
+    if (rc != BA_OK) return rc;
+    BA_REQUIRE(!r.joint || r.g.nb < (1u << 23) - r.h.nb, "attention: too many tiles for a call");
+    return BA_OK;
+}
+
 static int attend_scored(const ba_kv_scored_args& s, hipStream_t st) {
     ba_kv_attend_args a = s.a;
     if (a.window > SC_WINDOW) a.window = SC_WINDOW;
     a.n_splits = s.a.n_splits + s.shared_parts;
-    const int group = a.q_heads / a.heads;
-    const int64_t rows = a.max_rows * group, all = a.n_rows * group;
-    AtShape v = s.tile ? at_tile(s.tile, a.dim) : at_shape(rows, a.dim), w = s.shared_tile ? at_tile(s.shared_tile, a.dim) : at_shape(all, a.dim);
-    // both in one launch, where that takes the sequences' own no larger tile or they are few (2048 workgroups of tokens over 164
-    // tokens in tiles of 16 rows: 50 us, 63 in tiles of 32)
-    const bool joint = s.shared && joint_shape(v, w, (double)a.n_seqs * a.heads);
-    if (joint) v = w = v.rows > w.rows ? v : w;
-    auto least = [](const AtShape& x) { return x.ncb ? SC_MIN_BLOCKS : AT_MIN_BLOCKS; };
-    AtGrid g, h;
-    AtJoin j;
-    int rc = attend_grid(a, rows, a.n_seqs, s.a.n_splits, v, g);
-    if (rc == BA_OK && s.shared) rc = attend_grid(a, all, 1, s.shared_parts, w, h);
-    if (rc == BA_OK) rc = attend_join(a, j);
+    ScoredShape shape;
+    int rc = scored_shape(s, a, shape);
     if (rc != BA_OK) return rc;
-    BA_REQUIRE(!joint || g.nb < (1u << 23) - h.nb, "attention: too many tiles for a call");
+    const AtShape &v = shape.v, &w = shape.w;
+    const AtGrid &g = shape.g, &h = shape.h;
+    const AtJoin& j = shape.j;
+    const bool joint = shape.joint;
+    auto least = [](const AtShape& x) { return x.ncb ? SC_MIN_BLOCKS : AT_MIN_BLOCKS; };
     const unsigned at_once = BA_N_XCD * (unsigned)g.tiles;
     // unequal: what a tile sees grows with its place by a quarter of the longest's at least (2048 rows over 16384 tokens 1219 us, 1236 dealt out)
     const bool unequal = v.ncb && ((a.causal && !s.since) || s.until) && 4 * a.max_rows >= 64 * (int64_t)a.n_pages;
@@ -166,12 +185,28 @@ static Guess guess(int64_t rows, int64_t n_seqs, int heads, int dim, int64_t blo
     return best;
 }
 
+// What a plan may ask for: launches and a join that can be made, and less room for partial sums than 8 GB, 3% of the chip's
+// (64 x 2048 rows of 32 heads of 128 over shared blocks take 4.4 in two parts).
+#define SC_ROOM ((int64_t)8 << 30)
+
+static bool can_be_made(const ba_kv_scored_args& s) {
+    ba_kv_attend_args a = s.a;
+    a.n_splits = s.a.n_splits + s.shared_parts;
+    a.workspace = (void*)16;                                 // there will be one
+    a.workspace_bytes = (int64_t)1 << 62;
+    ScoredShape r;
+    const bool ok = scored_shape(s, a, r) == BA_OK && ba_kv_attend_workspace_bytes(a.n_rows, a.q_heads, a.dim, a.n_splits) <= SC_ROOM;
+    clear_error();
+    return ok;
+}
+
 }  // namespace ba
 
 using namespace ba;
 
 extern "C" void ba_kv_scored_plan(ba_kv_scored_args* args) {
     ba_kv_attend_args& a = args->a;
+    clear_error();
     a.n_splits = 1;
     args->shared_parts = args->shared > 0 ? 1 : 0;
     args->tile = args->shared_tile = 0;
@@ -187,21 +222,30 @@ extern "C" void ba_kv_scored_plan(ba_kv_scored_args* args) {
     }
     // causal tiles of a prompt see half of what is new on the average
     const double fresh = (double)a.max_rows / (64.0 * (blocks < 1 ? 1 : blocks)), share = a.causal ? 1.0 - 0.5 * (fresh < 1.0 ? fresh : 1.0) : 1.0;
-    Guess own = guess(rows, a.n_seqs, a.heads, a.dim, blocks, join, false, brief, share);
+    const Guess own = guess(rows, a.n_seqs, a.heads, a.dim, blocks, join, false, brief, share);
+    a.n_splits = own.parts;
+    args->tile = own.v.rows;
     if (args->shared > 0) {
         const int64_t rest = a.n_pages - args->shared;
         const Guess left = guess(rows, a.n_seqs, a.heads, a.dim, rest < blocks ? rest : blocks, join, true, brief, 1.0);
         const Guess common = guess(all, 1, a.heads, a.dim, args->shared, join, true, false, 1.0, &left, (double)a.n_seqs * a.heads);
         if (common.us < own.us) {
-            own = left;
-            args->shared_parts = common.parts;
-            args->shared_tile = common.v.rows;
-        } else {
-            args->shared = args->shared_parts = 0;
+            ba_kv_scored_args s = *args;
+            s.a.n_splits = left.parts;
+            s.tile = left.v.rows;
+            s.shared_parts = common.parts;
+            s.shared_tile = common.v.rows;
+            if (can_be_made(s)) {
+                *args = s;
+                return;
+            }
         }
+        args->shared = args->shared_parts = 0;
     }
-    a.n_splits = own.parts;
-    args->tile = own.v.rows;
+    if (!can_be_made(*args)) {                               // one part, in the largest tiles: what the chip is full of anyway
+        a.n_splits = 1;
+        args->tile = 0;
+    }
 }
 
 extern "C" int ba_kv_attend_scored(const ba_kv_scored_args* args, void* stream) {

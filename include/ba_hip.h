@@ -735,7 +735,7 @@ int64_t ba_kv_attend_workspace_bytes(int64_t n_rows, int32_t q_heads, int32_t di
  * the same as far as their tokens go, and none of them is missing: they are read once for all rows.  a.n_splits counts the parts of the sequences' own blocks,
  * shared_parts those of the shared ones (0 without any); tile and shared_tile are rows of a workgroup (16, 32, 128, 256; 0: by
  * their number).  ba_kv_scored_plan sets the four from everything else but pointers to rows and workspace, and sets shared to
- * 0 where reading each list by itself is expected to be faster.  With more than one part in all, a.workspace has
+ * 0 where reading each list by itself is expected to be faster, or the parts' sums would take more than 8 GB.  With more than one part in all, a.workspace has
  * ba_kv_attend_workspace_bytes for their sum. */
 typedef struct {
     ba_kv_attend_args a;

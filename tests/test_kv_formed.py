@@ -535,3 +535,45 @@ def test_windows_wider_than_64_bits_hold(n):
         for kw in (dict(cap=9.0), dict(slopes=torch.rand(4, device=DEV)), dict(prefix=_i32([70, 5]))):
             want = c.attend(q, pages, lens, causal=causal, **kw)
             assert torch.equal(c.attend(q, pages, lens, causal=causal, window=(1 << 63) - 1, **kw), want)
+
+
+# ---------------------------------------------------------------------------------- plans of large calls (CPU)
+
+def test_plans_are_not_refused_where_one_part_is_not():
+    """Whatever is planned for a call can be launched if the call can be without a plan; and its sums have room."""
+    if torch.cuda.is_available():
+        pytest.skip('would launch on addresses that are none')
+    from blast3r_amd import _lib
+    L, p = _lib.lib(), 4096
+    rng = np.random.default_rng(0)
+    base = dict(n_blocks=2, bits=0, dtype=2, scale=1.0, n_splits=1, k=p, v=p, scales=p, pages=p, lengths=p, q=p, o=p, workspace=p,
+                workspace_bytes=(1 << 63) - 1)
+    some = [dict(n_seqs=180, n_rows=3378240, max_rows=18768, heads=8, q_heads=64, dim=128, n_pages=20, shared=14, since=p),
+            dict(n_seqs=65536, n_rows=65536, max_rows=1, heads=64, q_heads=64, dim=64, n_pages=64),
+            dict(n_seqs=40000, n_rows=40000 * 32, max_rows=32, heads=64, q_heads=64, dim=256, n_pages=64),
+            dict(n_seqs=1 << 22, n_rows=1 << 22, max_rows=1, heads=1, q_heads=1, dim=64, n_pages=64, shared=40),
+            dict(n_seqs=1000, n_rows=4000000, max_rows=4000, heads=4, q_heads=32, dim=128, n_pages=300, shared=250)]
+    log = lambda lo, hi: int(2.0 ** rng.uniform(lo, hi))  # noqa: E731
+    while len(some) < 4000:
+        heads, rows, seqs = log(0, 7), log(0, 15), log(0, 22)
+        c = dict(n_seqs=seqs, n_rows=seqs * rows, max_rows=rows, heads=heads, q_heads=heads * log(0, 4), dim=int(rng.choice([32, 64, 96, 128, 256])), n_pages=log(0, 14))
+        if c['n_rows'] >= 1 << 31:
+            continue
+        c['shared'] = int(rng.integers(0, c['n_pages'] + 1)) if rng.random() < 0.5 else 0
+        c.update(since=p if rng.random() < 0.3 else None, prefix=p if rng.random() < 0.3 else None, window=log(0, 20) if rng.random() < 0.3 else 0,
+                 causal=int(rng.integers(0, 2)), offsets=p if rng.random() < 0.5 else None)
+        some.append(c)
+    planned = 0
+    for c in some:
+        c = {**base, **c, 'rows_per_seq': 0 if c.get('offsets') else c['max_rows']}
+        plain = _lib.BaKvScoredArgs(**{**c, 'shared': 0})
+        assert L.ba_kv_attend_scored(ctypes.byref(plain), None) != 0
+        if b'too many' in L.ba_last_error():
+            continue
+        a = _lib.BaKvScoredArgs(**c)
+        L.ba_kv_scored_plan(a)
+        n = a.n_splits + a.shared_parts
+        planned += n > 1
+        assert L.ba_kv_attend_scored(ctypes.byref(a), None) != 0 and b'too many' not in L.ba_last_error(), (c, L.ba_last_error())
+        assert L.ba_kv_attend_workspace_bytes(a.n_rows, a.q_heads, a.dim, n) <= 8 << 30, c
+    assert planned > 300
