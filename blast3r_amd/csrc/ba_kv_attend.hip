@@ -1,13 +1,18 @@
 // Attention over the 8-bit key/value cache: the plain form, and what its kernels share with the others (ba_kv_attend.h).
+#include <math.h>
+
 #include "ba_kv_attend.h"
 
 using namespace ba;
 
 extern "C" int32_t ba_kv_attend_splits(int32_t n_seqs, int32_t heads, int32_t q_heads, int32_t dim, int64_t max_rows,
                                        int32_t n_pages) {
-    if (n_seqs < 1 || heads < 1 || q_heads < heads || max_rows < 1 || n_pages < 1) return 1;
+    if (n_seqs < 1 || heads < 1 || q_heads < heads || max_rows < 1 || n_pages < 1 || dim < 4) return 1;
     const int64_t rows = max_rows * (q_heads / heads);
     const AtShape v = at_shape(rows, dim);
+    // two parts of so many workgroups, or the join of so many rows, are more than a launch can have
+    const double most_rows = ((1 << 24) - 1) * (double)(AT_T / (dim / 4)), all_rows = (double)n_seqs * max_rows * q_heads;
+    if ((double)n_seqs * heads * ceil((double)rows / v.rows) >= 1 << 22 || all_rows > most_rows || all_rows >= 2147483648.0) return 1;
     const int64_t base = (int64_t)n_seqs * heads * ((rows + v.rows - 1) / v.rows);
     const int64_t most = (n_pages + AT_MIN_BLOCKS - 1) / AT_MIN_BLOCKS;
     // Many rows: as many workgroups as the CUs hold at a time.  Few rows read memory: one and a half per CU do, and

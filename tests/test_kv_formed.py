@@ -577,3 +577,30 @@ def test_plans_are_not_refused_where_one_part_is_not():
         assert L.ba_kv_attend_scored(ctypes.byref(a), None) != 0 and b'too many' not in L.ba_last_error(), (c, L.ba_last_error())
         assert L.ba_kv_attend_workspace_bytes(a.n_rows, a.q_heads, a.dim, n) <= 8 << 30, c
     assert planned > 300
+
+
+def test_parts_of_plain_calls_are_not_refused_where_one_is_not():
+    """The same of plain attention: two parts of few rows were one workgroup, or as many rows to be joined, too many."""
+    if torch.cuda.is_available():
+        pytest.skip('would launch on addresses that are none')
+    from blast3r_amd import _lib
+    L, p = _lib.lib(), 4096
+    rng = np.random.default_rng(1)
+    log = lambda lo, hi: int(2.0 ** rng.uniform(lo, hi))  # noqa: E731
+    some = [(65536, 64, 64, 64, 1, 64), (40000, 64, 64, 256, 32, 64), (1 << 22, 1, 1, 64, 1, 64), ((1 << 22) - 1, 1, 1, 64, 1, 64), (1 << 20, 1, 16, 32, 2, 9000)]
+    some += [(log(8, 22), h, h * log(0, 4), int(rng.choice([32, 64, 96, 128, 256])), log(0, 10), log(0, 14)) for h in (log(0, 7) for _ in range(3000))]
+    two = 0
+    for seqs, heads, q_heads, dim, rows, pages in some:
+        if seqs * rows >= 1 << 31:
+            continue
+        a = _lib.BaKvAttendArgs(n_blocks=2, bits=0, dtype=2, scale=1.0, n_splits=1, k=p, v=p, scales=p, pages=p, lengths=p, q=p, o=p, n_seqs=seqs, heads=heads,
+                                q_heads=q_heads, dim=dim, n_rows=seqs * rows, rows_per_seq=rows, max_rows=rows, n_pages=pages, workspace=p, workspace_bytes=(1 << 63) - 1)
+        assert L.ba_kv_attend(ctypes.byref(a), None) != 0
+        if b'too many' in L.ba_last_error():
+            continue
+        a.n_splits = L.ba_kv_attend_splits(seqs, heads, q_heads, dim, rows, pages)
+        two += a.n_splits > 1
+        assert L.ba_kv_attend(ctypes.byref(a), None) != 0 and b'too many' not in L.ba_last_error(), (seqs, heads, q_heads, dim, rows, pages, L.ba_last_error())
+    assert two > 300
+    for bad in (((1 << 31) - 1, 65536, 65536, 256, (1 << 31) - 1, 1 << 24), (1 << 25, 65536, 65536, 64, (1 << 31) - 1, 9), (4, 4, 4, 0, 1, 9)):
+        assert L.ba_kv_attend_splits(*bad) == 1
