@@ -1527,6 +1527,9 @@ static inline AtShape at_tile(int rows, int dim) {
 }
 static inline AtShape at_shape(int64_t rows, int dim) { return at_tile(rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 128 ? 128 : 256, dim); }
 
+#define AT_WINDOW ((int64_t)1 << 40)      // wider ones are no narrower to any position, and sums with them pass 64 bits
+static inline int64_t at_window(int64_t window) { return window < AT_WINDOW ? window : AT_WINDOW; }
+
 // The checks and sizes of every attention call (ba_kv_attend.hip).
 struct AtGrid { unsigned nb; int tiles, packed; };
 struct AtJoin { int lanes; unsigned nb; };

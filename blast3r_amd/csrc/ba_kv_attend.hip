@@ -90,10 +90,11 @@ int ba::attend_wide(const ba_kv_attend_args& a) {
 extern "C" int ba_kv_attend(const ba_kv_attend_args* args, void* stream) {
     clear_error();
     BA_REQUIRE(args != nullptr, "null args");
-    const ba_kv_attend_args& a = *args;
+    ba_kv_attend_args a = *args;
     bool nothing;
     int rc = attend_check(a, nothing);
     if (rc != BA_OK || nothing) return rc;
+    a.window = at_window(a.window);
     const int64_t rows = a.max_rows * (a.q_heads / a.heads);
     const AtShape v = at_shape(rows, a.dim);
     AtGrid g;

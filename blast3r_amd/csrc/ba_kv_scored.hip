@@ -47,8 +47,6 @@ static bool joint_shape(const AtShape& own, const AtShape& common, double wgs) {
     return !own.ncb && !common.ncb && (own.rows >= common.rows || wgs <= 1024.0);
 }
 
-#define SC_WINDOW ((int64_t)1 << 40)      // wider ones are no narrower to any position, and sums with them pass 64 bits
-
 // The launches of a call: of the sequences' own blocks, of the shared ones, and the join's.
 struct ScoredShape {
     AtShape v, w;
@@ -77,7 +75,7 @@ static int scored_shape(const ba_kv_scored_args& s, const ba_kv_attend_args& a, 
 
 static int attend_scored(const ba_kv_scored_args& s, hipStream_t st) {
     ba_kv_attend_args a = s.a;
-    if (a.window > SC_WINDOW) a.window = SC_WINDOW;
+    a.window = at_window(a.window);
     a.n_splits = s.a.n_splits + s.shared_parts;
     ScoredShape shape;
     int rc = scored_shape(s, a, shape);
@@ -216,7 +214,7 @@ extern "C" void ba_kv_scored_plan(ba_kv_scored_args* args) {
     const double join = 8.0 * a.n_rows * a.q_heads * (a.dim + 2) / 9.0e6;        // mostly in the caches
     const bool brief = args->since != nullptr;
     int64_t blocks = a.n_pages;
-    if (a.window > 0 && a.window < SC_WINDOW && !args->prefix) {                     // what a tile's rows can see
+    if (a.window > 0 && a.window < AT_WINDOW && !args->prefix) {                     // what a tile's rows can see
         const int64_t at_once = 256 / group < a.max_rows ? 256 / group + 1 : a.max_rows, seen = (a.window + at_once + 62) / 64 + 1;
         blocks = seen < blocks ? seen : blocks;
     }

@@ -256,7 +256,7 @@ class KVCache:
         if window is not None:
             if window < 1:
                 raise ValueError(f'cache: window must be at least 1, got {window}')
-            a.window = window
+            a.window = min(window, 1 << 40)       # (a field of 64 bits keeps the low ones of a longer number)
         if scale is not None:
             if not 0.0 < scale < 1e30:
                 raise ValueError(f'cache: scale must be positive, got {scale}')

@@ -604,3 +604,49 @@ def test_parts_of_plain_calls_are_not_refused_where_one_is_not():
     assert two > 300
     for bad in (((1 << 31) - 1, 65536, 65536, 256, (1 << 31) - 1, 1 << 24), (1 << 25, 65536, 65536, 64, (1 << 31) - 1, 9), (4, 4, 4, 0, 1, 9)):
         assert L.ba_kv_attend_splits(*bad) == 1
+
+
+# ---------------------------------------------------------------------------------- windows wider than any list
+
+WIDE = (1 << 40, (1 << 62) + 1, (1 << 63) - 1, 1 << 63, (1 << 64) + 3, 10 ** 30)
+
+
+def test_wide_windows_are_not_cut_to_their_low_bits(host):
+    from blast3r_amd.kv_cache import KVCache
+    c = KVCache(4, 2, 64, device='cpu')
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    q, pages, lens = torch.zeros(4, 4, 64, dtype=torch.bfloat16), i32([[0, 1], [2, 3]]), i32([5, 6])
+    for window in WIDE:
+        for kw in (dict(), dict(cap=5.0)):
+            c.attend(q, pages, lens, window=window, **kw)
+            assert host[-1].window >= 1 << 40
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [3, 20, 90, 300])
+def test_windows_wider_than_any_list_are_none(n):
+    """Of rows before the first token too, whose positions are below 0; through the C entry point as well."""
+    from blast3r_amd import _lib
+    c, o = _cache(12, 2, 64, 'int8')
+    q = torch.randn((2 * n, 4, 64), device=DEV).bfloat16()
+    pages, lens = _i32(np.arange(12).reshape(2, 6)), _i32([300, n - 2])
+    print(f'wide windows {n}', flush=True)
+    real = _lib.launch
+    for kw in (dict(), dict(causal=False), dict(cap=9.0)):
+        want = c.attend(q, pages, lens, return_lse=True, **kw)
+        assert not want[0][n:n + 2].any() or kw.get('causal') is False
+        for window in WIDE:
+            for x, y in zip(c.attend(q, pages, lens, window=window, return_lse=True, **kw), want):
+                assert torch.equal(x, y), (kw, window)
+        from blast3r_amd import kv_cache
+        for window in ((1 << 63) - 1, (1 << 63) - n):
+            def put(call, args, device):
+                args.window = window
+                real(call, args, device)
+            kv_cache.launch = put
+            try:
+                got = c.attend(q, pages, lens, window=1 << 40, return_lse=True, **kw)
+            finally:
+                kv_cache.launch = real
+            for x, y in zip(got, want):
+                assert torch.equal(x, y), (kw, window)
