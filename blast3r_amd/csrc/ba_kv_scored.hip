@@ -164,8 +164,8 @@ static Guess guess(int64_t rows, int64_t n_seqs, int heads, int dim, int64_t blo
         best.us = with(best.v, (double)base * best.parts, few_us(dim, (double)base, blocks, best.parts) + parted(best.parts, false));
         return best;
     }
-    // documents are short beside their sequence: small tiles, whole (8192 tokens of documents of 50 to 2000: 143 us, 146 with
-    // tiles of 256 rows, 263 in two parts)
+    // documents packed into a prompt are short beside it: small tiles, whole (8192 tokens of documents of 50 to 2000, 32 heads of 128
+    // on 8, fp16: 143 us, 146 with tiles of 256 rows, 263 in two parts; 16 heads of 64, bf16: 74, 102)
     if (brief) return {at_tile(128, dim), 1, launch_us(at_tile(128, dim), dim, (double)n_seqs * heads * ((rows + 127) / 128), blocks, 1, 1.0)};
     static const int some[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20, 24, 32, 40, 48, 64};
     best.us = 1.0e30;
@@ -212,7 +212,10 @@ extern "C" void ba_kv_scored_plan(ba_kv_scored_args* args) {
     const int group = a.q_heads / a.heads;
     const int64_t rows = a.max_rows * group, all = a.n_rows * group;
     const double join = 8.0 * a.n_rows * a.q_heads * (a.dim + 2) / 9.0e6;        // mostly in the caches
-    const bool brief = args->since != nullptr;
+    // rows with a first token of their own are those of short documents where they are most of their list (half of 8192, 32 heads
+    // on 8: 98 us, 104 planned as without; of one long document 449 and 409).  A quarter or less may as well be the end of one:
+    // 16 rows over 65536 tokens 1666 us and 49, 256 over 8192 202 and 71 (of short documents 29.5 and 26)
+    const bool brief = args->since && 2 * a.max_rows >= 64 * (int64_t)a.n_pages;
     int64_t blocks = a.n_pages;
     if (a.window > 0 && a.window < AT_WINDOW && !args->prefix) {                     // what a tile's rows can see
         const int64_t at_once = 256 / group < a.max_rows ? 256 / group + 1 : a.max_rows, seen = (a.window + at_once + 62) / 64 + 1;
@@ -225,9 +228,10 @@ extern "C" void ba_kv_scored_plan(ba_kv_scored_args* args) {
     args->tile = own.v.rows;
     if (args->shared > 0) {
         const int64_t rest = a.n_pages - args->shared;
-        const Guess left = guess(rows, a.n_seqs, a.heads, a.dim, rest < blocks ? rest : blocks, join, true, brief, 1.0);
+        const Guess left = guess(rows, a.n_seqs, a.heads, a.dim, rest < blocks ? rest : blocks, join, true, false, 1.0);
+        const Guess whole = brief ? guess(rows, a.n_seqs, a.heads, a.dim, blocks, join, false, false, share) : own;    // as the two parts are
         const Guess common = guess(all, 1, a.heads, a.dim, args->shared, join, true, false, 1.0, &left, (double)a.n_seqs * a.heads);
-        if (common.us < own.us) {
+        if (common.us < whole.us) {
             ba_kv_scored_args s = *args;
             s.a.n_splits = left.parts;
             s.tile = left.v.rows;
