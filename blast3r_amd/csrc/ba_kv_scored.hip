@@ -15,8 +15,9 @@
 // Measured (heads of 128 int8, 32 on 8, unless said otherwise):
 //   memory   48 sequences of up to 8192 tokens, a token each, slopes: 91 us (4.6 TB/s) + join 5, as without slopes; 16 of 65000
 //            that see 64 + 4096 tokens, e4m3: 32 us (4.3 TB/s) + 5
-//   vector   2 x 2048 rows over 16384 tokens: 1030 us with masks, 960 with slopes (far weights vanish, and power with them), 1200
-//   units    capped (matrix unit busy 35%, vector units 64%: two more transcendentals a score), 1180 both
+//   issue    2 x 2048 rows over 16384 tokens: 1030 us with masks, 960 with slopes (far weights vanish, and power with them), 1200
+//            capped (vector units busy 64% of the time, 27 of it two transcendentals a score; the matrix unit 35%, 21 of it beside them;
+//            22% of the time neither: barriers, LDS and what waits for what in a wave), 1180 both
 //   latency  8192 tokens of documents of 50 to 2000: 149 us, where their products would take 65 (documents of 64, one block a tile:
 //            54, in four turns of two tiles a CU: that is what a tile takes to begin and end)
 //   shared   64 tokens over 16384 shared and 1 to 512 of their own: 45 + 6 us (41 + 16 + 6 as two launches); read by each, 460

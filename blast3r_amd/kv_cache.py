@@ -240,8 +240,9 @@ class KVCache:
                   given back is among them): they are read once for all sequences, where that is expected to be faster than
                   reading each list by itself
         A row that sees no token gives zeros.  q_heads is a multiple of the cache's heads; query head h reads cache
-        head h // (q_heads // heads).  With ``return_lse`` also log(sum(exp(scale q k^T))) as (tokens, q_heads) fp32,
-        -inf where no token is seen, with which results over different tokens can be joined."""
+        head h // (q_heads // heads).  With ``return_lse`` also the logarithm of the sum of exp(score) over the tokens that a
+        row sees (scale q k^T, capped and less its bias where these are given) as (tokens, q_heads) fp32, -inf where it sees
+        none, with which results over different tokens can be joined."""
         self._begin(q, q if out is None else out)
         shape = q.shape
         if len(shape) != 3 or shape[1] % self._heads or shape[1] == 0:
