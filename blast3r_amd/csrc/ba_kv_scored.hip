@@ -21,7 +21,7 @@
 //   latency  8192 tokens of documents of 50 to 2000: 149 us, where their products would take 65 (documents of 64, one block a tile:
 //            54, in four turns of two tiles a CU: that is what a tile takes to begin and end)
 //   shared   64 tokens over 16384 shared and 1 to 512 of their own: 45 + 6 us (41 + 16 + 6 as two launches); read by each, 460
-//   16 heads of 64, e4m3: 6144 rows of frames over 12288 tokens 288 us (0.83 PFLOP/s), 4608 rows of six frames over 16128 391 us
+//   16 heads of 64, e4m3: 6144 rows of frames over 12288 tokens 290 us (0.83 PFLOP/s), 4608 rows of six frames over 16128 391 us
 #include <math.h>
 
 #include "ba_kv_attend.h"

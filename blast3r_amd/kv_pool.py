@@ -18,7 +18,8 @@ Nothing here synchronises and every call can be captured in a graph; results do 
 the lowest free block is taken first, and sequences are served in their order.  What a call cannot do for want of blocks it
 counts in ``missing``.  The calls of one pool go one after the other (on one stream, or on streams that wait for each other).
 
-A table is (n_seqs, blocks) int32, -1 where a list has no block.  A block must not be written to by two lists: after a fork
+A table is (n_seqs, blocks) int32, -1 where a list has no block (and 2^30 more than its number where one may not be written
+to, see ``grow``).  A block must not be written to by two lists: after a fork
 the open last block is shared, and ``grow`` is what gives each its own before new tokens are appended.
 """
 import torch
@@ -127,17 +128,18 @@ class BlockPool:
 
     def grow(self, pages, lengths, new, max_new=None):
         """Blocks for ``new`` more tokens (a number, or (n_seqs,) int32) after the first ``lengths`` of each list, written into
-        ``pages``; blocks that are there already stay, unless other lists hold them too.  max_new (default: what lists can hold) bounds ``new``, and a close
-        bound saves time.  ``lengths`` stays as it is.
+        ``pages``; blocks that are there already stay, unless other lists hold them too.  max_new (default: what lists can
+        hold) bounds ``new``, and a close bound saves time.  ``lengths`` stays as it is.
 
         Returns (src, dst, n) for ``KVCache.copy``: where new tokens would go to a block that has tokens and that other lists
         hold too, it is exchanged for another one in this list, and src has to be copied to dst before anything is appended
         (and before the next call on this pool).  One list after the other, so the last holder of a block keeps it.
 
         ``missing`` says how many blocks there were not.  Lists that there were none left for have -1 at the places of their
-        new tokens; one whose shared block there was no other for holds it as before, with 2^30 added to its number.  Its
-        tokens are seen and read as ever, and rows appended to either are left out (``lengths`` must not count them).  When
-        blocks have been given back, the same call again gives such lists what they lacked."""
+        new tokens.  A shared block that there was no other for stays in all lists that were to write there and hold it still,
+        with 2^30 added to its number: its tokens are seen and read as ever.  Rows appended to either are left out, and
+        ``lengths`` must not count them.  When blocks have been given back, the same call again gives such lists what they
+        lacked."""
         a = self._args(BaKvGrowArgs)
         self._table(a.table, pages)
         S, width = a.table.n_seqs, a.table.n_pages

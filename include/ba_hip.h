@@ -735,8 +735,8 @@ int64_t ba_kv_attend_workspace_bytes(int64_t n_rows, int32_t q_heads, int32_t di
  * the same as far as their tokens go, and none of them is missing: they are read once for all rows.  a.n_splits counts the parts of the sequences' own blocks,
  * shared_parts those of the shared ones (0 without any); tile and shared_tile are rows of a workgroup (16, 32, 128, 256; 0: by
  * their number).  ba_kv_scored_plan sets the four from everything else but pointers to rows and workspace, and sets shared to
- * 0 where reading each list by itself is expected to be faster, or the parts' sums would take more than 8 GB.  With more than one part in all, a.workspace has
- * ba_kv_attend_workspace_bytes for their sum. */
+ * 0 where reading each list by itself is expected to be faster, or the parts' sums would take more than 8 GB.  With more than
+ * one part in all, a.workspace has ba_kv_attend_workspace_bytes for their sum. */
 typedef struct {
     ba_kv_attend_args a;
     const float* slopes;       /* (q_heads,) */
@@ -822,9 +822,9 @@ typedef struct {
 int ba_kv_pool_trim(const ba_kv_trim_args* args, void* stream);
 
 /* Blocks for more[s] (or `each`; at most max_new) tokens after the first lengths[s] of every list, taken in the order of the
- * lists, the lowest free block first; entries that are there already stay, but for those past the list's tokens whose
- * block other lists hold too (tokens that this one has no more): it is given back.  Where the first of them goes to a block that has
- * tokens and that other lists hold too, that block is exchanged for another: (src, dst)[0 .. n) are the blocks to be copied,
+ * lists, the lowest free block first; entries that are there already stay, but for those past the list's tokens whose block
+ * other lists hold too (tokens that this one has no more): it is given back.  Where the first of them goes to a block that
+ * has tokens and that other lists hold too, that block is exchanged for another: (src, dst)[0 .. n) are the blocks to be copied,
  * -1 after them ((n_seqs,) ints each).  One list after the other: the last holder of a block keeps it.  missing: blocks that
  * there were not; entries of new tokens without one are -1, and a block for which there was no other stays where it is, marked
  * (its number + 2^30) in all lists that were to write there and hold it still: it is read, rows appended to it are left out,
