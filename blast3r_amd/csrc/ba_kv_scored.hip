@@ -213,10 +213,11 @@ extern "C" void ba_kv_scored_plan(ba_kv_scored_args* args) {
     const int group = a.q_heads / a.heads;
     const int64_t rows = a.max_rows * group, all = a.n_rows * group;
     const double join = 8.0 * a.n_rows * a.q_heads * (a.dim + 2) / 9.0e6;        // mostly in the caches
-    // rows with a first token of their own are those of short documents where they are most of their list (half of 8192, 32 heads
-    // on 8: 98 us, 104 planned as without; of one long document 449 and 409).  A quarter or less may as well be the end of one:
-    // 16 rows over 65536 tokens 1666 us and 49, 256 over 8192 202 and 71 (of short documents 29.5 and 26)
-    const bool brief = args->since && 2 * a.max_rows >= 64 * (int64_t)a.n_pages;
+    // rows with a first token of their own are taken for those of short documents where they are half of their list (4096 of 8192,
+    // 32 heads on 8: 98 us, 104 planned as without; of one long document 449 and 409), or as many as fill the chip whatever they
+    // see (2048 in a table of 131072: 47 and 53; 16 heads of 64, 4096: 52 and 65; of one document of 32768: 696 and 587).  Fewer may
+    // as well be the end of a long one: 16 rows over 65536 tokens 1666 us and 49, 256 over 8192 202 and 71 (of short documents 29.5 and 26)
+    const bool brief = args->since && (2 * a.max_rows >= 64 * (int64_t)a.n_pages || (double)a.n_seqs * a.heads * (rows / 128) >= 512.0);
     int64_t blocks = a.n_pages;
     if (a.window > 0 && a.window < AT_WINDOW && !args->prefix) {                     // what a tile's rows can see
         const int64_t at_once = 256 / group < a.max_rows ? 256 / group + 1 : a.max_rows, seen = (a.window + at_once + 62) / 64 + 1;

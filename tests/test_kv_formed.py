@@ -654,7 +654,7 @@ def test_windows_wider_than_any_list_are_none(n):
 
 def test_plans_of_rows_with_a_first_token_of_their_own():
     """What a row's first token is, the host does not know: a few rows over a long list are planned as without, shared blocks
-    are weighed alike, and a prompt packed with documents is taken whole."""
+    are weighed alike, and a prompt packed with documents is taken whole, also in a table that is wider."""
     from blast3r_amd import _lib
     L, p = _lib.lib(), 4096
 
@@ -663,11 +663,12 @@ def test_plans_of_rows_with_a_first_token_of_their_own():
         L.ba_kv_scored_plan(a)
         return a.n_splits, a.tile, a.shared, a.shared_parts, a.shared_tile
 
-    for seqs, rows, pages in ((1, 1, 1024), (1, 16, 1024), (1, 64, 1024), (1, 512, 1024), (4, 100, 300), (1, 2048, 256), (64, 64, 40)):
+    for seqs, rows, pages in ((1, 1, 1024), (1, 16, 1024), (1, 64, 1024), (1, 512, 1024), (4, 100, 300), (1, 1024, 256), (32, 16, 64)):
         kw = dict(n_seqs=seqs, n_rows=seqs * rows, max_rows=rows, rows_per_seq=rows, n_pages=pages)
         for shared in (0, pages // 4, pages - 3):
             assert plan(since=p, shared=shared, **kw) == plan(shared=shared, **kw)
     for seqs, rows, pages, shared in ((16, 768, 252, 240), (64, 768, 252, 240), (64, 2048, 288, 256)):
         kw = dict(n_seqs=seqs, n_rows=seqs * rows, max_rows=rows, rows_per_seq=rows, n_pages=pages, shared=shared)
-        assert plan(since=p, **kw) == plan(**kw)
-    assert plan(since=p, n_seqs=1, n_rows=8192, max_rows=8192, rows_per_seq=8192, n_pages=128) == (1, 128, 0, 0, 0)
+        assert plan(since=p, **kw)[2:] == plan(**kw)[2:]
+    for pages in (128, 2048):
+        assert plan(since=p, n_seqs=1, n_rows=8192, max_rows=8192, rows_per_seq=8192, n_pages=pages) == (1, 128, 0, 0, 0)
