@@ -814,3 +814,67 @@ def test_tokens_of_others_stay_when_a_list_is_cut_short():
         k, v = cache.read(pages, _i32([0, 0]), _i32([0, 300, 500 + cut]), 500 + cut, dtype=torch.float32)
         for got in (k, v):
             assert torch.equal(got[:300], x) and torch.equal(got[300:300 + cut], x[:cut]) and torch.equal(got[300 + cut:], y)
+
+
+def test_caches_have_fewer_blocks_than_marks_leave_numbers_for():
+    from blast3r_amd import _lib
+    L, p = _lib.lib(), 4096
+    same = dict(k=p, v=p, scales=p, heads=1, dim=64, bits=1, n_seqs=1, pages=p, n_pages=1, dtype=2, n_rows=1, rows_per_seq=1, max_rows=1, n_blocks=(1 << 30) + 1)
+    at = dict(lengths=p, q=p, o=p, q_heads=1, scale=1.0, n_splits=1)
+    for call, a in ((L.ba_kv_write, _lib.BaKvArgs(**same, starts=p, rk=p, rv=p)), (L.ba_kv_read, _lib.BaKvArgs(**same, starts=p, rk=p, rv=p)),
+                    (L.ba_kv_attend, _lib.BaKvAttendArgs(**same, **at)), (L.ba_kv_attend_scored, _lib.BaKvScoredArgs(**same, **at))):
+        assert call(ctypes.byref(a), None) != 0 and b'bad sizes' in L.ba_last_error()
+
+
+@pytest.mark.gpu
+def test_steps_that_run_out_of_blocks_in_a_graph():
+    """A captured step of samples whose pool runs full, with sequences ended between the replays, as the same step run eagerly:
+    lists, lengths, counts and codes are equal after each."""
+    from blast3r_amd.kv_cache import KVCache
+    from blast3r_amd.kv_pool import BlockPool
+    S = 6
+    print('full pool in a graph', flush=True)
+
+    def start():
+        cache, pool = KVCache(9, 2, 32, torch.int8, device=DEV), BlockPool(9, device=DEV)
+        pages, lens = torch.full((S, 4), -1, dtype=torch.int32, device=DEV), _i32([0] * S)
+        x = torch.randn((90, 2, 32), device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+        pool.grow(pages, lens, _i32([90, 0, 0, 0, 0, 0]))
+        cache.append(x, x, pages, lens, offsets=_i32([0] + [90] * S))
+        lens[0] = 90
+        pool.fork(pages, lens, _i32([0] * 5), _i32([1, 2, 3, 4, 5]))
+        new = torch.zeros((S, 2, 32), device=DEV)
+
+        def step():
+            cache.copy(*pool.grow(pages, lens, 1))
+            cache.append(new, new, pages, lens)
+            at = pages.gather(1, (lens // 64).long()[:, None])[:, 0]
+            lens.add_(((at >= 0) & (at < KEPT)).int())       # of the lists that had room
+            return cache.attend(new.bfloat16(), pages, lens)
+
+        return cache, pool, pages, lens, new, step
+
+    one, two = start(), start()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        start()[-1]()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = one[-1]()
+    seen = 0
+    for t in range(60):
+        x = torch.randn((S, 2, 32), device=DEV, generator=torch.Generator(device=DEV).manual_seed(t))
+        for state in (one, two):
+            state[4].copy_(x)
+            if t in (10, 45):
+                state[1].free(state[2], state[3], _i32([t // 10]))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = two[-1]()
+        assert torch.equal(y, want), t
+        seen += int((two[2] >= KEPT).any()) + int(two[1].missing > 0)
+        for a, b in ((one[2], two[2]), (one[3], two[3]), (one[1].counts, two[1].counts), (one[1].missing, two[1].missing), (one[0].k, two[0].k), (one[0].v, two[0].v)):
+            assert torch.equal(a, b), t
+    assert seen > 10
